@@ -109,6 +109,17 @@ SIGNATURES = {
     "fvq_fp8_ffn_profile": (_c.c_int, [_vp, _i64, _c.POINTER(FvqLinearFp8),
                                        _c.POINTER(FvqLinearFp8), _vp, _vp, _sz, _vp,
                                        _c.POINTER(_c.c_float)]),
+    "fvq_rms_norm": (_c.c_int, [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _c.c_float, _vp, _c.c_int,
+                                _vp, _vp, _vp, _vp, _vp]),
+    "fvq_linear_act": (_c.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _c.c_int, _c.c_int, _vp,
+                                  _vp, _vp]),
+    "fvq_fp8_scaled_mm_act": (_c.c_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _c.c_int,
+                                         _c.c_int, _vp, _vp, _vp]),
+    "fvq_set_linear_kernel": (_c.c_int, [_c.c_int]),
+    "fvq_fp8_cache_write": (_c.c_int, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp,
+                                       _vp, _vp, _vp, _i64, _vp]),
+    "fvq_fp8_cache_read": (_c.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64,
+                                      _vp, _i64, _vp, _vp, _vp]),
     "fvq_div_full_probe": (_c.c_int, [_vp, _vp, _vp, _i64, _vp]),
     "fvq_pil_resize": (_c.c_int, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                   _vp, _vp, _vp]),

@@ -23,7 +23,7 @@ BUILD = HERE / "_build"
 LIB = HERE / "libfvq.so"
 
 SOURCES = ["fvq_quant.cu", "fvq_fp8.cu", "fvq_resize.cu", "fvq_block.cu", "fvq_gemm.cu",
-           "fvq_api.cu", "fvq_noalloc.cu"]
+           "fvq_norm.cu", "fvq_linear.cu", "fvq_cache.cu", "fvq_api.cu", "fvq_noalloc.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
     "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2",

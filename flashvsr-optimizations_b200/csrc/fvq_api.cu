@@ -1005,6 +1005,174 @@ int fvq_pil_normalize(const uint8_t* src, int64_t frames, int64_t h, int64_t w,
   return FVQ_OK;
 }
 
+int fvq_rms_norm(const uint16_t* x, int64_t rows, int64_t inner, int64_t outer_stride,
+                 int64_t inner_stride, int64_t d, const uint16_t* weight, float eps,
+                 const void* residual, int residual_fp32, void* residual_out, uint16_t* y,
+                 uint8_t* q, float* scale, void* stream) {
+  if (rows <= 0 || rows > (int64_t(1) << 30) || inner <= 0 || rows % inner != 0)
+    return fail(FVQ_EINVAL, "fvq_rms_norm: rows must be in [1, 2^30] and a multiple of inner "
+                "(got %lld, %lld)", (long long)rows, (long long)inner);
+  if (d <= 0 || d > fvq::rms_norm_max_d())
+    return fail(FVQ_EINVAL, "fvq_rms_norm: d must be in [1, %lld] (got %lld)",
+                (long long)fvq::rms_norm_max_d(), (long long)d);
+  if (outer_stride < 0 || inner_stride < 0)
+    return fail(FVQ_EINVAL, "fvq_rms_norm: negative stride");
+  if (!(eps >= 0.0f)) return fail(FVQ_EINVAL, "fvq_rms_norm: eps must be >= 0");
+  if (!x || (!y && !q) || (q != nullptr) != (scale != nullptr) ||
+      (residual != nullptr) != (residual_out != nullptr))
+    return fail(FVQ_EINVAL, "fvq_rms_norm: NULL pointer (x; y or q; scale with q; residual_out "
+                "with residual)");
+  const auto off = [](const void* p, uintptr_t mask) {
+    return (reinterpret_cast<uintptr_t>(p) & mask) != 0;
+  };
+  if (off(x, 1) || off(weight, 1) || off(y, 1) || off(scale, 3) ||
+      off(residual, residual_fp32 ? 3 : 1) || off(residual_out, residual_fp32 ? 3 : 1))
+    return fail(FVQ_EALIGN, "fvq_rms_norm: pointers must be aligned to their element");
+  if (int rc = check_device()) return rc;
+  fvq::NormArgs a = {x, rows, inner, outer_stride, inner_stride, static_cast<int>(d), weight, eps,
+                     residual, residual_out, residual_fp32 != 0, y, q, scale};
+  cudaError_t e = fvq::launch_rms_norm(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "fvq_rms_norm launch");
+  return FVQ_OK;
+}
+
+namespace {
+
+int linear_impl(const fvq::LinearProblem& l, const char* who, void* stream) {
+  const int per16 = l.fp8 ? 16 : 8;  // elements in 16 bytes
+  if (l.m <= 0 || l.m > (int64_t(1) << 28))
+    return fail(FVQ_EINVAL, "%s: m must be in [1, 2^28] (got %lld)", who, (long long)l.m);
+  if (l.n <= 0 || l.n % 8 != 0 || l.n > (int64_t(1) << 28))
+    return fail(FVQ_EINVAL, "%s: n must be a positive multiple of 8 up to 2^28 (got %lld)", who,
+                (long long)l.n);
+  if (l.k <= 0 || l.k % per16 != 0 || l.k > (int64_t(1) << 24))
+    return fail(FVQ_EINVAL, "%s: k must be a positive multiple of %d up to 2^24 (got %lld)", who,
+                per16, (long long)l.k);
+  if (l.x_stride < l.k || l.x_stride % per16 != 0 || l.x_stride > (int64_t(1) << 32))
+    return fail(FVQ_EINVAL, "%s: the row stride must be a multiple of %d, at least k (got %lld)",
+                who, per16, (long long)l.x_stride);
+  if (l.act < FVQ_ACT_NONE || l.act > FVQ_ACT_SILU)
+    return fail(FVQ_EINVAL, "%s: unknown activation %d", who, l.act);
+  if (!l.x || !l.w || !l.y || (l.fp8 && (!l.sx || !l.sw)))
+    return fail(FVQ_EINVAL, "%s: NULL pointer", who);
+  if (!aligned16(l.x) || !aligned16(l.w) || !aligned16(l.sw) || !aligned16(l.bias) ||
+      !aligned16(l.residual) || !aligned16(l.y) || !aligned4(l.sx))
+    return fail(FVQ_EALIGN, "%s: operands, W scales, bias, residual and y must be 16-byte aligned",
+                who);
+  if (int rc = check_device()) return rc;
+  const char* why = nullptr;
+  cudaError_t e = fvq::launch_linear(l, wait_limit(), static_cast<cudaStream_t>(stream), &why);
+  if (e != cudaSuccess) {
+    if (why) return fail(FVQ_ECUDA, "%s: %s", who, why);
+    return cuda_fail(e, who);
+  }
+  return FVQ_OK;
+}
+
+}  // namespace
+
+int fvq_linear_act(const uint16_t* x, int64_t m, int64_t k, int64_t x_stride, const uint16_t* w,
+                   int64_t n, const uint16_t* bias, int act, int gated, const uint16_t* residual,
+                   uint16_t* y, void* stream) {
+  const fvq::LinearProblem l = {x, w, nullptr, nullptr, bias, residual, y, m, n, k, x_stride,
+                                act, gated != 0, false};
+  return linear_impl(l, "fvq_linear_act", stream);
+}
+
+int fvq_fp8_scaled_mm_act(const uint8_t* a, const float* scale_a, int64_t m, int64_t k,
+                          int64_t a_stride, const uint8_t* w, const float* scale_w, int64_t n,
+                          const uint16_t* bias, int act, int gated, const uint16_t* residual,
+                          uint16_t* y, void* stream) {
+  const fvq::LinearProblem l = {a, w, scale_a, scale_w, bias, residual, y, m, n, k, a_stride,
+                                act, gated != 0, true};
+  return linear_impl(l, "fvq_fp8_scaled_mm_act", stream);
+}
+
+int fvq_set_linear_kernel(int mode) {
+  if (mode < 0 || mode > 2)
+    return fail(FVQ_EINVAL, "fvq_set_linear_kernel: mode must be 0, 1 or 2 (got %d)", mode);
+  fvq::set_linear_kernel_mode(mode);
+  return FVQ_OK;
+}
+
+namespace {
+
+int check_cache(int64_t heads, int64_t d, int64_t slots, const void* kc, const void* ks,
+                const void* vc, const void* vs, const char* who) {
+  if (heads <= 0 || heads > 65535 || d <= 0 || d % 8 != 0 || d > 512)
+    return fail(FVQ_EINVAL, "%s: heads must be in [1, 65535], d a multiple of 8 up to 512 "
+                "(got %lld, %lld)", who, (long long)heads, (long long)d);
+  if (slots < 0 || slots > (int64_t(1) << 40))
+    return fail(FVQ_EINVAL, "%s: bad store size", who);
+  if (!kc || !ks || !vc || !vs) return fail(FVQ_EINVAL, "%s: NULL pointer", who);
+  const auto off = [](const void* p, uintptr_t mask) {
+    return (reinterpret_cast<uintptr_t>(p) & mask) != 0;
+  };
+  if (off(kc, 7) || off(vc, 7) || off(ks, 3) || off(vs, 3))
+    return fail(FVQ_EALIGN, "%s: codes must be 8-byte, scales 4-byte aligned", who);
+  return FVQ_OK;
+}
+
+}  // namespace
+
+int fvq_fp8_cache_write(const uint16_t* k, const uint16_t* v, int64_t tokens, int64_t heads,
+                        int64_t d, int64_t k_token_stride, int64_t k_head_stride,
+                        int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots,
+                        uint8_t* k_codes, float* k_scale, uint8_t* v_codes, float* v_scale,
+                        int64_t num_slots, void* stream) {
+  const char* who = "fvq_fp8_cache_write";
+  if (int rc = check_cache(heads, d, num_slots, k_codes, k_scale, v_codes, v_scale, who)) return rc;
+  if (tokens <= 0 || tokens > (int64_t(1) << 31) || tokens * heads > (int64_t(1) << 31))
+    return fail(FVQ_EINVAL, "%s: tokens must be > 0 and tokens * heads at most 2^31 (got %lld)",
+                who, (long long)tokens);
+  if (k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0 ||
+      (k_token_stride | k_head_stride | v_token_stride | v_head_stride) % 8 != 0)
+    return fail(FVQ_EINVAL, "%s: strides must be non-negative multiples of 8", who);
+  if (!k || !v || !slots) return fail(FVQ_EINVAL, "%s: NULL pointer", who);
+  if (!aligned16(k) || !aligned16(v) || (reinterpret_cast<uintptr_t>(slots) & 7u) != 0)
+    return fail(FVQ_EALIGN, "%s: k and v must be 16-byte, slots 8-byte aligned", who);
+  if (int rc = check_device()) return rc;
+  uint32_t* err = fvq::error_word_ptr();
+  if (err == nullptr) return cuda_fail(cudaErrorInvalidSymbol, who);
+  fvq::CacheWriteArgs a = {{k, k_token_stride, k_head_stride, k_codes, k_scale},
+                           {v, v_token_stride, v_head_stride, v_codes, v_scale},
+                           slots, tokens * heads, static_cast<int>(heads), static_cast<int>(d),
+                           num_slots};
+  cudaError_t e = fvq::launch_cache_write(a, err, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return FVQ_OK;
+}
+
+int fvq_fp8_cache_read(const uint8_t* k_codes, const float* k_scale, const uint8_t* v_codes,
+                       const float* v_scale, int64_t num_pages, int64_t page, int64_t heads,
+                       int64_t d, const int32_t* page_table, int64_t batch, int64_t pages_per_seq,
+                       const int32_t* lengths, int64_t max_len, uint16_t* k_out, uint16_t* v_out,
+                       void* stream) {
+  const char* who = "fvq_fp8_cache_read";
+  if (page <= 0 || page > (int64_t(1) << 31) || num_pages < 0 || num_pages > (int64_t(1) << 31))
+    return fail(FVQ_EINVAL, "%s: bad page size or count (%lld, %lld)", who, (long long)page,
+                (long long)num_pages);
+  if (int rc = check_cache(heads, d, 0, k_codes, k_scale, v_codes, v_scale, who)) return rc;
+  if (batch <= 0 || batch > 65535 || pages_per_seq <= 0 || pages_per_seq > (int64_t(1) << 31))
+    return fail(FVQ_EINVAL, "%s: batch must be in [1, 65535] and pages_per_seq in [1, 2^31] "
+                "(got %lld, %lld)", who, (long long)batch, (long long)pages_per_seq);
+  if (max_len <= 0 || max_len > (int64_t(1) << 31) || max_len * heads * (d / 8) > (int64_t(1) << 38))
+    return fail(FVQ_EINVAL, "%s: max_len must be positive and max_len * heads * d at most 2^41 "
+                "(got %lld)", who, (long long)max_len);
+  if (!page_table || !lengths || !k_out || !v_out) return fail(FVQ_EINVAL, "%s: NULL pointer", who);
+  if (!aligned16(k_out) || !aligned16(v_out) || !aligned4(page_table) || !aligned4(lengths))
+    return fail(FVQ_EALIGN, "%s: outputs must be 16-byte, table and lengths 4-byte aligned", who);
+  if (int rc = check_device()) return rc;
+  uint32_t* err = fvq::error_word_ptr();
+  if (err == nullptr) return cuda_fail(cudaErrorInvalidSymbol, who);
+  fvq::CacheReadArgs a = {k_codes, v_codes, k_scale, v_scale, page_table, lengths, k_out, v_out,
+                          batch, pages_per_seq, max_len, page, num_pages,
+                          static_cast<int>(heads), static_cast<int>(d)};
+  cudaError_t e = fvq::launch_cache_read(a, err, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return FVQ_OK;
+}
+
 int fvq_rcp_approx_probe(const float* in, float* out, int64_t n, void* stream) {
   if (n < 0 || (n > 0 && (!in || !out))) return fail(FVQ_EINVAL, "fvq_rcp_approx_probe: bad args");
   if (int rc = check_device()) return rc;

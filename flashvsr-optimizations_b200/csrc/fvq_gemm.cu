@@ -2014,6 +2014,8 @@ cudaError_t launch_gemm(const uint8_t* a_codes, const uint8_t* a_sf, const float
                                  amax_out, wait_limit, st);
 }
 
+void* tensor_map_encode_fn() { return reinterpret_cast<void*>(get_encode_fn()); }
+
 cudaError_t launch_gelu_probe(const uint16_t* in, uint16_t* out, int64_t count, cudaStream_t st) {
   if (count <= 0) return cudaSuccess;
   int64_t blocks = (count + 255) / 256;

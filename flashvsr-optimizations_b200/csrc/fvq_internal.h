@@ -15,6 +15,8 @@ constexpr uint32_t kErrWaitEpilogue = 1u << 2;  // epilogue gave up on the accum
 constexpr uint32_t kErrWaitTeardown = 1u << 3;  // teardown gave up on in-flight work
 constexpr uint32_t kErrSmemAlign = 1u << 4;     // dynamic shared memory not 1024-byte aligned
 constexpr uint32_t kErrWaitGrid = 1u << 5;      // fused quantizer gave up at its grid barrier
+constexpr uint32_t kErrCacheSlot = 1u << 6;     // a key/value slot past the store (nothing written)
+constexpr uint32_t kErrCachePage = 1u << 7;     // a page or length past the store (read as zeros)
 
 // Bound on any single pipeline wait inside a kernel (wall time, ns).
 constexpr uint64_t kDefaultWaitLimit = 2000000000ull;
@@ -193,6 +195,73 @@ cudaError_t launch_pil_normalize(const uint8_t* src, int64_t frames, int h, int 
 // (fvq_block.cu).
 cudaError_t launch_ln_modulate(const uint16_t* x, int64_t rows, int64_t d, const uint16_t* shift,
                                const uint16_t* scale, float eps, uint16_t* u, cudaStream_t st);
+// RMS norm with the residual's addition (fvq_norm.cu).  Row r of x starts at
+// (r / inner) * outer_stride + (r % inner) * inner_stride elements; every other tensor is
+// contiguous [rows, d].  d <= rms_norm_max_d().
+struct NormArgs {
+  const uint16_t* x;
+  int64_t rows, inner, outer_stride, inner_stride;
+  int d;
+  const uint16_t* weight;     // bf16 [d] or null (ones)
+  float eps;
+  const void* residual;       // bf16 or fp32 [rows, d], or null
+  void* residual_out;         // residual's type; set exactly when residual is
+  int residual_f32;
+  uint16_t* y;                // bf16, or null
+  uint8_t* q;                 // E4M3, or null
+  float* scale;               // fp32 [rows], with q
+};
+int64_t rms_norm_max_d();
+cudaError_t launch_rms_norm(const NormArgs& a, cudaStream_t st);
+
+// y = bf16(act(x W^T [* sx * sw] + bias) [* gate's other half] [+ residual]) (fvq_linear.cu).
+// x: m rows of k elements, x_stride elements apart; w: [n, k], gated [2n, k] (the activated
+// half first).  n % 8 == 0; k a multiple of 16 bytes' worth of elements.
+struct LinearProblem {
+  const void* x;
+  const void* w;
+  const float* sx;            // fp32 [m], with fp8
+  const float* sw;            // fp32 [n or 2n], with fp8
+  const uint16_t* bias;       // bf16 [n or 2n] or null
+  const uint16_t* residual;   // bf16 [m, n] or null
+  uint16_t* y;                // bf16 [m, n]
+  int64_t m, n, k, x_stride;
+  int act;
+  bool gated, fp8;
+};
+cudaError_t launch_linear(const LinearProblem& l, uint64_t wait_limit, cudaStream_t st,
+                          const char** why);
+void set_linear_kernel_mode(int mode);  // 0 by size, 1 the split kernel, 2 the pair kernel
+int linear_kernel_mode();
+void* tensor_map_encode_fn();           // cuTensorMapEncodeTiled, or null (fvq_gemm.cu)
+
+// Paged FP8 key/value store (fvq_cache.cu).  codes [num_slots, heads, d], scale
+// [num_slots, heads]; a page is `page` consecutive slots.
+struct CacheRows {
+  const uint16_t* x;          // bf16, element strides between tokens and heads
+  int64_t token_stride, head_stride;
+  uint8_t* codes;
+  float* scale;
+};
+struct CacheWriteArgs {
+  CacheRows k, v;
+  const int64_t* slots;       // [tokens]; negative: not stored
+  int64_t rows;               // tokens * heads
+  int heads, d;
+  int64_t num_slots;
+};
+struct CacheReadArgs {
+  const uint8_t *k_codes, *v_codes;
+  const float *k_scale, *v_scale;
+  const int32_t* table;       // [batch, pages_per_seq]
+  const int32_t* lengths;     // [batch]
+  uint16_t *k_out, *v_out;    // bf16 [batch, max_len, heads, d]
+  int64_t batch, pages_per_seq, max_len, page, num_pages;
+  int heads, d;
+};
+cudaError_t launch_cache_write(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st);
+cudaError_t launch_cache_read(const CacheReadArgs& a, uint32_t* err_word, cudaStream_t st);
+
 cudaError_t set_error_word(uint32_t v, cudaStream_t st);
 uint32_t* error_word_ptr();   // device address of the error word (current device)
 cudaError_t read_error_word(uint32_t* v, cudaStream_t st);

@@ -1,0 +1,943 @@
+// fvq_linear.cu -- matrix product with bias, activation, gate and residual in its epilogue.
+//
+//   z = x W^T  [* sx_m * sw_n]  + b                     fp32 accumulation (tcgen05)
+//   h = act(z)   or, gated (W = [Wg; Wu], 2n rows),  act(z_g) * z_u
+//   y = bf16(h + r)                                     one rounding
+//
+// Operands bf16 (kind::f16) or E4M3 with one fp32 scale per row (kind::f8f6f4); both take
+// 128 bytes of K per row and tile, so one code serves both and only the instruction
+// descriptor differs.  Two kernels:
+//
+//   linear_pair_kernel   many tokens: tensor-bound.  Persistent clusters of two CTAs
+//     (cta_group::2, M = 256 tokens, N = bn columns), W and x tiles by TMA through a ring of
+//     stages, two accumulators in TMEM so that the next tile's products run under the
+//     epilogue.  Gated: the even CTA loads the tile's Wg rows, the odd one its Wu rows, so
+//     both halves of an output column meet in the same TMEM lane and no pass over h is made.
+//   linear_split_kernel  few tokens: bound by reading W once.  The operands change places:
+//     `wr` rows of W are the M side, up to 256 tokens the N side, so that a single token
+//     costs one N = 16 instruction and not a 128-row tile; K is split over a cluster of up
+//     to eight CTAs until every SM streams its share of W, and the partial sums are joined
+//     through distributed shared memory in rank order (no atomics, no workspace, the same
+//     bits on every run).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cstring>
+
+#include "fvq_internal.h"
+#include "fvq_ptx.cuh"
+
+namespace fvq {
+
+namespace {
+
+constexpr int kKB = 128;  // bytes of K per row and tile: one 128B swizzle row
+
+// ---------------------------------------------------------------- activations
+enum Act { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
+
+// z * sigmoid(t), t and z of one sign: one exponential and one fast division (a few fp32 ulp,
+// against bf16's 2^-8), without the cancellation that 1 + tanh has for negative z.  The
+// exponential is of -|t|, so the divisor stays in [1, 2] and the negative tail keeps its
+// digits down to the smallest values.
+__device__ __forceinline__ float z_sigmoid(float z, float t) {
+  const float e = __expf(-fabsf(t));
+  return __fdividef(z < 0.0f ? z * e : z, 1.0f + e);
+}
+
+// act(z) in fp32; silu and the tanh form of gelu are z * sigmoid(t).  relu keeps NaN.
+template <int kAct>
+__device__ __forceinline__ float activate(float z) {
+  if constexpr (kAct == kActRelu) {
+    return z < 0.0f ? 0.0f : z;
+  } else if constexpr (kAct == kActGelu) {
+    return 0.5f * z * erfcf(-0.70710678118654752f * z);
+  } else if constexpr (kAct == kActGeluTanh) {
+    const float t = 1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.0f);  // 2 sqrt(2/pi) (z + ..)
+    return z_sigmoid(z, t);
+  } else if constexpr (kAct == kActSilu) {
+    return z_sigmoid(z, z);
+  } else {
+    return z;
+  }
+}
+
+__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// ---------------------------------------------------------------- MMA
+template <bool kF8>
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                         uint32_t accumulate) {
+  if constexpr (kF8)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+template <bool kF8>
+__device__ __forceinline__ void mma_one(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  if constexpr (kF8)
+    mma_f8(d, a, b, idesc, accumulate);
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// fp32 accumulator; both operands BF16 (kind::f16) or both E4M3 (kind::f8f6f4), K-major
+template <bool kF8>
+__host__ __device__ constexpr uint32_t instr_desc(int m, int n) {
+  return (1u << 4) | (kF8 ? 0u : (1u << 7) | (1u << 10)) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void flag(int* abort_flag, uint32_t* err_word, uint32_t bit) {
+  atomicOr(err_word, bit);
+  *reinterpret_cast<volatile int*>(abort_flag) = 1;
+}
+
+// from one lane of a converged warp
+__device__ __forceinline__ void warp_flag(int* abort_flag, uint32_t* err_word, uint32_t bit) {
+  if (elect_one()) flag(abort_flag, err_word, bit);
+  __syncwarp();
+}
+
+__device__ __forceinline__ bool warp_aborted(const int* abort_flag) {
+  return __shfl_sync(0xFFFFFFFFu, *reinterpret_cast<const volatile int*>(abort_flag), 0) != 0;
+}
+
+// ---------------------------------------------------------------- many tokens
+constexpr int kPairTokens = 256;                  // per pair; 128 per CTA
+constexpr int kPairABytes = 128 * kKB;            // 16 KB
+constexpr int kPairBBytes = 128 * kKB;            // half of the (up to 256) W rows
+constexpr int kPairStageBytes = kPairABytes + kPairBBytes;
+constexpr int kPairStages = 5;
+constexpr int kPairEpiWarps = 8;                  // two per TMEM lane quadrant
+constexpr int kPairThreads = 64 + 32 * kPairEpiWarps;
+constexpr int kChunk = 64;                        // output columns staged at a time (128 bytes)
+constexpr int kChunkBytes = 32 * kChunk * 2;      // of one warp's 32 rows
+constexpr int kPairStagingOff = kPairStages * kPairStageBytes;
+constexpr int kPairBarrierOff = kPairStagingOff + kPairEpiWarps * 2 * kChunkBytes;
+constexpr int kPairSmemBytes = kPairBarrierOff + 512;
+constexpr int kAccCols = 256;                     // TMEM columns per accumulator
+static_assert(kPairSmemBytes <= 232448, "pair plan exceeds shared memory");
+
+struct PairBars {
+  uint64_t full[kPairStages];     // even CTA: both CTAs' loads of the stage landed
+  uint64_t empty[kPairStages];    // the pair's MMAs on the stage completed
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];          // even CTA: both epilogues drained the accumulator
+  uint64_t res_full[kPairEpiWarps][2];  // residual chunk landed in the warp's staging buffer
+  uint64_t teardown;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(PairBars) <= 512, "pair barrier area");
+
+struct LinearArgs {
+  const float* sx;        // [m] or null
+  const float* sw;        // [wn] or null
+  const uint16_t* bias;   // [wn] or null
+  int m, n, k_tiles;
+  int act;
+  int bn;                 // accumulator columns per tile (pair kernel)
+  int residual;           // 0 / 1
+  uint64_t wait_limit;
+  uint32_t* err_word;
+};
+
+// 32 accumulator columns of one row -> z = acc [* sx * sw] + b.  `col`: first W row index;
+// `left`: how many of the 32 are inside the matrix (a multiple of 8).
+template <bool kF8>
+__device__ __forceinline__ void affine32(uint32_t (&r)[32], float sx, const float* sw,
+                                         const uint16_t* bias, int col, int left) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (8 * q < left) {
+      if constexpr (kF8) {
+        const float4 s0 = __ldg(reinterpret_cast<const float4*>(sw + col) + 2 * q);
+        const float4 s1 = __ldg(reinterpret_cast<const float4*>(sw + col) + 2 * q + 1);
+        const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          r[8 * q + j] = __float_as_uint(__uint_as_float(r[8 * q + j]) * sx * s[j]);
+      }
+      if (bias != nullptr) {
+        const uint4 b = __ldg(reinterpret_cast<const uint4*>(bias + col) + q);
+        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          r[8 * q + 2 * j] = __float_as_uint(__uint_as_float(r[8 * q + 2 * j]) + bf_lo(w[j]));
+          r[8 * q + 2 * j + 1] = __float_as_uint(__uint_as_float(r[8 * q + 2 * j + 1]) + bf_hi(w[j]));
+        }
+      }
+    }
+  }
+}
+
+template <int kAct, bool kGated>
+__device__ __forceinline__ void act32_t(uint32_t (&r)[32], const uint32_t (&u)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    float h = activate<kAct>(__uint_as_float(r[j]));
+    if constexpr (kGated) h *= __uint_as_float(u[j]);
+    r[j] = __float_as_uint(h);
+  }
+}
+
+template <bool kGated>
+__device__ __forceinline__ void act32(int act, uint32_t (&r)[32], const uint32_t (&u)[32]) {
+  switch (act) {
+    case kActRelu: act32_t<kActRelu, kGated>(r, u); break;
+    case kActGelu: act32_t<kActGelu, kGated>(r, u); break;
+    case kActGeluTanh: act32_t<kActGeluTanh, kGated>(r, u); break;
+    case kActSilu: act32_t<kActSilu, kGated>(r, u); break;
+    default: act32_t<kActNone, kGated>(r, u); break;
+  }
+}
+
+template <bool kF8, bool kGated>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_x,
+                       const __grid_constant__ CUtensorMap tmap_w,
+                       const __grid_constant__ CUtensorMap tmap_r,
+                       const __grid_constant__ CUtensorMap tmap_y, const LinearArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicOr(a.err_word, kErrSmemAlign);
+    return;  // both CTAs see the same layout, so both return here
+  }
+  auto* bars = reinterpret_cast<PairBars*>(smem + kPairBarrierOff);
+  int* abort_flag = &bars->abort_flag;
+  const int warp = warp_index_uniform();
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool even = rank == 0;
+  const int pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+  const int bn = a.bn, out_cols = kGated ? bn / 2 : bn;
+  const int n_blocks = (a.n + out_cols - 1) / out_cols;
+  const int tiles = ((a.m + kPairTokens - 1) / kPairTokens) * n_blocks;
+  const int count = pair < tiles ? (tiles - 1 - pair) / pairs + 1 : 0;  // same in both CTAs
+  const uint64_t wait_limit = a.wait_limit;
+  const uint64_t teardown_limit = wait_limit > kDefaultWaitLimit ? wait_limit : kDefaultWaitLimit;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->acc_full[b], 1);
+      mbar_init(&bars->acc_empty[b], 2 * kPairEpiWarps);
+      for (int w = 0; w < kPairEpiWarps; ++w) mbar_init(&bars->res_full[w][b], 1);
+    }
+    mbar_init(&bars->teardown, 1);
+    bars->abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+    prefetch_tmap(&tmap_x);
+    prefetch_tmap(&tmap_w);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&bars->tmem_base, 2 * kAccCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();  // barriers of both CTAs initialised before any remote arrive
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const auto even_addr = [&](const void* p) { return mapa_shared(smem_u32(p), 0); };
+  const auto odd_addr = [&](const void* p) { return mapa_shared(smem_u32(p), 1); };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer (both CTAs)
+    uint32_t armed[kPairStages];
+#pragma unroll
+    for (int s = 0; s < kPairStages; ++s) armed[s] = 0;
+    const uint32_t w_bytes = static_cast<uint32_t>(bn / 2) * kKB;
+    const int k_step = kF8 ? kKB : kKB / 2;  // elements
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < count && !warp_aborted(abort_flag); ++i) {
+      const int t = pair + i * pairs;
+      const int nb = t % n_blocks, mb = t / n_blocks;  // N block fastest: x rows stay in L2
+      const int x_row = mb * kPairTokens + static_cast<int>(rank) * 128;
+      // gated: Wg rows in the even CTA, the same columns' Wu rows in the odd one
+      const int w_row = kGated ? nb * out_cols + static_cast<int>(rank) * a.n
+                               : nb * bn + static_cast<int>(rank) * (bn / 2);
+      for (int kt = 0; kt < a.k_tiles; ++kt) {
+        if (!warp_wait_cluster_bounded(&bars->empty[stage], phase ^ 1u, wait_limit)) {
+          warp_flag(abort_flag, a.err_word, kErrWaitProducer);
+          break;
+        }
+        uint8_t* sa = smem + stage * kPairStageBytes;
+        const uint32_t bar = even_addr(&bars->full[stage]);
+        if (elect_one()) {
+          if (even) mbar_arrive_expect_tx(&bars->full[stage], 2 * (kPairABytes + w_bytes));
+          tma_load_2d_pair(sa, &tmap_x, bar, kt * k_step, x_row);
+          tma_load_2d_pair(sa + kPairABytes, &tmap_w, bar, kt * k_step, w_row);
+        }
+        __syncwarp();
+        armed[stage] += 1;
+        if (++stage == kPairStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    // the even CTA's stage barriers count both CTAs' loads; the odd CTA's land before the
+    // even CTA passes the final cluster barrier
+    for (int s = 0; even && s < kPairStages; ++s) {
+      if (armed[s] > 0 &&
+          !warp_wait_cluster_bounded(&bars->full[s], (armed[s] - 1) & 1u, teardown_limit))
+        warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
+    }
+  } else if (warp == 1) {
+    if (even) {
+      // ---------------------------------------------------------- MMA issuer (even CTA)
+      const uint32_t idesc = instr_desc<kF8>(kPairTokens, bn);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool issued_any = false, ok = true;
+      for (int i = 0; ok && i < count && !warp_aborted(abort_flag); ++i) {
+        const int buf = i & 1;
+        if (!warp_wait_cluster_bounded(&bars->acc_empty[buf],
+                                       (static_cast<uint32_t>(i >> 1) & 1u) ^ 1u, wait_limit)) {
+          warp_flag(abort_flag, a.err_word, kErrWaitMma);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(buf * kAccCols);
+        for (int kt = 0; kt < a.k_tiles; ++kt) {
+          if (!warp_wait_cluster_bounded(&bars->full[stage], phase, wait_limit)) {
+            warp_flag(abort_flag, a.err_word, kErrWaitMma);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * kPairStageBytes);
+          const uint64_t adesc = make_smem_desc(sa, 16, 1024, 2);
+          const uint64_t bdesc = make_smem_desc(sa + kPairABytes, 16, 1024, 2);
+          const uint32_t empty_odd = odd_addr(&bars->empty[stage]);
+          if (elect_one()) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)  // 32-byte K steps inside the 128B swizzle atom
+              mma_pair<kF8>(d, adesc + static_cast<uint64_t>(2 * j),
+                            bdesc + static_cast<uint64_t>(2 * j), idesc,
+                            (kt > 0 || j > 0) ? 1u : 0u);
+            tc_commit_pair(smem_u32(&bars->empty[stage]));
+            tc_commit_pair(empty_odd);
+          }
+          __syncwarp();
+          issued_any = true;
+          if (++stage == kPairStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        const uint32_t acc_odd = odd_addr(&bars->acc_full[buf]);
+        if (elect_one()) {
+          tc_commit_pair(smem_u32(&bars->acc_full[buf]));
+          tc_commit_pair(acc_odd);
+        }
+        __syncwarp();
+      }
+      if (warp_aborted(abort_flag) && issued_any) {
+        if (elect_one()) tc_commit_pair(smem_u32(&bars->teardown));
+        __syncwarp();
+        if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))
+          warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    // Warp w: TMEM lanes 32 * (w % 4).., every second 64-column chunk of the tile.  A chunk
+    // goes through one of the warp's two staging buffers: the residual chunk is loaded into
+    // it, the results take its place and leave by a TMA store (which also clips the edges).
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const int trow = quad * 32 + lane;
+    uint8_t* staging = smem + kPairStagingOff + (warp - 2) * 2 * kChunkBytes;
+    uint64_t* res_full = bars->res_full[warp - 2];
+    const int chunks = out_cols / kChunk;
+    uint32_t uses = 0;  // chunks through the staging buffers so far
+    bool ok = true;
+    for (int i = 0; ok && i < count; ++i) {
+      const int t = pair + i * pairs;
+      const int nb = t % n_blocks, mb = t / n_blocks;
+      const int row0 = mb * kPairTokens + static_cast<int>(rank) * 128 + quad * 32;
+      const int row = mb * kPairTokens + static_cast<int>(rank) * 128 + trow;
+      const float sx = kF8 && row < a.m ? __ldg(a.sx + row) : 0.0f;
+      const int buf = i & 1;
+      bool waited = false;
+      for (int c = half; c < chunks; c += 2) {
+        const int col0 = nb * out_cols + c * kChunk;
+        const bool inside = col0 < a.n && row0 < a.m;  // warp-uniform
+        uint8_t* stage_buf = staging + (uses & 1u) * kChunkBytes;
+        if (inside) {
+          // at most one committed store (of the other buffer) may still be reading
+          if (lane == 0) {
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            if (a.residual) {
+              mbar_arrive_expect_tx(&res_full[uses & 1u], kChunkBytes);
+              tma_load_2d(stage_buf, &tmap_r, &res_full[uses & 1u], col0, row0);
+            }
+          }
+          __syncwarp();
+        }
+        if (!waited) {
+          if (!mbar_wait_cluster_bounded(&bars->acc_full[buf], static_cast<uint32_t>(i >> 1) & 1u,
+                                         wait_limit)) {
+            flag(abort_flag, a.err_word, kErrWaitEpilogue);
+            ok = false;
+          }
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          tc_fence_after();
+          waited = true;
+        }
+        if (inside && a.residual) {
+          // a residual load in flight has to land before its buffer is used or the CTA exits
+          if (!mbar_wait_bounded(&res_full[uses & 1u], (uses >> 1) & 1u, teardown_limit)) {
+            flag(abort_flag, a.err_word, kErrWaitEpilogue);
+            ok = false;
+          }
+          ok = __all_sync(0xFFFFFFFFu, ok);
+        }
+        if (!ok) break;
+        if (!inside) continue;
+        const uint32_t taddr = tmem + static_cast<uint32_t>(buf * kAccCols + c * kChunk) +
+                               (static_cast<uint32_t>(quad * 32) << 16);
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          const int col = col0 + 32 * h;
+          uint32_t r[32], u[32];
+          tmem_ld_32x32b_x32(taddr + 32 * h, r);
+          if constexpr (kGated) tmem_ld_32x32b_x32(taddr + 32 * h + out_cols, u);
+          tmem_ld_wait();
+          affine32<kF8>(r, sx, a.sw, a.bias, col, a.n - col);
+          if constexpr (kGated)
+            affine32<kF8>(u, sx, a.sw + a.n, a.bias == nullptr ? nullptr : a.bias + a.n, col,
+                          a.n - col);
+          act32<kGated>(a.act, r, u);
+          // 16-byte chunk q of row l sits at l * 128 + ((q ^ (l & 7)) * 16) (128B swizzle)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint4* at = reinterpret_cast<uint4*>(stage_buf + lane * 128 +
+                                                 (((4 * h + q) ^ (lane & 7)) * 16));
+            uint32_t o[4];
+            if (a.residual) {
+              const uint4 v = *at;
+              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                o[j] = pack_bf16x2(__uint_as_float(r[8 * q + 2 * j]) + bf_lo(w[j]),
+                                   __uint_as_float(r[8 * q + 2 * j + 1]) + bf_hi(w[j]));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                o[j] = pack_bf16x2(__uint_as_float(r[8 * q + 2 * j]),
+                                   __uint_as_float(r[8 * q + 2 * j + 1]));
+            }
+            *at = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&tmap_y, stage_buf, col0, row0);
+          bulk_commit_group();
+        }
+        ++uses;
+      }
+      if (!ok) break;
+      if (!waited) {  // fewer chunks than warps: still wait for and release the accumulator
+        ok = mbar_wait_cluster_bounded(&bars->acc_full[buf], static_cast<uint32_t>(i >> 1) & 1u,
+                                       wait_limit);
+        if (!ok) flag(abort_flag, a.err_word, kErrWaitEpilogue);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(even_addr(&bars->acc_empty[buf]));
+    }
+    if (lane == 0) bulk_wait_group0();  // stores complete before the CTA exits
+  }
+
+  tc_fence_before();
+  cluster_sync();  // neither CTA leaves while the pair's MMAs or arrivals may touch it
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem, 2 * kAccCols);
+}
+
+// ---------------------------------------------------------------- few tokens
+constexpr int kSplitStagesMax = 16;
+constexpr int kSplitThreads = 320;                // producer, MMA issuer, eight epilogue warps
+constexpr int kSplitBarrierBytes = 512;
+// An MMA reads 128 W rows; a tile of fewer rows is followed by whatever comes next in shared
+// memory (it ends in accumulator rows that nobody reads), so the ring is followed by a pad.
+constexpr int kSplitPad = 128 * kKB;
+constexpr int kSplitRing = 232448 - kSplitBarrierBytes - kSplitPad - 1024;
+constexpr int kSplitRingBytes = kSplitRing / 1024 * 1024;
+constexpr int kSplitBarrierOff = kSplitRingBytes + kSplitPad;
+constexpr int kSplitSmemBytes = kSplitBarrierOff + kSplitBarrierBytes;
+static_assert(kSplitSmemBytes <= 232448, "split plan exceeds shared memory");
+
+struct SplitBars {
+  uint64_t full[kSplitStagesMax];
+  uint64_t empty[kSplitStagesMax];
+  uint64_t acc_full;
+  uint64_t teardown;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+static_assert(sizeof(SplitBars) <= kSplitBarrierBytes, "split barrier area");
+
+struct SplitPlan {
+  int wr;         // W rows per CTA: 32, 64 or 128 (gated: half of them Wg rows, half Wu rows)
+  int tn;         // tokens per CTA: a multiple of 16, at most 256
+  int split;      // CTAs per cluster sharing one tile's K
+  int group;      // K tiles per stage
+  int stages;
+};
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+__device__ __forceinline__ float activate_any(int act, float z) {
+  switch (act) {
+    case kActRelu: return activate<kActRelu>(z);
+    case kActGelu: return activate<kActGelu>(z);
+    case kActGeluTanh: return activate<kActGeluTanh>(z);
+    case kActSilu: return activate<kActSilu>(z);
+    default: return z;
+  }
+}
+
+template <bool kF8>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+    linear_split_kernel(const __grid_constant__ CUtensorMap tmap_x,
+                        const __grid_constant__ CUtensorMap tmap_w, const SplitPlan p,
+                        const int gated, const uint16_t* __restrict__ residual,
+                        uint16_t* __restrict__ y, const LinearArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0) {
+    if (threadIdx.x == 0) atomicOr(a.err_word, kErrSmemAlign);
+    return;  // every CTA of the cluster sees the same layout
+  }
+  auto* bars = reinterpret_cast<SplitBars*>(smem + kSplitBarrierOff);
+  int* abort_flag = &bars->abort_flag;
+  const int warp = warp_index_uniform();
+  const int lane = threadIdx.x & 31;
+  const int split = p.split, rank = static_cast<int>(blockIdx.x) % split;  // = cluster rank
+  const int tile = static_cast<int>(blockIdx.x) / split;
+  const int m_tiles = (a.m + p.tn - 1) / p.tn;
+  const int nb = tile / m_tiles, mb = tile % m_tiles;
+  const int out_rows = gated ? p.wr / 2 : p.wr;  // output columns of y per tile
+  const int kt0 = static_cast<int>(static_cast<int64_t>(a.k_tiles) * rank / split);
+  const int kt1 = static_cast<int>(static_cast<int64_t>(a.k_tiles) * (rank + 1) / split);
+  const int steps = (kt1 - kt0 + p.group - 1) / p.group;  // stages filled; >= 1 (split <= k_tiles)
+  const uint32_t w_bytes = static_cast<uint32_t>(p.wr) * kKB;
+  const uint32_t x_bytes = static_cast<uint32_t>(p.tn) * kKB;
+  const uint32_t stage_bytes = (w_bytes + x_bytes) * p.group;
+  const uint64_t wait_limit = a.wait_limit;
+  const uint64_t teardown_limit = wait_limit > kDefaultWaitLimit ? wait_limit : kDefaultWaitLimit;
+  uint32_t cols = 32;
+  while (static_cast<int>(cols) < p.tn) cols *= 2;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    mbar_init(&bars->acc_full, 1);
+    mbar_init(&bars->teardown, 1);
+    bars->abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+    prefetch_tmap(&tmap_x);
+    prefetch_tmap(&tmap_w);
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    const int k_step = kF8 ? kKB : kKB / 2;
+    int stage = 0;
+    uint32_t phase = 0, filled = 0;
+    for (int i = 0; i < steps; ++i) {
+      if (!warp_wait_bounded(&bars->empty[stage], phase ^ 1u, wait_limit)) {
+        warp_flag(abort_flag, a.err_word, kErrWaitProducer);
+        break;
+      }
+      const int kt = kt0 + i * p.group;
+      const int g = min(p.group, kt1 - kt);
+      uint8_t* sw = smem + stage * stage_bytes;
+      uint64_t* full = &bars->full[stage];
+      if (elect_one()) {
+        mbar_arrive_expect_tx(full, (w_bytes + x_bytes) * g);
+        for (int j = 0; j < g; ++j) {
+          uint8_t* at = sw + j * w_bytes;
+          const int k = (kt + j) * k_step;
+          if (gated) {  // boxes of wr / 2 rows: Wg, then the same columns' Wu
+            tma_load_2d(at, &tmap_w, full, k, nb * out_rows);
+            tma_load_2d(at + w_bytes / 2, &tmap_w, full, k, a.n + nb * out_rows);
+          } else {
+            tma_load_2d(at, &tmap_w, full, k, nb * out_rows);
+          }
+          tma_load_2d(sw + p.group * w_bytes + j * x_bytes, &tmap_x, full, k, mb * p.tn);
+        }
+      }
+      __syncwarp();
+      filled = i + 1;
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    // no load may be in flight when the ring is reused or the CTA exits
+    for (int s = 0; s < p.stages; ++s) {
+      const uint32_t times = filled > static_cast<uint32_t>(s) ? (filled - 1 - s) / p.stages + 1 : 0;
+      if (times > 0 && !warp_wait_bounded(&bars->full[s], (times - 1) & 1u, teardown_limit))
+        warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    const uint32_t idesc = instr_desc<kF8>(128, p.tn);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool issued_any = false;
+    for (int i = 0; i < steps; ++i) {
+      if (!warp_wait_bounded(&bars->full[stage], phase, wait_limit)) {
+        warp_flag(abort_flag, a.err_word, kErrWaitMma);
+        break;
+      }
+      tc_fence_after();
+      const int g = min(p.group, kt1 - kt0 - i * p.group);
+      const uint32_t sw = smem_u32(smem + stage * stage_bytes);
+      if (elect_one()) {
+        for (int t = 0; t < g; ++t) {
+          const uint64_t wdesc = make_smem_desc(sw + t * w_bytes, 16, 1024, 2);
+          const uint64_t xdesc = make_smem_desc(sw + p.group * w_bytes + t * x_bytes, 16, 1024, 2);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_one<kF8>(tmem, wdesc + static_cast<uint64_t>(2 * j),
+                         xdesc + static_cast<uint64_t>(2 * j), idesc,
+                         (i > 0 || t > 0 || j > 0) ? 1u : 0u);
+        }
+        tc_commit(&bars->empty[stage]);
+        if (i == steps - 1) tc_commit(&bars->acc_full);
+      }
+      __syncwarp();
+      issued_any = true;
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    if (warp_aborted(abort_flag) && issued_any) {
+      if (elect_one()) tc_commit(&bars->teardown);
+      __syncwarp();
+      if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))
+        warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
+    }
+  }
+  // ------------------------------------------------------------ partial sums to shared memory
+  // part[t * wr + row]: fp32, over the ring (every load has landed and every MMA is done)
+  float* part = reinterpret_cast<float*>(smem);
+  __syncthreads();  // warps 0 and 1 have issued everything; the producer saw every load land
+  if (!mbar_wait_bounded(&bars->acc_full, 0, wait_limit) &&
+      *reinterpret_cast<volatile int*>(abort_flag) == 0)
+    flag(abort_flag, a.err_word, kErrWaitEpilogue);
+  __syncwarp();
+  tc_fence_after();
+  if (warp >= 2) {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const int row = quad * 32 + lane;
+    if (quad * 32 < p.wr) {
+      for (int c = half * 16; c < p.tn; c += 32) {
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c + j) * p.wr + row] = __uint_as_float(r[j]);
+      }
+    }
+    tc_fence_before();
+  }
+  if (split > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+
+  // ------------------------------------------------------------ join and epilogue
+  // This CTA's share of the tile's tokens; four output columns per thread, the ranks' partial
+  // sums added in rank order.
+  const int t0 = p.tn * rank / split, t1 = p.tn * (rank + 1) / split;
+  const int quads = out_rows / 4;
+  const uint32_t part_addr = smem_u32(part);
+  const bool good = *reinterpret_cast<volatile int*>(abort_flag) == 0;
+  for (int i = threadIdx.x; good && i < (t1 - t0) * quads; i += kSplitThreads) {
+    const int t = t0 + i / quads, row = (i % quads) * 4;
+    const int token = mb * p.tn + t, col = nb * out_rows + row;
+    if (token >= a.m || col >= a.n) continue;
+    const uint32_t at = part_addr + static_cast<uint32_t>((t * p.wr + row) * 4);
+    float z[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int q = 0; q < split; ++q) {
+      const uint32_t peer = mapa_shared(at, static_cast<uint32_t>(q));
+      const float4 v = ld_cluster_f4(peer);
+      z[0] += v.x, z[1] += v.y, z[2] += v.z, z[3] += v.w;
+      if (gated) {
+        const float4 g = ld_cluster_f4(peer + static_cast<uint32_t>(out_rows * 4));
+        u[0] += g.x, u[1] += g.y, u[2] += g.z, u[3] += g.w;
+      }
+    }
+    const float sx = kF8 ? __ldg(a.sx + token) : 1.0f;
+    float o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kF8) z[j] = z[j] * sx * __ldg(a.sw + col + j);
+      if (a.bias != nullptr) z[j] += __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + col + j)) << 16);
+      o[j] = activate_any(a.act, z[j]);
+      if (gated) {
+        if constexpr (kF8) u[j] = u[j] * sx * __ldg(a.sw + a.n + col + j);
+        if (a.bias != nullptr)
+          u[j] += __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + a.n + col + j)) << 16);
+        o[j] *= u[j];
+      }
+    }
+    const int64_t dst = static_cast<int64_t>(token) * a.n + col;
+    if (residual != nullptr) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(residual + dst));
+      o[0] += bf_lo(v.x), o[1] += bf_hi(v.x), o[2] += bf_lo(v.y), o[3] += bf_hi(v.y);
+    }
+    *reinterpret_cast<uint2*>(y + dst) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+  }
+  tc_fence_before();
+  if (split > 1)
+    cluster_sync();  // no CTA leaves while a peer reads its partial sums
+  else
+    __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, cols);
+}
+
+// ---------------------------------------------------------------- host side
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// 2-D map over [rows, cols] elements of 1 or 2 bytes, rows `stride_bytes` apart; the box is
+// `box_rows` x 128 bytes, 128B swizzle.  Reads outside give zeros.
+bool make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t stride_bytes,
+              int elem, int box_rows) {
+  auto enc = reinterpret_cast<EncodeTiledFn>(tensor_map_encode_fn());
+  if (enc == nullptr) return false;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride_bytes)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(kKB / elem), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(map, elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
+             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool kF8, bool kGated>
+cudaError_t launch_pair(const LinearProblem& l, const LinearArgs& a, cudaStream_t st,
+                        const char** why) {
+  const int elem = kF8 ? 1 : 2;
+  alignas(64) CUtensorMap mx, mw, mr, my;
+  std::memset(&mr, 0, sizeof(mr));
+  if (!make_map(&mx, l.x, l.m, l.k, l.x_stride * elem, elem, 128) ||
+      !make_map(&mw, l.w, kGated ? 2 * l.n : l.n, l.k, l.k * elem, elem, a.bn / 2) ||
+      !make_map(&my, l.y, l.m, l.n, l.n * 2, 2, 32) ||
+      (l.residual != nullptr && !make_map(&mr, l.residual, l.m, l.n, l.n * 2, 2, 32))) {
+    *why = "cuTensorMapEncodeTiled failed";
+    return cudaErrorInvalidValue;
+  }
+  static ContextCache attr_done;
+  auto* kernel = linear_pair_kernel<kF8, kGated>;
+  if (cudaError_t e = ensure_max_dynamic_smem(attr_done, reinterpret_cast<const void*>(kernel),
+                                              kPairSmemBytes))
+    return e;
+  const int64_t out_cols = kGated ? a.bn / 2 : a.bn;
+  const int64_t tiles = ((l.m + kPairTokens - 1) / kPairTokens) * ((l.n + out_cols - 1) / out_cols);
+  int64_t pairs = sm_count() / 2;
+  if (pairs > tiles) pairs = tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, mx, mw, mr, my, a);
+}
+
+template <bool kF8>
+cudaError_t launch_split(const LinearProblem& l, const LinearArgs& a, const SplitPlan& p,
+                         cudaStream_t st, const char** why) {
+  const int elem = kF8 ? 1 : 2;
+  alignas(64) CUtensorMap mx, mw;
+  if (!make_map(&mx, l.x, l.m, l.k, l.x_stride * elem, elem, p.tn) ||
+      !make_map(&mw, l.w, l.gated ? 2 * l.n : l.n, l.k, l.k * elem, elem,
+                l.gated ? p.wr / 2 : p.wr)) {
+    *why = "cuTensorMapEncodeTiled failed";
+    return cudaErrorInvalidValue;
+  }
+  static ContextCache attr_done;
+  auto* kernel = linear_split_kernel<kF8>;
+  if (cudaError_t e = ensure_max_dynamic_smem(attr_done, reinterpret_cast<const void*>(kernel),
+                                              kSplitSmemBytes))
+    return e;
+  const int64_t out_rows = l.gated ? p.wr / 2 : p.wr;
+  const int64_t tiles = ((l.m + p.tn - 1) / p.tn) * ((l.n + out_rows - 1) / out_rows);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.split));
+  cfg.blockDim = dim3(kSplitThreads);
+  cfg.dynamicSmemBytes = kSplitSmemBytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(p.split);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, mx, mw, p, l.gated ? 1 : 0, l.residual, l.y, a);
+}
+
+// The split kernel's tile and split: the plan whose busiest SM moves the fewest bytes.  A CTA
+// reads (wr + tn) * 128 bytes per K tile; kJoin stands for the cluster's two barriers and the
+// exchange of partial sums.
+SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
+  constexpr double kJoin = 12e3;
+  const int sms = sm_count();
+  SplitPlan best = {};
+  *cost = 1e30;
+  const int64_t wn = l.gated ? 2 * l.n : l.n;
+  for (int wr = 32; wr <= 128; wr *= 2) {
+    const int64_t n_tiles = (wn + wr - 1) / wr;
+    for (int tn_max = 64; tn_max <= 256; tn_max *= 2) {
+      const int64_t m_tiles = (l.m + tn_max - 1) / tn_max;
+      const int tn = static_cast<int>(((l.m + m_tiles - 1) / m_tiles + 15) / 16 * 16);
+      for (int split = 1; split <= 8 && split <= k_tiles; ++split) {
+        const int64_t ctas = n_tiles * m_tiles * split;
+        const int64_t waves = (ctas + sms - 1) / sms;
+        const double c = static_cast<double>(waves) *
+                         (static_cast<double>((k_tiles + split - 1) / split) * (wr + tn) * kKB +
+                          (split > 1 ? kJoin : 0.0) + 4.0 * wr * tn / split);
+        if (c < *cost) {
+          *cost = c;
+          best.wr = wr;
+          best.tn = tn;
+          best.split = split;
+        }
+      }
+    }
+  }
+  const int tile_bytes = (best.wr + best.tn) * kKB;
+  int group = 16384 / tile_bytes;
+  group = group < 1 ? 1 : group > 4 ? 4 : group;
+  best.group = group;
+  best.stages = kSplitRingBytes / (tile_bytes * group);
+  if (best.stages > kSplitStagesMax) best.stages = kSplitStagesMax;
+  return best;
+}
+
+// Pair tiles: rounds of the persistent grid times what one tile streams per K tile.
+int plan_pair(const LinearProblem& l, int k_tiles, double* cost) {
+  const int64_t pairs = sm_count() / 2, mb = (l.m + kPairTokens - 1) / kPairTokens;
+  int best = 256;
+  *cost = 1e30;
+  for (int bn = l.gated ? 256 : 128; bn <= 256; bn += 64) {
+    const int64_t out_cols = l.gated ? bn / 2 : bn;
+    const int64_t tiles = mb * ((l.n + out_cols - 1) / out_cols);
+    const int64_t rounds = (tiles + pairs - 1) / pairs;
+    const double c = static_cast<double>(rounds) * k_tiles * (128 + bn / 2) * kKB;
+    if (c < *cost) {
+      *cost = c;
+      best = bn;
+    }
+  }
+  return best;
+}
+
+}  // namespace
+
+static std::atomic<int> g_linear_mode{0};
+void set_linear_kernel_mode(int mode) { g_linear_mode.store(mode, std::memory_order_relaxed); }
+int linear_kernel_mode() { return g_linear_mode.load(std::memory_order_relaxed); }
+
+cudaError_t launch_linear(const LinearProblem& l, uint64_t wait_limit, cudaStream_t st,
+                          const char** why) {
+  const char* unused = nullptr;
+  if (why == nullptr) why = &unused;
+  LinearArgs a = {};
+  a.sx = l.sx;
+  a.sw = l.sw;
+  a.bias = l.bias;
+  a.m = static_cast<int>(l.m);
+  a.n = static_cast<int>(l.n);
+  const int per = l.fp8 ? kKB : kKB / 2;
+  a.k_tiles = static_cast<int>((l.k + per - 1) / per);
+  a.act = l.act;
+  a.residual = l.residual != nullptr ? 1 : 0;
+  a.wait_limit = wait_limit;
+  a.err_word = error_word_ptr();
+  if (a.err_word == nullptr) return cudaErrorInvalidSymbol;
+  double split_cost, pair_cost;
+  const SplitPlan p = plan_split(l, a.k_tiles, &split_cost);
+  a.bn = plan_pair(l, a.k_tiles, &pair_cost);
+  const int mode = linear_kernel_mode();
+  if (mode == 1 || (mode == 0 && split_cost < pair_cost))
+    return l.fp8 ? launch_split<true>(l, a, p, st, why) : launch_split<false>(l, a, p, st, why);
+  if (l.fp8)
+    return l.gated ? launch_pair<true, true>(l, a, st, why) : launch_pair<true, false>(l, a, st, why);
+  return l.gated ? launch_pair<false, true>(l, a, st, why) : launch_pair<false, false>(l, a, st, why);
+}
+
+}  // namespace fvq

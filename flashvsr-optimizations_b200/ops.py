@@ -24,6 +24,8 @@ __all__ = [
     "nvfp4_linear", "nvfp4_ffn", "rcp_approx_probe", "sf_rows", "read_device_error",
     "fp8_row_quant", "fp8_quantize_activation", "fp8_scaled_mm", "fp8_linear", "fp8_ffn",
     "div_full_probe", "ln_modulate", "nvfp4_ffn_block",
+    "rms_norm", "add_rms_norm", "rms_norm_fp8", "add_rms_norm_fp8", "linear_act",
+    "fp8_scaled_mm_act", "fp8_cache_write", "fp8_cache_read", "ACTIVATIONS",
 ]
 
 
@@ -593,6 +595,366 @@ def _(x, q1, s1, b1, q2, s2, b2):
     return x.new_empty(x.shape, dtype=torch.bfloat16)
 
 
+# ---------------------------------------------------------------- the block around the linears
+# These operators are called once or more per block and token, where a decode step is bound by
+# its host side: they are defined directly on a torch.library.Library (about 5 us of dispatch a
+# call against 20 us for the decorator's wrapper) and the public functions below add what it
+# leaves out.  Inference only, like the rest: a call that would need a gradient raises when the
+# gradient is asked for.
+_BLOCK_LIB = torch.library.Library("fvq", "FRAGMENT")
+
+
+class _NoGradient(torch.autograd.Function):
+    """Runs an operator on inputs that require gradients; asking for them raises."""
+
+    @staticmethod
+    def forward(ctx, name, fn, *args):
+        ctx.name = name
+        return fn(*args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name}: no gradient formula (this library's operators are for inference)")
+
+
+def _define(schema: str, impl, fake):
+    name = schema.split("(", 1)[0]
+    _BLOCK_LIB.define(schema)
+    _BLOCK_LIB.impl(name, impl, "CompositeExplicitAutograd")
+    torch.library.register_fake(f"fvq::{name}", fake, lib=_BLOCK_LIB)
+    fn = getattr(torch.ops.fvq, name).default
+
+    def call(*args):
+        if torch.is_grad_enabled() and any(isinstance(a, torch.Tensor) and a.requires_grad for a in args):
+            return _NoGradient.apply(name, fn, *args)
+        return fn(*args)
+
+    return call
+
+
+def _launch(name: str, device: torch.device, *args) -> None:
+    """The C entry point on `device`'s current stream, with `device` current."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _same_device(name: str, x: torch.Tensor, *ts: torch.Tensor | None) -> None:
+    _check_cuda(name, x)
+    for t in ts:
+        if t is not None and t.device != x.device:
+            raise RuntimeError(f"{name}: expected every tensor on {x.device}, got {t.device}")
+
+
+def _norm_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """(x, inner, outer_stride, inner_stride): x's rows as the kernel walks them; a tensor whose
+    rows are no two-level pattern of adjacent values is copied."""
+    d = x.shape[-1]
+    if x.is_contiguous():
+        return x, 1, d, 0
+    if d == 1 or x.stride(-1) == 1:
+        if x.dim() == 2:
+            return x, 1, x.stride(0), 0
+        if x.dim() == 3:
+            return x, x.shape[1], x.stride(0), x.stride(1)
+    return x.contiguous(), 1, d, 0
+
+
+def _norm(name: str, x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None,
+          eps: float, fp8: bool):
+    _same_device(name, x, weight, residual)
+    _check_bf16(name, x)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"{name}: expected rows of at least one value, got shape {tuple(x.shape)}")
+    d = x.shape[-1]
+    rows = x.numel() // d
+    if weight is not None:
+        if weight.dtype != torch.bfloat16 or weight.numel() != d:
+            raise ValueError(f"{name}: expected a bf16 weight of {d} values")
+        weight = weight.reshape(-1).contiguous()
+    new = None
+    if residual is not None:
+        if residual.dtype not in (torch.bfloat16, torch.float32) or residual.shape != x.shape:
+            raise ValueError(f"{name}: expected a bf16 or fp32 residual of x's shape {tuple(x.shape)}")
+        residual = residual.contiguous()
+        new = torch.empty_like(residual)
+    out = torch.empty(x.shape, dtype=torch.float8_e4m3fn if fp8 else torch.bfloat16, device=x.device)
+    scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device) if fp8 else None
+    if rows:
+        x, inner, outer, step = _norm_rows(x)
+        _launch("fvq_rms_norm", x.device, x.data_ptr(), rows, inner, outer, step, d, _ptr(weight),
+                eps, _ptr(residual), 1 if new is not None and new.dtype == torch.float32 else 0,
+                _ptr(new), None if fp8 else out.data_ptr(), out.data_ptr() if fp8 else None,
+                _ptr(scale))
+    return out, scale, new
+
+
+def _fp8_like(x: torch.Tensor):
+    return (torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device),
+            x.new_empty((*x.shape[:-1], 1), dtype=torch.float32))
+
+
+_rms_norm = _define(
+    "rms_norm(Tensor x, Tensor? weight, float eps) -> Tensor",
+    lambda x, weight, eps: _norm("rms_norm", x, weight, None, eps, False)[0],
+    lambda x, weight, eps: x.new_empty(x.shape))
+_add_rms_norm = _define(
+    "add_rms_norm(Tensor x, Tensor residual, Tensor? weight, float eps) -> (Tensor, Tensor)",
+    lambda x, residual, weight, eps: _norm("add_rms_norm", x, weight, residual, eps, False)[::2],
+    lambda x, residual, weight, eps: (x.new_empty(x.shape), residual.new_empty(x.shape)))
+_rms_norm_fp8 = _define(
+    "rms_norm_fp8(Tensor x, Tensor? weight, float eps) -> (Tensor, Tensor)",
+    lambda x, weight, eps: _norm("rms_norm_fp8", x, weight, None, eps, True)[:2],
+    lambda x, weight, eps: _fp8_like(x))
+_add_rms_norm_fp8 = _define(
+    "add_rms_norm_fp8(Tensor x, Tensor residual, Tensor? weight, float eps) -> (Tensor, Tensor, Tensor)",
+    lambda x, residual, weight, eps: _norm("add_rms_norm_fp8", x, weight, residual, eps, True),
+    lambda x, residual, weight, eps: (*_fp8_like(x), residual.new_empty(x.shape)))
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
+    """bf16(x * rsqrt(mean(x^2) + eps) * weight) over the last dimension, in fp32 with one rounding.
+
+    x: bf16 [..., d], d <= 16384; views of two or three dimensions with adjacent values (heads
+    inside a fused projection's rows) are read in place.  weight: bf16 [d] or None (ones)."""
+    return _rms_norm(x, weight, eps)
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
+                 eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """(rms_norm(s), s) with s = x + residual: the branch's output joins the stream and the next
+    branch's input is normalised in one pass.  residual: bf16 or fp32, x's shape; s is returned in
+    its type, and normalised before that rounding."""
+    return _add_rms_norm(x, residual, weight, eps)
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor | None = None,
+                 eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q float8_e4m3fn like x, scale fp32 [..., 1]): rms_norm's fp32 value v quantized with one scale
+    per row, scale = max(max|v| / 448, 1e-12), q = v / scale -- the input of ``fp8_scaled_mm`` and
+    ``fp8_scaled_mm_act`` without a bf16 copy in between."""
+    return _rms_norm_fp8(x, weight, eps)
+
+
+def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
+                     eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(q, scale, s): ``rms_norm_fp8`` of s = x + residual, and s (see ``add_rms_norm``)."""
+    return _add_rms_norm_fp8(x, residual, weight, eps)
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _matrix(x: torch.Tensor, per16: int) -> tuple[torch.Tensor, int, int]:
+    """(x, rows, row stride) of x [..., k] as rows that TMA can read (16-byte aligned); copied when
+    they are not."""
+    k = x.shape[-1]
+    if x.dim() != 2:
+        x = x.reshape(-1, k)
+    m = x.shape[0]
+    stride = x.stride(0) if m > 1 else k
+    if x.stride(1) != 1 and k > 1 or stride < k or stride % per16 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        stride = k
+    return x, m, stride
+
+
+def _epilogue(name, x, weight, bias, act, gated, residual):
+    """Checks shared by the two products; (n, bias, residual, act code)."""
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"{name}: expected x [..., k] and weight [n, k], got {tuple(x.shape)} and "
+                         f"{tuple(weight.shape)}")
+    wn = weight.shape[0]
+    if gated and wn % 2:
+        raise ValueError(f"{name}: a gated weight has an even number of rows (the activated half first)")
+    n = wn // 2 if gated else wn
+    if act not in ACTIVATIONS:
+        raise ValueError(f"{name}: act must be one of {', '.join(ACTIVATIONS)}, got {act!r}")
+    if bias is not None:
+        if bias.dtype != torch.bfloat16 or bias.numel() != wn:
+            raise ValueError(f"{name}: expected a bf16 bias of {wn} values")
+        bias = _aligned16(bias)
+    if residual is not None:
+        if residual.dtype != torch.bfloat16 or residual.shape != (*x.shape[:-1], n):
+            raise ValueError(f"{name}: expected a bf16 residual of shape {(*x.shape[:-1], n)}")
+        residual = _aligned16(residual)
+    return n, bias, residual, ACTIVATIONS[act]
+
+
+def _linear_act_impl(x, weight, bias, act, gated, residual):
+    _same_device("linear_act", x, weight, bias, residual)
+    _check_bf16("linear_act", x)
+    _check_bf16("linear_act", weight)
+    n, bias, residual, code = _epilogue("linear_act", x, weight, bias, act, gated, residual)
+    y = torch.empty((*x.shape[:-1], n), dtype=torch.bfloat16, device=x.device)
+    if y.numel():
+        k = x.shape[-1]
+        x, m, stride = _matrix(x, 8)
+        weight = _aligned16(weight)
+        _launch("fvq_linear_act", y.device, x.data_ptr(), m, k, stride, weight.data_ptr(), n,
+                _ptr(bias), code, gated, _ptr(residual), y.data_ptr())
+    return y
+
+
+def _fp8_scaled_mm_act_impl(a, scale_a, w, scale_w, bias, act, gated, residual):
+    name = "fp8_scaled_mm_act"
+    _same_device(name, a, scale_a, w, scale_w, bias, residual)
+    _check_fp8(name, a, w)
+    n, bias, residual, code = _epilogue(name, a, w, bias, act, gated, residual)
+    k = a.shape[-1]
+    if scale_a.dtype != torch.float32 or scale_w.dtype != torch.float32 or \
+            scale_a.numel() * k != a.numel() or scale_w.numel() != w.shape[0]:
+        raise ValueError(f"{name}: expected fp32 scales, one per row of a and one per row of w")
+    y = torch.empty((*a.shape[:-1], n), dtype=torch.bfloat16, device=a.device)
+    if y.numel():
+        a, m, stride = _matrix(a, 16)
+        scale_a, scale_w, w = scale_a.contiguous(), _aligned16(scale_w), _aligned16(w)
+        _launch("fvq_fp8_scaled_mm_act", y.device, a.data_ptr(), scale_a.data_ptr(), m, k, stride,
+                w.data_ptr(), scale_w.data_ptr(), n, _ptr(bias), code, gated, _ptr(residual),
+                y.data_ptr())
+    return y
+
+
+def _product_fake(x, weight, gated):
+    n = weight.shape[0] // 2 if gated else weight.shape[0]
+    return x.new_empty((*x.shape[:-1], n), dtype=torch.bfloat16)
+
+
+_linear_act = _define(
+    "linear_act(Tensor x, Tensor weight, Tensor? bias, str act, bool gated, Tensor? residual) -> Tensor",
+    _linear_act_impl,
+    lambda x, weight, bias, act, gated, residual: _product_fake(x, weight, gated))
+_fp8_scaled_mm_act = _define(
+    "fp8_scaled_mm_act(Tensor a, Tensor scale_a, Tensor w, Tensor scale_w, Tensor? bias, str act, "
+    "bool gated, Tensor? residual) -> Tensor",
+    _fp8_scaled_mm_act_impl,
+    lambda a, scale_a, w, scale_w, bias, act, gated, residual: _product_fake(a, w, gated))
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+               act: str = "none", gated: bool = False,
+               residual: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16(h + residual) with z = x @ weight^T + bias and h = act(z), or with gated=True
+    h = act(z[..., :n]) * z[..., n:] (weight [2n, k], the activated half first).
+
+    fp32 accumulation and epilogue, one rounding.  x: bf16 [..., k] (rows may be strided), weight
+    in nn.Linear's layout, k and n multiples of 8; act: one of ``ACTIVATIONS`` ("gelu" is the erf
+    form).  From one row to many: few rows run on a kernel bound by reading the weight once."""
+    return _linear_act(x, weight, bias, act, gated, residual)
+
+
+def fp8_scaled_mm_act(a: torch.Tensor, scale_a: torch.Tensor, w: torch.Tensor, scale_w: torch.Tensor,
+                      bias: torch.Tensor | None = None, act: str = "none", gated: bool = False,
+                      residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``linear_act`` with E4M3 operands and one fp32 scale per row of each (those of
+    ``fp8_row_quant``, ``rms_norm_fp8`` and ``QuantLinear(mode='fp8')``):
+    z = (a @ w^T) * scale_a * scale_w + bias.  k a multiple of 16, n of 8."""
+    return _fp8_scaled_mm_act(a, scale_a, w, scale_w, bias, act, gated, residual)
+
+
+# ---------------------------------------------------------------- paged FP8 keys and values
+def _check_cache(name, k_codes, k_scale, v_codes, v_scale):
+    _check_fp8(name, k_codes, v_codes)
+    if k_codes.dim() != 4 or v_codes.shape != k_codes.shape or \
+            k_scale.shape != k_codes.shape[:3] or v_scale.shape != k_codes.shape[:3] or \
+            k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise ValueError(f"{name}: expected codes [pages, page, heads, d] and fp32 scales "
+                         "[pages, page, heads], the same for keys and values")
+    if not (k_codes.is_contiguous() and v_codes.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous()):
+        raise ValueError(f"{name}: the store's tensors must be contiguous")
+
+
+def _cache_rows(x: torch.Tensor) -> torch.Tensor:
+    if x.stride(-1) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _fp8_cache_write_impl(k, v, slots, k_codes, k_scale, v_codes, v_scale):
+    name = "fp8_cache_write"
+    _same_device(name, k, v, slots, k_codes, k_scale, v_codes, v_scale)
+    _check_bf16(name, k)
+    _check_bf16(name, v)
+    _check_cache(name, k_codes, k_scale, v_codes, v_scale)
+    pages, page, heads, d = k_codes.shape
+    if k.dim() != 3 or k.shape[1:] != (heads, d) or v.shape != k.shape:
+        raise ValueError(f"{name}: expected k and v [tokens, {heads}, {d}], got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    if slots.dtype != torch.int64 or slots.shape != (k.shape[0],):
+        raise ValueError(f"{name}: expected int64 slots, one per token")
+    if k.numel():
+        k, v, slots = _cache_rows(k), _cache_rows(v), slots.contiguous()
+        _launch("fvq_fp8_cache_write", k.device, k.data_ptr(), v.data_ptr(), k.shape[0], heads, d,
+                k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(),
+                k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(),
+                pages * page)
+
+
+def _fp8_cache_read_impl(k_codes, k_scale, v_codes, v_scale, page_table, lengths, max_len):
+    name = "fp8_cache_read"
+    _same_device(name, k_codes, k_scale, v_codes, v_scale, page_table, lengths)
+    _check_cache(name, k_codes, k_scale, v_codes, v_scale)
+    pages, page, heads, d = k_codes.shape
+    if page_table.dtype != torch.int32 or lengths.dtype != torch.int32 or page_table.dim() != 2 or \
+            lengths.shape != page_table.shape[:1]:
+        raise ValueError(f"{name}: expected an int32 page table [batch, pages] and int32 lengths [batch]")
+    if max_len < 0:
+        raise ValueError(f"{name}: max_len must not be negative")
+    batch, per = page_table.shape
+    shape = (batch, max_len, heads, d)
+    k = torch.empty(shape, dtype=torch.bfloat16, device=k_codes.device)
+    v = torch.empty(shape, dtype=torch.bfloat16, device=k_codes.device)
+    if k.numel():
+        if per == 0:
+            raise ValueError(f"{name}: the page table has no pages")
+        page_table, lengths = page_table.contiguous(), lengths.contiguous()
+        _launch("fvq_fp8_cache_read", k.device, k_codes.data_ptr(), k_scale.data_ptr(),
+                v_codes.data_ptr(), v_scale.data_ptr(), pages, page, heads, d, page_table.data_ptr(),
+                batch, per, lengths.data_ptr(), max_len, k.data_ptr(), v.data_ptr())
+    return k, v
+
+
+def _cache_read_fake(k_codes, k_scale, v_codes, v_scale, page_table, lengths, max_len):
+    shape = (page_table.shape[0], max_len, *k_codes.shape[2:])
+    return (k_codes.new_empty(shape, dtype=torch.bfloat16), k_codes.new_empty(shape, dtype=torch.bfloat16))
+
+
+_fp8_cache_write = _define(
+    "fp8_cache_write(Tensor k, Tensor v, Tensor slots, Tensor(a!) k_codes, Tensor(b!) k_scale, "
+    "Tensor(c!) v_codes, Tensor(d!) v_scale) -> ()",
+    _fp8_cache_write_impl, lambda *args: None)
+_fp8_cache_read = _define(
+    "fp8_cache_read(Tensor k_codes, Tensor k_scale, Tensor v_codes, Tensor v_scale, Tensor page_table, "
+    "Tensor lengths, SymInt max_len) -> (Tensor, Tensor)",
+    _fp8_cache_read_impl, _cache_read_fake)
+
+
+def fp8_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_codes: torch.Tensor,
+                    k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor) -> None:
+    """Quantize the keys and values of new tokens into a paged store, one launch for both.
+
+    k, v: bf16 [tokens, heads, d] (strided views of a fused projection are read in place); codes
+    float8_e4m3fn [pages, page, heads, d] and scales fp32 [pages, page, heads], written in place.
+    Token t goes to slot slots[t] = page index * page + offset (int64): one scale per token and
+    head, scale = max(max|x| / 448, 1e-12), q = x / scale.  A negative slot is padding (nothing is
+    stored); one past the store is skipped and sets bit 6 of ``read_device_error()``.  The slots
+    of one call must differ: what a repeated slot then holds is undefined."""
+    _fp8_cache_write(k, v, slots, k_codes, k_scale, v_codes, v_scale)
+
+
+def fp8_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor,
+                   v_scale: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                   max_len: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) bf16 [batch, max_len, heads, d] of the sequences whose pages page_table (int32
+    [batch, pages]) lists in order: bf16(q * scale) below lengths[b] (int32), zero from there on.
+    A page outside the store, or a length past max_len or past the table, reads as zeros and sets
+    bit 7 of ``read_device_error()``."""
+    return _fp8_cache_read(k_codes, k_scale, v_codes, v_scale, page_table, lengths, max_len)
+
+
 def div_full_probe(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     """div.full.f32(a, b) elementwise on the GPU, the FP8 quantizers' division (test support)."""
     _check_cuda("div_full_probe", a, b)
@@ -620,6 +982,12 @@ def read_device_error(device: torch.device | None = None) -> int:
     _lib.call("fvq_read_device_error", torch.cuda.current_stream(dev).cuda_stream,
               ctypes.byref(flags))
     return int(flags.value)
+
+
+def set_linear_kernel(mode: int) -> None:
+    """Which kernel ``linear_act`` and ``fp8_scaled_mm_act`` run: 0 by size (default), 1 the split
+    kernel (few rows), 2 the SM-pair kernel."""
+    _lib.call("fvq_set_linear_kernel", mode)
 
 
 def set_wait_limit(nanoseconds: int) -> None:

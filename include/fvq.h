@@ -368,6 +368,104 @@ int fvq_fp8_ffn_profile(const uint16_t* x, int64_t rows, const fvq_linear_fp8* l
 
 /*
  * ---------------------------------------------------------------------------
+ * The block around the bf16 and FP8 linears: no counterpart in the reference
+ * (whose DiT blocks are upstream code).  Outputs must not overlap inputs.
+ * ---------------------------------------------------------------------------
+ */
+
+/*
+ * RMS norm with the residual's addition, in bf16, in E4M3 with one scale per row, or both:
+ *   s = x + residual;  v = s * rsqrt(mean(s^2) + eps) * weight          (fp32)
+ *   residual_out = s (residual's type),  y = bf16(v)
+ *   scale[r] = max(max|v| / 448, 1e-12),  q = e4m3_rn(v * (1 / scale[r]))
+ * Row r of x starts at element (r / inner) * outer_stride + (r % inner) * inner_stride (a
+ * plain [rows, d] matrix: inner 1, outer_stride its row stride); weight is bf16 [d] or NULL
+ * (ones); residual NULL, or contiguous [rows, d] in bf16 (residual_fp32 0) or fp32 (1), then
+ * residual_out is required.  At least one of y (bf16 [rows, d]) and q (E4M3 [rows, d], with
+ * scale fp32 [rows]).  rows a multiple of inner, d in [1, 16384]; 2-byte aligned bf16,
+ * 4-byte aligned fp32 pointers (16-byte aligned pointers, d and strides that are multiples
+ * of 8 run on 16-byte accesses).  A NaN makes its row NaN.
+ */
+int fvq_rms_norm(const uint16_t* x, int64_t rows, int64_t inner, int64_t outer_stride,
+                 int64_t inner_stride, int64_t d, const uint16_t* weight, float eps,
+                 const void* residual, int residual_fp32, void* residual_out, uint16_t* y,
+                 uint8_t* q, float* scale, void* stream);
+
+/* Activations of the product's epilogue. */
+#define FVQ_ACT_NONE 0
+#define FVQ_ACT_RELU 1
+#define FVQ_ACT_GELU 2      /* 0.5 z erfc(-z / sqrt(2)) */
+#define FVQ_ACT_GELU_TANH 3
+#define FVQ_ACT_SILU 4
+
+/*
+ * Matrix product with bias, activation, gate and residual in its epilogue:
+ *   z = x W^T + bias;  h = act(z), or gated  act(z[:, :n]) * z[:, n:];  y = bf16(h + residual)
+ * fp32 accumulation and epilogue, one rounding.  x: bf16, m rows of k elements, x_stride
+ * elements apart (a multiple of 8, at least k); w: bf16 [n, k], gated [2n, k]; bias: bf16 of
+ * as many values as w has rows, or NULL; residual: bf16 [m, n] or NULL; y: bf16 [m, n].
+ * n % 8 == 0, k % 8 == 0; every pointer 16-byte aligned.  From one row up; no workspace.
+ * Few rows run on a kernel that splits k over clusters (fvq_set_linear_kernel); either
+ * kernel gives the same bits on every run, the two differ in the order of the sum over k.
+ */
+int fvq_linear_act(const uint16_t* x, int64_t m, int64_t k, int64_t x_stride, const uint16_t* w,
+                   int64_t n, const uint16_t* bias, int act, int gated, const uint16_t* residual,
+                   uint16_t* y, void* stream);
+
+/*
+ * The same with E4M3 operands and one fp32 scale per row of each (fvq_fp8_scaled_mm's):
+ *   z = (sum_k a w) * scale_a[m] * scale_w[n] + bias
+ * a: m rows of k codes, a_stride bytes apart (a multiple of 16); k % 16 == 0; scale_a 4-byte,
+ * every other pointer 16-byte aligned.
+ */
+int fvq_fp8_scaled_mm_act(const uint8_t* a, const float* scale_a, int64_t m, int64_t k,
+                          int64_t a_stride, const uint8_t* w, const float* scale_w, int64_t n,
+                          const uint16_t* bias, int act, int gated, const uint16_t* residual,
+                          uint16_t* y, void* stream);
+
+/*
+ * Library setting: which kernel fvq_linear_act and fvq_fp8_scaled_mm_act run: 0 (the default)
+ * by size, 1 the split kernel (few rows), 2 the SM-pair kernel.  Applies to later launches
+ * from any thread.
+ */
+int fvq_set_linear_kernel(int mode);
+
+/*
+ * Paged FP8 store of attention keys and values: codes E4M3 [num_slots, heads, d], scales fp32
+ * [num_slots, heads], `page` consecutive slots being one page.  A row of k and v (one token,
+ * one head) is stored as fvq_fp8_row_quantize's formula has it,
+ *   scale = max(max|x| / 448, 1e-12),  q = e4m3_rn(x * (1 / scale)),
+ * and read back as bf16(q * scale).
+ *
+ * write: token t goes to slot slots[t] (device int64); a negative slot is padding and stores
+ * nothing; a slot >= num_slots stores nothing and sets bit 6 of the device error word
+ * (fvq_read_device_error).  The non-negative slots of one call are distinct: of two tokens
+ * with the same slot, that slot's rows hold an undefined mixture.  k and v: bf16, element
+ * strides between tokens and between heads (multiples of 8), 16-byte aligned, the d values
+ * adjacent.  codes 8-byte, scales 4-byte aligned.  d % 8 == 0, d <= 512.
+ */
+int fvq_fp8_cache_write(const uint16_t* k, const uint16_t* v, int64_t tokens, int64_t heads,
+                        int64_t d, int64_t k_token_stride, int64_t k_head_stride,
+                        int64_t v_token_stride, int64_t v_head_stride, const int64_t* slots,
+                        uint8_t* k_codes, float* k_scale, uint8_t* v_codes, float* v_scale,
+                        int64_t num_slots, void* stream);
+
+/*
+ * read: position p of sequence b comes from slot page_table[b, p / page] * page + p % page
+ * (device int32 [batch, pages_per_seq]) for p < lengths[b] (device int32), and is zero from
+ * there up to max_len.  k_out, v_out: bf16 [batch, max_len, heads, d], 16-byte aligned.  A
+ * page outside [0, num_pages), or a length past max_len or past pages_per_seq * page, reads
+ * as zeros and sets bit 7 of the device error word; table entries past a sequence's length
+ * are not read.  batch <= 65535.
+ */
+int fvq_fp8_cache_read(const uint8_t* k_codes, const float* k_scale, const uint8_t* v_codes,
+                       const float* v_scale, int64_t num_pages, int64_t page, int64_t heads,
+                       int64_t d, const int32_t* page_table, int64_t batch, int64_t pages_per_seq,
+                       const int32_t* lengths, int64_t max_len, uint16_t* k_out, uint16_t* v_out,
+                       void* stream);
+
+/*
+ * ---------------------------------------------------------------------------
  * Pillow-exact bicubic resize of the input pipeline (reference pil_exact_gpu.py:
  * 30-150, used by chunked_input.py:111-113).
  * ---------------------------------------------------------------------------

@@ -1,0 +1,613 @@
+"""The operators around the bf16 / FP8 linears on the GPU against plain 64-bit implementations.
+
+Tolerances (bf16 rounds by at most 2^-8 of the value, E4M3 by 2^-4, or half its subnormal step 2^-9):
+
+* norm: a row of d values sums its squares in fp32 with at most 64 + 13 additions in a chain
+  (each 2^-24, halved by the square root), and makes six more roundings: under 2^-17 of the value;
+* product: the accumulator adds one partial sum per 16 values of K; every addition, in the tensor
+  core or after it, is taken as a full fp32 ulp (2^-23) of the largest partial sum, for which
+  sum |x w| stands: (k / 16 + 64) 2^-23 sum |x w|.  The activations change a value by at most 1.13
+  times its argument's change, and evaluate to 2^-17 of |z|.
+"""
+import math
+
+import pytest
+import torch
+
+import flashvsr_optimizations_b200 as fvq
+from flashvsr_optimizations_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, F8, F64 = torch.bfloat16, torch.float32, torch.float8_e4m3fn, torch.float64
+HALF_BF16, HALF_E4M3 = 2.0 ** -8, 2.0 ** -4
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(*shape, seed=0, std=1.0, dtype=BF16):
+    return (torch.randn(*shape, generator=gen(seed), device="cuda") * std).to(dtype)
+
+
+@pytest.fixture(autouse=True)
+def no_device_error():
+    yield
+    assert ops.read_device_error() == 0
+
+
+def inside(got, want, bound):
+    """|got - want| <= bound everywhere, with the same NaN and infinities."""
+    got, want = got.double(), want.double()
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got[~fine & ~torch.isnan(want)], want[~fine & ~torch.isnan(want)])
+    over = ((got - want).abs() - bound)[fine]
+    assert over.numel() == 0 or over.max().item() <= 0, f"exceeds the bound by {over.max().item():.3e}"
+
+
+def codes_inside(q, scale, v, extra):
+    """q are E4M3 codes of v / scale up to `extra` (relative) and half a step."""
+    t = v / scale.double()
+    inside(q.float(), t, torch.maximum(t.abs() * HALF_E4M3, torch.full_like(t, 2.0 ** -10)) + t.abs() * extra)
+
+
+# ---------------------------------------------------------------- norm
+def norm64(x, r, w, eps):
+    s = x.double() if r is None else x.double() + r.double()
+    v = s / torch.sqrt((s * s).mean(-1, keepdim=True) + eps)
+    return s, v if w is None else v * w.double()
+
+
+def check_norm(x, r, w, eps=1e-6):
+    s, v = norm64(x, r, w, eps)
+    tol = 2.0 ** -17
+    if r is None:
+        y = ops.rms_norm(x, w, eps)
+        q, scale = ops.rms_norm_fp8(x, w, eps)
+    else:
+        y, new = ops.add_rms_norm(x, r, w, eps)
+        q, scale, new2 = ops.add_rms_norm_fp8(x, r, w, eps)
+        assert new.dtype == r.dtype and torch.equal(new, new2)
+        want = (x.float() + r.float()).to(r.dtype)     # one fp32 addition, one rounding
+        assert torch.equal(new, want)
+    assert y.dtype == BF16 and y.shape == x.shape and q.dtype == F8 and scale.shape == (*x.shape[:-1], 1)
+    inside(y, v, v.abs() * (HALF_BF16 + tol))
+    want = (v.abs().amax(-1, keepdim=True) / 448).clamp_min(1e-12)
+    inside(scale, want, want * tol)
+    codes_inside(q, scale, v, tol)
+
+
+@pytest.mark.parametrize("d", [1, 2, 7, 8, 24, 64, 72, 127, 128, 129, 256, 264, 500, 512, 1000, 1024, 1536, 1544,
+                               2040, 2047, 2048, 2049, 4096, 4104, 6000, 8192, 8960, 10240, 12288, 12296, 16384])
+@pytest.mark.parametrize("residual", [None, BF16, F32])
+def test_norm_row_lengths(d, residual):
+    rows = 37 if d < 2048 else 5
+    x, w = randn(rows, d, seed=d), randn(d, seed=d + 1)
+    r = None if residual is None else randn(rows, d, seed=d + 2, std=2.0, dtype=residual)
+    check_norm(x, r, w)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 7, 8, 9, 16, 33, 1000])
+@pytest.mark.parametrize("d", [64, 128, 1536, 4096])
+def test_norm_row_counts_and_no_weight(rows, d):
+    check_norm(randn(rows, d, seed=rows), randn(rows, d, seed=rows + 1), None)
+    check_norm(randn(rows, d, seed=rows), None, randn(d, seed=3), eps=0.0)
+
+
+@pytest.mark.parametrize("d", [128, 80, 33])
+def test_norm_strided_views(d):
+    qkv = randn(50, 3 * 6 * d + 8, seed=d)
+    heads = qkv[:, 6 * d:12 * d].unflatten(1, (6, d))           # [tokens, heads, d] inside wider rows
+    w = randn(d, seed=1)
+    check_norm(heads, None, w)
+    check_norm(heads, randn(50, 6, d, seed=2), w)
+    check_norm(qkv[:, 5:5 + d], None, w)                          # two-dimensional, odd offset
+    check_norm(qkv[::2, :d], None, w)
+    check_norm(heads.transpose(0, 1), None, w)
+    check_norm(qkv[:12, :d].view(2, 2, 3, d).transpose(0, 2), None, w)   # four dimensions: copied
+    check_norm(qkv[:1, :d].expand(9, d), None, w)                 # broadcast rows
+    check_norm(qkv[0, :d], None, w)                               # a single vector
+    check_norm(qkv[:4, :d].t(), None, None)                       # no adjacent values: copied
+
+
+def test_norm_special_rows():
+    d = 1536
+    x = randn(8, d, seed=4)
+    x[0] = 0.0
+    x[1, 5] = float("inf")
+    x[2, 7] = float("nan")
+    x[3] = 1e-30
+    x[4, 9] = float("-inf")
+    x[5] = 1e15
+    x[6, ::2] = -0.0
+    w = randn(d, seed=5)
+    s, v = norm64(x, None, w, 1e-6)
+    y = ops.rms_norm(x, w)
+    inside(y, v, v.abs() * (HALF_BF16 + 2.0 ** -17))
+    q, scale = ops.rms_norm_fp8(x, w)
+    assert (q[0].float() == 0).all() and scale[0].item() == pytest.approx(1e-12, rel=1e-6)
+    # an infinity makes one NaN, a NaN all: the maximum is NaN then, and with it every code
+    assert torch.isnan(scale[[1, 2, 4]]).all() and torch.isnan(q[[1, 2, 4]].float()).all()
+    ok = [3, 5, 6, 7]
+    codes_inside(q[ok], scale[ok], v[ok], 2.0 ** -17)
+    assert torch.isfinite(ops.rms_norm(x[:1], w, 1e-6)).all()
+
+
+def test_norm_empty_and_refusals():
+    w = randn(64, seed=1)
+    assert ops.rms_norm(randn(0, 64), w).shape == (0, 64)
+    q, s, new = ops.add_rms_norm_fp8(randn(0, 3, 64), randn(0, 3, 64), w)
+    assert q.shape == (0, 3, 64) and s.shape == (0, 3, 1) and new.shape == (0, 3, 64)
+    x = randn(4, 64)
+    with pytest.raises(TypeError):
+        ops.rms_norm(x.float(), w)
+    with pytest.raises(ValueError):
+        ops.rms_norm(x, w[:32])
+    with pytest.raises(ValueError):
+        ops.rms_norm(x, w.float())
+    with pytest.raises(ValueError):
+        ops.add_rms_norm(x, x[:2], w)
+    with pytest.raises(ValueError):
+        ops.add_rms_norm(x, x.half(), w)
+    with pytest.raises(ValueError):
+        ops.rms_norm(randn(4, 0), None)
+    with pytest.raises(RuntimeError):
+        ops.rms_norm(x, w.cpu())
+    with pytest.raises(fvq.FvqError):
+        ops.rms_norm(randn(2, 16385))
+    with pytest.raises(fvq.FvqError):
+        ops.rms_norm(x, w, -1.0)
+
+
+# ---------------------------------------------------------------- product
+ACT64 = {
+    "none": lambda z: z,
+    "relu": lambda z: torch.where(z < 0, torch.zeros_like(z), z),
+    "gelu": lambda z: 0.5 * z * torch.special.erfc(-z / math.sqrt(2)),
+    "gelu_tanh": lambda z: 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))),
+    "silu": lambda z: z * torch.sigmoid(z),
+}
+
+
+def product64(x, w, sx, sw, bias, act, gated, residual):
+    """(y, bound) of the formulas in 64 bits."""
+    x2 = x.double().reshape(-1, x.shape[-1])
+    w = w.double()
+    z, mag = x2 @ w.t(), x2.abs() @ w.abs().t()
+    if sx is not None:
+        f = sx.double().reshape(-1, 1) * sw.double().reshape(1, -1)
+        z, mag = z * f, mag * f
+    if bias is not None:
+        z, mag = z + bias.double(), mag + bias.double().abs()
+    dz = (x.shape[-1] / 16 + 64) * 2.0 ** -23 * mag
+    f = ACT64[act]
+    if gated:
+        n = w.shape[0] // 2
+        h = f(z[:, :n]) * z[:, n:]
+        dh = (1.13 * dz[:, :n] + 2.0 ** -17 * z[:, :n].abs()) * (z[:, n:].abs() + dz[:, n:]) \
+            + f(z[:, :n]).abs() * dz[:, n:]
+    else:
+        h, dh = f(z), 1.13 * dz + 2.0 ** -17 * z.abs()
+    if residual is not None:
+        h = h + residual.double().reshape(h.shape)
+    shape = (*x.shape[:-1], h.shape[1])
+    return h.reshape(shape), (HALF_BF16 * h.abs() + (1 + HALF_BF16) * dh).reshape(shape)
+
+
+def fp8_rows(rows, k, seed, std=1.0):
+    return ops.fp8_row_quant(randn(rows, k, seed=seed, std=std)) if k % 8 == 0 else None
+
+
+def check_product(m, n, k, fp8=False, bias=True, act="none", gated=False, residual=True, seed=0):
+    wn = 2 * n if gated else n
+    b = randn(wn, seed=seed + 2) if bias else None
+    r = randn(m, n, seed=seed + 3) if residual else None
+    std = 1 / math.sqrt(k)
+    if fp8:
+        x, sx = fp8_rows(m, k, seed)
+        w, sw = fp8_rows(wn, k, seed + 1, std)
+        y = ops.fp8_scaled_mm_act(x, sx, w, sw, b, act, gated, r)
+        again = ops.fp8_scaled_mm_act(x, sx, w, sw, b, act, gated, r)
+    else:
+        x, w, sx, sw = randn(m, k, seed=seed), randn(wn, k, seed=seed + 1, std=std), None, None
+        y = ops.linear_act(x, w, b, act, gated, r)
+        again = ops.linear_act(x, w, b, act, gated, r)
+    assert y.dtype == BF16 and y.shape == (m, n)
+    assert torch.equal(y, again)
+    want, bound = product64(x.float() if fp8 else x, w.float() if fp8 else w, sx, sw, b, act, gated, r)
+    inside(y, want, bound)
+
+
+@pytest.fixture(params=[1, 2], ids=["split", "pair"])
+def kernel(request):
+    ops.set_linear_kernel(request.param)
+    yield request.param
+    ops.set_linear_kernel(0)
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("m", [1, 2, 15, 16, 17, 100, 128, 129, 256, 257, 300, 515])
+def test_product_row_counts(kernel, fp8, m):
+    check_product(m, 264, 192, fp8)
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("n", [8, 16, 56, 64, 72, 128, 136, 192, 200, 256, 264, 520])
+def test_product_column_counts(kernel, fp8, n):
+    check_product(70, n, 128, fp8)
+    check_product(70, n, 128, fp8, act="silu", gated=True, residual=False)
+
+
+@pytest.mark.parametrize("k", [8, 16, 24, 56, 64, 72, 136, 320, 1536, 1544, 8960])
+def test_product_depths_bf16(kernel, k):
+    check_product(33, 72, k)
+
+
+@pytest.mark.parametrize("k", [16, 48, 128, 144, 400, 1536, 1552, 8960])
+def test_product_depths_fp8(kernel, k):
+    check_product(33, 72, k, True)
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
+def test_product_epilogues(kernel, fp8, gated, act):
+    for bias in (False, True):
+        for residual in (False, True):
+            check_product(150, 168, 96, fp8, bias, act, gated, residual, seed=11)
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("m,n,k,gated", [(1, 8960, 1536, False), (24, 1536, 8960, False), (129, 4104, 512, True),
+                                         (777, 1536, 1536, True), (2500, 1536, 1024, False),
+                                         (4096, 2304, 128, False), (1, 8, 16, False), (20000, 8, 64, False),
+                                         (3, 20000, 64, True)])
+def test_product_by_size(fp8, m, n, k, gated):
+    check_product(m, n, k, fp8, act="gelu_tanh" if gated else "none", gated=gated)
+
+
+def test_product_extreme_values(kernel):
+    """Activations far out on both sides, infinities and NaN go where the formulas put them."""
+    k, n, m = 64, 64, 40
+    x = torch.zeros(m, k, dtype=BF16, device="cuda")
+    z = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 3.0, -3.0, 20.0, -20.0, 88.0, -88.0, 100.0, -100.0, 1e4, -1e4,
+                      1e13, -1e13, 1e30, -1e30, float("inf"), float("nan")], dtype=BF16, device="cuda")
+    x[:20, 0] = z
+    x[20:, 0] = z
+    w = torch.zeros(n, k, dtype=BF16, device="cuda")
+    w[:, 0] = 1.0
+    # the other products of a row are 0 * 0, an infinity meets only its own 1
+    for act in ops.ACTIVATIONS:
+        y = ops.linear_act(x, w, act=act).double()
+        zz = x[:, :1].double().expand(m, n)
+        want = ACT64[act](zz)
+        if act in ("gelu_tanh", "gelu", "silu"):
+            want = torch.where(zz == float("inf"), zz, want)
+        assert torch.equal(torch.isnan(y), torch.isnan(want)), act
+        fine = torch.isfinite(want)
+        assert torch.equal(y[~fine & ~torch.isnan(want)], want[~fine & ~torch.isnan(want)])
+        # 88 * 2^-23 from the exponent's argument; tails under the smallest normal may be flushed
+        tol = want.abs() * (HALF_BF16 + 2.0 ** -15) + 2.0 ** -125
+        assert ((y - want).abs() <= tol)[fine].all(), act
+
+
+def test_product_views_and_leading_dimensions(kernel):
+    wide = randn(2, 40, 400, seed=1)
+    w = randn(72, 128, seed=2)
+    cases = [wide[0, :, 8:136], wide[0, :, 4:132], wide[0, ::2, 16:144], wide[:, :, :128],
+             wide[:, :, 200:328].transpose(0, 1), wide[0, 0, :128], wide[0, :1, :128].expand(9, 128),
+             wide[0, :1, 8:136]]
+    for x in cases:
+        r = randn(*x.shape[:-1], 72, seed=3)
+        y = ops.linear_act(x, w, act="silu", residual=r)
+        want, bound = product64(x, w, None, None, None, "silu", False, r)
+        inside(y, want, bound)
+    q, s = ops.fp8_row_quant(randn(40, 400, seed=4))
+    wq, ws = ops.fp8_row_quant(w)
+    for x in (q[:, 16:144], q[:, 8:136], q[::3, :128]):
+        sx = s[::3] if x.shape[0] != 40 else s
+        y = ops.fp8_scaled_mm_act(x, sx, wq, ws.flatten())
+        want, bound = product64(x.float(), wq.float(), sx, ws, None, "none", False, None)
+        inside(y, want, bound)
+    off = randn(73 * 128 + 4, seed=5)[4:4 + 72 * 128].view(72, 128)     # weight at 8 bytes past alignment
+    y = ops.linear_act(wide[0, :, :128], off, bias=randn(73, seed=6)[1:])
+    want, bound = product64(wide[0, :, :128], off, None, None, randn(73, seed=6)[1:], "none", False, None)
+    inside(y, want, bound)
+
+
+def test_product_rows_do_not_see_one_another(kernel):
+    """A NaN row of x, a NaN row of W and a NaN residual stay where they are."""
+    m, n, k = 140, 136, 256
+    x, w, r = randn(m, k, seed=1), randn(n, k, seed=2), randn(m, n, seed=3)
+    clean = ops.linear_act(x, w, residual=r)
+    x[17], w[33], r[50, 60] = float("nan"), float("nan"), float("nan")
+    y = ops.linear_act(x, w, residual=r)
+    hit = torch.zeros(m, n, dtype=torch.bool, device="cuda")
+    hit[17], hit[:, 33], hit[50, 60] = True, True, True
+    assert torch.equal(torch.isnan(y), hit) and torch.equal(y[~hit], clean[~hit])
+
+
+def test_product_empty_and_refusals():
+    x, w = randn(4, 64), randn(72, 64)
+    assert ops.linear_act(x[:0], w).shape == (0, 72)
+    assert ops.linear_act(randn(2, 0, 64), w, act="silu", gated=True).shape == (2, 0, 36)
+    assert ops.linear_act(x, w[:0]).shape == (4, 0)
+    q, s = ops.fp8_row_quant(x)
+    wq, ws = ops.fp8_row_quant(w)
+    for bad, kind in ((lambda: ops.linear_act(x.float(), w), TypeError),
+                      (lambda: ops.linear_act(x, w.float()), TypeError),
+                      (lambda: ops.linear_act(x, w[:, :56]), ValueError),
+                      (lambda: ops.linear_act(x, w[:71], gated=True), ValueError),
+                      (lambda: ops.linear_act(x, w, act="tanh"), ValueError),
+                      (lambda: ops.linear_act(x, w, bias=x[0]), ValueError),
+                      (lambda: ops.linear_act(x, w, residual=x), ValueError),
+                      (lambda: ops.linear_act(x, w, residual=randn(4, 72).float()), ValueError),
+                      (lambda: ops.linear_act(x, w.cpu()), RuntimeError),
+                      (lambda: ops.linear_act(x, w[:71]), fvq.FvqError),            # n % 8
+                      (lambda: ops.linear_act(x[:, :60], w[:, :60]), fvq.FvqError),  # k % 8
+                      (lambda: ops.fp8_scaled_mm_act(x, s, wq, ws), TypeError),
+                      (lambda: ops.fp8_scaled_mm_act(q, s[:3], wq, ws), ValueError),
+                      (lambda: ops.fp8_scaled_mm_act(q, s.double(), wq, ws), ValueError),
+                      (lambda: ops.fp8_scaled_mm_act(q[:, :56], s, wq[:, :56], ws), fvq.FvqError)):
+        with pytest.raises(kind):
+            bad()
+
+
+def test_no_gradient():
+    x, w = randn(4, 64), randn(72, 64).requires_grad_()
+    y = ops.linear_act(x, w)
+    with pytest.raises(RuntimeError, match="no gradient formula"):
+        y.float().sum().backward()
+    with torch.no_grad():
+        assert not ops.linear_act(x, w).requires_grad
+    y, s = ops.add_rms_norm(x.requires_grad_(), x.detach())
+    with pytest.raises(RuntimeError, match="no gradient formula"):
+        s.float().sum().backward()
+
+
+# ---------------------------------------------------------------- paged FP8 keys and values
+def store(pages, page, heads, d, seed=0):
+    codes = [randn(pages, page, heads, d, seed=seed + i).to(F8) for i in (0, 1)]
+    scales = [torch.rand(pages, page, heads, generator=gen(seed + 5 + i), device="cuda") + 0.5 for i in (0, 1)]
+    return codes[0], scales[0], codes[1], scales[1]
+
+
+def row_scale(x):
+    return torch.maximum(x.float().abs().amax(-1) / torch.tensor(448.0, device=x.device),
+                         torch.tensor(1e-12, device=x.device))
+
+
+def check_written(x, slots, codes, scale, before_codes, before_scale):
+    codes, scale = codes.flatten(0, 1), scale.flatten(0, 1)
+    kept = torch.ones(codes.shape[0], dtype=torch.bool, device="cuda")
+    live = (slots >= 0) & (slots < codes.shape[0])
+    kept[slots[live]] = False
+    assert torch.equal(codes.view(torch.uint8)[kept], before_codes.view(torch.uint8).flatten(0, 1)[kept])
+    assert torch.equal(scale[kept], before_scale.flatten(0, 1)[kept])
+    got, x = scale[slots[live]], x[live]
+    assert torch.equal(got, row_scale(x))                    # an exact maximum and one IEEE division
+    # x * (1 / scale): two roundings of 2^-24 before E4M3's
+    codes_inside(codes[slots[live]], got[..., None], x.double(), 2.0 ** -22)
+
+
+@pytest.mark.parametrize("tokens", [1, 2, 3, 40, 300])
+@pytest.mark.parametrize("heads,d,page", [(1, 8, 1), (12, 128, 16), (5, 64, 48), (3, 80, 16), (2, 256, 64), (7, 264, 5),
+                                          (2, 512, 16)])
+def test_cache_write(tokens, heads, d, page):
+    pages = (tokens + page - 1) // page + 2
+    cache = store(pages, page, heads, d)
+    before = [t.clone() for t in cache]
+    qkv = randn(tokens, 3, heads, d, seed=7)
+    qkv[0, :, 0] = 0.0                                      # a row of zeros: the smallest scale
+    slots = torch.randperm(pages * page, generator=gen(1), device="cuda")[:tokens]
+    if tokens > 2:
+        slots[1], slots[tokens - 1] = -1, -7
+    ops.fp8_cache_write(qkv[:, 1], qkv[:, 2], slots, *cache)
+    check_written(qkv[:, 1], slots, cache[0], cache[1], before[0], before[1])
+    check_written(qkv[:, 2], slots, cache[2], cache[3], before[2], before[3])
+
+
+def test_cache_write_views_special_values_and_bad_slots():
+    heads, d = 4, 64
+    cache = store(4, 16, heads, d)
+    before = [t.clone() for t in cache]
+    base = randn(heads, 30, d + 8, seed=3)
+    k = base[:, :, :d].transpose(0, 1)                       # heads outermost
+    v = base[:, :, 4:4 + d].transpose(0, 1)                  # off 16 bytes: copied
+    slots = torch.randperm(64, generator=gen(2), device="cuda")[:30]
+    slots[3], slots[4] = 64, 1 << 40                         # past the store: skipped and reported
+    ops.fp8_cache_write(k, v, slots, *cache)
+    assert ops.read_device_error() == 64
+    check_written(k, slots, cache[0], cache[1], before[0], before[1])
+    check_written(v, slots, cache[2], cache[3], before[2], before[3])
+    x = randn(3, heads, d, seed=4)
+    x[0, 0, 1], x[1, 1, 2] = float("inf"), float("nan")
+    ops.fp8_cache_write(x, x, torch.arange(3, device="cuda"), *cache)
+    codes, scale = cache[0].flatten(0, 1).float(), cache[1].flatten(0, 1)
+    assert scale[0, 0] == float("inf") and torch.isnan(codes[0, 0, 1]) and (codes[0, 0, 2:] == 0).all()
+    assert torch.isnan(scale[1, 1]) and torch.isnan(codes[1, 1]).all()
+    assert torch.isfinite(codes[2]).all() and torch.isfinite(codes[0, 1:]).all()
+
+
+def read64(cache, table, lens, most):
+    """bf16(q * scale) below the length, zero above; one fp32 product, one rounding: exact."""
+    out = []
+    page = cache[0].shape[1]
+    for codes, scale in ((cache[0], cache[1]), (cache[2], cache[3])):
+        full = codes.float() * scale[..., None]
+        o = torch.zeros(len(lens), most, *codes.shape[2:], device="cuda")
+        for b, n in enumerate(lens):
+            n = min(max(n, 0), most, table.shape[1] * page)
+            for p in range(n):
+                at = int(table[b, p // page])
+                if 0 <= at < codes.shape[0]:
+                    o[b, p] = full[at, p % page]
+        out.append(o.to(BF16))
+    return out
+
+
+@pytest.mark.parametrize("heads,d,page,lens,most", [(1, 8, 1, [0, 1, 3], 3), (12, 128, 16, [33, 0, 16, 17], 40),
+                                                    (5, 80, 7, [1], 1), (2, 264, 48, [50, 48], 61),
+                                                    (3, 512, 16, [15, 20], 20)])
+def test_cache_read(heads, d, page, lens, most):
+    per = -(-most // page)
+    cache = store(per * len(lens) + 2, page, heads, d)
+    table = torch.randperm(per * len(lens) + 2, generator=gen(3), device="cuda")[:per * len(lens)]
+    table = table.view(len(lens), per).to(torch.int32)
+    for b, n in enumerate(lens):                             # entries past a length are not read
+        table[b, -(-n // page):] = 1 << 30
+    k, v = ops.fp8_cache_read(*cache, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), most)
+    want = read64(cache, table.cpu(), lens, most)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+def test_cache_read_bad_pages_and_lengths():
+    cache = store(6, 16, 2, 64)
+    table = torch.tensor([[0, 1], [6, 2], [-1, 3], [4, 5]], dtype=torch.int32, device="cuda")
+    lens = [20, 20, 20, 20]
+    k, v = ops.fp8_cache_read(*cache, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), 32)
+    assert ops.read_device_error() == 128
+    want = read64(cache, table.cpu(), lens, 32)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+    good = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device="cuda")
+    for lens, most, bits in (([-5, 3], 32, 0), ([33, 3], 40, 128), ([12, 3], 10, 128), ([10, 3], 10, 0)):
+        k, v = ops.fp8_cache_read(*cache, good, torch.tensor(lens, dtype=torch.int32, device="cuda"), most)
+        assert ops.read_device_error() == bits
+        want = read64(cache, good.cpu(), lens, most)
+        assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+def test_cache_empty_and_refusals():
+    cache = store(2, 16, 2, 64)
+    before = [t.clone() for t in cache]
+    kv, slots = randn(3, 2, 64), torch.arange(3, device="cuda")
+    ops.fp8_cache_write(kv[:0], kv[:0], slots[:0], *cache)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(cache, before))
+    table, lens = torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    assert ops.fp8_cache_read(*cache, table, lens, 0)[0].shape == (2, 0, 2, 64)
+    assert ops.fp8_cache_read(*cache, table[:0], lens[:0], 5)[1].shape == (0, 5, 2, 64)
+    for bad, kind in ((lambda: ops.fp8_cache_write(kv.float(), kv, slots, *cache), TypeError),
+                      (lambda: ops.fp8_cache_write(kv, kv[:2], slots, *cache), ValueError),
+                      (lambda: ops.fp8_cache_write(kv[:, :1], kv[:, :1], slots, *cache), ValueError),
+                      (lambda: ops.fp8_cache_write(kv, kv, slots.int(), *cache), ValueError),
+                      (lambda: ops.fp8_cache_write(kv, kv, slots[:2], *cache), ValueError),
+                      (lambda: ops.fp8_cache_write(kv, kv, slots.cpu(), *cache), RuntimeError),
+                      (lambda: ops.fp8_cache_write(kv, kv, slots, cache[0][:, ::2], cache[1][:, ::2],
+                                                   cache[2][:, ::2], cache[3][:, ::2]), ValueError),
+                      (lambda: ops.fp8_cache_read(*cache, table.long(), lens, 4), ValueError),
+                      (lambda: ops.fp8_cache_read(*cache, table, lens[:1], 4), ValueError),
+                      (lambda: ops.fp8_cache_read(*cache, table, lens, -1), ValueError),
+                      (lambda: ops.fp8_cache_read(*cache, table[:, :0], lens, 4), ValueError),
+                      (lambda: ops.fp8_cache_read(cache[0], cache[1].double(), cache[2], cache[3], table, lens, 4),
+                       ValueError)):
+        with pytest.raises(kind):
+            bad()
+
+
+# ---------------------------------------------------------------- streams and graphs
+def block_inputs(m, seed):
+    d, f, heads = 256, 512, 2
+    return {"x": randn(m, d, seed=seed), "r": randn(m, d, seed=seed + 1), "slots": torch.arange(m, device="cuda") * 2}
+
+
+def block_weights():
+    d, f = 256, 512
+    quant = lambda n, k, seed: ops.fp8_row_quant(randn(n, k, seed=seed, std=k ** -0.5))  # noqa: E731
+    return {"norm": randn(d, seed=50), "qkv": quant(3 * d, d, 51), "o": quant(d, d, 52), "up": quant(2 * f, d, 53),
+            "down": quant(d, f, 54), "bias": randn(d, seed=55)}
+
+
+def run_block(i, w, cache, table, lens, most):
+    """norm -> product -> store -> read -> attention in torch -> product + residual -> norm ->
+    gated product -> product + residual: the operators as a block uses them."""
+    d, heads = 256, 2
+    q, s, r = ops.add_rms_norm_fp8(i["x"], i["r"], w["norm"])
+    qkv = ops.fp8_scaled_mm_act(q, s, *w["qkv"]).unflatten(1, (3, heads, d // heads))
+    ops.fp8_cache_write(qkv[:, 1], qkv[:, 2], i["slots"], *cache)
+    k, v = ops.fp8_cache_read(*cache, table, lens, most)
+    p = torch.softmax(torch.einsum("mhd,lhd->hml", qkv[:, 0].float(), k[0].float()) * (d // heads) ** -0.5, -1)
+    att = torch.einsum("hml,lhd->mhd", p, v[0].float()).flatten(1).to(BF16)
+    r = ops.fp8_scaled_mm_act(*ops.fp8_row_quant(att), *w["o"], residual=r)
+    h = ops.fp8_scaled_mm_act(*ops.rms_norm_fp8(r, w["norm"]), *w["up"], act="silu", gated=True)
+    return ops.fp8_scaled_mm_act(*ops.fp8_row_quant(h), *w["down"], w["bias"], residual=r)
+
+
+def plain_block(i, w):
+    """run_block in 64 bits on the dequantized weights, nothing else quantized."""
+    d, heads = 256, 2
+    full = {n: w[n][0].double() * w[n][1].double() for n in ("qkv", "o", "up", "down")}
+    r, u = norm64(i["x"], i["r"], w["norm"], 1e-6)
+    qkv = (u @ full["qkv"].t()).unflatten(1, (3, heads, d // heads))
+    p = torch.softmax(torch.einsum("mhd,lhd->hml", qkv[:, 0], qkv[:, 1]) * (d // heads) ** -0.5, -1)
+    r = r + torch.einsum("hml,lhd->mhd", p, qkv[:, 2]).flatten(1) @ full["o"].t()
+    a, b = (norm64(r, None, w["norm"], 1e-6)[1] @ full["up"].t()).chunk(2, -1)
+    return r + (a * torch.sigmoid(a) * b) @ full["down"].t() + w["bias"].double()
+
+
+def fresh_store(m):
+    cache = store(m, 2, 2, 128)
+    table = torch.arange(m, dtype=torch.int32, device="cuda").view(1, m)
+    return cache, table
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_block_run(m):
+    """Frobenius-relative: every E4M3 rounding is at most 2^-4 (rms 2^-4 / sqrt(3) of the value,
+    under 0.036) and independent; a branch passes at most five of them (norm, weight is exact,
+    keys, values, attention output, gated product), so the output, which also carries the exact
+    stream, is off by less than 0.036 * sqrt(5) < 0.09."""
+    w, i = block_weights(), block_inputs(m, 60)
+    cache, _ = fresh_store(2 * m)
+    # slots 0, 2, 4, ...: one token per two-slot page is stored at its first slot
+    i["slots"] = torch.randperm(4 * m, generator=gen(9), device="cuda")[:m]
+    flat = [t.view(4 * m, 1, *t.shape[2:]) for t in cache]    # the same store as pages of one slot
+    table = i["slots"].to(torch.int32).view(1, m)
+    y = run_block(i, w, flat, table, torch.tensor([m], dtype=torch.int32, device="cuda"), m)
+    want = plain_block(i, w)
+    assert ((y.double() - want).norm() / want.norm()).item() < 0.09
+
+
+def test_block_run_in_a_graph_and_on_streams():
+    """The captured run replays with new inputs, two graphs and a side stream included."""
+    m, w = 24, block_weights()
+    lens = torch.tensor([m], dtype=torch.int32, device="cuda")
+
+    def make(seed):
+        i = block_inputs(m, seed)
+        i["slots"] = torch.randperm(2 * m, generator=gen(seed), device="cuda")[:m]
+        cache = store(2 * m, 1, 2, 128, seed=seed)
+        return i, cache, i["slots"].to(torch.int32).view(1, m)
+
+    want = {}
+    for seed in (1, 2, 3):
+        i, cache, table = make(seed)
+        want[seed] = run_block(i, w, cache, table, lens, m)
+    sets, graphs, outs = [make(1), make(2)], [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for i, cache, table in sets:
+            run_block(i, w, cache, table, lens, m)
+    torch.cuda.current_stream().wait_stream(side)
+    for i, cache, table in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run_block(i, w, cache, table, lens, m))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):                                     # both at once
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[1]) and torch.equal(outs[1], want[2])
+    third, _, _ = make(3)
+    sets[0][0]["x"].copy_(third["x"])
+    sets[0][0]["r"].copy_(third["r"])
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[3])                   # the slots differ, the attention does not see them
