@@ -1031,7 +1031,7 @@ int fvq_rms_norm(const uint16_t* x, int64_t rows, int64_t inner, int64_t outer_s
   if (int rc = check_device()) return rc;
   fvq::NormArgs a = {x, rows, inner, outer_stride, inner_stride, static_cast<int>(d), weight, eps,
                      residual, residual_out, residual_fp32 != 0, y, q, scale};
-  cudaError_t e = fvq::launch_rms_norm(a, static_cast<cudaStream_t>(stream));
+  cudaError_t e = fvq::launch_rms_norm(a, wait_limit(), static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "fvq_rms_norm launch");
   return FVQ_OK;
 }

@@ -210,9 +210,11 @@ struct NormArgs {
   uint16_t* y;                // bf16, or null
   uint8_t* q;                 // E4M3, or null
   float* scale;               // fp32 [rows], with q
+  uint32_t inner_mul;         // set by the launcher: row / inner without a division
+  int inner_shift;
 };
 int64_t rms_norm_max_d();
-cudaError_t launch_rms_norm(const NormArgs& a, cudaStream_t st);
+cudaError_t launch_rms_norm(const NormArgs& a, uint64_t wait_limit, cudaStream_t st);
 
 // y = bf16(act(x W^T [* sx * sw] + bias) [* gate's other half] [+ residual]) (fvq_linear.cu).
 // x: m rows of k elements, x_stride elements apart; w: [n, k], gated [2n, k] (the activated

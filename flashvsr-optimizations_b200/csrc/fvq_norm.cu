@@ -1,21 +1,26 @@
 // fvq_norm.cu -- root-mean-square norm with the residual's addition, in bf16 or E4M3.
 //
 //   s = x + r                                   fp32; r bf16 or fp32 (optional)
-//   v = s * rsqrt(mean(s^2) + eps) * w          fp32; w bf16 (optional)
+//   v = s * w * rsqrt(mean(s^2) + eps)          fp32; w bf16 (optional)
 //   r_out = s in r's type,  y = bf16(v)         and / or
-//   scale = max(max|v| / 448, 1e-12),  q = e4m3(v * (1 / scale))
+//   scale = max(max|v| / 448, 1e-12),  q = e4m3(s * w * (rsqrt(..) / scale))
 //
 // Everything up to the outputs is fp32 in registers; each output is rounded once.  q multiplies
-// by the correctly rounded reciprocal of the scale instead of dividing: two roundings of 2^-24
-// ahead of E4M3's 2^-4, a third of the instructions.  A NaN in a row makes the row NaN, an
+// by one factor per row instead of dividing: three roundings of 2^-24 ahead of E4M3's 2^-4, a
+// third of the instructions.  A NaN in a row makes the row NaN, an
 // infinity gives what the formulas give (0 for the finite values, NaN for the infinite ones).
 //
 // HBM-bound: x and r are read once, every output is written once; the row stays in registers
-// between the two reductions (sum of squares, then max |v| for E4M3).  Short rows go to
-// sub-warp groups of lanes so that a warp's 16-byte loads stay dense, rows of at most 2048
-// values to one warp (no barrier), longer ones to one CTA.  Row starts or lengths that are no
-// multiple of 16 bytes take element-wise loads (kVec = 1): neighbouring lanes read
-// neighbouring elements, so the sectors fetched are the same.
+// between the two reductions (sum of squares, then max |v| for E4M3).  Three forms:
+//   * rows of at most 256 values: sub-warp groups of lanes, several rows a group when there
+//     are many, so that their loads overlap;
+//   * few rows: a CTA per row with 8 or 16 values a thread, the shortest chain for one token;
+//   * many rows: persistent CTAs whose warps stream rows through rings in shared memory
+//     filled by bulk copies (rms_norm_stream_kernel), so that loads stay in flight while
+//     earlier rows are reduced and written.  A row that starts or ends off 16 bytes is
+//     fetched as the 16-byte aligned window around it.
+// In the first two forms such rows take element-wise loads (kVec = 1): neighbouring lanes
+// read neighbouring elements, so the sectors fetched are the same.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -26,250 +31,595 @@ namespace fvq {
 
 namespace {
 
-constexpr int kNormThreads = 256;
-constexpr int kNormMaxPerThread = 64;  // row elements a thread holds in registers
+constexpr int kNormThreads = 256;      // of the sub-warp form
+constexpr int kNormMaxThreads = 1024;  // of the CTA form
+constexpr int kNormMaxD = 16384;
 
-__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+// ---------------------------------------------------------------- pairs
+// Row elements are held as pairs of fp32 in 64-bit registers, so that the products and sums
+// are the packed f32x2 instructions (two IEEE operations each, half the issue slots).
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
 
-__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+__device__ __forceinline__ void split(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+
+__device__ __forceinline__ uint64_t pair_of_bf16(uint32_t w) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(w << 16), "r"(w & 0xFFFF0000u));
+  return v;
+}
+
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t bf16x2(uint64_t v) {
+  float lo, hi;
   uint32_t r;
+  split(v, lo, hi);
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+__device__ __forceinline__ uint32_t e4m3x2(uint64_t v) {
+  float lo, hi;
   uint16_t r;
+  split(v, lo, hi);
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
 
-// kVec consecutive bf16 / fp32 elements <-> fp32 registers (kVec 8: 16-byte accesses)
-template <int kVec>
-__device__ __forceinline__ void load_bf16(const uint16_t* p, float* f) {
+// max with a NaN of either side kept
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// A thread's share of a row: kPairs pairs.  kVec 8: pairs 4i .. 4i+3 are the eight adjacent
+// elements of its i-th 16-byte vector; kVec 1: pair i holds its elements 2i and 2i + 1, one
+// row stride of lanes apart.  `at(i)` is the element index of vector (kVec 8) or element
+// (kVec 1) i; elements past d are zero and not stored.
+template <int kPairs, int kVec, class At>
+__device__ __forceinline__ void load_bf16(uint32_t (&w)[kPairs], const uint16_t* p, int d, At at) {
   if constexpr (kVec == 8) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[2 * j] = bf_lo(w[j]);
-      f[2 * j + 1] = bf_hi(w[j]);
+    for (int i = 0; i < kPairs / 4; ++i) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (at(i) < d) v = *reinterpret_cast<const uint4*>(p + at(i));
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
     }
   } else {
-    f[0] = __uint_as_float(static_cast<uint32_t>(__ldg(p)) << 16);
-  }
-}
-
-template <int kVec>
-__device__ __forceinline__ void load_f32(const float* p, float* f) {
-  if constexpr (kVec == 8) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
-    f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
-    f[0] = __ldg(p);
-  }
-}
-
-template <int kVec>
-__device__ __forceinline__ void store_bf16(uint16_t* p, const float* f) {
-  if constexpr (kVec == 8)
-    *reinterpret_cast<uint4*>(p) = make_uint4(bf16x2(f[0], f[1]), bf16x2(f[2], f[3]),
-                                              bf16x2(f[4], f[5]), bf16x2(f[6], f[7]));
-  else
-    *p = __bfloat16_as_ushort(__float2bfloat16_rn(f[0]));
-}
-
-template <int kVec>
-__device__ __forceinline__ void store_f32(float* p, const float* f) {
-  if constexpr (kVec == 8) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-  } else {
-    *p = f[0];
-  }
-}
-
-// kLanes threads share a row: 8, 16 or 32 lanes of a warp, or all kNormThreads of the CTA.
-template <int kLanes>
-__device__ __forceinline__ float row_sum(float v, float* smem) {
-  constexpr int kWidth = kLanes < 32 ? kLanes : 32;
 #pragma unroll
-  for (int o = kWidth / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  if constexpr (kLanes > 32) {
-    if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0f;
+    for (int i = 0; i < kPairs; ++i) {
+      const uint32_t lo = at(2 * i) < d ? p[at(2 * i)] : 0u;
+      const uint32_t hi = at(2 * i + 1) < d ? p[at(2 * i + 1)] : 0u;
+      w[i] = lo | (hi << 16);
+    }
+  }
+}
+
+// s += the fp32 elements at p
+template <int kPairs, int kVec, class At>
+__device__ __forceinline__ void add_f32(uint64_t (&s)[kPairs], const float* p, int d, At at) {
+  if constexpr (kVec == 8) {
 #pragma unroll
-    for (int w = 0; w < kLanes / 32; ++w) v += smem[w];
+    for (int i = 0; i < kPairs / 4; ++i) {
+      if (at(i) < d) {
+        const float4 a = *reinterpret_cast<const float4*>(p + at(i));
+        const float4 b = *reinterpret_cast<const float4*>(p + at(i) + 4);
+        s[4 * i] = add2(s[4 * i], pair_of(a.x, a.y));
+        s[4 * i + 1] = add2(s[4 * i + 1], pair_of(a.z, a.w));
+        s[4 * i + 2] = add2(s[4 * i + 2], pair_of(b.x, b.y));
+        s[4 * i + 3] = add2(s[4 * i + 3], pair_of(b.z, b.w));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const float lo = at(2 * i) < d ? p[at(2 * i)] : 0.0f;
+      const float hi = at(2 * i + 1) < d ? p[at(2 * i + 1)] : 0.0f;
+      s[i] = add2(s[i], pair_of(lo, hi));
+    }
+  }
+}
+
+template <int kPairs, int kVec, class At>
+__device__ __forceinline__ void store_f32(float* p, const uint64_t (&s)[kPairs], int d, At at) {
+  if constexpr (kVec == 8) {
+#pragma unroll
+    for (int i = 0; i < kPairs / 4; ++i) {
+      if (at(i) < d) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split(s[4 * i + e], f[2 * e], f[2 * e + 1]);
+        reinterpret_cast<float4*>(p + at(i))[0] = make_float4(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<float4*>(p + at(i))[1] = make_float4(f[4], f[5], f[6], f[7]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      float lo, hi;
+      split(s[i], lo, hi);
+      if (at(2 * i) < d) p[at(2 * i)] = lo;
+      if (at(2 * i + 1) < d) p[at(2 * i + 1)] = hi;
+    }
+  }
+}
+
+// bf16(s * f)
+template <int kPairs, int kVec, class At>
+__device__ __forceinline__ void store_bf16(uint16_t* p, const uint64_t (&s)[kPairs], uint64_t f, int d,
+                                           At at) {
+  if constexpr (kVec == 8) {
+#pragma unroll
+    for (int i = 0; i < kPairs / 4; ++i)
+      if (at(i) < d)
+        *reinterpret_cast<uint4*>(p + at(i)) =
+            make_uint4(bf16x2(mul2(s[4 * i], f)), bf16x2(mul2(s[4 * i + 1], f)),
+                       bf16x2(mul2(s[4 * i + 2], f)), bf16x2(mul2(s[4 * i + 3], f)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const uint32_t w = bf16x2(mul2(s[i], f));
+      if (at(2 * i) < d) p[at(2 * i)] = static_cast<uint16_t>(w);
+      if (at(2 * i + 1) < d) p[at(2 * i + 1)] = static_cast<uint16_t>(w >> 16);
+    }
+  }
+}
+
+// e4m3(s * f)
+template <int kPairs, int kVec, class At>
+__device__ __forceinline__ void store_e4m3(uint8_t* p, const uint64_t (&s)[kPairs], uint64_t f, int d,
+                                           At at) {
+  if constexpr (kVec == 8) {
+#pragma unroll
+    for (int i = 0; i < kPairs / 4; ++i)
+      if (at(i) < d)
+        *reinterpret_cast<uint2*>(p + at(i)) =
+            make_uint2(e4m3x2(mul2(s[4 * i], f)) | (e4m3x2(mul2(s[4 * i + 1], f)) << 16),
+                       e4m3x2(mul2(s[4 * i + 2], f)) | (e4m3x2(mul2(s[4 * i + 3], f)) << 16));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const uint32_t w = e4m3x2(mul2(s[i], f));
+      if (at(2 * i) < d) p[at(2 * i)] = static_cast<uint8_t>(w);
+      if (at(2 * i + 1) < d) p[at(2 * i + 1)] = static_cast<uint8_t>(w >> 8);
+    }
+  }
+}
+
+// s = x + r, and r_out = s; p at the row's residual (global or shared memory).
+template <int kPairs, int kVec, class At>
+__device__ __forceinline__ void add_residual(uint64_t (&s)[kPairs], const void* p, bool f32, void* out,
+                                             bool store, int d, At at) {
+  if (f32) {
+    add_f32<kPairs, kVec>(s, static_cast<const float*>(p), d, at);
+    if (store) store_f32<kPairs, kVec>(static_cast<float*>(out), s, d, at);
+  } else {
+    uint32_t w[kPairs];
+    load_bf16<kPairs, kVec>(w, static_cast<const uint16_t*>(p), d, at);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) s[i] = add2(s[i], pair_of_bf16(w[i]));
+    if (store)
+      store_bf16<kPairs, kVec>(static_cast<uint16_t*>(out), s, pair_of(1.0f, 1.0f), d, at);
+  }
+}
+
+template <int kPairs>
+__device__ __forceinline__ float sum_squares(const uint64_t (&s)[kPairs]) {
+  uint64_t q = 0;
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) q = fma2(s[i], s[i], q);
+  float lo, hi;
+  split(q, lo, hi);
+  return lo + hi;
+}
+
+// s *= w (when there is a weight)
+template <int kPairs>
+__device__ __forceinline__ void apply_weight(uint64_t (&s)[kPairs], const uint32_t (&w)[kPairs]) {
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) s[i] = mul2(s[i], pair_of_bf16(w[i]));
+}
+
+template <int kPairs>
+__device__ __forceinline__ float max_abs(const uint64_t (&s)[kPairs]) {
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    float lo, hi;
+    split(s[i], lo, hi);
+    m = max_nan(max_nan(m, fabsf(lo)), fabsf(hi));
+  }
+  return m;
+}
+
+// max(m / 448, 1e-12); NaN stays NaN
+__device__ __forceinline__ float scale448(float m) {
+  const float by448 = __fdiv_rn(m, 448.0f);
+  return by448 < 1e-12f ? 1e-12f : by448;
+}
+
+// Sum / maximum over the threads of a row: kLanes (8, 16 or 32) lanes of a warp, or with
+// kLanes = 0 the whole CTA.
+template <int kLanes, class Op>
+__device__ __forceinline__ float row_reduce(float v, float* smem, Op op) {
+  constexpr int kWidth = kLanes == 0 ? 32 : kLanes;
+#pragma unroll
+  for (int o = kWidth / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  if constexpr (kLanes == 0) {
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (warps > 1) {
+      if (lane == 0) smem[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = lane < warps ? smem[lane] : 0.0f;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    }
   }
   return v;
 }
 
-// Maximum of magnitude bits: orders like the values, infinities above finite ones, NaN on top.
-template <int kLanes>
-__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* smem) {
-  constexpr int kWidth = kLanes < 32 ? kLanes : 32;
-#pragma unroll
-  for (int o = kWidth / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-  if constexpr (kLanes > 32) {
-    if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int w = 0; w < kLanes / 32; ++w) v = max(v, smem[w]);
-  }
-  return v;
+__device__ __forceinline__ const uint16_t* x_row(const NormArgs& a, int64_t row) {
+  if (a.inner == 1) return a.x + row * a.outer_stride;
+  // row / inner, exact below 2^31: (n + umulhi(n, m)) >> l with m, l of the launcher
+  const uint32_t n = static_cast<uint32_t>(row);
+  const uint32_t outer = (n + __umulhi(n, a.inner_mul)) >> a.inner_shift;
+  const uint32_t in = n - outer * static_cast<uint32_t>(a.inner);
+  return a.x + outer * a.outer_stride + in * a.inner_stride;
 }
 
-// kPer: elements per thread (a multiple of kVec); a row has at most kLanes * kPer.
-template <int kLanes, int kPer, int kVec>
-__global__ void __launch_bounds__(kNormThreads) rms_norm_kernel(const NormArgs a) {
-  __shared__ float sum_smem[kNormThreads / 32];
-  __shared__ uint32_t max_smem[kNormThreads / 32];
-  constexpr int kIter = kPer / kVec;
-  const int lane = threadIdx.x % kLanes;
-  int64_t row = static_cast<int64_t>(blockIdx.x) * (kNormThreads / kLanes) + threadIdx.x / kLanes;
-  // a group past the last row repeats the last one without storing: the warp's shuffles stay whole
-  const bool live = row < a.rows;
-  if (!live) row = a.rows - 1;
-  const int64_t outer = row / a.inner;
-  const uint16_t* x = a.x + outer * a.outer_stride + (row - outer * a.inner) * a.inner_stride;
+// ---------------------------------------------------------------- short rows, few rows
+// kPer: elements per thread.  kLanes 0: one CTA per row; otherwise kLanes lanes per row and
+// kRows rows per group, whose loads overlap.  A row has at most (threads of the row) * kPer
+// elements.
+template <int kLanes, int kRows, int kPer, int kVec>
+__global__ void __launch_bounds__(kLanes == 0 ? kNormMaxThreads : kNormThreads)
+    rms_norm_kernel(const NormArgs a) {
+  static_assert(kLanes != 0 || kRows == 1, "one row per CTA");
+  __shared__ float sum_smem[32];
+  __shared__ float max_smem[32];
+  constexpr int kPairs = kPer / 2;
+  const int lanes = kLanes == 0 ? static_cast<int>(blockDim.x) : kLanes;
+  const int lane = kLanes == 0 ? static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x) % lanes;
   const int d = a.d;
-  const int64_t base = row * d;
-
-  float s[kPer];
+  const auto at = [lane, lanes](int i) { return (lane + i * lanes) * kVec; };
+  // kRows rows, `step` apart, so that neighbouring groups read neighbouring rows
+  const int64_t step = kLanes == 0 ? 1 : kNormThreads / lanes;
+  const int64_t first = kLanes == 0 ? static_cast<int64_t>(blockIdx.x)
+                                    : blockIdx.x * step * kRows + static_cast<int>(threadIdx.x) / lanes;
+  uint32_t xw[kRows][kPairs];
 #pragma unroll
-  for (int i = 0; i < kIter; ++i) {
-    const int j = (lane + i * kLanes) * kVec;
-    if (j < d) {
-      load_bf16<kVec>(x + j, &s[i * kVec]);
-    } else {
+  for (int k = 0; k < kRows; ++k)  // a row past the last one repeats it: the warp's shuffles stay whole
+    load_bf16<kPairs, kVec>(xw[k], x_row(a, min(first + k * step, a.rows - 1)), d, at);
+  uint32_t w[kPairs];
+  if (a.weight != nullptr) load_bf16<kPairs, kVec>(w, a.weight, d, at);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) s[i * kVec + e] = 0.0f;
+  for (int k = 0; k < kRows; ++k) {
+    const bool live = first + k * step < a.rows;
+    const int64_t row = min(first + k * step, a.rows - 1);
+    const int64_t base = row * d;
+    uint64_t s[kPairs];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) s[i] = pair_of_bf16(xw[k][i]);
+    if (a.residual != nullptr) {
+      const int64_t bytes = base * (a.residual_f32 ? 4 : 2);
+      add_residual<kPairs, kVec>(s, static_cast<const uint8_t*>(a.residual) + bytes, a.residual_f32,
+                                 static_cast<uint8_t*>(a.residual_out) + bytes, live, d, at);
     }
-  }
-  if (a.residual != nullptr) {
-    float r[kPer];
-    if (a.residual_f32) {
-      const float* p = static_cast<const float*>(a.residual) + base;
-#pragma unroll
-      for (int i = 0; i < kIter; ++i) {
-        const int j = (lane + i * kLanes) * kVec;
-        if (j < d) load_f32<kVec>(p + j, &r[i * kVec]);
-      }
-    } else {
-      const uint16_t* p = static_cast<const uint16_t*>(a.residual) + base;
-#pragma unroll
-      for (int i = 0; i < kIter; ++i) {
-        const int j = (lane + i * kLanes) * kVec;
-        if (j < d) load_bf16<kVec>(p + j, &r[i * kVec]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kIter; ++i) {
-      const int j = (lane + i * kLanes) * kVec;
-      if (j < d) {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) s[i * kVec + e] += r[i * kVec + e];
-        if (live) {
-          if (a.residual_f32)
-            store_f32<kVec>(static_cast<float*>(a.residual_out) + base + j, &s[i * kVec]);
-          else
-            store_bf16<kVec>(static_cast<uint16_t*>(a.residual_out) + base + j, &s[i * kVec]);
-        }
-      }
-    }
-  }
-  float sq = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) sq = fmaf(s[i], s[i], sq);
-  sq = row_sum<kLanes>(sq, sum_smem);
-  const float rstd = rsqrtf(sq / static_cast<float>(d) + a.eps);
-
-  uint32_t mag = 0;
-#pragma unroll
-  for (int i = 0; i < kIter; ++i) {
-    const int j = (lane + i * kLanes) * kVec;
-    if (j < d) {
-      float w[kVec];
-      if (a.weight != nullptr) {
-        load_bf16<kVec>(a.weight + j, w);
-      } else {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) w[e] = 1.0f;
-      }
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        float& v = s[i * kVec + e];
-        v = v * rstd * w[e];
-        mag = max(mag, __float_as_uint(v) & 0x7FFFFFFFu);
-      }
-      if (a.y != nullptr && live) store_bf16<kVec>(a.y + base + j, &s[i * kVec]);
-    }
-  }
-  if (a.q != nullptr) {
-    mag = row_max<kLanes>(mag, max_smem);
-    const float by448 = __fdiv_rn(__uint_as_float(mag), 448.0f);
-    const float scale = by448 < 1e-12f ? 1e-12f : by448;  // NaN stays NaN
-    const float inv = __frcp_rn(scale);
-    if (!live) return;
-    if (lane == 0) a.scale[row] = scale;
-    uint8_t* q = a.q + base;
-#pragma unroll
-    for (int i = 0; i < kIter; ++i) {
-      const int j = (lane + i * kLanes) * kVec;
-      if (j < d) {
-        if constexpr (kVec == 8) {
-          uint32_t c[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            c[e] = e4m3x2(s[i * kVec + 2 * e] * inv, s[i * kVec + 2 * e + 1] * inv);
-          *reinterpret_cast<uint2*>(q + j) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
-        } else {
-          q[j] = static_cast<uint8_t>(e4m3x2(s[i] * inv, 0.0f) & 0xFFu);
-        }
-      }
+    const float sq = row_reduce<kLanes>(sum_squares(s), sum_smem, [](float p, float q) { return p + q; });
+    const float rstd = rsqrtf(sq / static_cast<float>(d) + a.eps);
+    if (a.weight != nullptr) apply_weight(s, w);
+    if (a.y != nullptr && live) store_bf16<kPairs, kVec>(a.y + base, s, pair_of(rstd, rstd), d, at);
+    if (a.q != nullptr) {
+      const float m = row_reduce<kLanes>(max_abs(s), max_smem, [](float p, float q) { return max_nan(p, q); });
+      const float scale = scale448(m * rstd), f = rstd * __frcp_rn(scale);
+      if (!live) continue;
+      if (lane == 0) a.scale[row] = scale;
+      store_e4m3<kPairs, kVec>(a.q + base, s, pair_of(f, f), d, at);
     }
   }
 }
 
-template <int kLanes, int kPer>
-void norm_launch(const NormArgs& a, bool vec, cudaStream_t st) {
-  constexpr int kRows = kNormThreads / kLanes;
-  const unsigned grid = static_cast<unsigned>((a.rows + kRows - 1) / kRows);
-  if (vec)
-    rms_norm_kernel<kLanes, kPer, 8><<<grid, kNormThreads, 0, st>>>(a);
+// ---------------------------------------------------------------- many long rows
+// One CTA of 16 warps per SM.  A group of `kGroup` warps walks rows group by group over the
+// grid; each group owns a ring of `slots` row buffers (x's row, then the residual's), one
+// mbarrier each.  A slot is refilled as soon as the group holds its row in registers.
+constexpr int kStreamWarps = 16;
+constexpr int kStreamThreads = 32 * kStreamWarps;
+constexpr int kStreamSmem = 216 * 1024;
+constexpr int kStreamSlotsMax = 8;
+constexpr int kStreamHead = 2048;  // barriers and the reductions' partials
+
+struct StreamPlan {
+  int x_bytes;     // bytes of x's window in a slot (a multiple of 16)
+  int slot_bytes;
+  int slots;
+};
+
+// The 16-byte window around a row of `bytes` at p; whole: it lies inside [begin, end).
+struct Window {
+  const uint8_t* lo;
+  uint32_t bytes;
+  uint32_t off;    // of the row in the window
+  bool whole;
+};
+
+__device__ __forceinline__ Window window(const void* p, uint32_t bytes, const void* begin,
+                                         const void* end) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  Window w;
+  w.off = static_cast<uint32_t>(at & 15u);
+  w.lo = reinterpret_cast<const uint8_t*>(at - w.off);
+  w.bytes = (w.off + bytes + 15u) & ~15u;
+  w.whole = w.lo >= static_cast<const uint8_t*>(begin) && w.lo + w.bytes <= static_cast<const uint8_t*>(end);
+  return w;
+}
+
+template <int kGroup>
+__device__ __forceinline__ void group_sync(int group) {
+  if constexpr (kGroup == 1)
+    __syncwarp();
   else
-    rms_norm_kernel<kLanes, kPer, 1><<<grid, kNormThreads, 0, st>>>(a);
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * kGroup) : "memory");
+}
+
+template <int kGroup, class Op>
+__device__ __forceinline__ float group_reduce(float v, float* smem, int group, int warp_in_group, Op op) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  if constexpr (kGroup > 1) {
+    if ((threadIdx.x & 31) == 0) smem[warp_in_group] = v;
+    group_sync<kGroup>(group);
+    v = smem[0];
+#pragma unroll
+    for (int k = 1; k < kGroup; ++k) v = op(v, smem[k]);
+  }
+  return v;
+}
+
+template <int kGroup, int kPer, int kVec>
+__global__ void __launch_bounds__(kStreamThreads, 1)
+    rms_norm_stream_kernel(const NormArgs a, const StreamPlan p, const uint64_t wait_limit,
+                           uint32_t* err_word) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int kGroups = kStreamWarps / kGroup;
+  constexpr int kLanes = 32 * kGroup;
+  constexpr int kPairs = kPer / 2;
+  auto* bars = reinterpret_cast<uint64_t*>(smem);                          // [groups][slots]
+  auto* sums = reinterpret_cast<float*>(smem + kStreamWarps * kStreamSlotsMax * 8);
+  auto* maxima = sums + kStreamWarps;
+  auto* lost = reinterpret_cast<volatile int*>(maxima + kStreamWarps);      // a load never landed
+  const int warp = threadIdx.x >> 5;
+  const int group = warp / kGroup, in_group = warp % kGroup;
+  const int lane = static_cast<int>(threadIdx.x) - group * kLanes;
+  const bool leader = lane == 0;
+  uint64_t* bar = bars + group * kStreamSlotsMax;
+  uint8_t* ring = smem + kStreamHead + group * p.slots * p.slot_bytes;
+  const int d = a.d;
+  const auto at = [lane](int i) { return (lane + i * kLanes) * kVec; };
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kGroups;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+  const int res_bytes = a.residual == nullptr ? 0 : a.residual_f32 ? 4 : 2;
+
+  const auto x_window = [&](int64_t row) {
+    return window(x_row(a, row), 2u * d, a.x, x_row(a, a.rows - 1) + d);
+  };
+  const auto r_row = [&](int64_t row) {
+    return static_cast<const uint8_t*>(a.residual) + row * d * res_bytes;
+  };
+  const auto r_window = [&](int64_t row) {
+    return window(r_row(row), static_cast<uint32_t>(d * res_bytes), a.residual, r_row(a.rows));
+  };
+  // A row whose window would leave its tensor (the first or last one, off 16 bytes) is copied
+  // by the group itself when its turn comes.
+  const auto fetch = [&](int64_t row, int slot) {
+    const Window x = x_window(row);
+    Window r = {nullptr, 0u, 0u, true};
+    if (res_bytes != 0) r = r_window(row);
+    if (!x.whole || !r.whole) return;
+    mbar_arrive_expect_tx(&bar[slot], x.bytes + r.bytes);
+    uint8_t* to = ring + slot * p.slot_bytes;
+    bulk_load(to, x.lo, x.bytes, &bar[slot]);
+    if (res_bytes != 0) bulk_load(to + p.x_bytes, r.lo, r.bytes, &bar[slot]);
+  };
+
+  if (threadIdx.x == 0) *lost = 0;
+  if (leader) {
+    for (int s = 0; s < p.slots; ++s) mbar_init(&bar[s], 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+    for (int s = 0; s < p.slots; ++s)
+      if (row0 + s * stride < a.rows) fetch(row0 + s * stride, s);
+  }
+  uint32_t w[kPairs];
+  if (a.weight != nullptr) load_bf16<kPairs, kVec>(w, a.weight, d, at);
+  __syncthreads();  // the barriers are initialised
+
+  int slot = 0;
+  uint32_t phases = 0;        // bit s: parity of slot s
+  for (int64_t row = row0; row < a.rows; row += stride) {
+    uint8_t* xs = ring + slot * p.slot_bytes;
+    uint8_t* rs = xs + p.x_bytes;
+    bool whole = true;
+    if constexpr (kVec == 1) {  // with 16-byte rows every window is its row
+      const Window xw = x_window(row);
+      xs += xw.off;
+      whole = xw.whole;
+      if (res_bytes != 0) {
+        const Window rw = r_window(row);
+        rs += rw.off;
+        whole = whole && rw.whole;
+      }
+    }
+    if (whole) {
+      // A wait that runs out is reported, and waited for once more: the ring stays in step,
+      // and no load is in flight when the CTA exits.
+      const uint32_t parity = (phases >> slot) & 1u;
+      if (*lost == 0 && !mbar_wait_bounded(&bar[slot], parity, wait_limit)) {
+        atomicOr(err_word, kErrWaitProducer);
+        if (!mbar_wait_bounded(&bar[slot], parity, wait_limit > kDefaultWaitLimit ? wait_limit : kDefaultWaitLimit))
+          *lost = 1;  // later rows are not waited for; their outputs are undefined
+      }
+      phases ^= 1u << slot;
+    } else {
+      for (int j = lane; j < d; j += kLanes) {
+        reinterpret_cast<uint16_t*>(xs)[j] = __ldg(x_row(a, row) + j);
+        if (res_bytes == 4)
+          reinterpret_cast<float*>(rs)[j] = __ldg(reinterpret_cast<const float*>(r_row(row)) + j);
+        else if (res_bytes == 2)
+          reinterpret_cast<uint16_t*>(rs)[j] = __ldg(reinterpret_cast<const uint16_t*>(r_row(row)) + j);
+      }
+      fence_proxy_async_smem();  // the slot's next bulk copy comes after these stores
+      group_sync<kGroup>(group);
+    }
+    uint32_t xw[kPairs];
+    load_bf16<kPairs, kVec>(xw, reinterpret_cast<const uint16_t*>(xs), d, at);
+    uint64_t s[kPairs];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) s[i] = pair_of_bf16(xw[i]);
+    const int64_t base = row * d;
+    if (res_bytes != 0)
+      add_residual<kPairs, kVec>(s, rs, res_bytes == 4, static_cast<uint8_t*>(a.residual_out) + base * res_bytes,
+                                 true, d, at);
+    float sq = sum_squares(s);
+    group_sync<kGroup>(group);  // the group holds the row (and has left the partials)
+    if (leader && row + p.slots * stride < a.rows) fetch(row + p.slots * stride, slot);
+    sq = group_reduce<kGroup>(sq, sums + group * kGroup, group, in_group,
+                              [](float x, float y) { return x + y; });
+    const float rstd = rsqrtf(sq / static_cast<float>(d) + a.eps);
+    if (a.weight != nullptr) apply_weight(s, w);
+    if (a.y != nullptr) store_bf16<kPairs, kVec>(a.y + base, s, pair_of(rstd, rstd), d, at);
+    if (a.q != nullptr) {
+      const float m = group_reduce<kGroup>(max_abs(s), maxima + group * kGroup, group, in_group,
+                                           [](float x, float y) { return max_nan(x, y); });
+      const float scale = scale448(m * rstd), f = rstd * __frcp_rn(scale);
+      if (leader) a.scale[row] = scale;
+      store_e4m3<kPairs, kVec>(a.q + base, s, pair_of(f, f), d, at);
+    }
+    if (++slot == p.slots) slot = 0;
+  }
+}
+
+template <int kLanes, int kRows, int kPer>
+void norm_launch(const NormArgs& a, bool vec, cudaStream_t st) {
+  const int threads = kLanes != 0 ? kNormThreads : ((a.d + kPer - 1) / kPer + 31) / 32 * 32;
+  const int rows = kLanes != 0 ? kNormThreads / kLanes * kRows : 1;
+  const unsigned grid = static_cast<unsigned>((a.rows + rows - 1) / rows);
+  if (vec)
+    rms_norm_kernel<kLanes, kRows, kPer, 8><<<grid, threads, 0, st>>>(a);
+  else
+    rms_norm_kernel<kLanes, kRows, kPer, 1><<<grid, threads, 0, st>>>(a);
+}
+
+template <int kLanes>
+void norm_short(const NormArgs& a, bool vec, cudaStream_t st) {
+  // four rows a group once that still leaves every SM its threads
+  if (a.rows * kLanes >= static_cast<int64_t>(sm_count()) * 2048 * 4)
+    norm_launch<kLanes, 4, 8>(a, vec, st);
+  else
+    norm_launch<kLanes, 1, 8>(a, vec, st);
+}
+
+template <int kGroup, int kPer, int kVec>
+cudaError_t stream_launch(const NormArgs& a, const StreamPlan& p, uint64_t wait_limit,
+                          uint32_t* err_word, cudaStream_t st) {
+  static ContextCache attr_done;
+  auto* kernel = rms_norm_stream_kernel<kGroup, kPer, kVec>;
+  const int bytes = kStreamHead + kStreamSmem;
+  if (cudaError_t e = ensure_max_dynamic_smem(attr_done, reinterpret_cast<const void*>(kernel), bytes))
+    return e;
+  kernel<<<static_cast<unsigned>(sm_count()), kStreamThreads, bytes, st>>>(a, p, wait_limit, err_word);
+  return cudaGetLastError();
+}
+
+template <int kGroup, int kVec>
+cudaError_t stream_by_width(const NormArgs& a, const StreamPlan& p, uint64_t wait_limit,
+                            uint32_t* err_word, cudaStream_t st) {
+  const int per = (a.d + 32 * kGroup - 1) / (32 * kGroup);
+  if (per <= 16) return stream_launch<kGroup, 16, kVec>(a, p, wait_limit, err_word, st);
+  if (per <= 32) return stream_launch<kGroup, 32, kVec>(a, p, wait_limit, err_word, st);
+  if (per <= 48) return stream_launch<kGroup, 48, kVec>(a, p, wait_limit, err_word, st);
+  return stream_launch<kGroup, 64, kVec>(a, p, wait_limit, err_word, st);
 }
 
 }  // namespace
 
-int64_t rms_norm_max_d() { return static_cast<int64_t>(kNormThreads) * kNormMaxPerThread; }
+int64_t rms_norm_max_d() { return kNormMaxD; }
 
-cudaError_t launch_rms_norm(const NormArgs& a, cudaStream_t st) {
-  if (a.rows <= 0) return cudaSuccess;
+cudaError_t launch_rms_norm(const NormArgs& args, uint64_t wait_limit, cudaStream_t st) {
+  if (args.rows <= 0) return cudaSuccess;
+  NormArgs a = args;
+  a.inner_shift = 0;
+  while ((int64_t(1) << a.inner_shift) < a.inner) ++a.inner_shift;
+  a.inner_mul = static_cast<uint32_t>(
+      ((uint64_t(1) << 32) * ((uint64_t(1) << a.inner_shift) - static_cast<uint64_t>(a.inner))) /
+          static_cast<uint64_t>(a.inner) + 1);
   const auto at16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   const bool vec = a.d % 8 == 0 && a.outer_stride % 8 == 0 && a.inner_stride % 8 == 0 &&
                    at16(a.x) && at16(a.weight) && at16(a.residual) && at16(a.residual_out) &&
                    at16(a.y) && at16(a.q);
   const int d = a.d;
-  if (d <= 64) norm_launch<8, 8>(a, vec, st);
-  else if (d <= 128) norm_launch<16, 8>(a, vec, st);
-  else if (d <= 256) norm_launch<32, 8>(a, vec, st);
-  else if (d <= 512) norm_launch<32, 16>(a, vec, st);
-  else if (d <= 1024) norm_launch<32, 32>(a, vec, st);
-  else if (d <= 1536) norm_launch<32, 48>(a, vec, st);
-  else if (d <= 2048) norm_launch<32, 64>(a, vec, st);
-  else if (d <= 4096) norm_launch<256, 16>(a, vec, st);
-  else if (d <= 6144) norm_launch<256, 24>(a, vec, st);
-  else if (d <= 8192) norm_launch<256, 32>(a, vec, st);
-  else if (d <= 10240) norm_launch<256, 40>(a, vec, st);
-  else if (d <= 12288) norm_launch<256, 48>(a, vec, st);
-  else if (d <= rms_norm_max_d()) norm_launch<256, 64>(a, vec, st);
-  else return cudaErrorInvalidValue;
+  if (d > kNormMaxD) return cudaErrorInvalidValue;
+  if (d <= 64) {
+    norm_short<8>(a, vec, st);
+  } else if (d <= 128) {
+    norm_short<16>(a, vec, st);
+  } else if (d <= 256) {
+    norm_short<32>(a, vec, st);
+  } else {
+    // warps per row: rings of two rows per group within the shared memory, 64 values a lane
+    StreamPlan p;
+    const int res = a.residual == nullptr ? 0 : a.residual_f32 ? 4 : 2, slack = vec ? 0 : 16;
+    p.x_bytes = (2 * d + slack + 15) / 16 * 16;
+    p.slot_bytes = p.x_bytes + (res == 0 ? 0 : (res * d + slack + 15) / 16 * 16);
+    int group = 1;
+    while (group < 16 && (d > 32 * group * 64 || kStreamWarps / group * 2 * p.slot_bytes > kStreamSmem))
+      group *= 2;
+    p.slots = kStreamSmem / (kStreamWarps / group) / p.slot_bytes;
+    if (p.slots > kStreamSlotsMax) p.slots = kStreamSlotsMax;
+    if (a.rows >= static_cast<int64_t>(sm_count()) * (kStreamWarps / group) * 2) {
+      uint32_t* err_word = error_word_ptr();
+      if (err_word == nullptr) return cudaErrorInvalidSymbol;
+      switch (group * 2 + (vec ? 1 : 0)) {
+        case 2: return stream_by_width<1, 1>(a, p, wait_limit, err_word, st);
+        case 3: return stream_by_width<1, 8>(a, p, wait_limit, err_word, st);
+        case 4: return stream_by_width<2, 1>(a, p, wait_limit, err_word, st);
+        case 5: return stream_by_width<2, 8>(a, p, wait_limit, err_word, st);
+        case 8: return stream_by_width<4, 1>(a, p, wait_limit, err_word, st);
+        case 9: return stream_by_width<4, 8>(a, p, wait_limit, err_word, st);
+        case 16: return stream_by_width<8, 1>(a, p, wait_limit, err_word, st);
+        case 17: return stream_by_width<8, 8>(a, p, wait_limit, err_word, st);
+        case 32: return stream_by_width<16, 1>(a, p, wait_limit, err_word, st);
+        default: return stream_by_width<16, 8>(a, p, wait_limit, err_word, st);
+      }
+    }
+    if (d <= 8 * kNormMaxThreads)
+      norm_launch<0, 1, 8>(a, vec, st);
+    else
+      norm_launch<0, 1, 16>(a, vec, st);
+  }
   return cudaGetLastError();
 }
 

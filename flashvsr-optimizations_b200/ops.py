@@ -597,10 +597,10 @@ def _(x, q1, s1, b1, q2, s2, b2):
 
 # ---------------------------------------------------------------- the block around the linears
 # These operators are called once or more per block and token, where a decode step is bound by
-# its host side: they are defined directly on a torch.library.Library (about 5 us of dispatch a
-# call against 20 us for the decorator's wrapper) and the public functions below add what it
-# leaves out.  Inference only, like the rest: a call that would need a gradient raises when the
-# gradient is asked for.
+# its host side: they are defined directly on a torch.library.Library (about 6 us of dispatch a
+# call against 20 us for the decorator's wrapper), and a plain eager call -- no subclass, no
+# mode, no tracing, no gradient -- runs the implementation without the dispatcher.  Inference
+# only, like the rest: a call that would need a gradient raises when the gradient is asked for.
 _BLOCK_LIB = torch.library.Library("fvq", "FRAGMENT")
 
 
@@ -625,20 +625,32 @@ def _define(schema: str, impl, fake):
     fn = getattr(torch.ops.fvq, name).default
 
     def call(*args):
-        if torch.is_grad_enabled() and any(isinstance(a, torch.Tensor) and a.requires_grad for a in args):
-            return _NoGradient.apply(name, fn, *args)
-        return fn(*args)
+        if torch.compiler.is_compiling():
+            return fn(*args)
+        plain = not (_dispatch_modes() or _function_modes())
+        if plain:
+            for a in args:
+                kind = type(a)
+                if issubclass(kind, torch.Tensor):
+                    if a.requires_grad and torch.is_grad_enabled():
+                        return _NoGradient.apply(name, fn, *args)
+                    plain = plain and (kind is torch.Tensor or kind is torch.nn.Parameter)
+        return impl(*args) if plain else fn(*args)
 
     return call
+
+
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(d).cuda_stream, without its object
 
 
 def _launch(name: str, device: torch.device, *args) -> None:
     """The C entry point on `device`'s current stream, with `device` current."""
     if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+        _lib.call(name, *args, _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
-            _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+            _lib.call(name, *args, _raw_stream(device.index))
 
 
 def _same_device(name: str, x: torch.Tensor, *ts: torch.Tensor | None) -> None:
@@ -680,8 +692,8 @@ def _norm(name: str, x: torch.Tensor, weight: torch.Tensor | None, residual: tor
             raise ValueError(f"{name}: expected a bf16 or fp32 residual of x's shape {tuple(x.shape)}")
         residual = residual.contiguous()
         new = torch.empty_like(residual)
-    out = torch.empty(x.shape, dtype=torch.float8_e4m3fn if fp8 else torch.bfloat16, device=x.device)
-    scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device) if fp8 else None
+    out = x.new_empty(x.shape, dtype=torch.float8_e4m3fn) if fp8 else x.new_empty(x.shape)
+    scale = x.new_empty((*x.shape[:-1], 1), dtype=torch.float32) if fp8 else None
     if rows:
         x, inner, outer, step = _norm_rows(x)
         _launch("fvq_rms_norm", x.device, x.data_ptr(), rows, inner, outer, step, d, _ptr(weight),
@@ -788,7 +800,7 @@ def _linear_act_impl(x, weight, bias, act, gated, residual):
     _check_bf16("linear_act", x)
     _check_bf16("linear_act", weight)
     n, bias, residual, code = _epilogue("linear_act", x, weight, bias, act, gated, residual)
-    y = torch.empty((*x.shape[:-1], n), dtype=torch.bfloat16, device=x.device)
+    y = x.new_empty((*x.shape[:-1], n))
     if y.numel():
         k = x.shape[-1]
         x, m, stride = _matrix(x, 8)
@@ -807,7 +819,7 @@ def _fp8_scaled_mm_act_impl(a, scale_a, w, scale_w, bias, act, gated, residual):
     if scale_a.dtype != torch.float32 or scale_w.dtype != torch.float32 or \
             scale_a.numel() * k != a.numel() or scale_w.numel() != w.shape[0]:
         raise ValueError(f"{name}: expected fp32 scales, one per row of a and one per row of w")
-    y = torch.empty((*a.shape[:-1], n), dtype=torch.bfloat16, device=a.device)
+    y = a.new_empty((*a.shape[:-1], n), dtype=torch.bfloat16)
     if y.numel():
         a, m, stride = _matrix(a, 16)
         scale_a, scale_w, w = scale_a.contiguous(), _aligned16(scale_w), _aligned16(w)
@@ -905,8 +917,8 @@ def _fp8_cache_read_impl(k_codes, k_scale, v_codes, v_scale, page_table, lengths
         raise ValueError(f"{name}: max_len must not be negative")
     batch, per = page_table.shape
     shape = (batch, max_len, heads, d)
-    k = torch.empty(shape, dtype=torch.bfloat16, device=k_codes.device)
-    v = torch.empty(shape, dtype=torch.bfloat16, device=k_codes.device)
+    k = k_codes.new_empty(shape, dtype=torch.bfloat16)
+    v = k_codes.new_empty(shape, dtype=torch.bfloat16)
     if k.numel():
         if per == 0:
             raise ValueError(f"{name}: the page table has no pages")

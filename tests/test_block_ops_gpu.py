@@ -112,6 +112,44 @@ def test_norm_strided_views(d):
     check_norm(qkv[:4, :d].t(), None, None)                       # no adjacent values: copied
 
 
+@pytest.mark.parametrize("rows,d", [(9600, 264), (5001, 1536), (4800, 2047), (4740, 2048), (2400, 2050), (2400, 4096),
+                                    (1300, 5555), (1250, 8960), (650, 12288), (700, 16384), (4737, 301)])
+@pytest.mark.parametrize("residual", [None, BF16, F32])
+def test_norm_many_rows(rows, d, residual):
+    """Enough rows for the streaming form, from storage whose ends are the rows' ends."""
+    x = randn(rows, d, seed=d)
+    r = None if residual is None else randn(rows, d, seed=d + 1, dtype=residual)
+    check_norm(x, r, randn(d, seed=d + 2))
+    if d < 3000:
+        check_norm(x[:, 1:], None if r is None else r[:, 1:], None)
+        check_norm(x.view(-1)[3:3 + (rows - 1) * d].view(rows - 1, d), None, randn(d, seed=d + 3))
+
+
+def test_norm_many_strided_rows():
+    wide = randn(800, 6 * 512 + 24, seed=3)
+    check_norm(wide[:, 8:8 + 6 * 512].unflatten(1, (6, 512)), None, randn(512, seed=4))
+    check_norm(wide[:, 5:5 + 6 * 501].unflatten(1, (6, 501)), randn(800, 6, 501, seed=6), randn(501, seed=4))
+    heads = randn(30000, 3 * 256, seed=5)
+    check_norm(heads[:, 256:].unflatten(1, (4, 128)), None, randn(128, seed=4))
+    check_norm(heads[:, 256:].unflatten(1, (8, 64)), randn(30000, 8, 64, seed=6, dtype=F32), randn(64, seed=4))
+    check_norm(heads[:29999, 3:242], None, randn(239, seed=4))
+    check_norm(wide[0, :300].expand(20000, 300), None, None)
+
+
+def test_norm_wait_limit():
+    """Whether or not a wait runs out of a limit of one test, the rows are waited for."""
+    x, w = randn(60000, 1536, seed=1), randn(1536, seed=2)
+    want = ops.rms_norm(x, w)
+    torch.cuda.synchronize()
+    ops.set_wait_limit(1)
+    try:
+        y = ops.rms_norm(x, w)
+        assert ops.read_device_error() in (0, 1)
+    finally:
+        ops.set_wait_limit(0)
+    assert torch.equal(y, want) and torch.equal(ops.rms_norm(x, w), want)
+
+
 def test_norm_special_rows():
     d = 1536
     x = randn(8, d, seed=4)
