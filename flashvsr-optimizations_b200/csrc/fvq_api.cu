@@ -1122,8 +1122,8 @@ int fvq_fp8_cache_write(const uint16_t* k, const uint16_t* v, int64_t tokens, in
                         int64_t num_slots, void* stream) {
   const char* who = "fvq_fp8_cache_write";
   if (int rc = check_cache(heads, d, num_slots, k_codes, k_scale, v_codes, v_scale, who)) return rc;
-  if (tokens <= 0 || tokens > (int64_t(1) << 31) || tokens * heads > (int64_t(1) << 31))
-    return fail(FVQ_EINVAL, "%s: tokens must be > 0 and tokens * heads at most 2^31 (got %lld)",
+  if (tokens <= 0 || tokens > (int64_t(1) << 30) || tokens * heads > (int64_t(1) << 30))
+    return fail(FVQ_EINVAL, "%s: tokens must be > 0 and tokens * heads at most 2^30 (got %lld)",
                 who, (long long)tokens);
   if (k_token_stride < 0 || k_head_stride < 0 || v_token_stride < 0 || v_head_stride < 0 ||
       (k_token_stride | k_head_stride | v_token_stride | v_head_stride) % 8 != 0)
@@ -1149,15 +1149,15 @@ int fvq_fp8_cache_read(const uint8_t* k_codes, const float* k_scale, const uint8
                        const int32_t* lengths, int64_t max_len, uint16_t* k_out, uint16_t* v_out,
                        void* stream) {
   const char* who = "fvq_fp8_cache_read";
-  if (page <= 0 || page > (int64_t(1) << 31) || num_pages < 0 || num_pages > (int64_t(1) << 31))
+  if (page <= 0 || page > (int64_t(1) << 30) || num_pages < 0 || num_pages > (int64_t(1) << 31))
     return fail(FVQ_EINVAL, "%s: bad page size or count (%lld, %lld)", who, (long long)page,
                 (long long)num_pages);
   if (int rc = check_cache(heads, d, 0, k_codes, k_scale, v_codes, v_scale, who)) return rc;
   if (batch <= 0 || batch > 65535 || pages_per_seq <= 0 || pages_per_seq > (int64_t(1) << 31))
     return fail(FVQ_EINVAL, "%s: batch must be in [1, 65535] and pages_per_seq in [1, 2^31] "
                 "(got %lld, %lld)", who, (long long)batch, (long long)pages_per_seq);
-  if (max_len <= 0 || max_len > (int64_t(1) << 31) || max_len * heads * (d / 8) > (int64_t(1) << 38))
-    return fail(FVQ_EINVAL, "%s: max_len must be positive and max_len * heads * d at most 2^41 "
+  if (max_len <= 0 || max_len > (int64_t(1) << 30) || max_len * heads * (d / 8) > (int64_t(1) << 38))
+    return fail(FVQ_EINVAL, "%s: max_len must be in [1, 2^30] and max_len * heads * d at most 2^41 "
                 "(got %lld)", who, (long long)max_len);
   if (!page_table || !lengths || !k_out || !v_out) return fail(FVQ_EINVAL, "%s: NULL pointer", who);
   if (!aligned16(k_out) || !aligned16(v_out) || !aligned4(page_table) || !aligned4(lengths))

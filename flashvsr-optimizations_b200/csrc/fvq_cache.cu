@@ -4,9 +4,12 @@
 //   write: scale = max(max|x| / 448, 1e-12),  q = e4m3(x * (1 / scale))   per token and head
 //   read:  bf16(q * scale), rows past a sequence's length zero
 //
-// Both are HBM-bound copies with a conversion: keys and values go in one launch, a row of
-// d <= 512 values to a power-of-two group of lanes (8 values a lane, up to two vectors), so
-// that its maximum needs only shuffles.  Slot and page numbers come from the device and are
+// Both are HBM-bound copies with a conversion, keys and values in one launch.  Writing gives
+// a row of d <= 512 values to a power-of-two group of lanes (8 values a lane, up to two
+// vectors), so that its maximum needs only shuffles; reading gives 16 (or 8) codes to a thread,
+// four vectors in flight each.  Row and position arithmetic is 32-bit with multiplications in
+// place of divisions: with 64-bit divisions both were bound by issue slots (reading 4 x 7680
+// tokens of 12 heads of 128 took 78 us).  Slot and page numbers come from the device and are
 // checked there: a negative slot is padding and stores nothing, a slot or page past the store
 // touches nothing (the rows read are zero) and sets a bit of the device error word.
 #include <cuda_bf16.h>
@@ -36,112 +39,189 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// two E4M3 codes -> two fp32 values (exact)
-__device__ __forceinline__ void e4m3x2_to_f32(uint32_t codes, float& lo, float& hi) {
-  uint32_t h2;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(codes)));
-  const __half2 h = *reinterpret_cast<const __half2*>(&h2);
-  lo = __low2float(h);
-  hi = __high2float(h);
+// Division by a fixed divisor, exact below 2^31.
+struct Divider {
+  uint32_t d, mul;
+  int shift;
+};
+
+Divider divider(int64_t d) {
+  Divider r;
+  r.d = static_cast<uint32_t>(d);
+  r.shift = 0;
+  while ((int64_t(1) << r.shift) < d) ++r.shift;
+  r.mul = static_cast<uint32_t>(((uint64_t(1) << 32) * ((uint64_t(1) << r.shift) - static_cast<uint64_t>(d))) /
+                                    static_cast<uint64_t>(d) + 1);
+  return r;
 }
 
-// kLanes lanes a row; blockIdx.y: 0 keys, 1 values.
-template <int kLanes, int kVecs>
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Divider& by) {
+  return (n + __umulhi(n, by.mul)) >> by.shift;
+}
+
+// four E4M3 codes * scale -> four bf16 values (one fp32 product and one rounding each)
+__device__ __forceinline__ uint2 dequantize4(uint32_t codes, float scale) {
+  uint32_t h[2], w[2];
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h[0]) : "h"(static_cast<uint16_t>(codes)));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h[1]) : "h"(static_cast<uint16_t>(codes >> 16)));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(f.y * scale), "f"(f.x * scale));
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// kLanes lanes a row, kRows rows a group, whose loads overlap; blockIdx.y: 0 keys, 1 values.
+template <int kLanes, int kVecs, int kRows>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheWriteArgs a,
+                                                                   const Divider by_heads,
                                                                    uint32_t* err_word) {
   const CacheRows src = blockIdx.y == 0 ? a.k : a.v;
+  constexpr uint32_t kStep = kCacheThreads / kLanes;
   const int lane = threadIdx.x % kLanes;
-  int64_t row = static_cast<int64_t>(blockIdx.x) * (kCacheThreads / kLanes) + threadIdx.x / kLanes;
-  const bool live = row < a.rows;
-  if (!live) row = a.rows - 1;  // whole warps at the shuffles; nothing stored
-  const int64_t token = row / a.heads;
-  const int head = static_cast<int>(row - token * a.heads);
-  const int64_t slot = __ldg(a.slots + token);
-  const uint16_t* x = src.x + token * src.token_stride + head * src.head_stride;
+  const uint32_t first = blockIdx.x * (kStep * kRows) + threadIdx.x / kLanes;
+  const uint32_t rows = static_cast<uint32_t>(a.rows);
   const int nvec = a.d / 8;
-  uint4 v[kVecs];
-  uint32_t m2 = 0;  // max |x|, magnitude bits of the low and high halves (NaN on top)
+  uint4 v[kRows][kVecs];
+  int64_t slot[kRows];
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int j = lane + i * kLanes;
-    v[i] = j < nvec ? __ldg(reinterpret_cast<const uint4*>(x) + j) : make_uint4(0, 0, 0, 0);
-    m2 = max_u16x2(m2, max_u16x2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu));
-    m2 = max_u16x2(m2, max_u16x2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu));
+  for (int k = 0; k < kRows; ++k) {
+    const uint32_t row = min(first + k * kStep, rows - 1);  // whole warps at the shuffles
+    const uint32_t token = divide(row, by_heads), head = row - token * by_heads.d;
+    slot[k] = first + k * kStep < rows ? __ldg(a.slots + token) : -1;
+    const uint4* x = reinterpret_cast<const uint4*>(src.x + token * src.token_stride + head * src.head_stride);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int j = lane + i * kLanes;
+      v[k][i] = j < nvec ? __ldg(x + j) : make_uint4(0, 0, 0, 0);
+    }
   }
-  uint32_t m = max(m2 & 0xFFFFu, m2 >> 16);
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  if (!live || slot < 0) return;
-  if (slot >= a.num_slots) {
-    if (lane == 0 && head == 0 && blockIdx.y == 0) atomicOr(err_word, kErrCacheSlot);
-    return;
-  }
-  const float by448 = __fdiv_rn(__uint_as_float(m << 16), 448.0f);
-  const float scale = by448 < 1e-12f ? 1e-12f : by448;  // NaN stays NaN
-  const float inv = __frcp_rn(scale);
-  const int64_t at = slot * a.heads + head;
-  if (lane == 0) src.scale[at] = scale;
-  uint2* q = reinterpret_cast<uint2*>(src.codes + at * a.d);
+  for (int k = 0; k < kRows; ++k) {
+    uint32_t m2 = 0;  // max |x|, magnitude bits of the low and high halves (NaN on top)
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int j = lane + i * kLanes;
-    if (j >= nvec) continue;
-    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-    uint32_t c[4];
+    for (int i = 0; i < kVecs; ++i) {
+      m2 = max_u16x2(m2, max_u16x2(v[k][i].x & 0x7FFF7FFFu, v[k][i].y & 0x7FFF7FFFu));
+      m2 = max_u16x2(m2, max_u16x2(v[k][i].z & 0x7FFF7FFFu, v[k][i].w & 0x7FFF7FFFu));
+    }
+    uint32_t m = max(m2 & 0xFFFFu, m2 >> 16);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] = e4m3x2(bf_lo(w[e]) * inv, bf_hi(w[e]) * inv);
-    q[j] = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+    for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    const uint32_t row = min(first + k * kStep, rows - 1);
+    const uint32_t head = row - divide(row, by_heads) * by_heads.d;
+    if (slot[k] < 0) continue;
+    if (slot[k] >= a.num_slots) {
+      if (lane == 0 && head == 0 && blockIdx.y == 0) atomicOr(err_word, kErrCacheSlot);
+      continue;
+    }
+    const float by448 = __fdiv_rn(__uint_as_float(m << 16), 448.0f);
+    const float scale = by448 < 1e-12f ? 1e-12f : by448;  // NaN stays NaN
+    const float inv = __frcp_rn(scale);
+    const int64_t at = slot[k] * a.heads + head;
+    if (lane == 0) src.scale[at] = scale;
+    uint2* q = reinterpret_cast<uint2*>(src.codes + at * a.d);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      const int j = lane + i * kLanes;
+      if (j >= nvec) continue;
+      const uint32_t w[4] = {v[k][i].x, v[k][i].y, v[k][i].z, v[k][i].w};
+      uint32_t c[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[e] = e4m3x2(bf_lo(w[e]) * inv, bf_hi(w[e]) * inv);
+      q[j] = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+    }
   }
 }
 
-// One thread per 8 codes; blockIdx.y: sequence, blockIdx.z: 0 keys, 1 values; blockIdx.x
-// walks the sequence's positions x heads x d / 8.
-__global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const CacheReadArgs a,
-                                                                  uint32_t* err_word) {
+// A CTA reads `span` positions of one sequence: their span * heads * d / kCodes vectors, four
+// at a time per thread.  blockIdx.y: sequence, blockIdx.z: 0 keys, 1 values.
+constexpr int kReadUnroll = 4;
+template <int kCodes>
+__global__ void __launch_bounds__(kCacheThreads)
+    cache_read_kernel(const CacheReadArgs a, const int span, const Divider by_token,
+                      const Divider by_row, const Divider by_page, uint32_t* err_word) {
   const bool values = blockIdx.z != 0;
   const uint8_t* codes = values ? a.v_codes : a.k_codes;
   const float* scales = values ? a.v_scale : a.k_scale;
-  uint16_t* out = values ? a.v_out : a.k_out;
   const int64_t b = blockIdx.y;
   const int32_t len_raw = __ldg(a.lengths + b);
   const int64_t most = a.pages_per_seq * a.page < a.max_len ? a.pages_per_seq * a.page : a.max_len;
   const int64_t len = len_raw < most ? len_raw : most;
   if (len_raw > most && blockIdx.x == 0 && threadIdx.x == 0 && !values)
     atomicOr(err_word, kErrCachePage);
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kCacheThreads + threadIdx.x;
-  const int dv = a.d / 8;
-  const int64_t row = i / dv;  // position x heads + head
-  const int64_t pos = row / a.heads;
-  if (pos >= a.max_len) return;
-  uint4 o = make_uint4(0, 0, 0, 0);
-  if (pos < len) {
-    const int64_t p = pos / a.page;
-    const int64_t page = __ldg(a.table + b * a.pages_per_seq + p);
-    if (page >= 0 && page < a.num_pages) {
-      const int64_t at = (page * a.page + (pos - p * a.page)) * a.heads + (row - pos * a.heads);
-      const uint2 c = __ldg(reinterpret_cast<const uint2*>(codes + at * a.d) + (i - row * dv));
-      const float s = __ldg(scales + at);
-      const uint32_t cw[4] = {c.x & 0xFFFFu, c.x >> 16, c.y & 0xFFFFu, c.y >> 16};
-      uint32_t w[4];
+  const int64_t pos0 = static_cast<int64_t>(blockIdx.x) * span;
+  const int64_t left = a.max_len - pos0;  // > 0
+  const uint32_t count = static_cast<uint32_t>(left < span ? left : span) * by_token.d;  // vectors
+  uint16_t* out = (values ? a.v_out : a.k_out) + (b * a.max_len + pos0) * a.heads * a.d;
+  const int32_t* table = a.table + b * a.pages_per_seq;
+  for (uint32_t i0 = threadIdx.x; i0 < count; i0 += kCacheThreads * kReadUnroll) {
+    uint32_t c[kReadUnroll][kCodes / 4];
+    float s[kReadUnroll];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float lo, hi;
-        e4m3x2_to_f32(cw[e], lo, hi);
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[e]) : "f"(hi * s), "f"(lo * s));
+    for (int u = 0; u < kReadUnroll; ++u) {
+      const uint32_t i = i0 + u * kCacheThreads;
+#pragma unroll
+      for (int e = 0; e < kCodes / 4; ++e) c[u][e] = 0;
+      s[u] = 0.0f;
+      if (i >= count) continue;
+      const uint32_t t = divide(i, by_token), vec = i - t * by_token.d;  // vector in the token
+      const uint32_t pos = static_cast<uint32_t>(pos0) + t;              // below 2^31
+      if (pos >= len) continue;
+      const uint32_t p = divide(pos, by_page);
+      const int64_t page = __ldg(table + p);
+      if (page < 0 || page >= a.num_pages) {
+        if (vec == 0 && !values) atomicOr(err_word, kErrCachePage);
+        continue;
       }
-      o = make_uint4(w[0], w[1], w[2], w[3]);
-    } else if (!values) {
-      atomicOr(err_word, kErrCachePage);
+      const int64_t slot = page * a.page + (pos - p * by_page.d);
+      const uint8_t* at = codes + (slot * a.heads * a.d + static_cast<int64_t>(vec) * kCodes);
+      if constexpr (kCodes == 16) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
+        c[u][0] = v.x, c[u][1] = v.y, c[u][2] = v.z, c[u][3] = v.w;
+      } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+        c[u][0] = v.x, c[u][1] = v.y;
+      }
+      s[u] = __ldg(scales + slot * a.heads + divide(vec, by_row));
+    }
+#pragma unroll
+    for (int u = 0; u < kReadUnroll; ++u) {
+      const uint32_t i = i0 + u * kCacheThreads;
+      if (i >= count) continue;
+      uint4* to = reinterpret_cast<uint4*>(out + static_cast<int64_t>(i) * kCodes);
+#pragma unroll
+      for (int e = 0; e < kCodes / 8; ++e) {
+        const uint2 lo = dequantize4(c[u][2 * e], s[u]), hi = dequantize4(c[u][2 * e + 1], s[u]);
+        to[e] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      }
     }
   }
-  reinterpret_cast<uint4*>(out)[b * a.max_len * a.heads * dv + i] = o;
+}
+
+template <int kLanes, int kVecs, int kRows>
+void write_launch(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) {
+  constexpr int kCtaRows = kCacheThreads / kLanes * kRows;
+  const dim3 grid(static_cast<unsigned>((a.rows + kCtaRows - 1) / kCtaRows), 2);
+  cache_write_kernel<kLanes, kVecs, kRows><<<grid, kCacheThreads, 0, st>>>(a, divider(a.heads), err_word);
 }
 
 template <int kLanes, int kVecs>
-void write_launch(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) {
-  constexpr int kRows = kCacheThreads / kLanes;
-  const dim3 grid(static_cast<unsigned>((a.rows + kRows - 1) / kRows), 2);
-  cache_write_kernel<kLanes, kVecs><<<grid, kCacheThreads, 0, st>>>(a, err_word);
+void write_by_rows(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) {
+  // several rows a group once that still leaves every SM two thousand threads
+  if (2 * a.rows * kLanes >= static_cast<int64_t>(sm_count()) * 2048 * 2)
+    write_launch<kLanes, kVecs, 4 / kVecs>(a, err_word, st);
+  else
+    write_launch<kLanes, kVecs, 1>(a, err_word, st);
+}
+
+template <int kCodes>
+void read_launch(const CacheReadArgs& a, uint32_t* err_word, cudaStream_t st) {
+  const int64_t per_token = static_cast<int64_t>(a.heads) * a.d / kCodes;
+  int64_t span = (kCacheThreads * kReadUnroll + per_token - 1) / per_token;
+  const dim3 grid(static_cast<unsigned>((a.max_len + span - 1) / span), static_cast<unsigned>(a.batch), 2);
+  cache_read_kernel<kCodes><<<grid, kCacheThreads, 0, st>>>(a, static_cast<int>(span), divider(per_token),
+                                                            divider(a.d / kCodes), divider(a.page), err_word);
 }
 
 }  // namespace
@@ -149,20 +229,21 @@ void write_launch(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) 
 cudaError_t launch_cache_write(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) {
   if (a.rows <= 0) return cudaSuccess;
   const int nvec = a.d / 8;
-  if (nvec <= 8) write_launch<8, 1>(a, err_word, st);
-  else if (nvec <= 16) write_launch<16, 1>(a, err_word, st);
-  else if (nvec <= 32) write_launch<32, 1>(a, err_word, st);
-  else if (nvec <= 64) write_launch<32, 2>(a, err_word, st);
+  if (nvec <= 8) write_by_rows<8, 1>(a, err_word, st);
+  else if (nvec <= 16) write_by_rows<16, 1>(a, err_word, st);
+  else if (nvec <= 32) write_by_rows<32, 1>(a, err_word, st);
+  else if (nvec <= 64) write_by_rows<32, 2>(a, err_word, st);
   else return cudaErrorInvalidValue;
   return cudaGetLastError();
 }
 
 cudaError_t launch_cache_read(const CacheReadArgs& a, uint32_t* err_word, cudaStream_t st) {
-  const int64_t threads = a.max_len * a.heads * (a.d / 8);
-  if (threads <= 0 || a.batch <= 0) return cudaSuccess;
-  const dim3 grid(static_cast<unsigned>((threads + kCacheThreads - 1) / kCacheThreads),
-                  static_cast<unsigned>(a.batch), 2);
-  cache_read_kernel<<<grid, kCacheThreads, 0, st>>>(a, err_word);
+  if (a.max_len <= 0 || a.batch <= 0) return cudaSuccess;
+  const auto at16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  if (a.d % 16 == 0 && at16(a.k_codes) && at16(a.v_codes))
+    read_launch<16>(a, err_word, st);
+  else
+    read_launch<8>(a, err_word, st);
   return cudaGetLastError();
 }
 

@@ -618,6 +618,7 @@ class _NoGradient(torch.autograd.Function):
 
 
 def _define(schema: str, impl, fake):
+    """Registers fvq::<name>; returns its call for everything but a plain eager call."""
     name = schema.split("(", 1)[0]
     _BLOCK_LIB.define(schema)
     _BLOCK_LIB.impl(name, impl, "CompositeExplicitAutograd")
@@ -625,19 +626,22 @@ def _define(schema: str, impl, fake):
     fn = getattr(torch.ops.fvq, name).default
 
     def call(*args):
-        if torch.compiler.is_compiling():
-            return fn(*args)
-        plain = not (_dispatch_modes() or _function_modes())
-        if plain:
-            for a in args:
-                kind = type(a)
-                if issubclass(kind, torch.Tensor):
-                    if a.requires_grad and torch.is_grad_enabled():
-                        return _NoGradient.apply(name, fn, *args)
-                    plain = plain and (kind is torch.Tensor or kind is torch.nn.Parameter)
-        return impl(*args) if plain else fn(*args)
+        if torch.is_grad_enabled() and any(isinstance(a, torch.Tensor) and a.requires_grad for a in args):
+            return _NoGradient.apply(name, fn, *args)
+        return fn(*args)
 
     return call
+
+
+def _plain(*ts: torch.Tensor | None) -> bool:
+    """A plain eager call: tensors and parameters, no gradient to record, no mode, no tracing."""
+    for t in ts:
+        if t is not None:
+            kind = type(t)
+            if (kind is not torch.Tensor and kind is not torch.nn.Parameter) or \
+                    (t.requires_grad and torch.is_grad_enabled()):
+                return False
+    return not (_dispatch_modes() or _function_modes() or torch.compiler.is_compiling())
 
 
 _dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
@@ -664,8 +668,6 @@ def _norm_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     """(x, inner, outer_stride, inner_stride): x's rows as the kernel walks them; a tensor whose
     rows are no two-level pattern of adjacent values is copied."""
     d = x.shape[-1]
-    if x.is_contiguous():
-        return x, 1, d, 0
     if d == 1 or x.stride(-1) == 1:
         if x.dim() == 2:
             return x, 1, x.stride(0), 0
@@ -678,28 +680,39 @@ def _norm(name: str, x: torch.Tensor, weight: torch.Tensor | None, residual: tor
           eps: float, fp8: bool):
     _same_device(name, x, weight, residual)
     _check_bf16(name, x)
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"{name}: expected rows of at least one value, got shape {tuple(x.shape)}")
-    d = x.shape[-1]
+    shape = x.shape
+    d = shape[-1] if shape else 0
+    if d == 0:
+        raise ValueError(f"{name}: expected rows of at least one value, got shape {tuple(shape)}")
     rows = x.numel() // d
     if weight is not None:
         if weight.dtype != torch.bfloat16 or weight.numel() != d:
             raise ValueError(f"{name}: expected a bf16 weight of {d} values")
-        weight = weight.reshape(-1).contiguous()
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
     new = None
+    f32 = 0
     if residual is not None:
-        if residual.dtype not in (torch.bfloat16, torch.float32) or residual.shape != x.shape:
-            raise ValueError(f"{name}: expected a bf16 or fp32 residual of x's shape {tuple(x.shape)}")
-        residual = residual.contiguous()
+        if residual.dtype == torch.float32:
+            f32 = 1
+        elif residual.dtype != torch.bfloat16:
+            raise ValueError(f"{name}: expected a bf16 or fp32 residual, got {residual.dtype}")
+        if residual.shape != shape:
+            raise ValueError(f"{name}: expected a residual of x's shape {tuple(shape)}")
+        if not residual.is_contiguous():
+            residual = residual.contiguous()
         new = torch.empty_like(residual)
-    out = x.new_empty(x.shape, dtype=torch.float8_e4m3fn) if fp8 else x.new_empty(x.shape)
-    scale = x.new_empty((*x.shape[:-1], 1), dtype=torch.float32) if fp8 else None
-    if rows:
+    if x.is_contiguous():
+        inner, outer, step = 1, d, 0
+        out = torch.empty_like(x, dtype=torch.float8_e4m3fn) if fp8 else torch.empty_like(x)
+    else:
         x, inner, outer, step = _norm_rows(x)
-        _launch("fvq_rms_norm", x.device, x.data_ptr(), rows, inner, outer, step, d, _ptr(weight),
-                eps, _ptr(residual), 1 if new is not None and new.dtype == torch.float32 else 0,
-                _ptr(new), None if fp8 else out.data_ptr(), out.data_ptr() if fp8 else None,
-                _ptr(scale))
+        out = x.new_empty(shape, dtype=torch.float8_e4m3fn if fp8 else torch.bfloat16)
+    scale = x.new_empty((*shape[:-1], 1), dtype=torch.float32) if fp8 else None
+    if rows:
+        q = out.data_ptr()
+        _launch("fvq_rms_norm", x.device, x.data_ptr(), rows, inner, outer, step, d, _ptr(weight), eps,
+                _ptr(residual), f32, _ptr(new), None if fp8 else q, q if fp8 else None, _ptr(scale))
     return out, scale, new
 
 
@@ -731,6 +744,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1
 
     x: bf16 [..., d], d <= 16384; views of two or three dimensions with adjacent values (heads
     inside a fused projection's rows) are read in place.  weight: bf16 [d] or None (ones)."""
+    if _plain(x, weight):
+        return _norm("rms_norm", x, weight, None, eps, False)[0]
     return _rms_norm(x, weight, eps)
 
 
@@ -739,6 +754,8 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor |
     """(rms_norm(s), s) with s = x + residual: the branch's output joins the stream and the next
     branch's input is normalised in one pass.  residual: bf16 or fp32, x's shape; s is returned in
     its type, and normalised before that rounding."""
+    if _plain(x, residual, weight):
+        return _norm("add_rms_norm", x, weight, residual, eps, False)[::2]
     return _add_rms_norm(x, residual, weight, eps)
 
 
@@ -747,12 +764,16 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor | None = None,
     """(q float8_e4m3fn like x, scale fp32 [..., 1]): rms_norm's fp32 value v quantized with one scale
     per row, scale = max(max|v| / 448, 1e-12), q = v / scale -- the input of ``fp8_scaled_mm`` and
     ``fp8_scaled_mm_act`` without a bf16 copy in between."""
+    if _plain(x, weight):
+        return _norm("rms_norm_fp8", x, weight, None, eps, True)[:2]
     return _rms_norm_fp8(x, weight, eps)
 
 
 def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
                      eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(q, scale, s): ``rms_norm_fp8`` of s = x + residual, and s (see ``add_rms_norm``)."""
+    if _plain(x, residual, weight):
+        return _norm("add_rms_norm_fp8", x, weight, residual, eps, True)
     return _add_rms_norm_fp8(x, residual, weight, eps)
 
 
@@ -787,11 +808,13 @@ def _epilogue(name, x, weight, bias, act, gated, residual):
     if bias is not None:
         if bias.dtype != torch.bfloat16 or bias.numel() != wn:
             raise ValueError(f"{name}: expected a bf16 bias of {wn} values")
-        bias = _aligned16(bias)
+        if not bias.is_contiguous() or bias.data_ptr() % 16:
+            bias = _aligned16(bias)
     if residual is not None:
         if residual.dtype != torch.bfloat16 or residual.shape != (*x.shape[:-1], n):
             raise ValueError(f"{name}: expected a bf16 residual of shape {(*x.shape[:-1], n)}")
-        residual = _aligned16(residual)
+        if not residual.is_contiguous() or residual.data_ptr() % 16:
+            residual = _aligned16(residual)
     return n, bias, residual, ACTIVATIONS[act]
 
 
@@ -854,7 +877,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     fp32 accumulation and epilogue, one rounding.  x: bf16 [..., k] (rows may be strided), weight
     in nn.Linear's layout, k and n multiples of 8; act: one of ``ACTIVATIONS`` ("gelu" is the erf
     form).  From one row to many: few rows run on a kernel bound by reading the weight once."""
-    return _linear_act(x, weight, bias, act, gated, residual)
+    call = _linear_act_impl if _plain(x, weight, bias, residual) else _linear_act
+    return call(x, weight, bias, act, gated, residual)
 
 
 def fp8_scaled_mm_act(a: torch.Tensor, scale_a: torch.Tensor, w: torch.Tensor, scale_w: torch.Tensor,
@@ -863,26 +887,32 @@ def fp8_scaled_mm_act(a: torch.Tensor, scale_a: torch.Tensor, w: torch.Tensor, s
     """``linear_act`` with E4M3 operands and one fp32 scale per row of each (those of
     ``fp8_row_quant``, ``rms_norm_fp8`` and ``QuantLinear(mode='fp8')``):
     z = (a @ w^T) * scale_a * scale_w + bias.  k a multiple of 16, n of 8."""
-    return _fp8_scaled_mm_act(a, scale_a, w, scale_w, bias, act, gated, residual)
+    call = _fp8_scaled_mm_act_impl if _plain(a, scale_a, w, scale_w, bias, residual) else _fp8_scaled_mm_act
+    return call(a, scale_a, w, scale_w, bias, act, gated, residual)
 
 
 # ---------------------------------------------------------------- paged FP8 keys and values
 def _check_cache(name, k_codes, k_scale, v_codes, v_scale):
     _check_fp8(name, k_codes, v_codes)
-    if k_codes.dim() != 4 or v_codes.shape != k_codes.shape or \
-            k_scale.shape != k_codes.shape[:3] or v_scale.shape != k_codes.shape[:3] or \
+    shape = k_codes.shape
+    rows = shape[:3]
+    if len(shape) != 4 or v_codes.shape != shape or k_scale.shape != rows or v_scale.shape != rows or \
             k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
         raise ValueError(f"{name}: expected codes [pages, page, heads, d] and fp32 scales "
                          "[pages, page, heads], the same for keys and values")
     if not (k_codes.is_contiguous() and v_codes.is_contiguous() and k_scale.is_contiguous()
             and v_scale.is_contiguous()):
         raise ValueError(f"{name}: the store's tensors must be contiguous")
+    return shape
 
 
-def _cache_rows(x: torch.Tensor) -> torch.Tensor:
-    if x.stride(-1) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.data_ptr() % 16 == 0:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+def _cache_rows(x: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """(x, stride between tokens, stride between heads); copied when the kernel cannot read it."""
+    token, head, one = x.stride()
+    if one != 1 or token % 8 or head % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        token, head, one = x.stride()
+    return x, token, head
 
 
 def _fp8_cache_write_impl(k, v, slots, k_codes, k_scale, v_codes, v_scale):
@@ -890,26 +920,25 @@ def _fp8_cache_write_impl(k, v, slots, k_codes, k_scale, v_codes, v_scale):
     _same_device(name, k, v, slots, k_codes, k_scale, v_codes, v_scale)
     _check_bf16(name, k)
     _check_bf16(name, v)
-    _check_cache(name, k_codes, k_scale, v_codes, v_scale)
-    pages, page, heads, d = k_codes.shape
+    pages, page, heads, d = _check_cache(name, k_codes, k_scale, v_codes, v_scale)
     if k.dim() != 3 or k.shape[1:] != (heads, d) or v.shape != k.shape:
         raise ValueError(f"{name}: expected k and v [tokens, {heads}, {d}], got {tuple(k.shape)} and "
                          f"{tuple(v.shape)}")
     if slots.dtype != torch.int64 or slots.shape != (k.shape[0],):
         raise ValueError(f"{name}: expected int64 slots, one per token")
     if k.numel():
-        k, v, slots = _cache_rows(k), _cache_rows(v), slots.contiguous()
+        k, k_token, k_head = _cache_rows(k)
+        v, v_token, v_head = _cache_rows(v)
+        slots = slots.contiguous()
         _launch("fvq_fp8_cache_write", k.device, k.data_ptr(), v.data_ptr(), k.shape[0], heads, d,
-                k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(),
-                k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(),
+                k_token, k_head, v_token, v_head, slots.data_ptr(), k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(),
                 pages * page)
 
 
 def _fp8_cache_read_impl(k_codes, k_scale, v_codes, v_scale, page_table, lengths, max_len):
     name = "fp8_cache_read"
     _same_device(name, k_codes, k_scale, v_codes, v_scale, page_table, lengths)
-    _check_cache(name, k_codes, k_scale, v_codes, v_scale)
-    pages, page, heads, d = k_codes.shape
+    pages, page, heads, d = _check_cache(name, k_codes, k_scale, v_codes, v_scale)
     if page_table.dtype != torch.int32 or lengths.dtype != torch.int32 or page_table.dim() != 2 or \
             lengths.shape != page_table.shape[:1]:
         raise ValueError(f"{name}: expected an int32 page table [batch, pages] and int32 lengths [batch]")
@@ -918,7 +947,7 @@ def _fp8_cache_read_impl(k_codes, k_scale, v_codes, v_scale, page_table, lengths
     batch, per = page_table.shape
     shape = (batch, max_len, heads, d)
     k = k_codes.new_empty(shape, dtype=torch.bfloat16)
-    v = k_codes.new_empty(shape, dtype=torch.bfloat16)
+    v = torch.empty_like(k)
     if k.numel():
         if per == 0:
             raise ValueError(f"{name}: the page table has no pages")
@@ -954,7 +983,8 @@ def fp8_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cod
     head, scale = max(max|x| / 448, 1e-12), q = x / scale.  A negative slot is padding (nothing is
     stored); one past the store is skipped and sets bit 6 of ``read_device_error()``.  The slots
     of one call must differ: what a repeated slot then holds is undefined."""
-    _fp8_cache_write(k, v, slots, k_codes, k_scale, v_codes, v_scale)
+    plain = _plain(k, v, slots, k_codes, k_scale, v_codes, v_scale)
+    (_fp8_cache_write_impl if plain else _fp8_cache_write)(k, v, slots, k_codes, k_scale, v_codes, v_scale)
 
 
 def fp8_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor,
@@ -964,7 +994,9 @@ def fp8_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.
     [batch, pages]) lists in order: bf16(q * scale) below lengths[b] (int32), zero from there on.
     A page outside the store, or a length past max_len or past the table, reads as zeros and sets
     bit 7 of ``read_device_error()``."""
-    return _fp8_cache_read(k_codes, k_scale, v_codes, v_scale, page_table, lengths, max_len)
+    plain = _plain(k_codes, k_scale, v_codes, v_scale, page_table, lengths)
+    call = _fp8_cache_read_impl if plain else _fp8_cache_read
+    return call(k_codes, k_scale, v_codes, v_scale, page_table, lengths, max_len)
 
 
 def div_full_probe(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
