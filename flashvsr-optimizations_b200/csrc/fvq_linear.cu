@@ -64,15 +64,6 @@ __device__ __forceinline__ float activate(float z) {
   }
 }
 
-__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
 // ---------------------------------------------------------------- MMA
 template <bool kF8>
 __device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
@@ -137,10 +128,12 @@ constexpr int kPairStageBytes = kPairABytes + kPairBBytes;
 constexpr int kPairStages = 5;
 constexpr int kPairEpiWarps = 8;                  // two per TMEM lane quadrant
 constexpr int kPairThreads = 64 + 32 * kPairEpiWarps;
-constexpr int kChunk = 64;                        // output columns staged at a time (128 bytes)
+constexpr int kChunk = 32;                        // output columns staged at a time (64 bytes)
 constexpr int kChunkBytes = 32 * kChunk * 2;      // of one warp's 32 rows
+constexpr int kParamBytes = kChunk * 2 * 8;       // a chunk's scales and biases, both halves of a gate
 constexpr int kPairStagingOff = kPairStages * kPairStageBytes;
-constexpr int kPairBarrierOff = kPairStagingOff + kPairEpiWarps * 2 * kChunkBytes;
+constexpr int kPairParamOff = kPairStagingOff + kPairEpiWarps * 2 * kChunkBytes;
+constexpr int kPairBarrierOff = kPairParamOff + kPairEpiWarps * kParamBytes;
 constexpr int kPairSmemBytes = kPairBarrierOff + 512;
 constexpr int kAccCols = 256;                     // TMEM columns per accumulator
 static_assert(kPairSmemBytes <= 232448, "pair plan exceeds shared memory");
@@ -169,53 +162,72 @@ struct LinearArgs {
   uint32_t* err_word;
 };
 
-// 32 accumulator columns of one row -> z = acc [* sx * sw] + b.  `col`: first W row index;
-// `left`: how many of the 32 are inside the matrix (a multiple of 8).
+// Scales and biases of 32 W rows, one per lane, on their way to shared memory: fetched a chunk
+// ahead, so that their latency (an L2 miss for every new tile) is off the epilogue's path.
+struct ColumnParam {
+  float scale, bias;
+};
+
 template <bool kF8>
-__device__ __forceinline__ void affine32(uint32_t (&r)[32], float sx, const float* sw,
-                                         const uint16_t* bias, int col, int left) {
+__device__ __forceinline__ ColumnParam column_param(const LinearArgs& a, int row, bool inside) {
+  ColumnParam c = {1.0f, 0.0f};
+  if (inside) {
+    if constexpr (kF8) c.scale = __ldg(a.sw + row);
+    if (a.bias != nullptr) c.bias = __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + row)) << 16);
+  }
+  return c;
+}
+
+// Shared-memory layout of 32 columns: E4M3 16 bytes per column pair (two scales, two biases),
+// bf16 the 32 biases.
+template <bool kF8>
+__device__ __forceinline__ void put_param(float* at, int lane, ColumnParam c) {
+  if constexpr (kF8) {
+    at[(lane >> 1) * 4 + (lane & 1)] = c.scale;
+    at[(lane >> 1) * 4 + 2 + (lane & 1)] = c.bias;
+  } else {
+    at[lane] = c.bias;
+  }
+}
+
+// 32 accumulator columns of one row -> z = acc [* sx * sw] + b, in pairs.
+template <bool kF8>
+__device__ __forceinline__ void affine32(const uint32_t (&r)[32], uint64_t sx2, const float* param,
+                                         uint64_t (&z)[16]) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (8 * q < left) {
-      if constexpr (kF8) {
-        const float4 s0 = __ldg(reinterpret_cast<const float4*>(sw + col) + 2 * q);
-        const float4 s1 = __ldg(reinterpret_cast<const float4*>(sw + col) + 2 * q + 1);
-        const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          r[8 * q + j] = __float_as_uint(__uint_as_float(r[8 * q + j]) * sx * s[j]);
-      }
-      if (bias != nullptr) {
-        const uint4 b = __ldg(reinterpret_cast<const uint4*>(bias + col) + q);
-        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          r[8 * q + 2 * j] = __float_as_uint(__uint_as_float(r[8 * q + 2 * j]) + bf_lo(w[j]));
-          r[8 * q + 2 * j + 1] = __float_as_uint(__uint_as_float(r[8 * q + 2 * j + 1]) + bf_hi(w[j]));
-        }
-      }
+  for (int i = 0; i < 16; ++i) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(r[2 * i]), "r"(r[2 * i + 1]));
+    if constexpr (kF8) {
+      const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(param + 4 * i);
+      z[i] = f2_fma(f2_mul(v, sx2), c.x, c.y);
+    } else {
+      z[i] = f2_add(v, *reinterpret_cast<const uint64_t*>(param + 2 * i));
     }
   }
 }
 
 template <int kAct, bool kGated>
-__device__ __forceinline__ void act32_t(uint32_t (&r)[32], const uint32_t (&u)[32]) {
+__device__ __forceinline__ void act32_t(uint64_t (&z)[16], const uint64_t (&u)[16]) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    float h = activate<kAct>(__uint_as_float(r[j]));
-    if constexpr (kGated) h *= __uint_as_float(u[j]);
-    r[j] = __float_as_uint(h);
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (kAct != kActNone) {
+      float lo, hi;
+      f2_split(z[i], lo, hi);
+      z[i] = f2_pack(activate<kAct>(lo), activate<kAct>(hi));
+    }
+    if constexpr (kGated) z[i] = f2_mul(z[i], u[i]);
   }
 }
 
 template <bool kGated>
-__device__ __forceinline__ void act32(int act, uint32_t (&r)[32], const uint32_t (&u)[32]) {
+__device__ __forceinline__ void act32(int act, uint64_t (&z)[16], const uint64_t (&u)[16]) {
   switch (act) {
-    case kActRelu: act32_t<kActRelu, kGated>(r, u); break;
-    case kActGelu: act32_t<kActGelu, kGated>(r, u); break;
-    case kActGeluTanh: act32_t<kActGeluTanh, kGated>(r, u); break;
-    case kActSilu: act32_t<kActSilu, kGated>(r, u); break;
-    default: act32_t<kActNone, kGated>(r, u); break;
+    case kActRelu: act32_t<kActRelu, kGated>(z, u); break;
+    case kActGelu: act32_t<kActGelu, kGated>(z, u); break;
+    case kActGeluTanh: act32_t<kActGeluTanh, kGated>(z, u); break;
+    case kActSilu: act32_t<kActSilu, kGated>(z, u); break;
+    default: act32_t<kActNone, kGated>(z, u); break;
   }
 }
 
@@ -375,14 +387,17 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
-    // Warp w: TMEM lanes 32 * (w % 4).., every second 64-column chunk of the tile.  A chunk
+    // Warp w: TMEM lanes 32 * (w % 4).., every second 32-column chunk of the tile.  A chunk
     // goes through one of the warp's two staging buffers: the residual chunk is loaded into
     // it, the results take its place and leave by a TMA store (which also clips the edges).
     const int quad = warp & 3, half = (warp - 2) >> 2;
     const int trow = quad * 32 + lane;
     uint8_t* staging = smem + kPairStagingOff + (warp - 2) * 2 * kChunkBytes;
+    float* param = reinterpret_cast<float*>(smem + kPairParamOff + (warp - 2) * kParamBytes);
+    float* param_u = param + (kF8 ? 2 : 1) * kChunk;
     uint64_t* res_full = bars->res_full[warp - 2];
     const int chunks = out_cols / kChunk;
+    const uint32_t swizzle = (lane >> 1) & 3u;  // 64B swizzle of row `lane`
     uint32_t uses = 0;  // chunks through the staging buffers so far
     bool ok = true;
     for (int i = 0; ok && i < count; ++i) {
@@ -391,12 +406,26 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int row0 = mb * kPairTokens + static_cast<int>(rank) * 128 + quad * 32;
       const int row = mb * kPairTokens + static_cast<int>(rank) * 128 + trow;
       const float sx = kF8 && row < a.m ? __ldg(a.sx + row) : 0.0f;
+      const uint64_t sx2 = f2_pack(sx, sx);
       const int buf = i & 1;
+      const int tile_col = nb * out_cols;
+      const auto fetch = [&](int c, ColumnParam& g, ColumnParam& u) {
+        const int col = tile_col + c * kChunk + lane;
+        const bool in = c < chunks && col < a.n;
+        g = column_param<kF8>(a, col, in);
+        if constexpr (kGated) u = column_param<kF8>(a, a.n + col, in);
+      };
+      ColumnParam pg, pu;
+      fetch(half, pg, pu);
       bool waited = false;
       for (int c = half; c < chunks; c += 2) {
-        const int col0 = nb * out_cols + c * kChunk;
+        const int col0 = tile_col + c * kChunk;
         const bool inside = col0 < a.n && row0 < a.m;  // warp-uniform
         uint8_t* stage_buf = staging + (uses & 1u) * kChunkBytes;
+        __syncwarp();  // the previous chunk's parameters have been read
+        put_param<kF8>(param, lane, pg);
+        if constexpr (kGated) put_param<kF8>(param_u, lane, pu);
+        fetch(c + 2, pg, pu);
         if (inside) {
           // at most one committed store (of the other buffer) may still be reading
           if (lane == 0) {
@@ -406,8 +435,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
               tma_load_2d(stage_buf, &tmap_r, &res_full[uses & 1u], col0, row0);
             }
           }
-          __syncwarp();
         }
+        __syncwarp();
         if (!waited) {
           if (!mbar_wait_cluster_bounded(&bars->acc_full[buf], static_cast<uint32_t>(i >> 1) & 1u,
                                          wait_limit)) {
@@ -418,6 +447,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           tc_fence_after();
           waited = true;
         }
+        uint32_t r[32], v[32];
+        const uint32_t taddr = tmem + static_cast<uint32_t>(buf * kAccCols + c * kChunk) +
+                               (static_cast<uint32_t>(quad * 32) << 16);
+        if (ok && inside) {
+          tmem_ld_32x32b_x32(taddr, r);
+          if constexpr (kGated) tmem_ld_32x32b_x32(taddr + out_cols, v);
+        }
         if (inside && a.residual) {
           // a residual load in flight has to land before its buffer is used or the CTA exits
           if (!mbar_wait_bounded(&res_full[uses & 1u], (uses >> 1) & 1u, teardown_limit)) {
@@ -426,43 +462,26 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
           ok = __all_sync(0xFFFFFFFFu, ok);
         }
+        tmem_ld_wait();
         if (!ok) break;
         if (!inside) continue;
-        const uint32_t taddr = tmem + static_cast<uint32_t>(buf * kAccCols + c * kChunk) +
-                               (static_cast<uint32_t>(quad * 32) << 16);
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const int col = col0 + 32 * h;
-          uint32_t r[32], u[32];
-          tmem_ld_32x32b_x32(taddr + 32 * h, r);
-          if constexpr (kGated) tmem_ld_32x32b_x32(taddr + 32 * h + out_cols, u);
-          tmem_ld_wait();
-          affine32<kF8>(r, sx, a.sw, a.bias, col, a.n - col);
-          if constexpr (kGated)
-            affine32<kF8>(u, sx, a.sw + a.n, a.bias == nullptr ? nullptr : a.bias + a.n, col,
-                          a.n - col);
-          act32<kGated>(a.act, r, u);
-          // 16-byte chunk q of row l sits at l * 128 + ((q ^ (l & 7)) * 16) (128B swizzle)
+        uint64_t z[16], u[16];
+        affine32<kF8>(r, sx2, param, z);
+        if constexpr (kGated) affine32<kF8>(v, sx2, param_u, u);
+        act32<kGated>(a.act, z, u);
+        // 16-byte piece q of row l sits at l * 64 + ((q ^ ((l >> 1) & 3)) * 16)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint4* at = reinterpret_cast<uint4*>(stage_buf + lane * 128 +
-                                                 (((4 * h + q) ^ (lane & 7)) * 16));
-            uint32_t o[4];
-            if (a.residual) {
-              const uint4 v = *at;
-              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                o[j] = pack_bf16x2(__uint_as_float(r[8 * q + 2 * j]) + bf_lo(w[j]),
-                                   __uint_as_float(r[8 * q + 2 * j + 1]) + bf_hi(w[j]));
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                o[j] = pack_bf16x2(__uint_as_float(r[8 * q + 2 * j]),
-                                   __uint_as_float(r[8 * q + 2 * j + 1]));
-            }
-            *at = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int q = 0; q < 4; ++q) {
+          uint4* at = reinterpret_cast<uint4*>(stage_buf + lane * 64 + ((q ^ swizzle) * 16));
+          if (a.residual) {
+            const uint4 w = *at;
+            z[4 * q] = f2_add(z[4 * q], f2_of_bf16x2(w.x));
+            z[4 * q + 1] = f2_add(z[4 * q + 1], f2_of_bf16x2(w.y));
+            z[4 * q + 2] = f2_add(z[4 * q + 2], f2_of_bf16x2(w.z));
+            z[4 * q + 3] = f2_add(z[4 * q + 3], f2_of_bf16x2(w.w));
           }
+          *at = make_uint4(f2_to_bf16x2(z[4 * q]), f2_to_bf16x2(z[4 * q + 1]),
+                           f2_to_bf16x2(z[4 * q + 2]), f2_to_bf16x2(z[4 * q + 3]));
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -495,6 +514,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
 // ---------------------------------------------------------------- few tokens
 constexpr int kSplitStagesMax = 16;
+constexpr int kSplitMax = 8;                      // CTAs per cluster (the portable limit)
 constexpr int kSplitThreads = 320;                // producer, MMA issuer, eight epilogue warps
 constexpr int kSplitBarrierBytes = 512;
 // An MMA reads 128 W rows; a tile of fewer rows is followed by whatever comes next in shared
@@ -517,7 +537,7 @@ struct SplitBars {
 static_assert(sizeof(SplitBars) <= kSplitBarrierBytes, "split barrier area");
 
 struct SplitPlan {
-  int wr;         // W rows per CTA: 32, 64 or 128 (gated: half of them Wg rows, half Wu rows)
+  int wr;         // W rows per CTA: 64 or 128 (gated: half of them Wg rows, half Wu rows)
   int tn;         // tokens per CTA: a multiple of 16, at most 256
   int split;      // CTAs per cluster sharing one tile's K
   int group;      // K tiles per stage
@@ -574,20 +594,45 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   uint32_t cols = 32;
   while (static_cast<int>(cols) < p.tn) cols *= 2;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&bars->full[s], 1);
-      mbar_init(&bars->empty[s], 1);
+  const int k_step = kF8 ? kKB : kKB / 2;
+  const auto fill = [&](int i, int stage) {  // one lane: the copies of step i into its stage
+    const int kt = kt0 + i * p.group;
+    const int g = min(p.group, kt1 - kt);
+    uint8_t* sw = smem + stage * stage_bytes;
+    uint64_t* full = &bars->full[stage];
+    mbar_arrive_expect_tx(full, (w_bytes + x_bytes) * g);
+    for (int j = 0; j < g; ++j) {
+      uint8_t* at = sw + j * w_bytes;
+      const int k = (kt + j) * k_step;
+      if (gated) {  // boxes of wr / 2 rows: Wg, then the same columns' Wu
+        tma_load_2d(at, &tmap_w, full, k, nb * out_rows);
+        tma_load_2d(at + w_bytes / 2, &tmap_w, full, k, a.n + nb * out_rows);
+      } else {
+        tma_load_2d(at, &tmap_w, full, k, nb * out_rows);
+      }
+      tma_load_2d(sw + p.group * w_bytes + j * x_bytes, &tmap_x, full, k, mb * p.tn);
     }
-    mbar_init(&bars->acc_full, 1);
-    mbar_init(&bars->teardown, 1);
-    bars->abort_flag = 0;
+  };
+
+  // The ring's first fill is under way before the rest of the CTA is set up.
+  const int ahead = min(steps, p.stages);
+  if (warp == 0) {
+    if (lane < p.stages) {
+      mbar_init(&bars->full[lane], 1);
+      mbar_init(&bars->empty[lane], 1);
+    }
+    if (lane == 31) {
+      mbar_init(&bars->acc_full, 1);
+      mbar_init(&bars->teardown, 1);
+      bars->abort_flag = 0;
+    }
     fence_barrier_init();
     fence_proxy_async_smem();
-    prefetch_tmap(&tmap_x);
-    prefetch_tmap(&tmap_w);
-  }
-  if (warp == 1) {
+    __syncwarp();
+    if (elect_one())
+      for (int i = 0; i < ahead; ++i) fill(i, i);
+    __syncwarp();
+  } else if (warp == 1) {
     tmem_alloc(&bars->tmem_base, cols);
     tmem_relinquish();
   }
@@ -598,32 +643,15 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    const int k_step = kF8 ? kKB : kKB / 2;
-    int stage = 0;
-    uint32_t phase = 0, filled = 0;
-    for (int i = 0; i < steps; ++i) {
+    int stage = ahead == p.stages ? 0 : ahead;
+    uint32_t phase = ahead == p.stages ? 1u : 0u;
+    uint32_t filled = static_cast<uint32_t>(ahead);
+    for (int i = ahead; i < steps; ++i) {
       if (!warp_wait_bounded(&bars->empty[stage], phase ^ 1u, wait_limit)) {
         warp_flag(abort_flag, a.err_word, kErrWaitProducer);
         break;
       }
-      const int kt = kt0 + i * p.group;
-      const int g = min(p.group, kt1 - kt);
-      uint8_t* sw = smem + stage * stage_bytes;
-      uint64_t* full = &bars->full[stage];
-      if (elect_one()) {
-        mbar_arrive_expect_tx(full, (w_bytes + x_bytes) * g);
-        for (int j = 0; j < g; ++j) {
-          uint8_t* at = sw + j * w_bytes;
-          const int k = (kt + j) * k_step;
-          if (gated) {  // boxes of wr / 2 rows: Wg, then the same columns' Wu
-            tma_load_2d(at, &tmap_w, full, k, nb * out_rows);
-            tma_load_2d(at + w_bytes / 2, &tmap_w, full, k, a.n + nb * out_rows);
-          } else {
-            tma_load_2d(at, &tmap_w, full, k, nb * out_rows);
-          }
-          tma_load_2d(sw + p.group * w_bytes + j * x_bytes, &tmap_x, full, k, mb * p.tn);
-        }
-      }
+      if (elect_one()) fill(i, stage);
       __syncwarp();
       filled = i + 1;
       if (++stage == p.stages) {
@@ -710,44 +738,62 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   // This CTA's share of the tile's tokens; four output columns per thread, the ranks' partial
   // sums added in rank order.
   const int t0 = p.tn * rank / split, t1 = p.tn * (rank + 1) / split;
-  const int quads = out_rows / 4;
+  const int quad_shift = 31 - __clz(out_rows / 4);  // out_rows is a power of two
   const uint32_t part_addr = smem_u32(part);
   const bool good = *reinterpret_cast<volatile int*>(abort_flag) == 0;
-  for (int i = threadIdx.x; good && i < (t1 - t0) * quads; i += kSplitThreads) {
-    const int t = t0 + i / quads, row = (i % quads) * 4;
+  for (int i = threadIdx.x; good && i < (t1 - t0) << quad_shift; i += kSplitThreads) {
+    const int t = t0 + (i >> quad_shift), row = (i & ((1 << quad_shift) - 1)) * 4;
     const int token = mb * p.tn + t, col = nb * out_rows + row;
     if (token >= a.m || col >= a.n) continue;
-    const uint32_t at = part_addr + static_cast<uint32_t>((t * p.wr + row) * 4);
-    float z[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int q = 0; q < split; ++q) {
-      const uint32_t peer = mapa_shared(at, static_cast<uint32_t>(q));
-      const float4 v = ld_cluster_f4(peer);
-      z[0] += v.x, z[1] += v.y, z[2] += v.z, z[3] += v.w;
-      if (gated) {
-        const float4 g = ld_cluster_f4(peer + static_cast<uint32_t>(out_rows * 4));
-        u[0] += g.x, u[1] += g.y, u[2] += g.z, u[3] += g.w;
-      }
-    }
-    const float sx = kF8 ? __ldg(a.sx + token) : 1.0f;
-    float o[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (kF8) z[j] = z[j] * sx * __ldg(a.sw + col + j);
-      if (a.bias != nullptr) z[j] += __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + col + j)) << 16);
-      o[j] = activate_any(a.act, z[j]);
-      if (gated) {
-        if constexpr (kF8) u[j] = u[j] * sx * __ldg(a.sw + a.n + col + j);
-        if (a.bias != nullptr)
-          u[j] += __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + a.n + col + j)) << 16);
-        o[j] *= u[j];
-      }
-    }
     const int64_t dst = static_cast<int64_t>(token) * a.n + col;
-    if (residual != nullptr) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(residual + dst));
-      o[0] += bf_lo(v.x), o[1] += bf_hi(v.x), o[2] += bf_lo(v.y), o[3] += bf_hi(v.y);
+    uint2 res = make_uint2(0, 0), bg = make_uint2(0, 0), bu = make_uint2(0, 0);
+    float4 sg = make_float4(1.0f, 1.0f, 1.0f, 1.0f), su = sg;
+    float sx = 1.0f;
+    if (residual != nullptr) res = __ldg(reinterpret_cast<const uint2*>(residual + dst));
+    if (a.bias != nullptr) {
+      bg = __ldg(reinterpret_cast<const uint2*>(a.bias + col));
+      if (gated) bu = __ldg(reinterpret_cast<const uint2*>(a.bias + a.n + col));
     }
-    *reinterpret_cast<uint2*>(y + dst) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    if constexpr (kF8) {
+      sx = __ldg(a.sx + token);
+      sg = __ldg(reinterpret_cast<const float4*>(a.sw + col));
+      if (gated) su = __ldg(reinterpret_cast<const float4*>(a.sw + a.n + col));
+    }
+    const uint32_t at = part_addr + static_cast<uint32_t>((t * p.wr + row) * 4);
+    const auto total = [&](uint32_t where) {  // the ranks' sums in rank order, loads first
+      float4 v[kSplitMax];
+#pragma unroll
+      for (int q = 0; q < kSplitMax; ++q)
+        if (q < split) v[q] = ld_cluster_f4(mapa_shared(where, static_cast<uint32_t>(q)));
+      float4 z = v[0];
+#pragma unroll
+      for (int q = 1; q < kSplitMax; ++q)
+        if (q < split) z.x += v[q].x, z.y += v[q].y, z.z += v[q].z, z.w += v[q].w;
+      return z;
+    };
+    const auto affine = [&](float4 v, float4 scale, uint2 bias, uint64_t (&z)[2]) {
+      z[0] = f2_pack(v.x, v.y);
+      z[1] = f2_pack(v.z, v.w);
+      if constexpr (kF8) {
+        z[0] = f2_mul(f2_mul(z[0], f2_pack(sx, sx)), f2_pack(scale.x, scale.y));
+        z[1] = f2_mul(f2_mul(z[1], f2_pack(sx, sx)), f2_pack(scale.z, scale.w));
+      }
+      z[0] = f2_add(z[0], f2_of_bf16x2(bias.x));
+      z[1] = f2_add(z[1], f2_of_bf16x2(bias.y));
+    };
+    uint64_t z[2], u[2];
+    affine(total(at), sg, bg, z);
+    if (gated) affine(total(at + static_cast<uint32_t>(out_rows * 4)), su, bu, u);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float lo, hi;
+      f2_split(z[j], lo, hi);
+      z[j] = f2_pack(activate_any(a.act, lo), activate_any(a.act, hi));
+      if (gated) z[j] = f2_mul(z[j], u[j]);
+    }
+    z[0] = f2_add(z[0], f2_of_bf16x2(res.x));
+    z[1] = f2_add(z[1], f2_of_bf16x2(res.y));
+    *reinterpret_cast<uint2*>(y + dst) = make_uint2(f2_to_bf16x2(z[0]), f2_to_bf16x2(z[1]));
   }
   tc_fence_before();
   if (split > 1)
@@ -765,18 +811,19 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 // 2-D map over [rows, cols] elements of 1 or 2 bytes, rows `stride_bytes` apart; the box is
-// `box_rows` x 128 bytes, 128B swizzle.  Reads outside give zeros.
+// `box_rows` x `box_bytes` (64 or 128), with the swizzle of that width.  Reads outside give zeros.
 bool make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t stride_bytes,
-              int elem, int box_rows) {
+              int elem, int box_rows, int box_bytes = kKB) {
   auto enc = reinterpret_cast<EncodeTiledFn>(tensor_map_encode_fn());
   if (enc == nullptr) return false;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride_bytes)};
-  cuuint32_t box[2] = {static_cast<cuuint32_t>(kKB / elem), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_bytes / elem), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
   return enc(map, elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
              const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             box_bytes == kKB ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -788,8 +835,8 @@ cudaError_t launch_pair(const LinearProblem& l, const LinearArgs& a, cudaStream_
   std::memset(&mr, 0, sizeof(mr));
   if (!make_map(&mx, l.x, l.m, l.k, l.x_stride * elem, elem, 128) ||
       !make_map(&mw, l.w, kGated ? 2 * l.n : l.n, l.k, l.k * elem, elem, a.bn / 2) ||
-      !make_map(&my, l.y, l.m, l.n, l.n * 2, 2, 32) ||
-      (l.residual != nullptr && !make_map(&mr, l.residual, l.m, l.n, l.n * 2, 2, 32))) {
+      !make_map(&my, l.y, l.m, l.n, l.n * 2, 2, 32, 2 * kChunk) ||
+      (l.residual != nullptr && !make_map(&mr, l.residual, l.m, l.n, l.n * 2, 2, 32, 2 * kChunk))) {
     *why = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
@@ -850,26 +897,69 @@ cudaError_t launch_split(const LinearProblem& l, const LinearArgs& a, const Spli
   return cudaLaunchKernelEx(&cfg, kernel, mx, mw, p, l.gated ? 1 : 0, l.residual, l.y, a);
 }
 
-// The split kernel's tile and split: the plan whose busiest SM moves the fewest bytes.  A CTA
-// reads (wr + tn) * 128 bytes per K tile; kJoin stands for the cluster's two barriers and the
-// exchange of partial sums.
+// How many clusters of `split` of the split kernel's CTAs run at a time: a cluster stays inside
+// a GPC, and on a B200 sizes 3 to 8 leave up to a fifth of the SMs unused (74 pairs, 45 triples,
+// 33 fours, 26 fives, 22 sixes, 15 sevens and eights).  Asked once per device and size.
+template <bool kF8>
+int resident_clusters(int split) {
+  static std::atomic<int> known[64][kSplitMax + 1];
+  if (split == 1) return sm_count();
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count() / split;
+  int n = known[dev][split].load(std::memory_order_relaxed);
+  if (n == 0) {
+    static ContextCache attr_done;
+    auto* kernel = linear_split_kernel<kF8>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(split * sm_count()));
+    cfg.blockDim = dim3(kSplitThreads);
+    cfg.dynamicSmemBytes = kSplitSmemBytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (ensure_max_dynamic_smem(attr_done, reinterpret_cast<const void*>(kernel), kSplitSmemBytes) !=
+            cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();  // the estimate below stands in
+      n = sm_count() / split;
+    }
+    known[dev][split].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// Both planners estimate cycles per SM from measured rates and take the cheapest tile.
+//
+// Split: a K tile costs its four MMAs, about 137 cycles each whatever their N up to 128 (an
+// M = 128 MMA takes its A rows from shared memory at 32 bytes a cycle) and 164 at N = 256, or
+// its bytes: W at an SM's share of HBM (24 bytes a cycle), x from L2.  Half-empty MMAs (64 W
+// rows) pay only when W has few rows.  Setup, drain and output take about 6000 cycles, the
+// exchange of partial sums 2000 more.
+template <bool kF8>
 SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
-  constexpr double kJoin = 12e3;
-  const int sms = sm_count();
   SplitPlan best = {};
   *cost = 1e30;
   const int64_t wn = l.gated ? 2 * l.n : l.n;
-  for (int wr = 32; wr <= 128; wr *= 2) {
+  for (int wr = 64; wr <= 128; wr *= 2) {
     const int64_t n_tiles = (wn + wr - 1) / wr;
+    int last_tn = 0;
     for (int tn_max = 64; tn_max <= 256; tn_max *= 2) {
       const int64_t m_tiles = (l.m + tn_max - 1) / tn_max;
       const int tn = static_cast<int>(((l.m + m_tiles - 1) / m_tiles + 15) / 16 * 16);
-      for (int split = 1; split <= 8 && split <= k_tiles; ++split) {
-        const int64_t ctas = n_tiles * m_tiles * split;
-        const int64_t waves = (ctas + sms - 1) / sms;
+      if (tn == last_tn) continue;
+      last_tn = tn;
+      const double mma = tn <= 128 ? 550.0 : 550.0 + 0.85 * (tn - 128);
+      const double bytes = wr * kKB / 24.0 + tn * kKB / 64.0;
+      for (int split = 1; split <= kSplitMax && split <= k_tiles; ++split) {
+        const int64_t clusters = resident_clusters<kF8>(split);
+        const int64_t waves = (n_tiles * m_tiles + clusters - 1) / clusters;
         const double c = static_cast<double>(waves) *
-                         (static_cast<double>((k_tiles + split - 1) / split) * (wr + tn) * kKB +
-                          (split > 1 ? kJoin : 0.0) + 4.0 * wr * tn / split);
+                         ((k_tiles + split - 1) / split * (mma > bytes ? mma : bytes) + 6000.0 +
+                          (split > 1 ? 2000.0 : 0.0) + 0.1 * wr * tn / split);
         if (c < *cost) {
           *cost = c;
           best.wr = wr;
@@ -880,24 +970,26 @@ SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
     }
   }
   const int tile_bytes = (best.wr + best.tn) * kKB;
-  int group = 16384 / tile_bytes;
-  group = group < 1 ? 1 : group > 4 ? 4 : group;
+  int group = 24576 / tile_bytes;
+  group = group < 1 ? 1 : group;
   best.group = group;
   best.stages = kSplitRingBytes / (tile_bytes * group);
   if (best.stages > kSplitStagesMax) best.stages = kSplitStagesMax;
   return best;
 }
 
-// Pair tiles: rounds of the persistent grid times what one tile streams per K tile.
+// Pair: a K tile of a 256 x bn tile takes time in proportion to bn + 205 (7680 x 1536 x 8960
+// timed at bn 64 to 256: 0.21, 0.26, 0.29, 0.36 us), so narrower tiles pay only where they
+// fill a round of the persistent grid better.
 int plan_pair(const LinearProblem& l, int k_tiles, double* cost) {
   const int64_t pairs = sm_count() / 2, mb = (l.m + kPairTokens - 1) / kPairTokens;
   int best = 256;
   *cost = 1e30;
-  for (int bn = l.gated ? 256 : 128; bn <= 256; bn += 64) {
+  for (int bn = 256; bn >= 128; bn -= 64) {
     const int64_t out_cols = l.gated ? bn / 2 : bn;
     const int64_t tiles = mb * ((l.n + out_cols - 1) / out_cols);
     const int64_t rounds = (tiles + pairs - 1) / pairs;
-    const double c = static_cast<double>(rounds) * k_tiles * (128 + bn / 2) * kKB;
+    const double c = static_cast<double>(rounds) * k_tiles * (bn + 205) * 1.5 + 9000.0;
     if (c < *cost) {
       *cost = c;
       best = bn;
@@ -930,7 +1022,8 @@ cudaError_t launch_linear(const LinearProblem& l, uint64_t wait_limit, cudaStrea
   a.err_word = error_word_ptr();
   if (a.err_word == nullptr) return cudaErrorInvalidSymbol;
   double split_cost, pair_cost;
-  const SplitPlan p = plan_split(l, a.k_tiles, &split_cost);
+  const SplitPlan p = l.fp8 ? plan_split<true>(l, a.k_tiles, &split_cost)
+                            : plan_split<false>(l, a.k_tiles, &split_cost);
   a.bn = plan_pair(l, a.k_tiles, &pair_cost);
   const int mode = linear_kernel_mode();
   if (mode == 1 || (mode == 0 && split_cost < pair_cost))

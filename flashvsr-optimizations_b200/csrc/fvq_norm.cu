@@ -35,59 +35,6 @@ constexpr int kNormThreads = 256;      // of the sub-warp form
 constexpr int kNormMaxThreads = 1024;  // of the CTA form
 constexpr int kNormMaxD = 16384;
 
-// ---------------------------------------------------------------- pairs
-// Row elements are held as pairs of fp32 in 64-bit registers, so that the products and sums
-// are the packed f32x2 instructions (two IEEE operations each, half the issue slots).
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
-}
-
-__device__ __forceinline__ void split(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-
-__device__ __forceinline__ uint64_t pair_of_bf16(uint32_t w) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(w << 16), "r"(w & 0xFFFF0000u));
-  return v;
-}
-
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
-__device__ __forceinline__ uint32_t bf16x2(uint64_t v) {
-  float lo, hi;
-  uint32_t r;
-  split(v, lo, hi);
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
-__device__ __forceinline__ uint32_t e4m3x2(uint64_t v) {
-  float lo, hi;
-  uint16_t r;
-  split(v, lo, hi);
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
 // max with a NaN of either side kept
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -95,10 +42,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// A thread's share of a row: kPairs pairs.  kVec 8: pairs 4i .. 4i+3 are the eight adjacent
-// elements of its i-th 16-byte vector; kVec 1: pair i holds its elements 2i and 2i + 1, one
-// row stride of lanes apart.  `at(i)` is the element index of vector (kVec 8) or element
-// (kVec 1) i; elements past d are zero and not stored.
+// Row elements are held as pairs (f2_*); a thread's share of a row is kPairs of them.  kVec 8:
+// pairs 4i .. 4i+3 are the eight adjacent elements of its i-th 16-byte vector; kVec 1: pair i
+// holds its elements 2i and 2i + 1, as many elements apart as the row has lanes.  `at(i)` is
+// the index of vector (kVec 8) or element (kVec 1) i; elements past d are zero, not stored.
 template <int kPairs, int kVec, class At>
 __device__ __forceinline__ void load_bf16(uint32_t (&w)[kPairs], const uint16_t* p, int d, At at) {
   if constexpr (kVec == 8) {
@@ -127,10 +74,10 @@ __device__ __forceinline__ void add_f32(uint64_t (&s)[kPairs], const float* p, i
       if (at(i) < d) {
         const float4 a = *reinterpret_cast<const float4*>(p + at(i));
         const float4 b = *reinterpret_cast<const float4*>(p + at(i) + 4);
-        s[4 * i] = add2(s[4 * i], pair_of(a.x, a.y));
-        s[4 * i + 1] = add2(s[4 * i + 1], pair_of(a.z, a.w));
-        s[4 * i + 2] = add2(s[4 * i + 2], pair_of(b.x, b.y));
-        s[4 * i + 3] = add2(s[4 * i + 3], pair_of(b.z, b.w));
+        s[4 * i] = f2_add(s[4 * i], f2_pack(a.x, a.y));
+        s[4 * i + 1] = f2_add(s[4 * i + 1], f2_pack(a.z, a.w));
+        s[4 * i + 2] = f2_add(s[4 * i + 2], f2_pack(b.x, b.y));
+        s[4 * i + 3] = f2_add(s[4 * i + 3], f2_pack(b.z, b.w));
       }
     }
   } else {
@@ -138,7 +85,7 @@ __device__ __forceinline__ void add_f32(uint64_t (&s)[kPairs], const float* p, i
     for (int i = 0; i < kPairs; ++i) {
       const float lo = at(2 * i) < d ? p[at(2 * i)] : 0.0f;
       const float hi = at(2 * i + 1) < d ? p[at(2 * i + 1)] : 0.0f;
-      s[i] = add2(s[i], pair_of(lo, hi));
+      s[i] = f2_add(s[i], f2_pack(lo, hi));
     }
   }
 }
@@ -151,7 +98,7 @@ __device__ __forceinline__ void store_f32(float* p, const uint64_t (&s)[kPairs],
       if (at(i) < d) {
         float f[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) split(s[4 * i + e], f[2 * e], f[2 * e + 1]);
+        for (int e = 0; e < 4; ++e) f2_split(s[4 * i + e], f[2 * e], f[2 * e + 1]);
         reinterpret_cast<float4*>(p + at(i))[0] = make_float4(f[0], f[1], f[2], f[3]);
         reinterpret_cast<float4*>(p + at(i))[1] = make_float4(f[4], f[5], f[6], f[7]);
       }
@@ -160,7 +107,7 @@ __device__ __forceinline__ void store_f32(float* p, const uint64_t (&s)[kPairs],
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
       float lo, hi;
-      split(s[i], lo, hi);
+      f2_split(s[i], lo, hi);
       if (at(2 * i) < d) p[at(2 * i)] = lo;
       if (at(2 * i + 1) < d) p[at(2 * i + 1)] = hi;
     }
@@ -176,12 +123,12 @@ __device__ __forceinline__ void store_bf16(uint16_t* p, const uint64_t (&s)[kPai
     for (int i = 0; i < kPairs / 4; ++i)
       if (at(i) < d)
         *reinterpret_cast<uint4*>(p + at(i)) =
-            make_uint4(bf16x2(mul2(s[4 * i], f)), bf16x2(mul2(s[4 * i + 1], f)),
-                       bf16x2(mul2(s[4 * i + 2], f)), bf16x2(mul2(s[4 * i + 3], f)));
+            make_uint4(f2_to_bf16x2(f2_mul(s[4 * i], f)), f2_to_bf16x2(f2_mul(s[4 * i + 1], f)),
+                       f2_to_bf16x2(f2_mul(s[4 * i + 2], f)), f2_to_bf16x2(f2_mul(s[4 * i + 3], f)));
   } else {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
-      const uint32_t w = bf16x2(mul2(s[i], f));
+      const uint32_t w = f2_to_bf16x2(f2_mul(s[i], f));
       if (at(2 * i) < d) p[at(2 * i)] = static_cast<uint16_t>(w);
       if (at(2 * i + 1) < d) p[at(2 * i + 1)] = static_cast<uint16_t>(w >> 16);
     }
@@ -197,12 +144,12 @@ __device__ __forceinline__ void store_e4m3(uint8_t* p, const uint64_t (&s)[kPair
     for (int i = 0; i < kPairs / 4; ++i)
       if (at(i) < d)
         *reinterpret_cast<uint2*>(p + at(i)) =
-            make_uint2(e4m3x2(mul2(s[4 * i], f)) | (e4m3x2(mul2(s[4 * i + 1], f)) << 16),
-                       e4m3x2(mul2(s[4 * i + 2], f)) | (e4m3x2(mul2(s[4 * i + 3], f)) << 16));
+            make_uint2(f2_to_e4m3x2(f2_mul(s[4 * i], f)) | (f2_to_e4m3x2(f2_mul(s[4 * i + 1], f)) << 16),
+                       f2_to_e4m3x2(f2_mul(s[4 * i + 2], f)) | (f2_to_e4m3x2(f2_mul(s[4 * i + 3], f)) << 16));
   } else {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
-      const uint32_t w = e4m3x2(mul2(s[i], f));
+      const uint32_t w = f2_to_e4m3x2(f2_mul(s[i], f));
       if (at(2 * i) < d) p[at(2 * i)] = static_cast<uint8_t>(w);
       if (at(2 * i + 1) < d) p[at(2 * i + 1)] = static_cast<uint8_t>(w >> 8);
     }
@@ -220,9 +167,9 @@ __device__ __forceinline__ void add_residual(uint64_t (&s)[kPairs], const void* 
     uint32_t w[kPairs];
     load_bf16<kPairs, kVec>(w, static_cast<const uint16_t*>(p), d, at);
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) s[i] = add2(s[i], pair_of_bf16(w[i]));
+    for (int i = 0; i < kPairs; ++i) s[i] = f2_add(s[i], f2_of_bf16x2(w[i]));
     if (store)
-      store_bf16<kPairs, kVec>(static_cast<uint16_t*>(out), s, pair_of(1.0f, 1.0f), d, at);
+      store_bf16<kPairs, kVec>(static_cast<uint16_t*>(out), s, f2_pack(1.0f, 1.0f), d, at);
   }
 }
 
@@ -230,9 +177,9 @@ template <int kPairs>
 __device__ __forceinline__ float sum_squares(const uint64_t (&s)[kPairs]) {
   uint64_t q = 0;
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) q = fma2(s[i], s[i], q);
+  for (int i = 0; i < kPairs; ++i) q = f2_fma(s[i], s[i], q);
   float lo, hi;
-  split(q, lo, hi);
+  f2_split(q, lo, hi);
   return lo + hi;
 }
 
@@ -240,7 +187,7 @@ __device__ __forceinline__ float sum_squares(const uint64_t (&s)[kPairs]) {
 template <int kPairs>
 __device__ __forceinline__ void apply_weight(uint64_t (&s)[kPairs], const uint32_t (&w)[kPairs]) {
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) s[i] = mul2(s[i], pair_of_bf16(w[i]));
+  for (int i = 0; i < kPairs; ++i) s[i] = f2_mul(s[i], f2_of_bf16x2(w[i]));
 }
 
 template <int kPairs>
@@ -249,7 +196,7 @@ __device__ __forceinline__ float max_abs(const uint64_t (&s)[kPairs]) {
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
     float lo, hi;
-    split(s[i], lo, hi);
+    f2_split(s[i], lo, hi);
     m = max_nan(max_nan(m, fabsf(lo)), fabsf(hi));
   }
   return m;
@@ -322,7 +269,7 @@ __global__ void __launch_bounds__(kLanes == 0 ? kNormMaxThreads : kNormThreads)
     const int64_t base = row * d;
     uint64_t s[kPairs];
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) s[i] = pair_of_bf16(xw[k][i]);
+    for (int i = 0; i < kPairs; ++i) s[i] = f2_of_bf16x2(xw[k][i]);
     if (a.residual != nullptr) {
       const int64_t bytes = base * (a.residual_f32 ? 4 : 2);
       add_residual<kPairs, kVec>(s, static_cast<const uint8_t*>(a.residual) + bytes, a.residual_f32,
@@ -331,13 +278,13 @@ __global__ void __launch_bounds__(kLanes == 0 ? kNormMaxThreads : kNormThreads)
     const float sq = row_reduce<kLanes>(sum_squares(s), sum_smem, [](float p, float q) { return p + q; });
     const float rstd = rsqrtf(sq / static_cast<float>(d) + a.eps);
     if (a.weight != nullptr) apply_weight(s, w);
-    if (a.y != nullptr && live) store_bf16<kPairs, kVec>(a.y + base, s, pair_of(rstd, rstd), d, at);
+    if (a.y != nullptr && live) store_bf16<kPairs, kVec>(a.y + base, s, f2_pack(rstd, rstd), d, at);
     if (a.q != nullptr) {
       const float m = row_reduce<kLanes>(max_abs(s), max_smem, [](float p, float q) { return max_nan(p, q); });
       const float scale = scale448(m * rstd), f = rstd * __frcp_rn(scale);
       if (!live) continue;
       if (lane == 0) a.scale[row] = scale;
-      store_e4m3<kPairs, kVec>(a.q + base, s, pair_of(f, f), d, at);
+      store_e4m3<kPairs, kVec>(a.q + base, s, f2_pack(f, f), d, at);
     }
   }
 }
@@ -498,7 +445,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     load_bf16<kPairs, kVec>(xw, reinterpret_cast<const uint16_t*>(xs), d, at);
     uint64_t s[kPairs];
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) s[i] = pair_of_bf16(xw[i]);
+    for (int i = 0; i < kPairs; ++i) s[i] = f2_of_bf16x2(xw[i]);
     const int64_t base = row * d;
     if (res_bytes != 0)
       add_residual<kPairs, kVec>(s, rs, res_bytes == 4, static_cast<uint8_t*>(a.residual_out) + base * res_bytes,
@@ -510,13 +457,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                               [](float x, float y) { return x + y; });
     const float rstd = rsqrtf(sq / static_cast<float>(d) + a.eps);
     if (a.weight != nullptr) apply_weight(s, w);
-    if (a.y != nullptr) store_bf16<kPairs, kVec>(a.y + base, s, pair_of(rstd, rstd), d, at);
+    if (a.y != nullptr) store_bf16<kPairs, kVec>(a.y + base, s, f2_pack(rstd, rstd), d, at);
     if (a.q != nullptr) {
       const float m = group_reduce<kGroup>(max_abs(s), maxima + group * kGroup, group, in_group,
                                            [](float x, float y) { return max_nan(x, y); });
       const float scale = scale448(m * rstd), f = rstd * __frcp_rn(scale);
       if (leader) a.scale[row] = scale;
-      store_e4m3<kPairs, kVec>(a.q + base, s, pair_of(f, f), d, at);
+      store_e4m3<kPairs, kVec>(a.q + base, s, f2_pack(f, f), d, at);
     }
     if (++slot == p.slots) slot = 0;
   }
