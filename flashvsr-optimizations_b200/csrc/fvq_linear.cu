@@ -19,6 +19,9 @@
 //     to eight CTAs until every SM streams its share of W, and the partial sums are joined
 //     through distributed shared memory in rank order (no atomics, no workspace, the same
 //     bits on every run).
+//   linear_vector_kernel  one or two tokens: W streamed through registers by plain 16-byte
+//     loads and fp32 FMAs, x in shared memory.  No tensor-core pipeline to set up, fill and
+//     drain, which is half of the split kernel's time at this size.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -804,6 +807,175 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   if (warp == 1) tmem_dealloc(tmem, cols);
 }
 
+// ---------------------------------------------------------------- one or two tokens
+// A warp takes four W rows (gated: two Wg rows and the same columns' Wu rows) and every
+// `kw`-th 512-byte slice of their K; the `kw` warps of a row group are in one CTA and join
+// their sums through shared memory in warp order.
+constexpr int kVecWarps = 8;
+constexpr int kVecThreads = 32 * kVecWarps;
+constexpr int kVecRows = 4;
+constexpr int kVecUnroll = 2;          // slices in flight: 8 loads of 16 bytes a lane
+constexpr int kVecTokensMax = 2;
+constexpr int kVecCtas = 2;            // per SM (three: spills, and slower from 8960 x 1536 on)
+constexpr int kVecSmemMax = 72 * 1024;
+
+__device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// 16 bytes of operand -> pairs of fp32: 4 (bf16) or 8 (E4M3)
+template <bool kF8>
+__device__ __forceinline__ void unpack16(const uint4& v, uint64_t (&f)[kF8 ? 8 : 4]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kF8) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t h2;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(w[i] >> (16 * h))));
+        const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+        f[2 * i + h] = f2_pack(p.x, p.y);
+      }
+    } else {
+      f[i] = f2_of_bf16x2(w[i]);
+    }
+  }
+}
+
+template <bool kF8, int kM>
+__global__ void __launch_bounds__(kVecThreads, kVecCtas)
+    linear_vector_kernel(const uint8_t* __restrict__ x, const int64_t x_bytes,
+                         const uint8_t* __restrict__ w, const int k_bytes, const int kw,
+                         const int gated, const uint16_t* __restrict__ residual,
+                         uint16_t* __restrict__ y, const LinearArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr int kPairs = kF8 ? 8 : 4;
+  constexpr int kValues = kVecRows * kM;
+  uint4* xs = reinterpret_cast<uint4*>(smem);                     // [kM][k_bytes / 16]
+  float* part = reinterpret_cast<float*>(smem + kM * k_bytes);    // [warps][kValues]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slice = warp % kw;
+  const int slices = k_bytes / 16;                                // 16-byte pieces of a row
+  const int group = static_cast<int>(blockIdx.x) * (kVecWarps / kw) + warp / kw;
+  const int out_cols = gated ? kVecRows / 2 : kVecRows;
+  const int col0 = group * out_cols;
+  const uint4* rows[kVecRows];
+#pragma unroll
+  for (int r = 0; r < kVecRows; ++r) {
+    // a group past the last column reads the last rows and stores nothing
+    const int c = min(col0 + (gated ? r & 1 : r), a.n - 1);
+    rows[r] = reinterpret_cast<const uint4*>(w + (static_cast<int64_t>(c) + (gated && r >= 2 ? a.n : 0)) * k_bytes);
+  }
+  uint4 wv[kVecUnroll][kVecRows];
+  const auto load = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < kVecUnroll; ++u) {
+      const int at = base + u * kw * 32 + lane;
+#pragma unroll
+      for (int r = 0; r < kVecRows; ++r)
+        wv[u][r] = at < slices ? ld_stream_v4(rows[r] + at) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  const int step = kVecUnroll * kw * 32;
+  load(slice * 32);
+  for (int i = threadIdx.x; i < kM * slices; i += kVecThreads) {
+    const int t = i / slices;
+    xs[i] = t < a.m ? __ldg(reinterpret_cast<const uint4*>(x + t * x_bytes) + (i - t * slices))
+                    : make_uint4(0, 0, 0, 0);
+  }
+  __syncthreads();
+  uint64_t acc[kVecRows][kM];
+#pragma unroll
+  for (int r = 0; r < kVecRows; ++r)
+#pragma unroll
+    for (int t = 0; t < kM; ++t) acc[r][t] = 0;
+  for (int base = slice * 32; base < slices; base += step) {
+    uint4 now[kVecUnroll][kVecRows];
+#pragma unroll
+    for (int u = 0; u < kVecUnroll; ++u)
+#pragma unroll
+      for (int r = 0; r < kVecRows; ++r) now[u][r] = wv[u][r];
+    if (base + step < slices) load(base + step);
+#pragma unroll
+    for (int u = 0; u < kVecUnroll; ++u) {
+      const int at = base + u * kw * 32 + lane;
+      if (at >= slices) continue;
+      uint64_t xf[kM][kPairs];
+#pragma unroll
+      for (int t = 0; t < kM; ++t) unpack16<kF8>(xs[t * slices + at], xf[t]);
+#pragma unroll
+      for (int r = 0; r < kVecRows; ++r) {
+        uint64_t wf[kPairs];
+        unpack16<kF8>(now[u][r], wf);
+#pragma unroll
+        for (int t = 0; t < kM; ++t)
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i) acc[r][t] = f2_fma(wf[i], xf[t][i], acc[r][t]);
+      }
+    }
+  }
+  // Sums over the warp: while a lane holds several values, each step exchanges half of them
+  // (the upper lanes keep the upper half), so that the last lanes hold one value each.
+  float v[kValues];
+#pragma unroll
+  for (int r = 0; r < kVecRows; ++r)
+#pragma unroll
+    for (int t = 0; t < kM; ++t) {
+      float lo, hi;
+      f2_split(acc[r][t], lo, hi);
+      v[r * kM + t] = lo + hi;
+    }
+  int index = 0;
+#pragma unroll
+  for (int o = 16, have = kValues; o > 0; o >>= 1) {
+    if (have > 1) {
+      have /= 2;
+      const bool upper = (lane & o) != 0;
+#pragma unroll
+      for (int i = 0; i < kValues / 2; ++i) {
+        if (i >= have) break;
+        const float give = upper ? v[i] : v[i + have];
+        const float keep = upper ? v[i + have] : v[i];
+        v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
+      }
+      if (upper) index += have;
+    } else {
+      v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], o);
+    }
+  }
+  if ((lane & (32 / kValues - 1)) == 0) part[warp * kValues + index] = v[0];
+  __syncthreads();
+  // one thread per output of the CTA
+  const int outs = out_cols * kM;
+  const int id = static_cast<int>(threadIdx.x);
+  if (id >= kVecWarps / kw * outs) return;
+  const int g = id / outs, j = id - g * outs, c = j / kM, t = j - c * kM;
+  const int col = (static_cast<int>(blockIdx.x) * (kVecWarps / kw) + g) * out_cols + c;
+  if (col >= a.n || t >= a.m) return;
+  float z = 0.0f, u = 0.0f;
+  for (int q = 0; q < kw; ++q) {
+    const float* p = part + (g * kw + q) * kValues;
+    z += p[c * kM + t];
+    if (gated) u += p[(c + 2) * kM + t];
+  }
+  if constexpr (kF8) z = z * __ldg(a.sx + t) * __ldg(a.sw + col);
+  if (a.bias != nullptr) z += __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + col)) << 16);
+  z = activate_any(a.act, z);
+  if (gated) {
+    if constexpr (kF8) u = u * __ldg(a.sx + t) * __ldg(a.sw + a.n + col);
+    if (a.bias != nullptr) u += __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + a.n + col)) << 16);
+    z *= u;
+  }
+  const int64_t dst = static_cast<int64_t>(t) * a.n + col;
+  if (residual != nullptr) z += __uint_as_float(static_cast<uint32_t>(__ldg(residual + dst)) << 16);
+  y[dst] = __bfloat16_as_ushort(__float2bfloat16_rn(z));
+}
+
 // ---------------------------------------------------------------- host side
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                    const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -897,6 +1069,33 @@ cudaError_t launch_split(const LinearProblem& l, const LinearArgs& a, const Spli
   return cudaLaunchKernelEx(&cfg, kernel, mx, mw, p, l.gated ? 1 : 0, l.residual, l.y, a);
 }
 
+template <bool kF8, int kM>
+cudaError_t launch_vector(const LinearProblem& l, const LinearArgs& a, cudaStream_t st) {
+  const int elem = kF8 ? 1 : 2;
+  const int k_bytes = static_cast<int>(l.k * elem);
+  const int64_t out_cols = l.gated ? kVecRows / 2 : kVecRows;
+  const int64_t groups = (l.n + out_cols - 1) / out_cols;
+  // warps per row group: enough for sixteen warps an SM, while a warp keeps a slice of K
+  int kw = 1;
+  while (kw < kVecWarps && groups * kw < 16 * sm_count() && kw * 512 < k_bytes) kw *= 2;
+  const int bytes = kM * k_bytes + kVecWarps * kVecRows * kM * 4;
+  static ContextCache attr_done;
+  auto* kernel = linear_vector_kernel<kF8, kM>;
+  if (cudaError_t e = ensure_max_dynamic_smem(attr_done, reinterpret_cast<const void*>(kernel),
+                                              kVecSmemMax + kVecWarps * kVecRows * kM * 4))
+    return e;
+  const int64_t ctas = (groups + kVecWarps / kw - 1) / (kVecWarps / kw);
+  kernel<<<static_cast<unsigned>(ctas), kVecThreads, bytes, st>>>(
+      static_cast<const uint8_t*>(l.x), l.x_stride * elem, static_cast<const uint8_t*>(l.w), k_bytes, kw,
+      l.gated ? 1 : 0, l.residual, l.y, a);
+  return cudaGetLastError();
+}
+
+template <bool kF8>
+cudaError_t launch_vector_by_tokens(const LinearProblem& l, const LinearArgs& a, cudaStream_t st) {
+  return l.m == 1 ? launch_vector<kF8, 1>(l, a, st) : launch_vector<kF8, 2>(l, a, st);
+}
+
 // How many clusters of `split` of the split kernel's CTAs run at a time: a cluster stays inside
 // a GPC, and on a B200 sizes 3 to 8 leave up to a fifth of the SMs unused (74 pairs, 45 triples,
 // 33 fours, 26 fives, 22 sixes, 15 sevens and eights).  Asked once per device and size.
@@ -985,7 +1184,7 @@ int plan_pair(const LinearProblem& l, int k_tiles, double* cost) {
   const int64_t pairs = sm_count() / 2, mb = (l.m + kPairTokens - 1) / kPairTokens;
   int best = 256;
   *cost = 1e30;
-  for (int bn = 256; bn >= 128; bn -= 64) {
+  for (int bn = 256; bn >= 128; bn -= l.gated ? 64 : 32) {
     const int64_t out_cols = l.gated ? bn / 2 : bn;
     const int64_t tiles = mb * ((l.n + out_cols - 1) / out_cols);
     const int64_t rounds = (tiles + pairs - 1) / pairs;
@@ -1021,11 +1220,14 @@ cudaError_t launch_linear(const LinearProblem& l, uint64_t wait_limit, cudaStrea
   a.wait_limit = wait_limit;
   a.err_word = error_word_ptr();
   if (a.err_word == nullptr) return cudaErrorInvalidSymbol;
+  const int mode = linear_kernel_mode();
+  const int64_t x_smem = l.m * l.k * (l.fp8 ? 1 : 2);
+  if (mode == 0 && l.m <= kVecTokensMax && x_smem <= kVecSmemMax)
+    return l.fp8 ? launch_vector_by_tokens<true>(l, a, st) : launch_vector_by_tokens<false>(l, a, st);
   double split_cost, pair_cost;
   const SplitPlan p = l.fp8 ? plan_split<true>(l, a.k_tiles, &split_cost)
                             : plan_split<false>(l, a.k_tiles, &split_cost);
   a.bn = plan_pair(l, a.k_tiles, &pair_cost);
-  const int mode = linear_kernel_mode();
   if (mode == 1 || (mode == 0 && split_cost < pair_cost))
     return l.fp8 ? launch_split<true>(l, a, p, st, why) : launch_split<false>(l, a, p, st, why);
   if (l.fp8)

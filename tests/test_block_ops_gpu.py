@@ -235,7 +235,10 @@ def product64(x, w, sx, sw, bias, act, gated, residual):
 
 
 def fp8_rows(rows, k, seed, std=1.0):
-    return ops.fp8_row_quant(randn(rows, k, seed=seed, std=std)) if k % 8 == 0 else None
+    """Codes and row scales; any will do, and the row quantizer ends at 16384 values."""
+    x = randn(rows, k, seed=seed, std=std).float()
+    scale = x.abs().amax(-1, keepdim=True) / 448
+    return (x / scale).to(F8), scale
 
 
 def check_product(m, n, k, fp8=False, bias=True, act="none", gated=False, residual=True, seed=0):
@@ -304,6 +307,25 @@ def test_product_epilogues(kernel, fp8, gated, act):
                                          (3, 20000, 64, True)])
 def test_product_by_size(fp8, m, n, k, gated):
     check_product(m, n, k, fp8, act="gelu_tanh" if gated else "none", gated=gated)
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("n,k", [(8, 16), (16, 528), (72, 1536), (1000, 8960), (8960, 1536), (264, 12288), (40, 20480)])
+def test_product_few_rows(fp8, m, n, k):
+    """One or two rows (the form that reads W through registers), and the next counts."""
+    check_product(m, n, k, fp8)
+    check_product(m, n, k, fp8, act="gelu_tanh", gated=True, residual=False)
+    check_product(m, n, k, fp8, bias=False, act="silu", gated=True)
+
+
+@pytest.mark.parametrize("m", [1, 3])
+def test_product_few_rows_views(m):
+    wide = randn(m, 400, seed=1)
+    w = randn(72, 128, seed=2)
+    for x in (wide[:, 8:136], wide[:, 4:132], wide[:1, :128].expand(m, 128)):
+        want, bound = product64(x, w, None, None, None, "silu", False, None)
+        inside(ops.linear_act(x, w, act="silu"), want, bound)
 
 
 def test_product_extreme_values(kernel):
