@@ -7,11 +7,14 @@ raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import threading
 from pathlib import Path
 
 _HERE = Path(__file__).resolve().parent
 LIB_PATH = _HERE / "libfvq.so"
+BINDING_PATH = _HERE / "_fvq_torch.so"
 
 FVQ_OK = 0
 FVQ_EINVAL = -1
@@ -162,6 +165,27 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
         if path is None:
             _lib = lib
         return lib
+
+
+_binding = None
+
+
+def binding():
+    """The module _fvq_torch (csrc/fvq_torch.cpp), bound to libfvq.so's entry points."""
+    global _binding
+    if _binding is None:
+        if not BINDING_PATH.exists():
+            raise FileNotFoundError(
+                f"{BINDING_PATH} is missing: build it with `python flashvsr-optimizations_b200/build.py`")
+        lib = load()
+        loader = importlib.machinery.ExtensionFileLoader("_fvq_torch", str(BINDING_PATH))
+        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_fvq_torch", loader))
+        loader.exec_module(mod)
+        mod.bind(*(ctypes.cast(getattr(lib, f"fvq_{n}"), _vp).value
+                   for n in ("rms_norm", "linear_act", "fp8_scaled_mm_act", "fp8_cache_write",
+                             "fp8_cache_read")))
+        _binding = mod
+    return _binding
 
 
 def check(fn_name: str, rc: int) -> None:

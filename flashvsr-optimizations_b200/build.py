@@ -1,4 +1,4 @@
-"""Build libfvq.so (the C-ABI CUDA library) in-tree for sm_100a.
+"""Build libfvq.so (the C-ABI CUDA library) and _fvq_torch.so (torch's short path to it) in-tree.
 
     python flashvsr-optimizations_b200/build.py [--force] [--verbose]
 
@@ -6,6 +6,7 @@ Each .cu file is compiled separately (nvcc -c, cached by mtime) and linked
 into ``libfvq.so`` beside this file.  cudart is linked statically so the
 library works inside any process that already has a CUDA context (torch's
 included) without depending on which libcudart that process loaded.
+``_fvq_torch.so`` is host code only, compiled against the installed torch.
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
 BUILD = HERE / "_build"
 LIB = HERE / "libfvq.so"
+BINDING = HERE / "_fvq_torch.so"
 
 SOURCES = ["fvq_quant.cu", "fvq_fp8.cu", "fvq_resize.cu", "fvq_block.cu", "fvq_gemm.cu",
            "fvq_norm.cu", "fvq_linear.cu", "fvq_cache.cu", "fvq_api.cu", "fvq_noalloc.cu"]
@@ -73,9 +75,41 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     return LIB
 
 
+def build_binding(force: bool = False) -> Path:
+    """_fvq_torch.so, rebuilt when its source, the C header or the installed torch changed."""
+    import sysconfig
+
+    import torch
+    src = CSRC / "fvq_torch.cpp"
+    stamp = BUILD / "fvq_torch.version.txt"
+    version = f"{torch.__version__} {sys.version}"
+    newest = max(src.stat().st_mtime, max(h.stat().st_mtime for h in INCLUDE.glob("*.h")))
+    if not force and BINDING.exists() and BINDING.stat().st_mtime >= newest and stamp.exists() \
+            and stamp.read_text() == version:
+        return BINDING
+    BUILD.mkdir(exist_ok=True)
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent / "include"
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in (root / "include", root / "include/torch/csrc/api/include",
+                                      sysconfig.get_paths()["include"], cuda)),
+           str(src), "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10",
+           "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("build of _fvq_torch.so failed")
+    os.replace(tmp, BINDING)
+    stamp.write_text(version)
+    return BINDING
+
+
 if __name__ == "__main__":
     ap = argparse.ArgumentParser()
     ap.add_argument("--force", action="store_true")
     ap.add_argument("--verbose", action="store_true")
     a = ap.parse_args()
     print(build(a.force, a.verbose))
+    print(build_binding(a.force))

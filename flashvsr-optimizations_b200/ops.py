@@ -597,10 +597,11 @@ def _(x, q1, s1, b1, q2, s2, b2):
 
 # ---------------------------------------------------------------- the block around the linears
 # These operators are called once or more per block and token, where a decode step is bound by
-# its host side: they are defined directly on a torch.library.Library (about 6 us of dispatch a
-# call against 20 us for the decorator's wrapper), and a plain eager call -- no subclass, no
-# mode, no tracing, no gradient -- runs the implementation without the dispatcher.  Inference
-# only, like the rest: a call that would need a gradient raises when the gradient is asked for.
+# its host side.  The common eager call goes straight to the C ABI through _fvq_torch (which
+# returns None for every other: views to copy, odd alignment, wrong arguments, gradients, modes,
+# subclasses); the rest goes through the registered operator, defined directly on a
+# torch.library.Library (about 6 us of dispatch a call against 20 us for the decorator's
+# wrapper).  Inference only: a call that would need a gradient raises when it is asked for.
 _BLOCK_LIB = torch.library.Library("fvq", "FRAGMENT")
 
 
@@ -633,19 +634,12 @@ def _define(schema: str, impl, fake):
     return call
 
 
-def _plain(*ts: torch.Tensor | None) -> bool:
-    """A plain eager call: tensors and parameters, no gradient to record, no mode, no tracing."""
-    for t in ts:
-        if t is not None:
-            kind = type(t)
-            if (kind is not torch.Tensor and kind is not torch.nn.Parameter) or \
-                    (t.requires_grad and torch.is_grad_enabled()):
-                return False
-    return not (_dispatch_modes() or _function_modes() or torch.compiler.is_compiling())
-
-
-_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
 _raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(d).cuda_stream, without its object
+
+
+def _fast():
+    """The short path's module; None while a graph is traced."""
+    return None if torch.compiler.is_compiling() else (_lib._binding or _lib.binding())
 
 
 def _launch(name: str, device: torch.device, *args) -> None:
@@ -744,9 +738,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1
 
     x: bf16 [..., d], d <= 16384; views of two or three dimensions with adjacent values (heads
     inside a fused projection's rows) are read in place.  weight: bf16 [d] or None (ones)."""
-    if _plain(x, weight):
-        return _norm("rms_norm", x, weight, None, eps, False)[0]
-    return _rms_norm(x, weight, eps)
+    fast = _fast()
+    got = fast.rms_norm(x, weight, None, eps, False) if fast else None
+    return _rms_norm(x, weight, eps) if got is None else got[0]
 
 
 def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
@@ -754,9 +748,9 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor |
     """(rms_norm(s), s) with s = x + residual: the branch's output joins the stream and the next
     branch's input is normalised in one pass.  residual: bf16 or fp32, x's shape; s is returned in
     its type, and normalised before that rounding."""
-    if _plain(x, residual, weight):
-        return _norm("add_rms_norm", x, weight, residual, eps, False)[::2]
-    return _add_rms_norm(x, residual, weight, eps)
+    fast = _fast()
+    got = fast.rms_norm(x, weight, residual, eps, False) if fast and residual is not None else None
+    return _add_rms_norm(x, residual, weight, eps) if got is None else got[::2]
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor | None = None,
@@ -764,17 +758,17 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor | None = None,
     """(q float8_e4m3fn like x, scale fp32 [..., 1]): rms_norm's fp32 value v quantized with one scale
     per row, scale = max(max|v| / 448, 1e-12), q = v / scale -- the input of ``fp8_scaled_mm`` and
     ``fp8_scaled_mm_act`` without a bf16 copy in between."""
-    if _plain(x, weight):
-        return _norm("rms_norm_fp8", x, weight, None, eps, True)[:2]
-    return _rms_norm_fp8(x, weight, eps)
+    fast = _fast()
+    got = fast.rms_norm(x, weight, None, eps, True) if fast else None
+    return _rms_norm_fp8(x, weight, eps) if got is None else got[:2]
 
 
 def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
                      eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(q, scale, s): ``rms_norm_fp8`` of s = x + residual, and s (see ``add_rms_norm``)."""
-    if _plain(x, residual, weight):
-        return _norm("add_rms_norm_fp8", x, weight, residual, eps, True)
-    return _add_rms_norm_fp8(x, residual, weight, eps)
+    fast = _fast()
+    got = fast.rms_norm(x, weight, residual, eps, True) if fast and residual is not None else None
+    return _add_rms_norm_fp8(x, residual, weight, eps) if got is None else got
 
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
@@ -877,8 +871,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     fp32 accumulation and epilogue, one rounding.  x: bf16 [..., k] (rows may be strided), weight
     in nn.Linear's layout, k and n multiples of 8; act: one of ``ACTIVATIONS`` ("gelu" is the erf
     form).  From one row to many: few rows run on a kernel bound by reading the weight once."""
-    call = _linear_act_impl if _plain(x, weight, bias, residual) else _linear_act
-    return call(x, weight, bias, act, gated, residual)
+    fast = _fast()
+    y = fast.linear_act(x, weight, bias, ACTIVATIONS.get(act), gated, residual) if fast else None
+    return _linear_act(x, weight, bias, act, gated, residual) if y is None else y
 
 
 def fp8_scaled_mm_act(a: torch.Tensor, scale_a: torch.Tensor, w: torch.Tensor, scale_w: torch.Tensor,
@@ -887,8 +882,10 @@ def fp8_scaled_mm_act(a: torch.Tensor, scale_a: torch.Tensor, w: torch.Tensor, s
     """``linear_act`` with E4M3 operands and one fp32 scale per row of each (those of
     ``fp8_row_quant``, ``rms_norm_fp8`` and ``QuantLinear(mode='fp8')``):
     z = (a @ w^T) * scale_a * scale_w + bias.  k a multiple of 16, n of 8."""
-    call = _fp8_scaled_mm_act_impl if _plain(a, scale_a, w, scale_w, bias, residual) else _fp8_scaled_mm_act
-    return call(a, scale_a, w, scale_w, bias, act, gated, residual)
+    fast = _fast()
+    y = fast.fp8_scaled_mm_act(a, scale_a, w, scale_w, bias, ACTIVATIONS.get(act), gated, residual) \
+        if fast else None
+    return _fp8_scaled_mm_act(a, scale_a, w, scale_w, bias, act, gated, residual) if y is None else y
 
 
 # ---------------------------------------------------------------- paged FP8 keys and values
@@ -983,8 +980,9 @@ def fp8_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cod
     head, scale = max(max|x| / 448, 1e-12), q = x / scale.  A negative slot is padding (nothing is
     stored); one past the store is skipped and sets bit 6 of ``read_device_error()``.  The slots
     of one call must differ: what a repeated slot then holds is undefined."""
-    plain = _plain(k, v, slots, k_codes, k_scale, v_codes, v_scale)
-    (_fp8_cache_write_impl if plain else _fp8_cache_write)(k, v, slots, k_codes, k_scale, v_codes, v_scale)
+    fast = _fast()
+    if not fast or fast.fp8_cache_write(k, v, slots, k_codes, k_scale, v_codes, v_scale) is None:
+        _fp8_cache_write(k, v, slots, k_codes, k_scale, v_codes, v_scale)
 
 
 def fp8_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor,
@@ -994,9 +992,9 @@ def fp8_cache_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.
     [batch, pages]) lists in order: bf16(q * scale) below lengths[b] (int32), zero from there on.
     A page outside the store, or a length past max_len or past the table, reads as zeros and sets
     bit 7 of ``read_device_error()``."""
-    plain = _plain(k_codes, k_scale, v_codes, v_scale, page_table, lengths)
-    call = _fp8_cache_read_impl if plain else _fp8_cache_read
-    return call(k_codes, k_scale, v_codes, v_scale, page_table, lengths, max_len)
+    fast = _fast()
+    got = fast.fp8_cache_read(k_codes, k_scale, v_codes, v_scale, page_table, lengths, max_len) if fast else None
+    return _fp8_cache_read(k_codes, k_scale, v_codes, v_scale, page_table, lengths, max_len) if got is None else got
 
 
 def div_full_probe(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
