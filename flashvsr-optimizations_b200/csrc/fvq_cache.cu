@@ -5,9 +5,9 @@
 //   read:  bf16(q * scale), rows past a sequence's length zero
 //
 // Both are HBM-bound copies with a conversion, keys and values in one launch.  Writing gives
-// a row of d <= 512 values to a power-of-two group of lanes (8 values a lane, up to two
-// vectors), so that its maximum needs only shuffles; reading gives 16 (or 8) codes to a thread,
-// four vectors in flight each.  Row and position arithmetic is 32-bit with multiplications in
+// a row of d <= 512 values to a power-of-two group of lanes (16 values a lane, 8 where
+// alignment allows no more), so that its maximum needs only shuffles; reading gives 16 (or 8)
+// codes to a thread, four vectors in flight each.  Row and position arithmetic is 32-bit with multiplications in
 // place of divisions: with 64-bit divisions both were bound by issue slots (reading 4 x 7680
 // tokens of 12 heads of 128 took 78 us).  Slot and page numbers come from the device and are
 // checked there: a negative slot is padding and stores nothing, a slot or page past the store
@@ -23,15 +23,6 @@ namespace fvq {
 namespace {
 
 constexpr int kCacheThreads = 256;
-
-__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -72,8 +63,23 @@ __device__ __forceinline__ uint2 dequantize4(uint32_t codes, float scale) {
   return make_uint2(w[0], w[1]);
 }
 
-// kLanes lanes a row, kRows rows a group, whose loads overlap; blockIdx.y: 0 keys, 1 values.
-template <int kLanes, int kVecs, int kRows>
+// 32-byte accesses: a warp's are whole sectors whichever way they are split up
+__device__ __forceinline__ void load32(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]),
+                 "=r"(w[7])
+               : "l"(p));
+}
+
+__device__ __forceinline__ void store32(void* p, const uint2 (&w)[4]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0].x), "r"(w[0].y),
+               "r"(w[1].x), "r"(w[1].y), "r"(w[2].x), "r"(w[2].y), "r"(w[3].x), "r"(w[3].y)
+               : "memory");
+}
+
+// kLanes lanes a row, kElems (8 or 16) values a lane and vector, kRows rows a group, whose
+// loads overlap; blockIdx.y: 0 keys, 1 values.
+template <int kLanes, int kElems, int kVecs, int kRows>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheWriteArgs a,
                                                                    const Divider by_heads,
                                                                    uint32_t* err_word) {
@@ -82,29 +88,37 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheW
   const int lane = threadIdx.x % kLanes;
   const uint32_t first = blockIdx.x * (kStep * kRows) + threadIdx.x / kLanes;
   const uint32_t rows = static_cast<uint32_t>(a.rows);
-  const int nvec = a.d / 8;
-  uint4 v[kRows][kVecs];
+  constexpr int kWords = kElems / 2;
+  const int nvec = a.d / kElems;
+  uint32_t v[kRows][kVecs][kWords];
   int64_t slot[kRows];
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
     const uint32_t row = min(first + k * kStep, rows - 1);  // whole warps at the shuffles
     const uint32_t token = divide(row, by_heads), head = row - token * by_heads.d;
     slot[k] = first + k * kStep < rows ? __ldg(a.slots + token) : -1;
-    const uint4* x = reinterpret_cast<const uint4*>(src.x + token * src.token_stride + head * src.head_stride);
+    const uint16_t* x = src.x + token * src.token_stride + head * src.head_stride;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       const int j = lane + i * kLanes;
-      v[k][i] = j < nvec ? __ldg(x + j) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < kWords; ++e) v[k][i][e] = 0;
+      if (j >= nvec) continue;
+      if constexpr (kElems == 16) {
+        load32(x + j * 16, v[k][i]);
+      } else {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(x + j * 8));
+        v[k][i][0] = q.x, v[k][i][1] = q.y, v[k][i][2] = q.z, v[k][i][3] = q.w;
+      }
     }
   }
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
     uint32_t m2 = 0;  // max |x|, magnitude bits of the low and high halves (NaN on top)
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      m2 = max_u16x2(m2, max_u16x2(v[k][i].x & 0x7FFF7FFFu, v[k][i].y & 0x7FFF7FFFu));
-      m2 = max_u16x2(m2, max_u16x2(v[k][i].z & 0x7FFF7FFFu, v[k][i].w & 0x7FFF7FFFu));
-    }
+    for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+      for (int e = 0; e < kWords; ++e) m2 = max_u16x2(m2, v[k][i][e] & 0x7FFF7FFFu);
     uint32_t m = max(m2 & 0xFFFFu, m2 >> 16);
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
@@ -120,16 +134,21 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheW
     const float inv = __frcp_rn(scale);
     const int64_t at = slot[k] * a.heads + head;
     if (lane == 0) src.scale[at] = scale;
-    uint2* q = reinterpret_cast<uint2*>(src.codes + at * a.d);
+    uint8_t* q = src.codes + at * a.d;
+    const uint64_t inv2 = f2_pack(inv, inv);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
       const int j = lane + i * kLanes;
       if (j >= nvec) continue;
-      const uint32_t w[4] = {v[k][i].x, v[k][i].y, v[k][i].z, v[k][i].w};
-      uint32_t c[4];
+      uint32_t c[kWords / 2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) c[e] = e4m3x2(bf_lo(w[e]) * inv, bf_hi(w[e]) * inv);
-      q[j] = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+      for (int e = 0; e < kWords / 2; ++e)
+        c[e] = f2_to_e4m3x2(f2_mul(f2_of_bf16x2(v[k][i][2 * e]), inv2)) |
+               (f2_to_e4m3x2(f2_mul(f2_of_bf16x2(v[k][i][2 * e + 1]), inv2)) << 16);
+      if constexpr (kElems == 16)
+        *reinterpret_cast<uint4*>(q + j * 16) = make_uint4(c[0], c[1], c[2], c[3]);
+      else
+        *reinterpret_cast<uint2*>(q + j * 8) = make_uint2(c[0], c[1]);
     }
   }
 }
@@ -189,36 +208,41 @@ __global__ void __launch_bounds__(kCacheThreads)
     for (int u = 0; u < kReadUnroll; ++u) {
       const uint32_t i = i0 + u * kCacheThreads;
       if (i >= count) continue;
-      uint4* to = reinterpret_cast<uint4*>(out + static_cast<int64_t>(i) * kCodes);
+      uint16_t* to = out + static_cast<int64_t>(i) * kCodes;
+      uint2 w[kCodes / 4];
 #pragma unroll
-      for (int e = 0; e < kCodes / 8; ++e) {
-        const uint2 lo = dequantize4(c[u][2 * e], s[u]), hi = dequantize4(c[u][2 * e + 1], s[u]);
-        to[e] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      }
+      for (int e = 0; e < kCodes / 4; ++e) w[e] = dequantize4(c[u][e], s[u]);
+      if constexpr (kCodes == 16)
+        store32(to, w);
+      else
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
     }
   }
 }
 
-template <int kLanes, int kVecs, int kRows>
+template <int kLanes, int kElems, int kVecs, int kRows>
 void write_launch(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) {
   constexpr int kCtaRows = kCacheThreads / kLanes * kRows;
   const dim3 grid(static_cast<unsigned>((a.rows + kCtaRows - 1) / kCtaRows), 2);
-  cache_write_kernel<kLanes, kVecs, kRows><<<grid, kCacheThreads, 0, st>>>(a, divider(a.heads), err_word);
+  cache_write_kernel<kLanes, kElems, kVecs, kRows>
+      <<<grid, kCacheThreads, 0, st>>>(a, divider(a.heads), err_word);
 }
 
-template <int kLanes, int kVecs>
+template <int kLanes, int kElems, int kVecs = 1>
 void write_by_rows(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) {
-  // several rows a group once that still leaves every SM two thousand threads
+  // two rows a group once that still leaves every SM two thousand threads
   if (2 * a.rows * kLanes >= static_cast<int64_t>(sm_count()) * 2048 * 2)
-    write_launch<kLanes, kVecs, 4 / kVecs>(a, err_word, st);
+    write_launch<kLanes, kElems, kVecs, 2>(a, err_word, st);
   else
-    write_launch<kLanes, kVecs, 1>(a, err_word, st);
+    write_launch<kLanes, kElems, kVecs, 1>(a, err_word, st);
 }
 
 template <int kCodes>
 void read_launch(const CacheReadArgs& a, uint32_t* err_word, cudaStream_t st) {
   const int64_t per_token = static_cast<int64_t>(a.heads) * a.d / kCodes;
-  int64_t span = (kCacheThreads * kReadUnroll + per_token - 1) / per_token;
+  // whole tokens that one pass of the CTA covers (a long token takes several passes)
+  const int64_t fit = kCacheThreads * kReadUnroll / per_token;
+  const int64_t span = fit < 1 ? 1 : fit;
   const dim3 grid(static_cast<unsigned>((a.max_len + span - 1) / span), static_cast<unsigned>(a.batch), 2);
   cache_read_kernel<kCodes><<<grid, kCacheThreads, 0, st>>>(a, static_cast<int>(span), divider(per_token),
                                                             divider(a.d / kCodes), divider(a.page), err_word);
@@ -228,19 +252,27 @@ void read_launch(const CacheReadArgs& a, uint32_t* err_word, cudaStream_t st) {
 
 cudaError_t launch_cache_write(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) {
   if (a.rows <= 0) return cudaSuccess;
-  const int nvec = a.d / 8;
-  if (nvec <= 8) write_by_rows<8, 1>(a, err_word, st);
-  else if (nvec <= 16) write_by_rows<16, 1>(a, err_word, st);
-  else if (nvec <= 32) write_by_rows<32, 1>(a, err_word, st);
-  else if (nvec <= 64) write_by_rows<32, 2>(a, err_word, st);
-  else return cudaErrorInvalidValue;
+  const auto at = [](const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; };
+  const bool wide = a.d % 16 == 0 && at(a.k.x, 32) && at(a.v.x, 32) && at(a.k.codes, 16) &&
+                    at(a.v.codes, 16) && (a.k.token_stride | a.k.head_stride | a.v.token_stride | a.v.head_stride) % 16 == 0;
+  if (wide) {
+    if (a.d <= 64) write_by_rows<4, 16>(a, err_word, st);
+    else if (a.d <= 128) write_by_rows<8, 16>(a, err_word, st);
+    else if (a.d <= 256) write_by_rows<16, 16>(a, err_word, st);
+    else write_by_rows<32, 16>(a, err_word, st);
+  } else {
+    if (a.d <= 64) write_by_rows<8, 8>(a, err_word, st);
+    else if (a.d <= 128) write_by_rows<16, 8>(a, err_word, st);
+    else if (a.d <= 256) write_by_rows<32, 8>(a, err_word, st);
+    else write_by_rows<32, 8, 2>(a, err_word, st);
+  }
   return cudaGetLastError();
 }
 
 cudaError_t launch_cache_read(const CacheReadArgs& a, uint32_t* err_word, cudaStream_t st) {
   if (a.max_len <= 0 || a.batch <= 0) return cudaSuccess;
-  const auto at16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
-  if (a.d % 16 == 0 && at16(a.k_codes) && at16(a.v_codes))
+  const auto at = [](const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; };
+  if (a.d % 16 == 0 && at(a.k_codes, 16) && at(a.v_codes, 16) && at(a.k_out, 32) && at(a.v_out, 32))
     read_launch<16>(a, err_word, st);
   else
     read_launch<8>(a, err_word, st);

@@ -7,8 +7,8 @@
 //
 // Everything up to the outputs is fp32 in registers; each output is rounded once.  q multiplies
 // by one factor per row instead of dividing: three roundings of 2^-24 ahead of E4M3's 2^-4, a
-// third of the instructions.  A NaN in a row makes the row NaN, an
-// infinity gives what the formulas give (0 for the finite values, NaN for the infinite ones).
+// third of the instructions.  A NaN in a row makes the row NaN, an infinity gives what the
+// formulas give (0 for the finite values, NaN for the infinite ones).
 //
 // HBM-bound: x and r are read once, every output is written once; the row stays in registers
 // between the two reductions (sum of squares, then max |v| for E4M3).  Three forms:
@@ -18,9 +18,11 @@
 //   * many rows: persistent CTAs whose warps stream rows through rings in shared memory
 //     filled by bulk copies (rms_norm_stream_kernel), so that loads stay in flight while
 //     earlier rows are reduced and written.  A row that starts or ends off 16 bytes is
-//     fetched as the 16-byte aligned window around it.
-// In the first two forms such rows take element-wise loads (kVec = 1): neighbouring lanes
-// read neighbouring elements, so the sectors fetched are the same.
+//     fetched as the 16-byte aligned window around it, and where rows lie end to end its
+//     elements are taken in the pairs that are 4-byte aligned and its outputs leave through
+//     the row's buffer, by bulk copies (kVec = 2).
+// In the first two forms, and with other strides, such rows take element-wise accesses
+// (kVec = 1): neighbouring lanes read neighbouring elements, so the sectors fetched are the same.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -44,8 +46,24 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // Row elements are held as pairs (f2_*); a thread's share of a row is kPairs of them.  kVec 8:
 // pairs 4i .. 4i+3 are the eight adjacent elements of its i-th 16-byte vector; kVec 1: pair i
-// holds its elements 2i and 2i + 1, as many elements apart as the row has lanes.  `at(i)` is
-// the index of vector (kVec 8) or element (kVec 1) i; elements past d are zero, not stored.
+// holds its elements 2i and 2i + 1, as many elements apart as the row has lanes; kVec 2 (rows
+// in shared memory, in the streaming form): pair i is two adjacent elements whose place is
+// 4-byte aligned, so that the first pair of a row may start one element before it, and the
+// last one end one after it; what lies there is the slot's slack.  `at(i)` is the index of
+// vector (kVec 8), pair (kVec 2) or element (kVec 1) i; elements outside [0, d) are zero, and
+// not stored but to the slack.
+// Where a thread's vectors (kVec 8), pairs (2) or elements (1) lie in a row.  kVec 2: pairs
+// [1, full) of every lane lie inside the row, so only the first and the last ones need bounds
+// (with bounds on every pair they were two thirds of the instructions).
+template <int kVec, int kLanes = 0>
+struct Place {
+  int lane, lanes, odd, full;
+  __device__ __forceinline__ int operator()(int i) const {
+    return (lane + i * (kLanes == 0 ? lanes : kLanes)) * kVec - (kVec == 2 ? odd : 0);
+  }
+  __device__ __forceinline__ bool inner(int i) const { return i > 0 && i < full; }
+};
+
 template <int kPairs, int kVec, class At>
 __device__ __forceinline__ void load_bf16(uint32_t (&w)[kPairs], const uint16_t* p, int d, At at) {
   if constexpr (kVec == 8) {
@@ -55,6 +73,14 @@ __device__ __forceinline__ void load_bf16(uint32_t (&w)[kPairs], const uint16_t*
       if (at(i) < d) v = *reinterpret_cast<const uint4*>(p + at(i));
       w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
     }
+  } else if constexpr (kVec == 2) {
+    // from a slot in shared memory, whose slack covers the elements on either side of the row;
+    // the caller drops them (mask_pairs)
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      w[i] = 0;
+      if (at.inner(i) || at(i) < d) w[i] = *reinterpret_cast<const uint32_t*>(p + at(i));
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
@@ -62,6 +88,21 @@ __device__ __forceinline__ void load_bf16(uint32_t (&w)[kPairs], const uint16_t*
       const uint32_t hi = at(2 * i + 1) < d ? p[at(2 * i + 1)] : 0u;
       w[i] = lo | (hi << 16);
     }
+  }
+}
+
+// The weight's share: global memory of any alignment.
+template <int kPairs, int kVec, class At>
+__device__ __forceinline__ void load_weight(uint32_t (&w)[kPairs], const uint16_t* p, int d, At at) {
+  if constexpr (kVec == 2) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const uint32_t lo = at(i) >= 0 && at(i) < d ? p[at(i)] : 0u;
+      const uint32_t hi = at(i) + 1 < d ? p[at(i) + 1] : 0u;
+      w[i] = lo | (hi << 16);
+    }
+  } else {
+    load_bf16<kPairs, kVec>(w, p, d, at);
   }
 }
 
@@ -80,6 +121,11 @@ __device__ __forceinline__ void add_f32(uint64_t (&s)[kPairs], const float* p, i
         s[4 * i + 3] = f2_add(s[4 * i + 3], f2_pack(b.z, b.w));
       }
     }
+  } else if constexpr (kVec == 2) {
+#pragma unroll
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i)
+      if (at.inner(i) || at(i) < d) s[i] = f2_add(s[i], *reinterpret_cast<const uint64_t*>(p + at(i)));
   } else {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
@@ -103,6 +149,10 @@ __device__ __forceinline__ void store_f32(float* p, const uint64_t (&s)[kPairs],
         reinterpret_cast<float4*>(p + at(i))[1] = make_float4(f[4], f[5], f[6], f[7]);
       }
     }
+  } else if constexpr (kVec == 2) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i)
+      if (at.inner(i) || at(i) < d) *reinterpret_cast<uint64_t*>(p + at(i)) = s[i];
   } else {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
@@ -125,6 +175,12 @@ __device__ __forceinline__ void store_bf16(uint16_t* p, const uint64_t (&s)[kPai
         *reinterpret_cast<uint4*>(p + at(i)) =
             make_uint4(f2_to_bf16x2(f2_mul(s[4 * i], f)), f2_to_bf16x2(f2_mul(s[4 * i + 1], f)),
                        f2_to_bf16x2(f2_mul(s[4 * i + 2], f)), f2_to_bf16x2(f2_mul(s[4 * i + 3], f)));
+  } else if constexpr (kVec == 2) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const uint32_t w = f2_to_bf16x2(f2_mul(s[i], f));
+      if (at.inner(i) || at(i) < d) *reinterpret_cast<uint32_t*>(p + at(i)) = w;
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
@@ -146,6 +202,12 @@ __device__ __forceinline__ void store_e4m3(uint8_t* p, const uint64_t (&s)[kPair
         *reinterpret_cast<uint2*>(p + at(i)) =
             make_uint2(f2_to_e4m3x2(f2_mul(s[4 * i], f)) | (f2_to_e4m3x2(f2_mul(s[4 * i + 1], f)) << 16),
                        f2_to_e4m3x2(f2_mul(s[4 * i + 2], f)) | (f2_to_e4m3x2(f2_mul(s[4 * i + 3], f)) << 16));
+  } else if constexpr (kVec == 2) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const uint32_t w = f2_to_e4m3x2(f2_mul(s[i], f));
+      if (at.inner(i) || at(i) < d) *reinterpret_cast<uint16_t*>(p + at(i)) = static_cast<uint16_t>(w);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
@@ -170,6 +232,17 @@ __device__ __forceinline__ void add_residual(uint64_t (&s)[kPairs], const void* 
     for (int i = 0; i < kPairs; ++i) s[i] = f2_add(s[i], f2_of_bf16x2(w[i]));
     if (store)
       store_bf16<kPairs, kVec>(static_cast<uint16_t*>(out), s, f2_pack(1.0f, 1.0f), d, at);
+  }
+}
+
+// kVec 2: zeros in place of the elements outside the row.
+template <int kPairs, class At>
+__device__ __forceinline__ void mask_pairs(uint64_t (&s)[kPairs], int d, At at) {
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    if (at.inner(i)) continue;
+    if (at(i) < 0 || at(i) >= d) s[i] &= 0xFFFFFFFF00000000ull;
+    if (at(i) + 1 >= d) s[i] &= 0x00000000FFFFFFFFull;
   }
 }
 
@@ -251,7 +324,7 @@ __global__ void __launch_bounds__(kLanes == 0 ? kNormMaxThreads : kNormThreads)
   const int lanes = kLanes == 0 ? static_cast<int>(blockDim.x) : kLanes;
   const int lane = kLanes == 0 ? static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x) % lanes;
   const int d = a.d;
-  const auto at = [lane, lanes](int i) { return (lane + i * lanes) * kVec; };
+  const Place<kVec> at = {lane, lanes, 0, 0};
   // kRows rows, `step` apart, so that neighbouring groups read neighbouring rows
   const int64_t step = kLanes == 0 ? 1 : kNormThreads / lanes;
   const int64_t first = kLanes == 0 ? static_cast<int64_t>(blockIdx.x)
@@ -261,7 +334,7 @@ __global__ void __launch_bounds__(kLanes == 0 ? kNormMaxThreads : kNormThreads)
   for (int k = 0; k < kRows; ++k)  // a row past the last one repeats it: the warp's shuffles stay whole
     load_bf16<kPairs, kVec>(xw[k], x_row(a, min(first + k * step, a.rows - 1)), d, at);
   uint32_t w[kPairs];
-  if (a.weight != nullptr) load_bf16<kPairs, kVec>(w, a.weight, d, at);
+  if (a.weight != nullptr) load_weight<kPairs, kVec>(w, a.weight, d, at);
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
     const bool live = first + k * step < a.rows;
@@ -346,6 +419,28 @@ __device__ __forceinline__ float group_reduce(float v, float* smem, int group, i
   return v;
 }
 
+// A row of `bytes` (elements of `elem`) from shared to global memory, both at the same offset
+// in 16 bytes: the whole 16-byte pieces by one bulk copy (lane 0's; committed by the caller),
+// the elements before and after them by the first lanes.
+__device__ __forceinline__ void flush_row(uint8_t* to, const uint8_t* from, int bytes, int elem, int lane) {
+  const int head = min(bytes, static_cast<int>((16u - (reinterpret_cast<uintptr_t>(to) & 15u)) & 15u));
+  const int body = (bytes - head) & ~15;
+  if (lane == 0 && body > 0)
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to + head),
+                 "r"(smem_u32(from + head)), "r"(body)
+                 : "memory");
+  const int tail = bytes - head - body;  // head and tail hold at most 15 elements each
+  const int at = lane < 16 ? lane * elem : head + body + (lane - 16) * elem;
+  if (lane < 32 && (lane < 16 ? lane * elem < head : (lane - 16) * elem < tail)) {
+    if (elem == 4)
+      *reinterpret_cast<uint32_t*>(to + at) = *reinterpret_cast<const uint32_t*>(from + at);
+    else if (elem == 2)
+      *reinterpret_cast<uint16_t*>(to + at) = *reinterpret_cast<const uint16_t*>(from + at);
+    else
+      to[at] = from[at];
+  }
+}
+
 template <int kGroup, int kPer, int kVec>
 __global__ void __launch_bounds__(kStreamThreads, 1)
     rms_norm_stream_kernel(const NormArgs a, const StreamPlan p, const uint64_t wait_limit,
@@ -365,9 +460,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   uint64_t* bar = bars + group * kStreamSlotsMax;
   uint8_t* ring = smem + kStreamHead + group * p.slots * p.slot_bytes;
   const int d = a.d;
-  const auto at = [lane](int i) { return (lane + i * kLanes) * kVec; };
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kGroups;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+  // kVec 2: rows of odd length start at odd elements every second time; `stride` is even, so
+  // all rows of a group start alike
+  const int odd = kVec == 2 ? static_cast<int>(row0 * d & 1) : 0;
+  const Place<kVec, kLanes> at = {lane, kLanes, odd, (d + odd) / (2 * kLanes)};
   const int res_bytes = a.residual == nullptr ? 0 : a.residual_f32 ? 4 : 2;
 
   const auto x_window = [&](int64_t row) {
@@ -401,7 +499,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       if (row0 + s * stride < a.rows) fetch(row0 + s * stride, s);
   }
   uint32_t w[kPairs];
-  if (a.weight != nullptr) load_bf16<kPairs, kVec>(w, a.weight, d, at);
+  if (a.weight != nullptr) load_weight<kPairs, kVec>(w, a.weight, d, at);
   __syncthreads();  // the barriers are initialised
 
   int slot = 0;
@@ -410,7 +508,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     uint8_t* xs = ring + slot * p.slot_bytes;
     uint8_t* rs = xs + p.x_bytes;
     bool whole = true;
-    if constexpr (kVec == 1) {  // with 16-byte rows every window is its row
+    if constexpr (kVec != 8) {  // with 16-byte rows every window is its row
       const Window xw = x_window(row);
       xs += xw.off;
       whole = xw.whole;
@@ -447,26 +545,51 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) s[i] = f2_of_bf16x2(xw[i]);
     const int64_t base = row * d;
-    if (res_bytes != 0)
-      add_residual<kPairs, kVec>(s, rs, res_bytes == 4, static_cast<uint8_t*>(a.residual_out) + base * res_bytes,
-                                 true, d, at);
+    if (res_bytes != 0) {
+      uint8_t* to = kVec == 2 ? rs : static_cast<uint8_t*>(a.residual_out) + base * res_bytes;
+      add_residual<kPairs, kVec>(s, rs, res_bytes == 4, to, true, d, at);
+    }
+    if constexpr (kVec == 2) mask_pairs(s, d, at);
     float sq = sum_squares(s);
     group_sync<kGroup>(group);  // the group holds the row (and has left the partials)
-    if (leader && row + p.slots * stride < a.rows) fetch(row + p.slots * stride, slot);
+    if constexpr (kVec == 2) {
+      // the previous row's slot held its outputs: free once their copies have read it
+      if (leader && row != row0) {
+        bulk_wait_group_read0();
+        const int64_t next = row + (p.slots - 1) * stride;
+        if (next < a.rows) fetch(next, slot == 0 ? p.slots - 1 : slot - 1);
+      }
+    } else {
+      if (leader && row + p.slots * stride < a.rows) fetch(row + p.slots * stride, slot);
+    }
     sq = group_reduce<kGroup>(sq, sums + group * kGroup, group, in_group,
                               [](float x, float y) { return x + y; });
     const float rstd = rsqrtf(sq / static_cast<float>(d) + a.eps);
     if (a.weight != nullptr) apply_weight(s, w);
-    if (a.y != nullptr) store_bf16<kPairs, kVec>(a.y + base, s, f2_pack(rstd, rstd), d, at);
+    if (a.y != nullptr)
+      store_bf16<kPairs, kVec>(kVec == 2 ? reinterpret_cast<uint16_t*>(xs) : a.y + base, s, f2_pack(rstd, rstd),
+                               d, at);
+    uint8_t* qs = a.q + base;  // kVec 2: in x's place, at its own offset in 16 bytes
+    if constexpr (kVec == 2) qs = ring + slot * p.slot_bytes + (reinterpret_cast<uintptr_t>(a.q + base) & 15u);
     if (a.q != nullptr) {
       const float m = group_reduce<kGroup>(max_abs(s), maxima + group * kGroup, group, in_group,
                                            [](float x, float y) { return max_nan(x, y); });
       const float scale = scale448(m * rstd), f = rstd * __frcp_rn(scale);
       if (leader) a.scale[row] = scale;
-      store_e4m3<kPairs, kVec>(a.q + base, s, f2_pack(f, f), d, at);
+      store_e4m3<kPairs, kVec>(qs, s, f2_pack(f, f), d, at);
+    }
+    if constexpr (kVec == 2) {
+      fence_proxy_async_smem();
+      group_sync<kGroup>(group);
+      if (res_bytes != 0)
+        flush_row(static_cast<uint8_t*>(a.residual_out) + base * res_bytes, rs, d * res_bytes, res_bytes, lane);
+      if (a.y != nullptr) flush_row(reinterpret_cast<uint8_t*>(a.y + base), xs, 2 * d, 2, lane);
+      if (a.q != nullptr) flush_row(a.q + base, qs, d, 1, lane);
+      if (leader) bulk_commit_group();
     }
     if (++slot == p.slots) slot = 0;
   }
+  if (kVec == 2 && leader) bulk_wait_group0();  // the copies out of shared memory are complete
 }
 
 template <int kLanes, int kRows, int kPer>
@@ -482,9 +605,10 @@ void norm_launch(const NormArgs& a, bool vec, cudaStream_t st) {
 
 template <int kLanes>
 void norm_short(const NormArgs& a, bool vec, cudaStream_t st) {
-  // four rows a group once that still leaves every SM its threads
-  if (a.rows * kLanes >= static_cast<int64_t>(sm_count()) * 2048 * 4)
-    norm_launch<kLanes, 4, 8>(a, vec, st);
+  // two rows a group once that still leaves every SM its threads (92160 rows of 128: 10.0 us
+  // with one, 9.0 with two, 9.4 with four)
+  if (a.rows * kLanes >= static_cast<int64_t>(sm_count()) * 2048 * 2)
+    norm_launch<kLanes, 2, 8>(a, vec, st);
   else
     norm_launch<kLanes, 1, 8>(a, vec, st);
 }
@@ -504,11 +628,19 @@ cudaError_t stream_launch(const NormArgs& a, const StreamPlan& p, uint64_t wait_
 template <int kGroup, int kVec>
 cudaError_t stream_by_width(const NormArgs& a, const StreamPlan& p, uint64_t wait_limit,
                             uint32_t* err_word, cudaStream_t st) {
-  const int per = (a.d + 32 * kGroup - 1) / (32 * kGroup);
+  const int per = (a.d + (kVec == 2 ? 1 : 0) + 32 * kGroup - 1) / (32 * kGroup);
   if (per <= 16) return stream_launch<kGroup, 16, kVec>(a, p, wait_limit, err_word, st);
   if (per <= 32) return stream_launch<kGroup, 32, kVec>(a, p, wait_limit, err_word, st);
   if (per <= 48) return stream_launch<kGroup, 48, kVec>(a, p, wait_limit, err_word, st);
   return stream_launch<kGroup, 64, kVec>(a, p, wait_limit, err_word, st);
+}
+
+template <int kGroup>
+cudaError_t stream_by_form(const NormArgs& a, const StreamPlan& p, int form, uint64_t wait_limit,
+                           uint32_t* err_word, cudaStream_t st) {
+  if (form == 8) return stream_by_width<kGroup, 8>(a, p, wait_limit, err_word, st);
+  if (form == 2) return stream_by_width<kGroup, 2>(a, p, wait_limit, err_word, st);
+  return stream_by_width<kGroup, 1>(a, p, wait_limit, err_word, st);
 }
 
 }  // namespace
@@ -542,24 +674,27 @@ cudaError_t launch_rms_norm(const NormArgs& args, uint64_t wait_limit, cudaStrea
     p.x_bytes = (2 * d + slack + 15) / 16 * 16;
     p.slot_bytes = p.x_bytes + (res == 0 ? 0 : (res * d + slack + 15) / 16 * 16);
     int group = 1;
-    while (group < 16 && (d > 32 * group * 64 || kStreamWarps / group * 2 * p.slot_bytes > kStreamSmem))
+    while (group < 16 && (d + 1 > 32 * group * 64 || kStreamWarps / group * 2 * p.slot_bytes > kStreamSmem))
       group *= 2;
     p.slots = kStreamSmem / (kStreamWarps / group) / p.slot_bytes;
     if (p.slots > kStreamSlotsMax) p.slots = kStreamSlotsMax;
+    const auto off = [](const void* q, uintptr_t mask) { return (reinterpret_cast<uintptr_t>(q) & mask) != 0; };
+    const bool even = (sm_count() * (kStreamWarps / group)) % 2 == 0;
+    // one output, rows end to end from 16-byte aligned starts: every row of every tensor but q
+    // then has its x's offset
+    const bool pairs = !vec && a.inner == 1 && a.outer_stride == d && even && !off(a.x, 15) && !off(a.y, 15) &&
+                       !off(a.q, 15) && !off(a.residual, 15) && !off(a.residual_out, 15) &&
+                       (a.y == nullptr || a.q == nullptr);
     if (a.rows >= static_cast<int64_t>(sm_count()) * (kStreamWarps / group) * 2) {
       uint32_t* err_word = error_word_ptr();
       if (err_word == nullptr) return cudaErrorInvalidSymbol;
-      switch (group * 2 + (vec ? 1 : 0)) {
-        case 2: return stream_by_width<1, 1>(a, p, wait_limit, err_word, st);
-        case 3: return stream_by_width<1, 8>(a, p, wait_limit, err_word, st);
-        case 4: return stream_by_width<2, 1>(a, p, wait_limit, err_word, st);
-        case 5: return stream_by_width<2, 8>(a, p, wait_limit, err_word, st);
-        case 8: return stream_by_width<4, 1>(a, p, wait_limit, err_word, st);
-        case 9: return stream_by_width<4, 8>(a, p, wait_limit, err_word, st);
-        case 16: return stream_by_width<8, 1>(a, p, wait_limit, err_word, st);
-        case 17: return stream_by_width<8, 8>(a, p, wait_limit, err_word, st);
-        case 32: return stream_by_width<16, 1>(a, p, wait_limit, err_word, st);
-        default: return stream_by_width<16, 8>(a, p, wait_limit, err_word, st);
+      const int form = vec ? 8 : pairs ? 2 : 1;
+      switch (group) {
+        case 1: return stream_by_form<1>(a, p, form, wait_limit, err_word, st);
+        case 2: return stream_by_form<2>(a, p, form, wait_limit, err_word, st);
+        case 4: return stream_by_form<4>(a, p, form, wait_limit, err_word, st);
+        case 8: return stream_by_form<8>(a, p, form, wait_limit, err_word, st);
+        default: return stream_by_form<16>(a, p, form, wait_limit, err_word, st);
       }
     }
     if (d <= 8 * kNormMaxThreads)
