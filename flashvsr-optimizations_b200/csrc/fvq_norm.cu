@@ -248,11 +248,11 @@ __device__ __forceinline__ void mask_pairs(uint64_t (&s)[kPairs], int d, At at) 
 
 template <int kPairs>
 __device__ __forceinline__ float sum_squares(const uint64_t (&s)[kPairs]) {
-  uint64_t q = 0;
+  uint64_t q[4] = {0, 0, 0, 0};  // four chains: one of 24 dependent steps is longer than the row's loads
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) q = f2_fma(s[i], s[i], q);
+  for (int i = 0; i < kPairs; ++i) q[i % 4] = f2_fma(s[i], s[i], q[i % 4]);
   float lo, hi;
-  f2_split(q, lo, hi);
+  f2_split(f2_add(f2_add(q[0], q[1]), f2_add(q[2], q[3])), lo, hi);
   return lo + hi;
 }
 
@@ -265,14 +265,15 @@ __device__ __forceinline__ void apply_weight(uint64_t (&s)[kPairs], const uint32
 
 template <int kPairs>
 __device__ __forceinline__ float max_abs(const uint64_t (&s)[kPairs]) {
-  float m = 0.0f;
+  float m[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
     float lo, hi;
     f2_split(s[i], lo, hi);
-    m = max_nan(max_nan(m, fabsf(lo)), fabsf(hi));
+    m[2 * (i % 2)] = max_nan(m[2 * (i % 2)], fabsf(lo));
+    m[2 * (i % 2) + 1] = max_nan(m[2 * (i % 2) + 1], fabsf(hi));
   }
-  return m;
+  return max_nan(max_nan(m[0], m[1]), max_nan(m[2], m[3]));
 }
 
 // max(m / 448, 1e-12); NaN stays NaN
@@ -378,23 +379,42 @@ struct StreamPlan {
   int slots;
 };
 
-// The 16-byte window around a row of `bytes` at p; whole: it lies inside [begin, end).
-struct Window {
-  const uint8_t* lo;
+// What a bulk copy fetches of a row: the 16-byte pieces around it, less those that are not
+// wholly inside the tensor (first and last row).  Both ends of the tensor are given rounded
+// inwards.
+struct Piece {
+  const uint8_t* lo;  // first byte fetched
   uint32_t bytes;
-  uint32_t off;    // of the row in the window
-  bool whole;
+  uint32_t off;       // of the row in its slot
+  uint32_t skip;      // of the fetched bytes in the slot
 };
 
-__device__ __forceinline__ Window window(const void* p, uint32_t bytes, const void* begin,
-                                         const void* end) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
-  Window w;
-  w.off = static_cast<uint32_t>(at & 15u);
-  w.lo = reinterpret_cast<const uint8_t*>(at - w.off);
-  w.bytes = (w.off + bytes + 15u) & ~15u;
-  w.whole = w.lo >= static_cast<const uint8_t*>(begin) && w.lo + w.bytes <= static_cast<const uint8_t*>(end);
-  return w;
+__device__ __forceinline__ Piece piece_of(const uint8_t* row, uint32_t bytes, const uint8_t* begin16,
+                                          const uint8_t* end16) {
+  Piece p;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row);
+  p.off = static_cast<uint32_t>(at & 15u);
+  const uint8_t* first = row - p.off;
+  const uint8_t* last = first + ((p.off + bytes + 15u) & ~15u);
+  p.lo = first < begin16 ? begin16 : first;
+  p.skip = static_cast<uint32_t>(p.lo - first);
+  p.bytes = static_cast<uint32_t>((last > end16 ? end16 : last) - p.lo);
+  return p;
+}
+
+// The elements of a row that its piece leaves out (at most 15 bytes at either end), by the
+// first lanes.  Returns whether there were any.
+template <class T>
+__device__ __forceinline__ bool patch_row(const uint8_t* row, uint8_t* slot_row, uint32_t bytes, const Piece& p,
+                                          int lane) {
+  const uint32_t head = p.lo > row ? static_cast<uint32_t>(p.lo - row) : 0u;
+  const uint32_t got = static_cast<uint32_t>(p.lo - row) + p.bytes;  // modulo 2^32: the end of the piece
+  const uint32_t tail = got < bytes ? bytes - got : 0u;
+  if (head == 0 && tail == 0) return false;
+  const uint32_t at = lane * static_cast<uint32_t>(sizeof(T));
+  if (at < head) *reinterpret_cast<T*>(slot_row + at) = *reinterpret_cast<const T*>(row + at);
+  if (at < tail) *reinterpret_cast<T*>(slot_row + got + at) = *reinterpret_cast<const T*>(row + got + at);
+  return true;
 }
 
 template <int kGroup>
@@ -451,7 +471,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   constexpr int kPairs = kPer / 2;
   auto* bars = reinterpret_cast<uint64_t*>(smem);                          // [groups][slots]
   auto* sums = reinterpret_cast<float*>(smem + kStreamWarps * kStreamSlotsMax * 8);
-  auto* maxima = sums + kStreamWarps;
+  auto* maxima = sums + 2 * kStreamWarps;
   auto* lost = reinterpret_cast<volatile int*>(maxima + kStreamWarps);      // a load never landed
   const int warp = threadIdx.x >> 5;
   const int group = warp / kGroup, in_group = warp % kGroup;
@@ -468,26 +488,37 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   const Place<kVec, kLanes> at = {lane, kLanes, odd, (d + odd) / (2 * kLanes)};
   const int res_bytes = a.residual == nullptr ? 0 : a.residual_f32 ? 4 : 2;
 
-  const auto x_window = [&](int64_t row) {
-    return window(x_row(a, row), 2u * d, a.x, x_row(a, a.rows - 1) + d);
-  };
   const auto r_row = [&](int64_t row) {
     return static_cast<const uint8_t*>(a.residual) + row * d * res_bytes;
   };
-  const auto r_window = [&](int64_t row) {
-    return window(r_row(row), static_cast<uint32_t>(d * res_bytes), a.residual, r_row(a.rows));
+  const uint32_t x_size = 2u * d, r_size = static_cast<uint32_t>(d * res_bytes);
+  const auto up16 = [](const void* q) {
+    return reinterpret_cast<const uint8_t*>((reinterpret_cast<uintptr_t>(q) + 15u) & ~static_cast<uintptr_t>(15u));
   };
-  // A row whose window would leave its tensor (the first or last one, off 16 bytes) is copied
-  // by the group itself when its turn comes.
-  const auto fetch = [&](int64_t row, int slot) {
-    const Window x = x_window(row);
-    Window r = {nullptr, 0u, 0u, true};
-    if (res_bytes != 0) r = r_window(row);
-    if (!x.whole || !r.whole) return;
+  const auto down16 = [](const void* q) {
+    return reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(q) & ~static_cast<uintptr_t>(15u));
+  };
+  const uint8_t* x_begin = up16(a.x);
+  const uint8_t* x_end = down16(x_row(a, a.rows - 1) + d);
+  const uint8_t* r_begin = up16(a.residual);
+  const uint8_t* r_end = res_bytes == 0 ? nullptr : down16(r_row(a.rows));
+  const auto x_piece = [&](const uint8_t* row) {
+    if constexpr (kVec == 8) return Piece{row, x_size, 0u, 0u};
+    return piece_of(row, x_size, x_begin, x_end);
+  };
+  const auto r_piece = [&](const uint8_t* row) {
+    if constexpr (kVec == 8) return Piece{row, r_size, 0u, 0u};
+    return piece_of(row, r_size, r_begin, r_end);
+  };
+  const auto fetch = [&](int64_t row, int slot) {  // the leader
+    if (row >= a.rows) return;
+    const Piece x = x_piece(reinterpret_cast<const uint8_t*>(x_row(a, row)));
+    Piece r = {nullptr, 0u, 0u, 0u};
+    if (res_bytes != 0) r = r_piece(r_row(row));
     mbar_arrive_expect_tx(&bar[slot], x.bytes + r.bytes);
     uint8_t* to = ring + slot * p.slot_bytes;
-    bulk_load(to, x.lo, x.bytes, &bar[slot]);
-    if (res_bytes != 0) bulk_load(to + p.x_bytes, r.lo, r.bytes, &bar[slot]);
+    bulk_load(to + x.skip, x.lo, x.bytes, &bar[slot]);
+    if (res_bytes != 0) bulk_load(to + p.x_bytes + r.skip, r.lo, r.bytes, &bar[slot]);
   };
 
   if (threadIdx.x == 0) *lost = 0;
@@ -495,76 +526,74 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     for (int s = 0; s < p.slots; ++s) mbar_init(&bar[s], 1);
     fence_barrier_init();
     fence_proxy_async_smem();
-    for (int s = 0; s < p.slots; ++s)
-      if (row0 + s * stride < a.rows) fetch(row0 + s * stride, s);
+    for (int s = 0; s < p.slots; ++s) fetch(row0 + s * stride, s);
   }
+  // the weight stays in registers up to 48 values a lane, and comes from L1 for every row beyond
+  constexpr bool kKeepWeight = kPer <= 48;
   uint32_t w[kPairs];
-  if (a.weight != nullptr) load_weight<kPairs, kVec>(w, a.weight, d, at);
+  if (kKeepWeight && a.weight != nullptr) load_weight<kPairs, kVec>(w, a.weight, d, at);
   __syncthreads();  // the barriers are initialised
 
+  const float inv_d = 1.0f / static_cast<float>(d);
+  int64_t base = row0 * d;
+  const int64_t base_step = stride * d;
   int slot = 0;
+  int turn = 0;
   uint32_t phases = 0;        // bit s: parity of slot s
-  for (int64_t row = row0; row < a.rows; row += stride) {
+  for (int64_t row = row0; row < a.rows; row += stride, base += base_step) {
     uint8_t* xs = ring + slot * p.slot_bytes;
     uint8_t* rs = xs + p.x_bytes;
-    bool whole = true;
-    if constexpr (kVec != 8) {  // with 16-byte rows every window is its row
-      const Window xw = x_window(row);
-      xs += xw.off;
-      whole = xw.whole;
-      if (res_bytes != 0) {
-        const Window rw = r_window(row);
-        rs += rw.off;
-        whole = whole && rw.whole;
-      }
+    // A wait that runs out is reported, and waited for once more: the ring stays in step, and
+    // no load is in flight when the CTA exits.
+    const uint32_t parity = (phases >> slot) & 1u;
+    if (*lost == 0 && !mbar_wait_bounded(&bar[slot], parity, wait_limit)) {
+      atomicOr(err_word, kErrWaitProducer);
+      if (!mbar_wait_bounded(&bar[slot], parity, wait_limit > kDefaultWaitLimit ? wait_limit : kDefaultWaitLimit))
+        *lost = 1;  // later rows are not waited for; their outputs are undefined
     }
-    if (whole) {
-      // A wait that runs out is reported, and waited for once more: the ring stays in step,
-      // and no load is in flight when the CTA exits.
-      const uint32_t parity = (phases >> slot) & 1u;
-      if (*lost == 0 && !mbar_wait_bounded(&bar[slot], parity, wait_limit)) {
-        atomicOr(err_word, kErrWaitProducer);
-        if (!mbar_wait_bounded(&bar[slot], parity, wait_limit > kDefaultWaitLimit ? wait_limit : kDefaultWaitLimit))
-          *lost = 1;  // later rows are not waited for; their outputs are undefined
+    phases ^= 1u << slot;
+    if constexpr (kVec != 8) {
+      const uint8_t* from = reinterpret_cast<const uint8_t*>(x_row(a, row));
+      const Piece x = x_piece(from);
+      xs += x.off;
+      bool patched = patch_row<uint16_t>(from, xs, x_size, x, lane);
+      if (res_bytes != 0) {
+        const Piece r = r_piece(r_row(row));
+        rs += r.off;
+        patched |= res_bytes == 4 ? patch_row<float>(r_row(row), rs, r_size, r, lane)
+                                  : patch_row<uint16_t>(r_row(row), rs, r_size, r, lane);
       }
-      phases ^= 1u << slot;
-    } else {
-      for (int j = lane; j < d; j += kLanes) {
-        reinterpret_cast<uint16_t*>(xs)[j] = __ldg(x_row(a, row) + j);
-        if (res_bytes == 4)
-          reinterpret_cast<float*>(rs)[j] = __ldg(reinterpret_cast<const float*>(r_row(row)) + j);
-        else if (res_bytes == 2)
-          reinterpret_cast<uint16_t*>(rs)[j] = __ldg(reinterpret_cast<const uint16_t*>(r_row(row)) + j);
+      if (patched) {
+        fence_proxy_async_smem();  // the slot's next bulk copy comes after these stores
+        group_sync<kGroup>(group);
       }
-      fence_proxy_async_smem();  // the slot's next bulk copy comes after these stores
-      group_sync<kGroup>(group);
     }
     uint32_t xw[kPairs];
     load_bf16<kPairs, kVec>(xw, reinterpret_cast<const uint16_t*>(xs), d, at);
     uint64_t s[kPairs];
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) s[i] = f2_of_bf16x2(xw[i]);
-    const int64_t base = row * d;
     if (res_bytes != 0) {
       uint8_t* to = kVec == 2 ? rs : static_cast<uint8_t*>(a.residual_out) + base * res_bytes;
       add_residual<kPairs, kVec>(s, rs, res_bytes == 4, to, true, d, at);
     }
     if constexpr (kVec == 2) mask_pairs(s, d, at);
-    float sq = sum_squares(s);
-    group_sync<kGroup>(group);  // the group holds the row (and has left the partials)
+    // the partial sums alternate between two places, so that the reduction's own barrier is the
+    // one that says the group holds the row and has left the last row's partials
+    const float sq = group_reduce<kGroup>(sum_squares(s), sums + (turn ^= 1) * kStreamWarps + group * kGroup, group,
+                                          in_group, [](float x, float y) { return x + y; });
+    if constexpr (kGroup == 1) __syncwarp();
     if constexpr (kVec == 2) {
       // the previous row's slot held its outputs: free once their copies have read it
       if (leader && row != row0) {
         bulk_wait_group_read0();
-        const int64_t next = row + (p.slots - 1) * stride;
-        if (next < a.rows) fetch(next, slot == 0 ? p.slots - 1 : slot - 1);
+        fetch(row + (p.slots - 1) * stride, slot == 0 ? p.slots - 1 : slot - 1);
       }
     } else {
-      if (leader && row + p.slots * stride < a.rows) fetch(row + p.slots * stride, slot);
+      if (leader) fetch(row + p.slots * stride, slot);
     }
-    sq = group_reduce<kGroup>(sq, sums + group * kGroup, group, in_group,
-                              [](float x, float y) { return x + y; });
-    const float rstd = rsqrtf(sq / static_cast<float>(d) + a.eps);
+    const float rstd = rsqrtf(fmaf(sq, inv_d, a.eps));
+    if (!kKeepWeight && a.weight != nullptr) load_weight<kPairs, kVec>(w, a.weight, d, at);
     if (a.weight != nullptr) apply_weight(s, w);
     if (a.y != nullptr)
       store_bf16<kPairs, kVec>(kVec == 2 ? reinterpret_cast<uint16_t*>(xs) : a.y + base, s, f2_pack(rstd, rstd),
@@ -632,7 +661,7 @@ cudaError_t stream_by_width(const NormArgs& a, const StreamPlan& p, uint64_t wai
   if (per <= 16) return stream_launch<kGroup, 16, kVec>(a, p, wait_limit, err_word, st);
   if (per <= 32) return stream_launch<kGroup, 32, kVec>(a, p, wait_limit, err_word, st);
   if (per <= 48) return stream_launch<kGroup, 48, kVec>(a, p, wait_limit, err_word, st);
-  return stream_launch<kGroup, 64, kVec>(a, p, wait_limit, err_word, st);
+  return stream_launch<kGroup, 72, kVec>(a, p, wait_limit, err_word, st);
 }
 
 template <int kGroup>
@@ -674,7 +703,7 @@ cudaError_t launch_rms_norm(const NormArgs& args, uint64_t wait_limit, cudaStrea
     p.x_bytes = (2 * d + slack + 15) / 16 * 16;
     p.slot_bytes = p.x_bytes + (res == 0 ? 0 : (res * d + slack + 15) / 16 * 16);
     int group = 1;
-    while (group < 16 && (d + 1 > 32 * group * 64 || kStreamWarps / group * 2 * p.slot_bytes > kStreamSmem))
+    while (group < 16 && (d + 1 > 32 * group * 72 || kStreamWarps / group * 2 * p.slot_bytes > kStreamSmem))
       group *= 2;
     p.slots = kStreamSmem / (kStreamWarps / group) / p.slot_bytes;
     if (p.slots > kStreamSlotsMax) p.slots = kStreamSlotsMax;
