@@ -519,6 +519,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 constexpr int kSplitStagesMax = 16;
 constexpr int kSplitMax = 8;                      // CTAs per cluster (the portable limit)
 constexpr int kSplitThreads = 320;                // producer, MMA issuer, eight epilogue warps
+constexpr int kJoinThreads = 256;                 // a power of two, so that a thread keeps its columns
 constexpr int kSplitBarrierBytes = 512;
 // An MMA reads 128 W rows; a tile of fewer rows is followed by whatever comes next in shared
 // memory (it ends in accumulator rows that nobody reads), so the ring is followed by a pad.
@@ -545,7 +546,15 @@ struct SplitPlan {
   int split;      // CTAs per cluster sharing one tile's K
   int group;      // K tiles per stage
   int stages;
+  int m_tiles;
+  int k_each, k_more, steps, steps_more;
 };
+
+__device__ __forceinline__ uint32_t cluster_id() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
+  return r;
+}
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
@@ -566,6 +575,17 @@ __device__ __forceinline__ float activate_any(int act, float z) {
   }
 }
 
+__device__ __forceinline__ void act4(int act, uint64_t (&z)[2]) {
+  if (act == kActNone) return;
+  float v[4];
+  f2_split(z[0], v[0], v[1]);
+  f2_split(z[1], v[2], v[3]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = activate_any(act, v[j]);
+  z[0] = f2_pack(v[0], v[1]);
+  z[1] = f2_pack(v[2], v[3]);
+}
+
 template <bool kF8>
 __global__ void __launch_bounds__(kSplitThreads, 1)
     linear_split_kernel(const __grid_constant__ CUtensorMap tmap_x,
@@ -581,14 +601,16 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   int* abort_flag = &bars->abort_flag;
   const int warp = warp_index_uniform();
   const int lane = threadIdx.x & 31;
-  const int split = p.split, rank = static_cast<int>(blockIdx.x) % split;  // = cluster rank
-  const int tile = static_cast<int>(blockIdx.x) / split;
-  const int m_tiles = (a.m + p.tn - 1) / p.tn;
-  const int nb = tile / m_tiles, mb = tile % m_tiles;
+  // one cluster of `split` CTAs per tile; a rank's K tiles: k_tiles / split, and one more for
+  // the first k_tiles % split ranks (the launcher divides, 32-bit and 64-bit divisions here
+  // were most of the time before the first copy)
+  const int split = p.split, rank = static_cast<int>(cluster_ctarank());
+  const int tile = static_cast<int>(cluster_id());
+  const int nb = p.m_tiles == 1 ? tile : tile / p.m_tiles, mb = tile - nb * p.m_tiles;
   const int out_rows = gated ? p.wr / 2 : p.wr;  // output columns of y per tile
-  const int kt0 = static_cast<int>(static_cast<int64_t>(a.k_tiles) * rank / split);
-  const int kt1 = static_cast<int>(static_cast<int64_t>(a.k_tiles) * (rank + 1) / split);
-  const int steps = (kt1 - kt0 + p.group - 1) / p.group;  // stages filled; >= 1 (split <= k_tiles)
+  const int kt0 = rank * p.k_each + min(rank, p.k_more);
+  const int kt1 = kt0 + p.k_each + (rank < p.k_more ? 1 : 0);
+  const int steps = rank < p.k_more ? p.steps_more : p.steps;  // stages filled; >= 1 (split <= k_tiles)
   const uint32_t w_bytes = static_cast<uint32_t>(p.wr) * kKB;
   const uint32_t x_bytes = static_cast<uint32_t>(p.tn) * kKB;
   const uint32_t stage_bytes = (w_bytes + x_bytes) * p.group;
@@ -617,8 +639,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     }
   };
 
-  // The ring's first fill is under way before the rest of the CTA is set up.
-  const int ahead = min(steps, p.stages);
+  // The first copies are under way before the rest of the CTA is set up (two steps of them:
+  // a copy takes a hundred cycles to issue, and the first stage should not wait for the rest).
+  const int ahead = min(min(steps, p.stages), 2);
   if (warp == 0) {
     if (lane < p.stages) {
       mbar_init(&bars->full[lane], 1);
@@ -732,73 +755,83 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     }
     tc_fence_before();
   }
-  if (split > 1)
-    cluster_sync();
-  else
-    __syncthreads();
+  __syncwarp();
+  if (split > 1) cluster_arrive();
 
   // ------------------------------------------------------------ join and epilogue
-  // This CTA's share of the tile's tokens; four output columns per thread, the ranks' partial
-  // sums added in rank order.
+  // This CTA's share of the tile's tokens: a thread keeps four output columns (whose scales and
+  // biases it fetches while the cluster's barrier fills) and takes every so many tokens, the
+  // ranks' partial sums added in rank order.
   const int t0 = p.tn * rank / split, t1 = p.tn * (rank + 1) / split;
   const int quad_shift = 31 - __clz(out_rows / 4);  // out_rows is a power of two
-  const uint32_t part_addr = smem_u32(part);
-  const bool good = *reinterpret_cast<volatile int*>(abort_flag) == 0;
-  for (int i = threadIdx.x; good && i < (t1 - t0) << quad_shift; i += kSplitThreads) {
-    const int t = t0 + (i >> quad_shift), row = (i & ((1 << quad_shift) - 1)) * 4;
-    const int token = mb * p.tn + t, col = nb * out_rows + row;
-    if (token >= a.m || col >= a.n) continue;
-    const int64_t dst = static_cast<int64_t>(token) * a.n + col;
-    uint2 res = make_uint2(0, 0), bg = make_uint2(0, 0), bu = make_uint2(0, 0);
-    float4 sg = make_float4(1.0f, 1.0f, 1.0f, 1.0f), su = sg;
-    float sx = 1.0f;
-    if (residual != nullptr) res = __ldg(reinterpret_cast<const uint2*>(residual + dst));
+  const int id = static_cast<int>(threadIdx.x);
+  const int row = (id & ((1 << quad_shift) - 1)) * 4, col = nb * out_rows + row;
+  const bool in_columns = id < kJoinThreads && col < a.n;
+  uint2 bg = make_uint2(0, 0), bu = make_uint2(0, 0);
+  float4 sg = make_float4(1.0f, 1.0f, 1.0f, 1.0f), su = sg;
+  if (in_columns) {
     if (a.bias != nullptr) {
       bg = __ldg(reinterpret_cast<const uint2*>(a.bias + col));
       if (gated) bu = __ldg(reinterpret_cast<const uint2*>(a.bias + a.n + col));
     }
     if constexpr (kF8) {
-      sx = __ldg(a.sx + token);
       sg = __ldg(reinterpret_cast<const float4*>(a.sw + col));
       if (gated) su = __ldg(reinterpret_cast<const float4*>(a.sw + a.n + col));
     }
-    const uint32_t at = part_addr + static_cast<uint32_t>((t * p.wr + row) * 4);
+  }
+  __syncwarp();
+  if (split > 1)
+    cluster_wait();
+  else
+    __syncthreads();
+  const bool good = *reinterpret_cast<volatile int*>(abort_flag) == 0;
+  const auto affine = [&](float4 v, float sx, float4 scale, uint2 bias, uint64_t (&z)[2]) {
+    z[0] = f2_pack(v.x, v.y);
+    z[1] = f2_pack(v.z, v.w);
+    if constexpr (kF8) {
+      z[0] = f2_mul(f2_mul(z[0], f2_pack(sx, sx)), f2_pack(scale.x, scale.y));
+      z[1] = f2_mul(f2_mul(z[1], f2_pack(sx, sx)), f2_pack(scale.z, scale.w));
+    }
+    z[0] = f2_add(z[0], f2_of_bf16x2(bias.x));
+    z[1] = f2_add(z[1], f2_of_bf16x2(bias.y));
+  };
+  if (good && in_columns) {
+    const uint32_t part_addr = smem_u32(part) + static_cast<uint32_t>(row * 4);
+    uint32_t peers[kSplitMax];
+#pragma unroll
+    for (int q = 0; q < kSplitMax; ++q) peers[q] = q < split ? mapa_shared(part_addr, static_cast<uint32_t>(q)) : 0u;
     const auto total = [&](uint32_t where) {  // the ranks' sums in rank order, loads first
       float4 v[kSplitMax];
 #pragma unroll
       for (int q = 0; q < kSplitMax; ++q)
-        if (q < split) v[q] = ld_cluster_f4(mapa_shared(where, static_cast<uint32_t>(q)));
+        if (q < split) v[q] = ld_cluster_f4(peers[q] + where);
       float4 z = v[0];
 #pragma unroll
       for (int q = 1; q < kSplitMax; ++q)
         if (q < split) z.x += v[q].x, z.y += v[q].y, z.z += v[q].z, z.w += v[q].w;
       return z;
     };
-    const auto affine = [&](float4 v, float4 scale, uint2 bias, uint64_t (&z)[2]) {
-      z[0] = f2_pack(v.x, v.y);
-      z[1] = f2_pack(v.z, v.w);
-      if constexpr (kF8) {
-        z[0] = f2_mul(f2_mul(z[0], f2_pack(sx, sx)), f2_pack(scale.x, scale.y));
-        z[1] = f2_mul(f2_mul(z[1], f2_pack(sx, sx)), f2_pack(scale.z, scale.w));
-      }
-      z[0] = f2_add(z[0], f2_of_bf16x2(bias.x));
-      z[1] = f2_add(z[1], f2_of_bf16x2(bias.y));
-    };
-    uint64_t z[2], u[2];
-    affine(total(at), sg, bg, z);
-    if (gated) affine(total(at + static_cast<uint32_t>(out_rows * 4)), su, bu, u);
+    for (int t = t0 + (id >> quad_shift); t < t1; t += kJoinThreads >> quad_shift) {
+      const int token = mb * p.tn + t;
+      if (token >= a.m) break;
+      const int64_t dst = static_cast<int64_t>(token) * a.n + col;
+      uint2 res = make_uint2(0, 0);
+      if (residual != nullptr) res = __ldg(reinterpret_cast<const uint2*>(residual + dst));
+      const float sx = kF8 ? __ldg(a.sx + token) : 1.0f;
+      uint64_t z[2], u[2];
+      affine(total(static_cast<uint32_t>(t * p.wr * 4)), sx, sg, bg, z);
+      if (gated) affine(total(static_cast<uint32_t>((t * p.wr + out_rows) * 4)), sx, su, bu, u);
+      act4(a.act, z);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float lo, hi;
-      f2_split(z[j], lo, hi);
-      z[j] = f2_pack(activate_any(a.act, lo), activate_any(a.act, hi));
-      if (gated) z[j] = f2_mul(z[j], u[j]);
+      for (int j = 0; j < 2; ++j)
+        if (gated) z[j] = f2_mul(z[j], u[j]);
+      z[0] = f2_add(z[0], f2_of_bf16x2(res.x));
+      z[1] = f2_add(z[1], f2_of_bf16x2(res.y));
+      *reinterpret_cast<uint2*>(y + dst) = make_uint2(f2_to_bf16x2(z[0]), f2_to_bf16x2(z[1]));
     }
-    z[0] = f2_add(z[0], f2_of_bf16x2(res.x));
-    z[1] = f2_add(z[1], f2_of_bf16x2(res.y));
-    *reinterpret_cast<uint2*>(y + dst) = make_uint2(f2_to_bf16x2(z[0]), f2_to_bf16x2(z[1]));
   }
   tc_fence_before();
+  __syncwarp();
   if (split > 1)
     cluster_sync();  // no CTA leaves while a peer reads its partial sums
   else
@@ -1174,6 +1207,11 @@ SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
   best.group = group;
   best.stages = kSplitRingBytes / (tile_bytes * group);
   if (best.stages > kSplitStagesMax) best.stages = kSplitStagesMax;
+  best.m_tiles = static_cast<int>((l.m + best.tn - 1) / best.tn);
+  best.k_each = k_tiles / best.split;
+  best.k_more = k_tiles % best.split;
+  best.steps = (best.k_each + group - 1) / group;
+  best.steps_more = (best.k_each + group) / group;
   return best;
 }
 
