@@ -32,7 +32,7 @@ from . import ops
 from ._lib import load as load_library
 
 __all__ = ["global_scale", "row_quant", "QuantLinear", "NVFP4FFN", "NVFP4FFNStack", "GraphedFFNStack",
-           "FP8FFN", "install_ffn"]
+           "FP8FFN", "FP8GatedFFN", "install_ffn"]
 
 
 def global_scale(x: torch.Tensor) -> torch.Tensor:
@@ -320,6 +320,83 @@ class FP8FFN(torch.nn.Sequential):
         x2 = x.reshape(-1, shape[-1]).contiguous()
         y = ops.fp8_ffn(x2, l1.qweight, l1.scale, l1.bias, l2.qweight, l2.scale, l2.bias)
         return y.reshape(*shape[:-1], l2.out_features)
+
+
+    def prenorm(self, x: torch.Tensor, weight: torch.Tensor | None, eps: float = 1e-6) -> torch.Tensor:
+        """The FFN step of a pre-RMS-norm block around this module: x + self(rms_norm(x) * weight),
+        in four launches: the norm quantizes its own output per row, the first product applies
+        bias and GELU, the second adds bias and x.  The norm's output, the pre-activation and
+        the sum with x stay in fp32 until the one rounding of each stored tensor (``forward``
+        rounds the pre-activation to bf16, as the reference does).  x: bf16 [..., d_model];
+        weight: bf16 [d_model] or None."""
+        l1, l2 = self[0], self[2]
+        if not _is_gelu_tanh(self[1]):
+            raise ValueError("FP8FFN.prenorm: the activation must be GELU(approximate='tanh')")
+        x2 = x.reshape(-1, x.shape[-1])
+        q, s = ops.rms_norm_fp8(x2, weight, eps)
+        h = ops.fp8_scaled_mm_act(q, s, l1.qweight, l1.scale, l1.bias, act="gelu_tanh")
+        q, s = ops.fp8_row_quant(h)
+        return ops.fp8_scaled_mm_act(q, s, l2.qweight, l2.scale, l2.bias, residual=x2).reshape(x.shape)
+
+
+class FP8GatedFFN(torch.nn.Module):
+    """``down(act(gate(x)) * up(x))`` in W8A8 (E4M3, one scale per row): the gated FFN, which the
+    reference's two-linear ``QuantLinear`` pair does not cover.
+
+    Built from three ``nn.Linear``; gate and up are quantized row by row and kept stacked
+    (buffers ``qweight`` [2 f, d], ``scale``, ``bias``), so that one product computes both and
+    joins them in its epilogue; ``down`` is quantized alike (``down_qweight``, ...).  act: one of
+    ``ops.ACTIVATIONS``.  d and f multiples of 16.  Inputs are bf16 [..., d]; four launches
+    (quantize x, or ``prenorm``'s norm which quantizes its own output; gated product; quantize h;
+    down product).
+    """
+
+    def __init__(self, gate: torch.nn.Linear, up: torch.nn.Linear, down: torch.nn.Linear, act: str = "silu"):
+        super().__init__()
+        if act not in ops.ACTIVATIONS:
+            raise ValueError(f"FP8GatedFFN: act must be one of {', '.join(ops.ACTIVATIONS)}")
+        d, f = gate.in_features, gate.out_features
+        if (up.in_features, up.out_features) != (d, f) or (down.in_features, down.out_features) != (f, d):
+            raise ValueError("FP8GatedFFN: linear shapes do not chain")
+        if (gate.bias is None) != (up.bias is None):
+            raise ValueError("FP8GatedFFN: gate and up need biases both or neither")
+        if not gate.weight.is_cuda:
+            raise RuntimeError("FP8GatedFFN: the weights must be on a CUDA device (no CPU path)")
+        self.act = act
+        both = torch.cat([gate.weight.detach(), up.weight.detach()]).to(torch.bfloat16)
+        bias = None if gate.bias is None else torch.cat([gate.bias.detach(), up.bias.detach()]).to(torch.bfloat16)
+        for name, w, b in (("", both, bias),
+                           ("down_", down.weight.detach().to(torch.bfloat16),
+                            None if down.bias is None else down.bias.detach().clone().to(torch.bfloat16))):
+            q, s = row_quant(w)
+            self.register_buffer(name + "qweight", q)
+            self.register_buffer(name + "scale", s)
+            self.register_buffer(name + "bias", b)
+
+    def _chain(self, q: torch.Tensor, scale: torch.Tensor, residual: torch.Tensor | None) -> torch.Tensor:
+        h = ops.fp8_scaled_mm_act(q, scale, self.qweight, self.scale, self.bias, act=self.act, gated=True)
+        q, scale = ops.fp8_row_quant(h)
+        return ops.fp8_scaled_mm_act(q, scale, self.down_qweight, self.down_scale, self.down_bias,
+                                     residual=residual)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        x2 = x.reshape(-1, x.shape[-1])
+        q, scale = ops.fp8_row_quant(x2)
+        return self._chain(q, scale, None).reshape(x.shape)
+
+    def prenorm(self, x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Tensor | None = None,
+                eps: float = 1e-6) -> torch.Tensor:
+        """s + self(rms_norm(s) * weight) with s = x, or x + residual (the branch before joins the
+        stream in the same pass); bf16 [..., d]."""
+        x2 = x.reshape(-1, x.shape[-1])
+        if residual is None:
+            q, scale = ops.rms_norm_fp8(x2, weight, eps)
+            return self._chain(q, scale, x2).reshape(x.shape)
+        q, scale, s = ops.add_rms_norm_fp8(x2, residual.reshape(x2.shape), weight, eps)
+        return self._chain(q, scale, s).reshape(x.shape)
+
+    def extra_repr(self) -> str:
+        return f"d={self.qweight.shape[1]}, f={self.qweight.shape[0] // 2}, act={self.act}"
 
 
 _FUSED = {"nvfp4": NVFP4FFN, "fp8": FP8FFN}

@@ -125,3 +125,32 @@ def test_fake_kernels_give_shapes_and_types():
         k, v = ops.fp8_cache_read(c, cs, c, cs, torch.empty(3, 4, dtype=torch.int32, device="cuda"),
                                   torch.empty(3, dtype=torch.int32, device="cuda"), 50)
         assert k.shape == v.shape == (3, 50, 2, 64) and k.dtype == BF16
+
+
+def test_modules_refuse_cpu_weights_and_bad_shapes():
+    lin = torch.nn.Linear
+    with pytest.raises(RuntimeError):
+        fvq.FP8GatedFFN(lin(64, 128), lin(64, 128), lin(128, 64))
+    with pytest.raises(ValueError):
+        fvq.FP8GatedFFN(lin(64, 128), lin(64, 96), lin(128, 64))
+    with pytest.raises(ValueError):
+        fvq.FP8GatedFFN(lin(64, 128), lin(64, 128), lin(128, 32))
+    with pytest.raises(ValueError):
+        fvq.FP8GatedFFN(lin(64, 128), lin(64, 128, bias=False), lin(128, 64))
+    with pytest.raises(ValueError):
+        fvq.FP8GatedFFN(lin(64, 128), lin(64, 128), lin(128, 64), act="swish")
+    with pytest.raises(ValueError):
+        fvq.FP8KVCache(4, 16, 2, 68)
+    with pytest.raises(ValueError):
+        fvq.FP8KVCache(0, 16, 2, 64)
+    with pytest.raises(RuntimeError):
+        fvq.FP8KVCache(4, 16, 2, 64, device="cpu")
+
+
+def test_cache_slot_numbers():
+    cache = object.__new__(fvq.FP8KVCache)
+    cache.k_codes = torch.zeros(9, 16, 1, 8)
+    table = torch.tensor([[4, 2], [7, 0]], dtype=torch.int32)
+    got = cache.slots(table, torch.tensor([[0, 15, 16, 31], [5, -1, 32, 17]]))
+    assert got.dtype == torch.int64
+    assert got.tolist() == [64, 79, 32, 47, 117, -1, -1, 1]

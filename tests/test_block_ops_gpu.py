@@ -671,3 +671,128 @@ def test_block_run_in_a_graph_and_on_streams():
     graphs[0].replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want[3])                   # the slots differ, the attention does not see them
+
+
+# ---------------------------------------------------------------- modules
+def linear(out_f, in_f, seed, bias=True):
+    lin = torch.nn.Linear(in_f, out_f, bias=bias, device="cuda", dtype=BF16)
+    with torch.no_grad():
+        lin.weight.copy_(randn(out_f, in_f, seed=seed, std=in_f ** -0.5))
+        if bias:
+            lin.bias.copy_(randn(out_f, seed=seed + 1, std=0.1))
+    return lin
+
+
+@pytest.mark.parametrize("shape", [(1, 512), (37, 512), (2, 150, 512), (0, 512)])
+def test_fp8_ffn_prenorm(shape):
+    """x + FFN(norm(x)) by the fused step: against its own launches one by one (the same bits), and
+    against 64 bits on the dequantized weights (three E4M3 roundings on the branch's path, each
+    at most 2^-4, rms 0.036: under 0.07 of the branch)."""
+    ffn = fvq.FP8FFN(fvq.QuantLinear(linear(1024, 512, 1), "fp8"), torch.nn.GELU(approximate="tanh"),
+                     fvq.QuantLinear(linear(512, 1024, 3), "fp8"))
+    x, w = randn(*shape, seed=5), randn(512, seed=6)
+    y = ffn.prenorm(x, w)
+    assert y.shape == x.shape and y.dtype == BF16
+    if not x.numel():
+        return
+    x2 = x.reshape(-1, 512)
+    branch = ops.fp8_scaled_mm_act(*ops.rms_norm_fp8(x2, w), ffn[0].qweight, ffn[0].scale, ffn[0].bias, "gelu_tanh")
+    again = ops.fp8_scaled_mm_act(*ops.fp8_row_quant(branch), ffn[2].qweight, ffn[2].scale, ffn[2].bias, residual=x2)
+    assert torch.equal(y, again.reshape(shape))
+    w1, w2 = (lin.qweight.double() * lin.scale.double() for lin in (ffn[0], ffn[2]))
+    h = ACT64["gelu_tanh"](norm64(x2, None, w, 1e-6)[1] @ w1.t() + ffn[0].bias.double())
+    want = h @ w2.t() + ffn[2].bias.double()
+    got = y.reshape(-1, 512).double() - x2.double()
+    # the output's own rounding, half a bf16 step of the sum, is counted apart
+    slack = HALF_BF16 * (want + x2.double()).norm()
+    assert (got - want).norm() <= 0.07 * want.norm() + slack
+    with pytest.raises(ValueError):
+        fvq.FP8FFN(ffn[0], torch.nn.GELU(), ffn[2]).prenorm(x, w)
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_fp8_gated_ffn(act, bias):
+    d, f = 256, 784
+    gate, up, down = linear(f, d, 1, bias), linear(f, d, 3, bias), linear(d, f, 5, bias)
+    ffn = fvq.FP8GatedFFN(gate, up, down, act)
+    x, r, w = randn(3, 50, d, seed=7), randn(3, 50, d, seed=8), randn(d, seed=9)
+
+    def branch(u):
+        wg, wd = ffn.qweight.double() * ffn.scale.double(), ffn.down_qweight.double() * ffn.down_scale.double()
+        z = u @ wg.t() + (0 if ffn.bias is None else ffn.bias.double())
+        h = ACT64[act](z[:, :f]) * z[:, f:]
+        return h @ wd.t() + (0 if ffn.down_bias is None else ffn.down_bias.double())
+
+    x2 = x.reshape(-1, d).double()
+    # x, and h from two products of x's roundings, and h's own: under 4 * 0.036 in all
+    want = branch(x2)
+    assert (ffn(x).reshape(-1, d).double() - want).norm() <= 0.15 * want.norm()
+    for residual in (None, r):
+        s, u = norm64(x, residual, w, 1e-6)
+        want = branch(u.reshape(-1, d))
+        got = ffn.prenorm(x, w, residual).reshape(-1, d).double() - s.reshape(-1, d)
+        assert (got - want).norm() <= 0.15 * want.norm() + 2 * HALF_BF16 * (want + s.reshape(-1, d)).norm()
+    assert set(ffn.state_dict()) >= {"qweight", "scale", "down_qweight", "down_scale"}
+
+
+def test_kv_cache_object():
+    heads, d, page = 3, 64, 16
+    cache = fvq.FP8KVCache(10, page, heads, d)
+    table = torch.tensor([[4, 2, 9], [7, 0, 1]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([40, 19], dtype=torch.int32, device="cuda")
+    at = torch.arange(40, device="cuda").repeat(2, 1)
+    at[1, 19:] = -1                                         # the shorter sequence is padded
+    kv = randn(2 * 40, 2, heads, d, seed=3)
+    cache.write(kv[:, 0], kv[:, 1], cache.slots(table, at))
+    k, v = cache.read(table, lens, 44)
+    for got, x in ((k, kv[:, 0]), (v, kv[:, 1])):
+        x = x.reshape(2, 40, heads, d)
+        step = x.float().abs().amax(-1, keepdim=True) / 448
+        for b, n in ((0, 40), (1, 19)):
+            y, want = got[b, :n].double(), x[b, :n].double()
+            # E4M3's half step (2^-10 of the scale below 2^-6), then bf16's
+            bound = torch.maximum(want.abs() * HALF_E4M3, step[b, :n].double() * 2.0 ** -10)
+            inside(y, want, bound * (1 + HALF_BF16) + HALF_BF16 * want.abs() + 2.0 ** -22 * want.abs())
+            assert (got[b, n:] == 0).all()
+
+
+def test_other_threads_and_modes():
+    """Calls from two threads on streams of their own, and under a dispatch mode."""
+    import threading
+    from torch.utils._python_dispatch import TorchDispatchMode
+    x, w = randn(64, 512, seed=1), randn(256, 512, seed=2)
+    want = ops.linear_act(x, w, act="silu")
+    got = [None, None]
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got[i] = ops.linear_act(x, w, act="silu")
+        s.synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert torch.equal(got[0], want) and torch.equal(got[1], want)
+    seen = []
+
+    class Log(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    with Log():
+        assert torch.equal(ops.linear_act(x, w, act="silu"), want)
+    assert any("fvq.linear_act" in s for s in seen)
+    with torch.inference_mode():
+        assert torch.equal(ops.linear_act(x, w, act="silu"), want)
+        cache = fvq.FP8KVCache(2, 4, 1, 64)
+        kv = randn(3, 1, 64)
+        cache.write(kv, kv, torch.arange(3, device="cuda"))
+    with torch.no_grad():
+        assert torch.equal(ops.linear_act(x, torch.nn.Parameter(w), act="silu"), want)
