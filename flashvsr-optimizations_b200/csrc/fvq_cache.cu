@@ -16,6 +16,7 @@
 #include <cuda_runtime.h>
 
 #include "fvq_internal.h"
+#include "fvq_launch.h"
 #include "fvq_ptx.cuh"
 
 namespace fvq {
@@ -83,6 +84,8 @@ template <int kLanes, int kElems, int kVecs, int kRows>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheWriteArgs a,
                                                                    const Divider by_heads,
                                                                    uint32_t* err_word) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   const CacheRows src = blockIdx.y == 0 ? a.k : a.v;
   constexpr uint32_t kStep = kCacheThreads / kLanes;
   const int lane = threadIdx.x % kLanes;
@@ -160,6 +163,8 @@ template <int kCodes>
 __global__ void __launch_bounds__(kCacheThreads)
     cache_read_kernel(const CacheReadArgs a, const int span, const Divider by_token,
                       const Divider by_row, const Divider by_page, uint32_t* err_word) {
+  grid_launch_dependents();
+  grid_dependency_wait();
   const bool values = blockIdx.z != 0;
   const uint8_t* codes = values ? a.v_codes : a.k_codes;
   const float* scales = values ? a.v_scale : a.k_scale;
@@ -221,31 +226,30 @@ __global__ void __launch_bounds__(kCacheThreads)
 }
 
 template <int kLanes, int kElems, int kVecs, int kRows>
-void write_launch(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) {
+cudaError_t write_launch(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) {
   constexpr int kCtaRows = kCacheThreads / kLanes * kRows;
   const dim3 grid(static_cast<unsigned>((a.rows + kCtaRows - 1) / kCtaRows), 2);
-  cache_write_kernel<kLanes, kElems, kVecs, kRows>
-      <<<grid, kCacheThreads, 0, st>>>(a, divider(a.heads), err_word);
+  return launch_dependent(cache_write_kernel<kLanes, kElems, kVecs, kRows>, grid, kCacheThreads, 0, st, 0, a,
+                          divider(a.heads), err_word);
 }
 
 template <int kLanes, int kElems, int kVecs = 1>
-void write_by_rows(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) {
+cudaError_t write_by_rows(const CacheWriteArgs& a, uint32_t* err_word, cudaStream_t st) {
   // two rows a group once that still leaves every SM two thousand threads
   if (2 * a.rows * kLanes >= static_cast<int64_t>(sm_count()) * 2048 * 2)
-    write_launch<kLanes, kElems, kVecs, 2>(a, err_word, st);
-  else
-    write_launch<kLanes, kElems, kVecs, 1>(a, err_word, st);
+    return write_launch<kLanes, kElems, kVecs, 2>(a, err_word, st);
+  return write_launch<kLanes, kElems, kVecs, 1>(a, err_word, st);
 }
 
 template <int kCodes>
-void read_launch(const CacheReadArgs& a, uint32_t* err_word, cudaStream_t st) {
+cudaError_t read_launch(const CacheReadArgs& a, uint32_t* err_word, cudaStream_t st) {
   const int64_t per_token = static_cast<int64_t>(a.heads) * a.d / kCodes;
   // whole tokens that one pass of the CTA covers (a long token takes several passes)
   const int64_t fit = kCacheThreads * kReadUnroll / per_token;
   const int64_t span = fit < 1 ? 1 : fit;
   const dim3 grid(static_cast<unsigned>((a.max_len + span - 1) / span), static_cast<unsigned>(a.batch), 2);
-  cache_read_kernel<kCodes><<<grid, kCacheThreads, 0, st>>>(a, static_cast<int>(span), divider(per_token),
-                                                            divider(a.d / kCodes), divider(a.page), err_word);
+  return launch_dependent(cache_read_kernel<kCodes>, grid, kCacheThreads, 0, st, 0, a, static_cast<int>(span),
+                          divider(per_token), divider(a.d / kCodes), divider(a.page), err_word);
 }
 
 }  // namespace
@@ -256,27 +260,23 @@ cudaError_t launch_cache_write(const CacheWriteArgs& a, uint32_t* err_word, cuda
   const bool wide = a.d % 16 == 0 && at(a.k.x, 32) && at(a.v.x, 32) && at(a.k.codes, 16) &&
                     at(a.v.codes, 16) && (a.k.token_stride | a.k.head_stride | a.v.token_stride | a.v.head_stride) % 16 == 0;
   if (wide) {
-    if (a.d <= 64) write_by_rows<4, 16>(a, err_word, st);
-    else if (a.d <= 128) write_by_rows<8, 16>(a, err_word, st);
-    else if (a.d <= 256) write_by_rows<16, 16>(a, err_word, st);
-    else write_by_rows<32, 16>(a, err_word, st);
-  } else {
-    if (a.d <= 64) write_by_rows<8, 8>(a, err_word, st);
-    else if (a.d <= 128) write_by_rows<16, 8>(a, err_word, st);
-    else if (a.d <= 256) write_by_rows<32, 8>(a, err_word, st);
-    else write_by_rows<32, 8, 2>(a, err_word, st);
+    if (a.d <= 64) return write_by_rows<4, 16>(a, err_word, st);
+    if (a.d <= 128) return write_by_rows<8, 16>(a, err_word, st);
+    if (a.d <= 256) return write_by_rows<16, 16>(a, err_word, st);
+    return write_by_rows<32, 16>(a, err_word, st);
   }
-  return cudaGetLastError();
+  if (a.d <= 64) return write_by_rows<8, 8>(a, err_word, st);
+  if (a.d <= 128) return write_by_rows<16, 8>(a, err_word, st);
+  if (a.d <= 256) return write_by_rows<32, 8>(a, err_word, st);
+  return write_by_rows<32, 8, 2>(a, err_word, st);
 }
 
 cudaError_t launch_cache_read(const CacheReadArgs& a, uint32_t* err_word, cudaStream_t st) {
   if (a.max_len <= 0 || a.batch <= 0) return cudaSuccess;
   const auto at = [](const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; };
   if (a.d % 16 == 0 && at(a.k_codes, 16) && at(a.v_codes, 16) && at(a.k_out, 32) && at(a.v_out, 32))
-    read_launch<16>(a, err_word, st);
-  else
-    read_launch<8>(a, err_word, st);
-  return cudaGetLastError();
+    return read_launch<16>(a, err_word, st);
+  return read_launch<8>(a, err_word, st);
 }
 
 }  // namespace fvq

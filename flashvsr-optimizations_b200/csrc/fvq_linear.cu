@@ -30,6 +30,7 @@
 #include <cstring>
 
 #include "fvq_internal.h"
+#include "fvq_launch.h"
 #include "fvq_ptx.cuh"
 
 namespace fvq {
@@ -283,6 +284,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   tc_fence_before();
   cluster_sync();  // barriers of both CTAs initialised before any remote arrive
   tc_fence_after();
+  grid_dependency_wait();
   const uint32_t tmem = bars->tmem_base;
   const auto even_addr = [&](const void* p) { return mapa_shared(smem_u32(p), 0); };
   const auto odd_addr = [&](const void* p) { return mapa_shared(smem_u32(p), 1); };
@@ -323,6 +325,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
       }
     }
+    grid_launch_dependents();  // this CTA's last tile is on its way
     // the even CTA's stage barriers count both CTAs' loads; the odd CTA's land before the
     // even CTA passes the final cluster barrier
     for (int s = 0; even && s < kPairStages; ++s) {
@@ -654,6 +657,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     }
     fence_barrier_init();
     fence_proxy_async_smem();
+    grid_launch_dependents();
+    grid_dependency_wait();
     __syncwarp();
     if (elect_one())
       for (int i = 0; i < ahead; ++i) fill(i, i);
@@ -662,6 +667,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     tmem_alloc(&bars->tmem_base, cols);
     tmem_relinquish();
   }
+  grid_dependency_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -887,6 +893,8 @@ __global__ void __launch_bounds__(kVecThreads, kVecCtas)
                          const int gated, const uint16_t* __restrict__ residual,
                          uint16_t* __restrict__ y, const LinearArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
+  grid_launch_dependents();
+  grid_dependency_wait();
   constexpr int kPairs = kF8 ? 8 : 4;
   constexpr int kValues = kVecRows * kM;
   uint4* xs = reinterpret_cast<uint4*>(smem);                     // [kM][k_bytes / 16]
@@ -1054,19 +1062,8 @@ cudaError_t launch_pair(const LinearProblem& l, const LinearArgs& a, cudaStream_
   const int64_t tiles = ((l.m + kPairTokens - 1) / kPairTokens) * ((l.n + out_cols - 1) / out_cols);
   int64_t pairs = sm_count() / 2;
   if (pairs > tiles) pairs = tiles;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
-  cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = kPairSmemBytes;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, mx, mw, mr, my, a);
+  return launch_dependent(kernel, static_cast<unsigned>(2 * pairs), kPairThreads, kPairSmemBytes, st, 2, mx, mw,
+                          mr, my, a);
 }
 
 template <bool kF8>
@@ -1087,19 +1084,8 @@ cudaError_t launch_split(const LinearProblem& l, const LinearArgs& a, const Spli
     return e;
   const int64_t out_rows = l.gated ? p.wr / 2 : p.wr;
   const int64_t tiles = ((l.m + p.tn - 1) / p.tn) * ((l.n + out_rows - 1) / out_rows);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.split));
-  cfg.blockDim = dim3(kSplitThreads);
-  cfg.dynamicSmemBytes = kSplitSmemBytes;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(p.split);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, mx, mw, p, l.gated ? 1 : 0, l.residual, l.y, a);
+  return launch_dependent(kernel, static_cast<unsigned>(tiles * p.split), kSplitThreads, kSplitSmemBytes, st,
+                          p.split, mx, mw, p, l.gated ? 1 : 0, l.residual, l.y, a);
 }
 
 template <bool kF8, int kM>
@@ -1118,10 +1104,9 @@ cudaError_t launch_vector(const LinearProblem& l, const LinearArgs& a, cudaStrea
                                               kVecSmemMax + kVecWarps * kVecRows * kM * 4))
     return e;
   const int64_t ctas = (groups + kVecWarps / kw - 1) / (kVecWarps / kw);
-  kernel<<<static_cast<unsigned>(ctas), kVecThreads, bytes, st>>>(
-      static_cast<const uint8_t*>(l.x), l.x_stride * elem, static_cast<const uint8_t*>(l.w), k_bytes, kw,
-      l.gated ? 1 : 0, l.residual, l.y, a);
-  return cudaGetLastError();
+  return launch_dependent(kernel, static_cast<unsigned>(ctas), kVecThreads, bytes, st, 0,
+                          static_cast<const uint8_t*>(l.x), l.x_stride * elem,
+                          static_cast<const uint8_t*>(l.w), k_bytes, kw, l.gated ? 1 : 0, l.residual, l.y, a);
 }
 
 template <bool kF8>

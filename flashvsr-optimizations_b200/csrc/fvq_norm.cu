@@ -27,6 +27,7 @@
 #include <cuda_runtime.h>
 
 #include "fvq_internal.h"
+#include "fvq_launch.h"
 #include "fvq_ptx.cuh"
 
 namespace fvq {
@@ -319,6 +320,8 @@ template <int kLanes, int kRows, int kPer, int kVec>
 __global__ void __launch_bounds__(kLanes == 0 ? kNormMaxThreads : kNormThreads)
     rms_norm_kernel(const NormArgs a) {
   static_assert(kLanes != 0 || kRows == 1, "one row per CTA");
+  grid_launch_dependents();
+  grid_dependency_wait();
   __shared__ float sum_smem[32];
   __shared__ float max_smem[32];
   constexpr int kPairs = kPer / 2;
@@ -364,7 +367,8 @@ __global__ void __launch_bounds__(kLanes == 0 ? kNormMaxThreads : kNormThreads)
 }
 
 // ---------------------------------------------------------------- many long rows
-// One CTA of 16 warps per SM.  A group of `kGroup` warps walks rows group by group over the
+// (No grid_launch_dependents here: with the next kernel let in early, 15360 rows of 1536 took
+// 29.5 us instead of 28.2.)  One CTA of 16 warps per SM.  A group of `kGroup` warps walks rows group by group over the
 // grid; each group owns a ring of `slots` row buffers (x's row, then the residual's), one
 // mbarrier each.  A slot is refilled as soon as the group holds its row in registers.
 constexpr int kStreamWarps = 16;
@@ -526,6 +530,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     for (int s = 0; s < p.slots; ++s) mbar_init(&bar[s], 1);
     fence_barrier_init();
     fence_proxy_async_smem();
+  }
+  grid_dependency_wait();
+  if (leader) {
     for (int s = 0; s < p.slots; ++s) fetch(row0 + s * stride, s);
   }
   // the weight stays in registers up to 48 values a lane, and comes from L1 for every row beyond
@@ -534,7 +541,6 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   if (kKeepWeight && a.weight != nullptr) load_weight<kPairs, kVec>(w, a.weight, d, at);
   __syncthreads();  // the barriers are initialised
 
-  const float inv_d = 1.0f / static_cast<float>(d);
   int64_t base = row0 * d;
   const int64_t base_step = stride * d;
   int slot = 0;
@@ -578,21 +584,25 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       add_residual<kPairs, kVec>(s, rs, res_bytes == 4, to, true, d, at);
     }
     if constexpr (kVec == 2) mask_pairs(s, d, at);
-    // the partial sums alternate between two places, so that the reduction's own barrier is the
-    // one that says the group holds the row and has left the last row's partials
+    // A warp refills its slot as soon as it holds the row.  A larger group does after the sum's
+    // barrier, which says the same (the partial sums alternate between two places, so that no
+    // other barrier is needed before them).
+    if constexpr (kGroup == 1) {
+      __syncwarp();
+      if (leader && kVec != 2) fetch(row + p.slots * stride, slot);
+    }
     const float sq = group_reduce<kGroup>(sum_squares(s), sums + (turn ^= 1) * kStreamWarps + group * kGroup, group,
                                           in_group, [](float x, float y) { return x + y; });
-    if constexpr (kGroup == 1) __syncwarp();
     if constexpr (kVec == 2) {
       // the previous row's slot held its outputs: free once their copies have read it
       if (leader && row != row0) {
         bulk_wait_group_read0();
         fetch(row + (p.slots - 1) * stride, slot == 0 ? p.slots - 1 : slot - 1);
       }
-    } else {
+    } else if constexpr (kGroup > 1) {
       if (leader) fetch(row + p.slots * stride, slot);
     }
-    const float rstd = rsqrtf(fmaf(sq, inv_d, a.eps));
+    const float rstd = rsqrtf(sq / static_cast<float>(d) + a.eps);
     if (!kKeepWeight && a.weight != nullptr) load_weight<kPairs, kVec>(w, a.weight, d, at);
     if (a.weight != nullptr) apply_weight(s, w);
     if (a.y != nullptr)
@@ -622,24 +632,21 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 }
 
 template <int kLanes, int kRows, int kPer>
-void norm_launch(const NormArgs& a, bool vec, cudaStream_t st) {
+cudaError_t norm_launch(const NormArgs& a, bool vec, cudaStream_t st) {
   const int threads = kLanes != 0 ? kNormThreads : ((a.d + kPer - 1) / kPer + 31) / 32 * 32;
   const int rows = kLanes != 0 ? kNormThreads / kLanes * kRows : 1;
   const unsigned grid = static_cast<unsigned>((a.rows + rows - 1) / rows);
-  if (vec)
-    rms_norm_kernel<kLanes, kRows, kPer, 8><<<grid, threads, 0, st>>>(a);
-  else
-    rms_norm_kernel<kLanes, kRows, kPer, 1><<<grid, threads, 0, st>>>(a);
+  if (vec) return launch_dependent(rms_norm_kernel<kLanes, kRows, kPer, 8>, grid, threads, 0, st, 0, a);
+  return launch_dependent(rms_norm_kernel<kLanes, kRows, kPer, 1>, grid, threads, 0, st, 0, a);
 }
 
 template <int kLanes>
-void norm_short(const NormArgs& a, bool vec, cudaStream_t st) {
+cudaError_t norm_short(const NormArgs& a, bool vec, cudaStream_t st) {
   // two rows a group once that still leaves every SM its threads (92160 rows of 128: 10.0 us
   // with one, 9.0 with two, 9.4 with four)
   if (a.rows * kLanes >= static_cast<int64_t>(sm_count()) * 2048 * 2)
-    norm_launch<kLanes, 2, 8>(a, vec, st);
-  else
-    norm_launch<kLanes, 1, 8>(a, vec, st);
+    return norm_launch<kLanes, 2, 8>(a, vec, st);
+  return norm_launch<kLanes, 1, 8>(a, vec, st);
 }
 
 template <int kGroup, int kPer, int kVec>
@@ -650,8 +657,8 @@ cudaError_t stream_launch(const NormArgs& a, const StreamPlan& p, uint64_t wait_
   const int bytes = kStreamHead + kStreamSmem;
   if (cudaError_t e = ensure_max_dynamic_smem(attr_done, reinterpret_cast<const void*>(kernel), bytes))
     return e;
-  kernel<<<static_cast<unsigned>(sm_count()), kStreamThreads, bytes, st>>>(a, p, wait_limit, err_word);
-  return cudaGetLastError();
+  return launch_dependent(kernel, static_cast<unsigned>(sm_count()), kStreamThreads, bytes, st, 0, a, p,
+                          wait_limit, err_word);
 }
 
 template <int kGroup, int kVec>
@@ -690,13 +697,10 @@ cudaError_t launch_rms_norm(const NormArgs& args, uint64_t wait_limit, cudaStrea
                    at16(a.y) && at16(a.q);
   const int d = a.d;
   if (d > kNormMaxD) return cudaErrorInvalidValue;
-  if (d <= 64) {
-    norm_short<8>(a, vec, st);
-  } else if (d <= 128) {
-    norm_short<16>(a, vec, st);
-  } else if (d <= 256) {
-    norm_short<32>(a, vec, st);
-  } else {
+  if (d <= 64) return norm_short<8>(a, vec, st);
+  if (d <= 128) return norm_short<16>(a, vec, st);
+  if (d <= 256) return norm_short<32>(a, vec, st);
+  {
     // warps per row: rings of two rows per group within the shared memory, 64 values a lane
     StreamPlan p;
     const int res = a.residual == nullptr ? 0 : a.residual_f32 ? 4 : 2, slack = vec ? 0 : 16;
@@ -726,12 +730,9 @@ cudaError_t launch_rms_norm(const NormArgs& args, uint64_t wait_limit, cudaStrea
         default: return stream_by_form<16>(a, p, form, wait_limit, err_word, st);
       }
     }
-    if (d <= 8 * kNormMaxThreads)
-      norm_launch<0, 1, 8>(a, vec, st);
-    else
-      norm_launch<0, 1, 16>(a, vec, st);
   }
-  return cudaGetLastError();
+  if (d <= 8 * kNormMaxThreads) return norm_launch<0, 1, 8>(a, vec, st);
+  return norm_launch<0, 1, 16>(a, vec, st);
 }
 
 }  // namespace fvq
