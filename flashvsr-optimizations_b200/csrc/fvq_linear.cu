@@ -14,11 +14,11 @@
 //     epilogue.  Gated: the even CTA loads the tile's Wg rows, the odd one its Wu rows, so
 //     both halves of an output column meet in the same TMEM lane and no pass over h is made.
 //   linear_split_kernel  few tokens: bound by reading W once.  The operands change places:
-//     `wr` rows of W are the M side, up to 256 tokens the N side, so that a single token
-//     costs one N = 16 instruction and not a 128-row tile; K is split over a cluster of up
-//     to eight CTAs until every SM streams its share of W, and the partial sums are joined
-//     through distributed shared memory in rank order (no atomics, no workspace, the same
-//     bits on every run).
+//     `wr` rows of W are the M side, up to 128 tokens the N side, so that a few tokens cost
+//     N = 16 instructions and not a 128-row tile; K is split over a cluster of up to eight
+//     CTAs until every SM streams its share of W, and each CTA sends its partial sums to the
+//     one that owns their tokens, through distributed shared memory; they are added in rank
+//     order (no atomics, no workspace, the same bits on every run).
 //   linear_vector_kernel  one or two tokens: W streamed through registers by plain 16-byte
 //     loads and fp32 FMAs, x in shared memory.  No tensor-core pipeline to set up, fill and
 //     drain, which is half of the split kernel's time at this size.
@@ -524,12 +524,13 @@ constexpr int kSplitMax = 8;                      // CTAs per cluster (the porta
 constexpr int kSplitThreads = 320;                // producer, MMA issuer, eight epilogue warps
 constexpr int kJoinThreads = 256;                 // a power of two, so that a thread keeps its columns
 constexpr int kSplitBarrierBytes = 512;
-// An MMA reads 128 W rows; a tile of fewer rows is followed by whatever comes next in shared
-// memory (it ends in accumulator rows that nobody reads), so the ring is followed by a pad.
+// Shared memory: the ring of stages, then the partial sums of this CTA's tokens, as the
+// cluster's CTAs send them (they may arrive while this CTA still multiplies).  An MMA reads
+// 128 W rows; a tile of fewer rows is followed by whatever comes next in shared memory (it
+// ends in accumulator rows that nobody reads), so what follows the ring is at least 16 KB.
 constexpr int kSplitPad = 128 * kKB;
-constexpr int kSplitRing = 232448 - kSplitBarrierBytes - kSplitPad - 1024;
-constexpr int kSplitRingBytes = kSplitRing / 1024 * 1024;
-constexpr int kSplitBarrierOff = kSplitRingBytes + kSplitPad;
+constexpr int kSplitDataBytes = (232448 - kSplitBarrierBytes) / 1024 * 1024;
+constexpr int kSplitBarrierOff = kSplitDataBytes;
 constexpr int kSplitSmemBytes = kSplitBarrierOff + kSplitBarrierBytes;
 static_assert(kSplitSmemBytes <= 232448, "split plan exceeds shared memory");
 
@@ -545,12 +546,15 @@ static_assert(sizeof(SplitBars) <= kSplitBarrierBytes, "split barrier area");
 
 struct SplitPlan {
   int wr;         // W rows per CTA: 64 or 128 (gated: half of them Wg rows, half Wu rows)
-  int tn;         // tokens per CTA: a multiple of 16, at most 256
+  int tn;         // tokens per CTA: a multiple of 16, at most 128
   int split;      // CTAs per cluster sharing one tile's K
   int group;      // K tiles per stage
   int stages;
   int m_tiles;
   int k_each, k_more, steps, steps_more;
+  int own;        // tokens per rank: rank r joins tokens [r * own, (r + 1) * own) of the tile
+  int own_mul;    // t / own = t * own_mul >> 16, exact for t * own < 2^16
+  int part_off;   // of the partial sums in shared memory
 };
 
 __device__ __forceinline__ uint32_t cluster_id() {
@@ -559,13 +563,8 @@ __device__ __forceinline__ uint32_t cluster_id() {
   return r;
 }
 
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
 __device__ __forceinline__ float activate_any(int act, float z) {
@@ -668,6 +667,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     tmem_relinquish();
   }
   grid_dependency_wait();
+  __syncwarp();
+  if (split > 1) cluster_arrive();  // this CTA runs: the others may send to it
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -738,25 +739,30 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
     }
   }
-  // ------------------------------------------------------------ partial sums to shared memory
-  // part[t * wr + row]: fp32, over the ring (every load has landed and every MMA is done)
-  float* part = reinterpret_cast<float*>(smem);
-  __syncthreads();  // warps 0 and 1 have issued everything; the producer saw every load land
+  // ------------------------------------------------------------ partial sums to their owners
+  // part[(source rank * own + t - owner's first token) * wr + row] of the owner of token t
+  float* part = reinterpret_cast<float*>(smem + p.part_off);
   if (!mbar_wait_bounded(&bars->acc_full, 0, wait_limit) &&
       *reinterpret_cast<volatile int*>(abort_flag) == 0)
     flag(abort_flag, a.err_word, kErrWaitEpilogue);
   __syncwarp();
+  if (split > 1) cluster_wait();
   tc_fence_after();
   if (warp >= 2) {
     const int quad = warp & 3, half = (warp - 2) >> 2;
     const int row = quad * 32 + lane;
     if (quad * 32 < p.wr) {
+      const uint32_t mine = smem_u32(part) + static_cast<uint32_t>((rank * p.own * p.wr + row) * 4);
       for (int c = half * 16; c < p.tn; c += 32) {
         uint32_t r[16];
         tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + c, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) part[(c + j) * p.wr + row] = __uint_as_float(r[j]);
+        for (int j = 0; j < 16; ++j) {
+          const int t = c + j, owner = (t * p.own_mul) >> 16;
+          const uint32_t at = mine + static_cast<uint32_t>((t - owner * p.own) * p.wr * 4);
+          st_cluster_f32(mapa_shared(at, static_cast<uint32_t>(owner)), __uint_as_float(r[j]));
+        }
       }
     }
     tc_fence_before();
@@ -768,7 +774,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   // This CTA's share of the tile's tokens: a thread keeps four output columns (whose scales and
   // biases it fetches while the cluster's barrier fills) and takes every so many tokens, the
   // ranks' partial sums added in rank order.
-  const int t0 = p.tn * rank / split, t1 = p.tn * (rank + 1) / split;
+  const int first = rank * p.own, count = min(p.own, p.tn - first);  // may be negative
   const int quad_shift = 31 - __clz(out_rows / 4);  // out_rows is a power of two
   const int id = static_cast<int>(threadIdx.x);
   const int row = (id & ((1 << quad_shift) - 1)) * 4, col = nb * out_rows + row;
@@ -802,31 +808,28 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     z[1] = f2_add(z[1], f2_of_bf16x2(bias.y));
   };
   if (good && in_columns) {
-    const uint32_t part_addr = smem_u32(part) + static_cast<uint32_t>(row * 4);
-    uint32_t peers[kSplitMax];
-#pragma unroll
-    for (int q = 0; q < kSplitMax; ++q) peers[q] = q < split ? mapa_shared(part_addr, static_cast<uint32_t>(q)) : 0u;
-    const auto total = [&](uint32_t where) {  // the ranks' sums in rank order, loads first
+    const auto total = [&](int t, int row) {  // the ranks' sums in rank order, loads first
       float4 v[kSplitMax];
+      const float* at = part + t * p.wr + row;
 #pragma unroll
       for (int q = 0; q < kSplitMax; ++q)
-        if (q < split) v[q] = ld_cluster_f4(peers[q] + where);
+        if (q < split) v[q] = *reinterpret_cast<const float4*>(at + q * p.own * p.wr);
       float4 z = v[0];
 #pragma unroll
       for (int q = 1; q < kSplitMax; ++q)
         if (q < split) z.x += v[q].x, z.y += v[q].y, z.z += v[q].z, z.w += v[q].w;
       return z;
     };
-    for (int t = t0 + (id >> quad_shift); t < t1; t += kJoinThreads >> quad_shift) {
-      const int token = mb * p.tn + t;
+    for (int t = id >> quad_shift; t < count; t += kJoinThreads >> quad_shift) {
+      const int token = mb * p.tn + first + t;
       if (token >= a.m) break;
       const int64_t dst = static_cast<int64_t>(token) * a.n + col;
       uint2 res = make_uint2(0, 0);
       if (residual != nullptr) res = __ldg(reinterpret_cast<const uint2*>(residual + dst));
       const float sx = kF8 ? __ldg(a.sx + token) : 1.0f;
       uint64_t z[2], u[2];
-      affine(total(static_cast<uint32_t>(t * p.wr * 4)), sx, sg, bg, z);
-      if (gated) affine(total(static_cast<uint32_t>((t * p.wr + out_rows) * 4)), sx, su, bu, u);
+      affine(total(t, row), sx, sg, bg, z);
+      if (gated) affine(total(t, row + out_rows), sx, su, bu, u);
       act4(a.act, z);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
@@ -836,12 +839,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       *reinterpret_cast<uint2*>(y + dst) = make_uint2(f2_to_bf16x2(z[0]), f2_to_bf16x2(z[1]));
     }
   }
-  tc_fence_before();
+  // nobody sends to this CTA any more; its warps have read TMEM before the barrier above
   __syncwarp();
-  if (split > 1)
-    cluster_sync();  // no CTA leaves while a peer reads its partial sums
-  else
-    __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, cols);
 }
@@ -1152,10 +1151,10 @@ int resident_clusters(int split) {
 // Both planners estimate cycles per SM from measured rates and take the cheapest tile.
 //
 // Split: a K tile costs its four MMAs, about 137 cycles each whatever their N up to 128 (an
-// M = 128 MMA takes its A rows from shared memory at 32 bytes a cycle) and 164 at N = 256, or
-// its bytes: W at an SM's share of HBM (24 bytes a cycle), x from L2.  Half-empty MMAs (64 W
-// rows) pay only when W has few rows.  Setup, drain and output take about 6000 cycles, the
-// exchange of partial sums 2000 more.
+// M = 128 MMA takes its A rows from shared memory at 32 bytes a cycle), or its bytes: W at an
+// SM's share of HBM (24 bytes a cycle), x from L2.  Half-empty MMAs (64 W rows) pay only when
+// W has few rows.  Setup, drain and output take about 6000 cycles, the exchange of partial
+// sums 2000 more.
 template <bool kF8>
 SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
   SplitPlan best = {};
@@ -1164,12 +1163,12 @@ SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
   for (int wr = 64; wr <= 128; wr *= 2) {
     const int64_t n_tiles = (wn + wr - 1) / wr;
     int last_tn = 0;
-    for (int tn_max = 64; tn_max <= 256; tn_max *= 2) {
+    for (int tn_max = 64; tn_max <= 128; tn_max *= 2) {
       const int64_t m_tiles = (l.m + tn_max - 1) / tn_max;
       const int tn = static_cast<int>(((l.m + m_tiles - 1) / m_tiles + 15) / 16 * 16);
       if (tn == last_tn) continue;
       last_tn = tn;
-      const double mma = tn <= 128 ? 550.0 : 550.0 + 0.85 * (tn - 128);
+      const double mma = 550.0;
       const double bytes = wr * kKB / 24.0 + tn * kKB / 64.0;
       for (int split = 1; split <= kSplitMax && split <= k_tiles; ++split) {
         const int64_t clusters = resident_clusters<kF8>(split);
@@ -1190,8 +1189,12 @@ SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
   int group = 24576 / tile_bytes;
   group = group < 1 ? 1 : group;
   best.group = group;
-  best.stages = kSplitRingBytes / (tile_bytes * group);
+  best.own = (best.tn + best.split - 1) / best.split;
+  best.own_mul = (65536 + best.own - 1) / best.own;
+  const int part_bytes = best.split * best.own * best.wr * 4;
+  best.stages = (kSplitDataBytes - (part_bytes > kSplitPad ? part_bytes : kSplitPad)) / (tile_bytes * group);
   if (best.stages > kSplitStagesMax) best.stages = kSplitStagesMax;
+  best.part_off = best.stages * tile_bytes * group;
   best.m_tiles = static_cast<int>((l.m + best.tn - 1) / best.tn);
   best.k_each = k_tiles / best.split;
   best.k_more = k_tiles % best.split;
