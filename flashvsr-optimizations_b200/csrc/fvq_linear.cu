@@ -13,6 +13,8 @@
 //     stages, two accumulators in TMEM so that the next tile's products run under the
 //     epilogue.  Gated: the even CTA loads the tile's Wg rows, the odd one its Wu rows, so
 //     both halves of an output column meet in the same TMEM lane and no pass over h is made.
+//     Where the tiles are few and K is long, two to four pairs share a tile's K and join their
+//     accumulators through distributed shared memory (kSplitK).
 //   linear_split_kernel  few tokens: bound by reading W once.  The operands change places:
 //     `wr` rows of W are the M side, up to 128 tokens the N side, so that a few tokens cost
 //     N = 16 instructions and not a 128-row tile; K is split over a cluster of up to eight
@@ -162,6 +164,7 @@ struct LinearArgs {
   int act;
   int bn;                 // accumulator columns per tile (pair kernel)
   int residual;           // 0 / 1
+  int split, k_each, k_more;  // pair kernel: pairs per tile; K tiles each, and one more for the first k_more
   uint64_t wait_limit;
   uint32_t* err_word;
 };
@@ -235,7 +238,23 @@ __device__ __forceinline__ void act32(int act, uint64_t (&z)[16], const uint64_t
   }
 }
 
-template <bool kF8, bool kGated>
+__device__ __forceinline__ uint32_t cluster_id() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// kSplitK: one tile per cluster of 2 * split CTAs, each pair taking its share of K.
+template <bool kF8, bool kGated, bool kSplitK>
 __global__ void __launch_bounds__(kPairThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_x,
                        const __grid_constant__ CUtensorMap tmap_w,
@@ -250,9 +269,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   int* abort_flag = &bars->abort_flag;
   const int warp = warp_index_uniform();
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
+  const uint32_t cta = cluster_ctarank(), rank = cta & 1u;  // in the cluster, in the pair
   const bool even = rank == 0;
-  const int pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+  const int split = kSplitK ? a.split : 1, part = kSplitK ? static_cast<int>(cta >> 1) : 0;
+  const int pairs = kSplitK ? static_cast<int>(gridDim.x) / (2 * split) : gridDim.x / 2;
+  const int pair = kSplitK ? static_cast<int>(cluster_id()) : blockIdx.x / 2;
+  const int kt0 = kSplitK ? part * a.k_each + min(part, a.k_more) : 0;
+  const int kt1 = kSplitK ? kt0 + a.k_each + (part < a.k_more ? 1 : 0) : a.k_tiles;
   const int bn = a.bn, out_cols = kGated ? bn / 2 : bn;
   const int n_blocks = (a.n + out_cols - 1) / out_cols;
   const int tiles = ((a.m + kPairTokens - 1) / kPairTokens) * n_blocks;
@@ -286,8 +309,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   tc_fence_after();
   grid_dependency_wait();
   const uint32_t tmem = bars->tmem_base;
-  const auto even_addr = [&](const void* p) { return mapa_shared(smem_u32(p), 0); };
-  const auto odd_addr = [&](const void* p) { return mapa_shared(smem_u32(p), 1); };
+  const auto even_addr = [&](const void* p) { return mapa_shared(smem_u32(p), cta & ~1u); };
+  const auto odd_addr = [&](const void* p) { return mapa_shared(smem_u32(p), cta | 1u); };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (both CTAs)
@@ -305,7 +328,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // gated: Wg rows in the even CTA, the same columns' Wu rows in the odd one
       const int w_row = kGated ? nb * out_cols + static_cast<int>(rank) * a.n
                                : nb * bn + static_cast<int>(rank) * (bn / 2);
-      for (int kt = 0; kt < a.k_tiles; ++kt) {
+      for (int kt = kt0; kt < kt1; ++kt) {
         if (!warp_wait_cluster_bounded(&bars->empty[stage], phase ^ 1u, wait_limit)) {
           warp_flag(abort_flag, a.err_word, kErrWaitProducer);
           break;
@@ -333,6 +356,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           !warp_wait_cluster_bounded(&bars->full[s], (armed[s] - 1) & 1u, teardown_limit))
         warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
     }
+    if constexpr (kSplitK) cluster_sync();  // the partial sums are in place
   } else if (warp == 1) {
     if (even) {
       // ---------------------------------------------------------- MMA issuer (even CTA)
@@ -349,7 +373,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(buf * kAccCols);
-        for (int kt = 0; kt < a.k_tiles; ++kt) {
+        for (int kt = kt0; kt < kt1; ++kt) {
           if (!warp_wait_cluster_bounded(&bars->full[stage], phase, wait_limit)) {
             warp_flag(abort_flag, a.err_word, kErrWaitMma);
             ok = false;
@@ -365,7 +389,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             for (int j = 0; j < 4; ++j)  // 32-byte K steps inside the 128B swizzle atom
               mma_pair<kF8>(d, adesc + static_cast<uint64_t>(2 * j),
                             bdesc + static_cast<uint64_t>(2 * j), idesc,
-                            (kt > 0 || j > 0) ? 1u : 0u);
+                            (kt > kt0 || j > 0) ? 1u : 0u);
             tc_commit_pair(smem_u32(&bars->empty[stage]));
             tc_commit_pair(empty_odd);
           }
@@ -391,6 +415,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
       }
     }
+    if constexpr (kSplitK) cluster_sync();
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
     // Warp w: TMEM lanes 32 * (w % 4).., every second 32-column chunk of the tile.  A chunk
@@ -406,6 +431,49 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t swizzle = (lane >> 1) & 3u;  // 64B swizzle of row `lane`
     uint32_t uses = 0;  // chunks through the staging buffers so far
     bool ok = true;
+    // Split K: the accumulator goes to shared memory, over the ring (its loads have landed and
+    // the MMAs that read it are complete), 16 bytes of columns by row: sums[col / 4][row].
+    // After the cluster's barrier CTA `cta` joins every split-th chunk, adding the sums of the
+    // CTAs of its parity in rank order.
+    float4* sums = reinterpret_cast<float4*>(smem);
+    if constexpr (kSplitK) {
+      if (!mbar_wait_cluster_bounded(&bars->acc_full[0], 0, wait_limit)) {
+        flag(abort_flag, a.err_word, kErrWaitEpilogue);
+        ok = false;
+      }
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      tc_fence_after();
+      for (int c = half; ok && c < bn / kChunk; c += 2) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tmem + static_cast<uint32_t>(c * kChunk) + (static_cast<uint32_t>(quad * 32) << 16), r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          sums[(c * 8 + j) * 128 + trow] =
+              make_float4(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1]),
+                          __uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3]));
+      }
+      tc_fence_before();
+      __syncwarp();
+      cluster_sync();
+    }
+    const auto joined = [&](int c, uint32_t (&r)[32]) {  // 32 columns of this row, all parts
+      const uint32_t at = smem_u32(sums + c * 8 * 128 + trow);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) r[j] = 0;
+      for (int q = 0; q < split; ++q) {
+        const uint32_t peer = mapa_shared(at, 2u * static_cast<uint32_t>(q) + rank);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 v = ld_cluster_f4(peer + static_cast<uint32_t>(j * 128 * 16));
+          r[4 * j] = __float_as_uint(__uint_as_float(r[4 * j]) + v.x);
+          r[4 * j + 1] = __float_as_uint(__uint_as_float(r[4 * j + 1]) + v.y);
+          r[4 * j + 2] = __float_as_uint(__uint_as_float(r[4 * j + 2]) + v.z);
+          r[4 * j + 3] = __float_as_uint(__uint_as_float(r[4 * j + 3]) + v.w);
+        }
+      }
+    };
+    const int c_first = part + split * half, c_step = 2 * split;  // split 1: every second chunk
     for (int i = 0; ok && i < count; ++i) {
       const int t = pair + i * pairs;
       const int nb = t % n_blocks, mb = t / n_blocks;
@@ -422,16 +490,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if constexpr (kGated) u = column_param<kF8>(a, a.n + col, in);
       };
       ColumnParam pg, pu;
-      fetch(half, pg, pu);
-      bool waited = false;
-      for (int c = half; c < chunks; c += 2) {
+      fetch(c_first, pg, pu);
+      bool waited = kSplitK;
+      for (int c = c_first; c < chunks; c += c_step) {
         const int col0 = tile_col + c * kChunk;
         const bool inside = col0 < a.n && row0 < a.m;  // warp-uniform
         uint8_t* stage_buf = staging + (uses & 1u) * kChunkBytes;
         __syncwarp();  // the previous chunk's parameters have been read
         put_param<kF8>(param, lane, pg);
         if constexpr (kGated) put_param<kF8>(param_u, lane, pu);
-        fetch(c + 2, pg, pu);
+        fetch(c + c_step, pg, pu);
         if (inside) {
           // at most one committed store (of the other buffer) may still be reading
           if (lane == 0) {
@@ -457,8 +525,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const uint32_t taddr = tmem + static_cast<uint32_t>(buf * kAccCols + c * kChunk) +
                                (static_cast<uint32_t>(quad * 32) << 16);
         if (ok && inside) {
-          tmem_ld_32x32b_x32(taddr, r);
-          if constexpr (kGated) tmem_ld_32x32b_x32(taddr + out_cols, v);
+          if constexpr (kSplitK) {
+            joined(c, r);
+            if constexpr (kGated) joined(c + chunks, v);
+          } else {
+            tmem_ld_32x32b_x32(taddr, r);
+            if constexpr (kGated) tmem_ld_32x32b_x32(taddr + out_cols, v);
+          }
         }
         if (inside && a.residual) {
           // a residual load in flight has to land before its buffer is used or the CTA exits
@@ -468,7 +541,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
           ok = __all_sync(0xFFFFFFFFu, ok);
         }
-        tmem_ld_wait();
+        if constexpr (!kSplitK) tmem_ld_wait();
         if (!ok) break;
         if (!inside) continue;
         uint64_t z[16], u[16];
@@ -497,7 +570,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         ++uses;
       }
-      if (!ok) break;
+      if (!ok || kSplitK) break;
       if (!waited) {  // fewer chunks than warps: still wait for and release the accumulator
         ok = mbar_wait_cluster_bounded(&bars->acc_full[buf], static_cast<uint32_t>(i >> 1) & 1u,
                                        wait_limit);
@@ -513,7 +586,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
 
   tc_fence_before();
-  cluster_sync();  // neither CTA leaves while the pair's MMAs or arrivals may touch it
+  __syncwarp();
+  cluster_sync();  // no CTA leaves while the MMAs, arrivals or reads of others may touch it
   tc_fence_after();
   if (warp == 1) tmem_dealloc_pair(tmem, 2 * kAccCols);
 }
@@ -556,12 +630,6 @@ struct SplitPlan {
   int own_mul;    // t / own = t * own_mul >> 16, exact for t * own < 2^16
   int part_off;   // of the partial sums in shared memory
 };
-
-__device__ __forceinline__ uint32_t cluster_id() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
-  return r;
-}
 
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
@@ -1039,7 +1107,7 @@ bool make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, in
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool kF8, bool kGated>
+template <bool kF8, bool kGated, bool kSplitK>
 cudaError_t launch_pair(const LinearProblem& l, const LinearArgs& a, cudaStream_t st,
                         const char** why) {
   const int elem = kF8 ? 1 : 2;
@@ -1053,12 +1121,15 @@ cudaError_t launch_pair(const LinearProblem& l, const LinearArgs& a, cudaStream_
     return cudaErrorInvalidValue;
   }
   static ContextCache attr_done;
-  auto* kernel = linear_pair_kernel<kF8, kGated>;
+  auto* kernel = linear_pair_kernel<kF8, kGated, kSplitK>;
   if (cudaError_t e = ensure_max_dynamic_smem(attr_done, reinterpret_cast<const void*>(kernel),
                                               kPairSmemBytes))
     return e;
   const int64_t out_cols = kGated ? a.bn / 2 : a.bn;
   const int64_t tiles = ((l.m + kPairTokens - 1) / kPairTokens) * ((l.n + out_cols - 1) / out_cols);
+  if (kSplitK)
+    return launch_dependent(kernel, static_cast<unsigned>(2 * a.split * tiles), kPairThreads, kPairSmemBytes, st,
+                            2 * a.split, mx, mw, mr, my, a);
   int64_t pairs = sm_count() / 2;
   if (pairs > tiles) pairs = tiles;
   return launch_dependent(kernel, static_cast<unsigned>(2 * pairs), kPairThreads, kPairSmemBytes, st, 2, mx, mw,
@@ -1205,22 +1276,41 @@ SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
 
 // Pair: a K tile of a 256 x bn tile takes time in proportion to bn + 205 (7680 x 1536 x 8960
 // timed at bn 64 to 256: 0.21, 0.26, 0.29, 0.36 us), so narrower tiles pay only where they
-// fill a round of the persistent grid better.
-int plan_pair(const LinearProblem& l, int k_tiles, double* cost) {
-  const int64_t pairs = sm_count() / 2, mb = (l.m + kPairTokens - 1) / kPairTokens;
-  int best = 256;
+// fill a round of the persistent grid better, and splitting K only where the tiles leave most
+// of it idle (1024 x 1536 x 8960: 37 us unsplit).
+struct PairPlan {
+  int bn, split;
+};
+
+template <bool kF8>
+PairPlan plan_pair(const LinearProblem& l, int k_tiles, double* cost) {
+  const int64_t mb = (l.m + kPairTokens - 1) / kPairTokens;
+  PairPlan best = {256, 1};
   *cost = 1e30;
-  for (int bn = 256; bn >= 128; bn -= l.gated ? 64 : 32) {
-    const int64_t out_cols = l.gated ? bn / 2 : bn;
-    const int64_t tiles = mb * ((l.n + out_cols - 1) / out_cols);
-    const int64_t rounds = (tiles + pairs - 1) / pairs;
-    const double c = static_cast<double>(rounds) * k_tiles * (bn + 205) * 1.5 + 9000.0;
-    if (c < *cost) {
-      *cost = c;
-      best = bn;
+  for (int split = 1; split <= kSplitMax / 2 && split <= k_tiles; ++split) {
+    // clusters of either kernel fill an SM per CTA, so the same number of them fits
+    const int64_t at_once = split == 1 ? sm_count() / 2 : resident_clusters<kF8>(2 * split);
+    for (int bn = 256; bn >= 128; bn -= l.gated ? 64 : 32) {
+      const int64_t out_cols = l.gated ? bn / 2 : bn;
+      const int64_t tiles = mb * ((l.n + out_cols - 1) / out_cols);
+      const int64_t rounds = (tiles + at_once - 1) / at_once;
+      const double c = static_cast<double>(rounds) * ((k_tiles + split - 1) / split) * (bn + 205) * 1.5 + 9000.0 +
+                       (split > 1 ? static_cast<double>(rounds) * 8000.0 : 0.0);
+      if (c < *cost) {
+        *cost = c;
+        best.bn = bn;
+        best.split = split;
+      }
     }
   }
   return best;
+}
+
+template <bool kF8>
+cudaError_t launch_pair_by_plan(const LinearProblem& l, const LinearArgs& a, cudaStream_t st, const char** why) {
+  if (a.split > 1)
+    return l.gated ? launch_pair<kF8, true, true>(l, a, st, why) : launch_pair<kF8, false, true>(l, a, st, why);
+  return l.gated ? launch_pair<kF8, true, false>(l, a, st, why) : launch_pair<kF8, false, false>(l, a, st, why);
 }
 
 }  // namespace
@@ -1253,12 +1343,14 @@ cudaError_t launch_linear(const LinearProblem& l, uint64_t wait_limit, cudaStrea
   double split_cost, pair_cost;
   const SplitPlan p = l.fp8 ? plan_split<true>(l, a.k_tiles, &split_cost)
                             : plan_split<false>(l, a.k_tiles, &split_cost);
-  a.bn = plan_pair(l, a.k_tiles, &pair_cost);
+  const PairPlan pp = l.fp8 ? plan_pair<true>(l, a.k_tiles, &pair_cost) : plan_pair<false>(l, a.k_tiles, &pair_cost);
+  a.bn = pp.bn;
+  a.split = pp.split;
+  a.k_each = a.k_tiles / pp.split;
+  a.k_more = a.k_tiles % pp.split;
   if (mode == 1 || (mode == 0 && split_cost < pair_cost))
     return l.fp8 ? launch_split<true>(l, a, p, st, why) : launch_split<false>(l, a, p, st, why);
-  if (l.fp8)
-    return l.gated ? launch_pair<true, true>(l, a, st, why) : launch_pair<true, false>(l, a, st, why);
-  return l.gated ? launch_pair<false, true>(l, a, st, why) : launch_pair<false, false>(l, a, st, why);
+  return l.fp8 ? launch_pair_by_plan<true>(l, a, st, why) : launch_pair_by_plan<false>(l, a, st, why);
 }
 
 }  // namespace fvq
