@@ -184,7 +184,8 @@ def binding():
         mod.bind(*(ctypes.cast(getattr(lib, f"fvq_{n}"), _vp).value
                    for n in ("rms_norm", "linear_act", "fp8_scaled_mm_act", "fp8_cache_write",
                              "fp8_cache_read")))
-        _binding = mod
+        with _lock:
+            _binding = _binding or mod
     return _binding
 
 

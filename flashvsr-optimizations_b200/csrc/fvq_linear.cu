@@ -126,6 +126,12 @@ __device__ __forceinline__ bool warp_aborted(const int* abort_flag) {
   return __shfl_sync(0xFFFFFFFFu, *reinterpret_cast<const volatile int*>(abort_flag), 0) != 0;
 }
 
+__device__ __forceinline__ void pause_ns(uint64_t ns) {
+  const uint64_t start = global_timer_ns();
+  for (int i = 0; i < (1 << 20) && global_timer_ns() - start < ns; ++i) {
+  }
+}
+
 // ---------------------------------------------------------------- many tokens
 constexpr int kPairTokens = 256;                  // per pair; 128 per CTA
 constexpr int kPairABytes = 128 * kKB;            // 16 KB
@@ -356,6 +362,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           !warp_wait_cluster_bounded(&bars->full[s], (armed[s] - 1) & 1u, teardown_limit))
         warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
     }
+    // after an abort the even CTA may not have armed a stage that this one has loads for: no
+    // barrier counts them, so give them time to land before the CTA may exit
+    if (!even && warp_aborted(abort_flag)) pause_ns(100000);
     if constexpr (kSplitK) cluster_sync();  // the partial sums are in place
   } else if (warp == 1) {
     if (even) {

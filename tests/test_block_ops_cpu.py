@@ -151,6 +151,6 @@ def test_cache_slot_numbers():
     cache = object.__new__(fvq.FP8KVCache)
     cache.k_codes = torch.zeros(9, 16, 1, 8)
     table = torch.tensor([[4, 2], [7, 0]], dtype=torch.int32)
-    got = cache.slots(table, torch.tensor([[0, 15, 16, 31], [5, -1, 32, 17]]))
+    got = cache.slots(table, torch.tensor([[0, 15, 16, 31], [5, -1, 32, 17]]))   # 32: past its table
     assert got.dtype == torch.int64
-    assert got.tolist() == [64, 79, 32, 47, 117, -1, -1, 1]
+    assert got.tolist() == [64, 79, 32, 47, 117, -1, 144, 1]

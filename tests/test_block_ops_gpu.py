@@ -389,6 +389,22 @@ def test_product_rows_do_not_see_one_another(kernel):
     assert torch.equal(torch.isnan(y), hit) and torch.equal(y[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("m,n,k,gated", [(24, 264, 1536, False), (600, 520, 4096, True), (2000, 1536, 512, False)])
+def test_product_wait_limit(kernel, m, n, k, gated):
+    """With a limit of one test per wait the kernels give up, drain and report; the next call is right."""
+    wn = 2 * n if gated else n
+    x, w, r = randn(m, k, seed=1), randn(wn, k, seed=2, std=k ** -0.5), randn(m, n, seed=3)
+    want = ops.linear_act(x, w, act="silu", gated=gated, residual=r)
+    assert ops.read_device_error() == 0
+    ops.set_wait_limit(1)
+    try:
+        ops.linear_act(x, w, act="silu", gated=gated, residual=r)
+        assert ops.read_device_error() != 0
+    finally:
+        ops.set_wait_limit(0)
+    assert torch.equal(ops.linear_act(x, w, act="silu", gated=gated, residual=r), want)
+
+
 def test_product_empty_and_refusals():
     x, w = randn(4, 64), randn(72, 64)
     assert ops.linear_act(x[:0], w).shape == (0, 72)
@@ -757,6 +773,52 @@ def test_kv_cache_object():
             assert (got[b, n:] == 0).all()
 
 
+@pytest.mark.parametrize("name", ["rms_norm", "add_rms_norm", "rms_norm_fp8", "add_rms_norm_fp8", "linear_act",
+                                  "fp8_scaled_mm_act", "fp8_cache_write", "fp8_cache_read"])
+def test_registered_operators(name):
+    """Schemas (what is written in place, no aliases) and fake kernels, as torch checks them."""
+    x, r, w = randn(6, 64, seed=1), randn(6, 64, seed=2, dtype=F32), randn(64, seed=3)
+    q, s = ops.fp8_row_quant(x)
+    wq, ws = ops.fp8_row_quant(randn(32, 64, seed=4))
+    cache = store(3, 4, 2, 32)
+    args = {"rms_norm": (x, w, 1e-6), "add_rms_norm": (x, r, w, 1e-6), "rms_norm_fp8": (x, None, 1e-6),
+            "add_rms_norm_fp8": (x, r, w, 1e-6), "linear_act": (x, randn(32, 64, seed=5), None, "silu", True, None),
+            "fp8_scaled_mm_act": (q, s, wq, ws, None, "none", False, randn(6, 32, seed=6)),
+            "fp8_cache_write": (x.view(6, 2, 32), x.view(6, 2, 32), torch.arange(6, device="cuda"), *cache),
+            "fp8_cache_read": (*cache, torch.zeros(1, 2, dtype=torch.int32, device="cuda"),
+                               torch.ones(1, dtype=torch.int32, device="cuda"), 5)}[name]
+    # torch's schema check multiplies its inputs, which E4M3 tensors do not do
+    plain = not any(isinstance(a, torch.Tensor) and a.dtype == F8 for a in args)
+    torch.library.opcheck(getattr(torch.ops.fvq, name).default, args,
+                          test_utils=("test_schema", "test_faketensor") if plain else ("test_faketensor",))
+
+
+def test_calls_that_the_short_path_leaves_to_python():
+    """The same results through the registered operators and through the short path."""
+    x, r, w = randn(40, 64, seed=1), randn(40, 64, seed=2), randn(64, seed=3)
+    m, b = randn(72, 64, seed=4), randn(72, seed=5)
+    op = torch.ops.fvq
+    for a, c in zip(ops.add_rms_norm_fp8(x, r, w), op.add_rms_norm_fp8.default(x, r, w, 1e-6)):
+        assert torch.equal(a.float(), c.float())
+    assert torch.equal(ops.linear_act(x, m, b, "relu"), op.linear_act.default(x, m, b, "relu", False, None))
+    q, s = ops.fp8_row_quant(x)
+    wq, ws = ops.fp8_row_quant(m[:64])                        # gated: 32 columns
+    assert torch.equal(ops.fp8_scaled_mm_act(q, s, wq, ws, act="silu", gated=True),
+                       op.fp8_scaled_mm_act.default(q, s, wq, ws, None, "silu", True, None))
+    c1, c2 = store(12, 4, 1, 64), store(12, 4, 1, 64)
+    slots = torch.arange(40, device="cuda")
+    ops.fp8_cache_write(x.view(40, 1, 64), r.view(40, 1, 64), slots, *c1)
+    before = c1[0]._version
+    ops.fp8_cache_write(x.view(40, 1, 64), r.view(40, 1, 64), slots, *c1)
+    assert c1[0]._version > before                            # an in-place write is seen by autograd
+    op.fp8_cache_write.default(x.view(40, 1, 64), r.view(40, 1, 64), slots, *c2)
+    assert all(torch.equal(i.view(torch.uint8), j.view(torch.uint8)) for i, j in zip(c1, c2))
+    table = torch.arange(12, dtype=torch.int32, device="cuda").view(1, 12)
+    lens = torch.tensor([40], dtype=torch.int32, device="cuda")
+    for a, c in zip(ops.fp8_cache_read(*c1, table, lens, 44), op.fp8_cache_read.default(*c1, table, lens, 44)):
+        assert torch.equal(a, c)
+
+
 def test_other_threads_and_modes():
     """Calls from two threads on streams of their own, and under a dispatch mode."""
     import threading
@@ -796,3 +858,54 @@ def test_other_threads_and_modes():
         cache.write(kv, kv, torch.arange(3, device="cuda"))
     with torch.no_grad():
         assert torch.equal(ops.linear_act(x, torch.nn.Parameter(w), act="silu"), want)
+
+
+# ---------------------------------------------------------------- past 2^31 elements
+def test_large_tensors():
+    """Offsets that pass 32 bits: the last rows of tensors of 2.4e9 elements."""
+    rows, d = 300_000, 8192
+    x = torch.empty(rows, d, dtype=BF16, device="cuda")
+    tail = randn(400, d, seed=1)
+    x[-400:] = tail
+    x[:400] = tail
+    w = randn(d, seed=2)
+    q, scale = ops.rms_norm_fp8(x, w)
+    _, v = norm64(tail, None, w, 1e-6)
+    for part in (slice(0, 400), slice(rows - 400, rows)):
+        codes_inside(q[part], scale[part], v, 2.0 ** -17)
+    del q, scale
+    wide = x.view(rows * 64, 128)                              # short rows: the sub-warp form
+    y = ops.rms_norm(wide)
+    _, v = norm64(tail.view(-1, 128), None, None, 1e-6)
+    inside(y[-400 * 64:], v, v.abs() * (HALF_BF16 + 2.0 ** -17))
+    del y, wide, x
+    torch.cuda.empty_cache()
+    x, m = randn(rows, 64, seed=3), randn(d, 64, seed=4)
+    r = torch.empty(rows, d, dtype=BF16, device="cuda")
+    r[-400:] = tail
+    y = ops.linear_act(x, m, act="silu", residual=r)
+    want, bound = product64(x[-400:], m, None, None, None, "silu", False, tail)
+    inside(y[-400:], want, bound)
+    del y, r
+    torch.cuda.empty_cache()
+
+
+def test_large_store():
+    """A store of 4.7e9 codes a side: slots and pages at its end."""
+    pages, page, heads, d = 48_000, 64, 12, 128
+    codes = [torch.empty(pages, page, heads, d, dtype=torch.uint8, device="cuda").view(F8) for _ in range(2)]
+    scales = [torch.zeros(pages, page, heads, device="cuda") for _ in range(2)]
+    cache = codes[0], scales[0], codes[1], scales[1]
+    kv = randn(100, 2, heads, d, seed=1)
+    table = torch.tensor([[pages - 1, pages - 3], [0, pages - 2]], dtype=torch.int32, device="cuda")
+    at = torch.arange(100, device="cuda")
+    slots = table[0].long()[at // page] * page + at % page
+    ops.fp8_cache_write(kv[:, 0], kv[:, 1], slots, *cache)
+    k, v = ops.fp8_cache_read(*cache, table, torch.tensor([100, 0], dtype=torch.int32, device="cuda"), 100)
+    for got, x in ((k, kv[:, 0]), (v, kv[:, 1])):
+        step = row_scale(x)[..., None].double()
+        bound = torch.maximum(x.double().abs() * HALF_E4M3, step * 2.0 ** -10)
+        inside(got[0], x.double(), bound * (1 + HALF_BF16) + (HALF_BF16 + 2.0 ** -22) * x.double().abs())
+        assert (got[1] == 0).all()
+    del codes, scales, cache
+    torch.cuda.empty_cache()
