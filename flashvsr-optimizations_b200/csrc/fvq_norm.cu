@@ -12,8 +12,9 @@
 //
 // HBM-bound: x and r are read once, every output is written once; the row stays in registers
 // between the two reductions (sum of squares, then max |v| for E4M3).  Three forms:
-//   * rows of at most 256 values: sub-warp groups of lanes, several rows a group when there
-//     are many, so that their loads overlap;
+//   * rows of at most 512 values: a warp or a part of one, several rows a group when they are
+//     short and there are many, so that their loads overlap (65317 rows of 271: 26.6 us, 48
+//     streamed; 20000 of 768: 31 us, 20.6 streamed);
 //   * few rows: a CTA per row with 8 or 16 values a thread, the shortest chain for one token;
 //   * many rows: persistent CTAs whose warps stream rows through rings in shared memory
 //     filled by bulk copies (rms_norm_stream_kernel), so that loads stay in flight while
@@ -640,13 +641,13 @@ cudaError_t norm_launch(const NormArgs& a, bool vec, cudaStream_t st) {
   return launch_dependent(rms_norm_kernel<kLanes, kRows, kPer, 1>, grid, threads, 0, st, 0, a);
 }
 
-template <int kLanes>
+template <int kLanes, int kPer = 8>
 cudaError_t norm_short(const NormArgs& a, bool vec, cudaStream_t st) {
   // two rows a group once that still leaves every SM its threads (92160 rows of 128: 10.0 us
   // with one, 9.0 with two, 9.4 with four)
   if (a.rows * kLanes >= static_cast<int64_t>(sm_count()) * 2048 * 2)
-    return norm_launch<kLanes, 2, 8>(a, vec, st);
-  return norm_launch<kLanes, 1, 8>(a, vec, st);
+    return norm_launch<kLanes, 16 / kPer, kPer>(a, vec, st);
+  return norm_launch<kLanes, 1, kPer>(a, vec, st);
 }
 
 template <int kGroup, int kPer, int kVec>
@@ -665,10 +666,15 @@ template <int kGroup, int kVec>
 cudaError_t stream_by_width(const NormArgs& a, const StreamPlan& p, uint64_t wait_limit,
                             uint32_t* err_word, cudaStream_t st) {
   const int per = (a.d + (kVec == 2 ? 1 : 0) + 32 * kGroup - 1) / (32 * kGroup);
-  if (per <= 16) return stream_launch<kGroup, 16, kVec>(a, p, wait_limit, err_word, st);
-  if (per <= 32) return stream_launch<kGroup, 32, kVec>(a, p, wait_limit, err_word, st);
-  if (per <= 48) return stream_launch<kGroup, 48, kVec>(a, p, wait_limit, err_word, st);
-  return stream_launch<kGroup, 72, kVec>(a, p, wait_limit, err_word, st);
+  // 17 values a lane at the least (rows are longer than 512, and groups grow when they have
+  // to); sixteen warps hold the longest row with 32
+  if (kGroup == kStreamWarps || per <= 32)
+    return stream_launch<kGroup, 32, kVec>(a, p, wait_limit, err_word, st);
+  if constexpr (kGroup < kStreamWarps) {
+    if (per <= 48) return stream_launch<kGroup, 48, kVec>(a, p, wait_limit, err_word, st);
+    return stream_launch<kGroup, 72, kVec>(a, p, wait_limit, err_word, st);
+  }
+  return cudaErrorInvalidValue;
 }
 
 template <int kGroup>
@@ -700,6 +706,7 @@ cudaError_t launch_rms_norm(const NormArgs& args, uint64_t wait_limit, cudaStrea
   if (d <= 64) return norm_short<8>(a, vec, st);
   if (d <= 128) return norm_short<16>(a, vec, st);
   if (d <= 256) return norm_short<32>(a, vec, st);
+  if (d <= 512) return norm_short<32, 16>(a, vec, st);
   {
     // warps per row: rings of two rows per group within the shared memory, 64 values a lane
     StreamPlan p;

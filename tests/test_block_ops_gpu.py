@@ -112,7 +112,7 @@ def test_norm_strided_views(d):
     check_norm(qkv[:4, :d].t(), None, None)                       # no adjacent values: copied
 
 
-@pytest.mark.parametrize("rows,d", [(9600, 264), (5001, 1536), (4800, 2047), (4740, 2048), (2400, 2050), (2400, 4096),
+@pytest.mark.parametrize("rows,d", [(9600, 264), (9600, 520), (4737, 515), (5001, 1536), (4800, 2047), (4740, 2048), (2400, 2050), (2400, 4096),
                                     (1300, 5555), (1250, 8960), (650, 12288), (700, 16384), (4737, 301)])
 @pytest.mark.parametrize("residual", [None, BF16, F32])
 def test_norm_many_rows(rows, d, residual):
