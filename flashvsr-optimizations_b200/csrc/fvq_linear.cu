@@ -44,29 +44,80 @@ constexpr int kKB = 128;  // bytes of K per row and tile: one 128B swizzle row
 // ---------------------------------------------------------------- activations
 enum Act { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
 
-// z * sigmoid(t), t and z of one sign: one exponential and one fast division (a few fp32 ulp,
-// against bf16's 2^-8), without the cancellation that 1 + tanh has for negative z.  The
-// exponential is of -|t|, so the divisor stays in [1, 2] and the negative tail keeps its
-// digits down to the smallest values.
-__device__ __forceinline__ float z_sigmoid(float z, float t) {
-  const float e = __expf(-fabsf(t));
-  return __fdividef(z < 0.0f ? z * e : z, 1.0f + e);
+// 2^x and 1/x as the hardware approximates them (about 2^-22), results below the smallest normal
+// flushed to zero.
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-// act(z) in fp32; silu and the tanh form of gelu are z * sigmoid(t).  relu keeps NaN.
+__device__ __forceinline__ uint64_t f2_both(float v) { return f2_pack(v, v); }
+
+// z * sigmoid(t) with t and z of one sign, u = t / ln 2, for two values: one exponential and one
+// reciprocal each, without the cancellation that 1 + tanh has for negative z.  The exponential
+// is of -|t|, so the divisor stays in [1, 2] and the negative tail keeps its digits; it is taken
+// 2^8 too large (and z 2^8 too small with it) so that it is not flushed before the product is.
+__device__ __forceinline__ uint64_t z_sigmoid2(uint64_t z2, uint64_t u2) {
+  float z[2], u[2], e[2], r[2];
+  f2_split(z2, z[0], z[1]);
+  f2_split(u2, u[0], u[1]);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) e[j] = ex2(8.0f - fabsf(u[j]));
+  const uint64_t e2 = f2_pack(e[0], e[1]);
+  float d[2];
+  f2_split(f2_fma(e2, f2_both(0x1p-8f), f2_both(1.0f)), d[0], d[1]);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) r[j] = rcp_approx_ftz(d[j]);
+  const uint64_t num = f2_mul(f2_mul(z2, f2_both(0x1p-8f)),
+                              f2_pack(z[0] < 0.0f ? e[0] : 256.0f, z[1] < 0.0f ? e[1] : 256.0f));
+  return f2_mul(num, f2_pack(r[0], r[1]));
+}
+
+// 0.5 z erfc(-z / sqrt 2) for two values.  With x = |z| / sqrt 2 and s = 1 / (1 + x / 2),
+// g = 0.5 erfc(x) = s 2^(p(s) - x^2 log2 e), where p is the polynomial of degree 7 that meets
+// log2(0.5 erfc(x) e^(x^2) / s) at the Chebyshev nodes of s over 0 <= x <= 9.6.  g is off by
+// 1e-6 of itself up to x = 2, and by 1e-5 at x = 9 for the rounding of x^2.  The result is
+// z (1 - g) for positive z and z g for the others, which has no cancellation.
+__device__ __forceinline__ uint64_t gelu2(uint64_t z2) {
+  float z[2], a[2], g[2], s[2];
+  f2_split(z2, z[0], z[1]);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) s[j] = rcp_approx_ftz(fmaf(fabsf(z[j]), 0.353553385f, 1.0f));
+  const uint64_t s2 = f2_pack(s[0], s[1]);
+  constexpr float kP[8] = {-2.82571697f, 1.44092202f, 0.566950738f, -0.0534122437f,
+                           0.498900861f, -1.43910909f, 1.08193898f, -0.270475209f};
+  uint64_t p = f2_both(kP[7]);
+#pragma unroll
+  for (int i = 6; i >= 0; --i) p = f2_fma(p, s2, f2_both(kP[i]));
+  f2_split(f2_fma(f2_mul(z2, z2), f2_both(-0.7213475204444817f), p), a[0], a[1]);  // log2(e) / 2
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    g[j] = s[j] * ex2(a[j]);
+    g[j] = z[j] > 0.0f ? 1.0f - g[j] : g[j];
+  }
+  return f2_mul(z2, f2_pack(g[0], g[1]));
+}
+
+// act(z) of two values in fp32; silu is z sigmoid(z), the tanh form of gelu z sigmoid(2 sqrt(2 /
+// pi) (z + 0.044715 z^3)).  relu keeps NaN.
 template <int kAct>
-__device__ __forceinline__ float activate(float z) {
+__device__ __forceinline__ uint64_t activate2(uint64_t z2) {
+  constexpr float kLog2e = 1.4426950408889634f;
   if constexpr (kAct == kActRelu) {
-    return z < 0.0f ? 0.0f : z;
+    float lo, hi;
+    f2_split(z2, lo, hi);
+    return f2_pack(lo < 0.0f ? 0.0f : lo, hi < 0.0f ? 0.0f : hi);
   } else if constexpr (kAct == kActGelu) {
-    return 0.5f * z * erfcf(-0.70710678118654752f * z);
+    return gelu2(z2);
   } else if constexpr (kAct == kActGeluTanh) {
-    const float t = 1.5957691216057308f * z * fmaf(0.044715f * z, z, 1.0f);  // 2 sqrt(2/pi) (z + ..)
-    return z_sigmoid(z, t);
+    constexpr float kA = 1.5957691216057308f * kLog2e;
+    const uint64_t q = f2_fma(f2_mul(z2, z2), f2_both(kA * 0.044715f), f2_both(kA));
+    return z_sigmoid2(z2, f2_mul(z2, q));
   } else if constexpr (kAct == kActSilu) {
-    return z_sigmoid(z, z);
+    return z_sigmoid2(z2, f2_mul(z2, f2_both(kLog2e)));
   } else {
-    return z;
+    return z2;
   }
 }
 
@@ -224,11 +275,7 @@ template <int kAct, bool kGated>
 __device__ __forceinline__ void act32_t(uint64_t (&z)[16], const uint64_t (&u)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    if constexpr (kAct != kActNone) {
-      float lo, hi;
-      f2_split(z[i], lo, hi);
-      z[i] = f2_pack(activate<kAct>(lo), activate<kAct>(hi));
-    }
+    z[i] = activate2<kAct>(z[i]);
     if constexpr (kGated) z[i] = f2_mul(z[i], u[i]);
   }
 }
@@ -644,25 +691,14 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
-__device__ __forceinline__ float activate_any(int act, float z) {
+__device__ __forceinline__ uint64_t activate2_any(int act, uint64_t z) {
   switch (act) {
-    case kActRelu: return activate<kActRelu>(z);
-    case kActGelu: return activate<kActGelu>(z);
-    case kActGeluTanh: return activate<kActGeluTanh>(z);
-    case kActSilu: return activate<kActSilu>(z);
+    case kActRelu: return activate2<kActRelu>(z);
+    case kActGelu: return activate2<kActGelu>(z);
+    case kActGeluTanh: return activate2<kActGeluTanh>(z);
+    case kActSilu: return activate2<kActSilu>(z);
     default: return z;
   }
-}
-
-__device__ __forceinline__ void act4(int act, uint64_t (&z)[2]) {
-  if (act == kActNone) return;
-  float v[4];
-  f2_split(z[0], v[0], v[1]);
-  f2_split(z[1], v[2], v[3]);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = activate_any(act, v[j]);
-  z[0] = f2_pack(v[0], v[1]);
-  z[1] = f2_pack(v[2], v[3]);
 }
 
 template <bool kF8>
@@ -907,7 +943,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       uint64_t z[2], u[2];
       affine(total(t, row), sx, sg, bg, z);
       if (gated) affine(total(t, row + out_rows), sx, su, bu, u);
-      act4(a.act, z);
+      z[0] = activate2_any(a.act, z[0]);
+      z[1] = activate2_any(a.act, z[1]);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         if (gated) z[j] = f2_mul(z[j], u[j]);
@@ -1082,7 +1119,8 @@ __global__ void __launch_bounds__(kVecThreads, kVecCtas)
   }
   if constexpr (kF8) z = z * __ldg(a.sx + t) * __ldg(a.sw + col);
   if (a.bias != nullptr) z += __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + col)) << 16);
-  z = activate_any(a.act, z);
+  float unused;
+  f2_split(activate2_any(a.act, f2_pack(z, 0.0f)), z, unused);
   if (gated) {
     if constexpr (kF8) u = u * __ldg(a.sx + t) * __ldg(a.sw + a.n + col);
     if (a.bias != nullptr) u += __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + a.n + col)) << 16);

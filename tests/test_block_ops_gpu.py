@@ -353,6 +353,29 @@ def test_product_extreme_values(kernel):
         assert ((y - want).abs() <= tol)[fine].all(), act
 
 
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_activations_of_every_bf16_between_2_to_minus_20_and_40(kernel, act, gated):
+    """The relative error holds down both tails, not only where the values are large."""
+    bits = torch.arange(0x3580, 0x4220, dtype=torch.int32, device="cuda")
+    z = torch.cat([bits, bits | 0x8000]).to(torch.uint16).view(BF16)
+    x = torch.zeros(z.numel(), 16, dtype=BF16, device="cuda")
+    x[:, 0], x[:, 1] = z, 1.0
+    w = torch.zeros(16 if gated else 8, 16, dtype=BF16, device="cuda")
+    w[:8, 0] = 1.0
+    if gated:
+        w[8:, 1] = 1.0
+    y = ops.linear_act(x, w, act=act, gated=gated).double()
+    # 1 + tanh(t) is 2 sigmoid(2 t); the former loses the tail's digits in 64 bits too
+    f = (lambda v: v * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3))) \
+        if act == "gelu_tanh" else ACT64[act]
+    want = f(z.double())[:, None].expand_as(y)
+    # the exponent's argument is at most 126 (in powers of two) where the result is not flushed and
+    # is rounded six times, constants included: 6 * 126 * ln 2 * 2^-24 < 2^-14.9; the exponential,
+    # the reciprocal and the products beside it add less than 2^-19
+    assert ((y - want).abs() <= want.abs() * (HALF_BF16 + 2.0 ** -14.8) + 2.0 ** -125).all()
+
+
 def test_product_views_and_leading_dimensions(kernel):
     wide = randn(2, 40, 400, seed=1)
     w = randn(72, 128, seed=2)
