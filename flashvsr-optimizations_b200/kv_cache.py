@@ -51,9 +51,11 @@ class FP8KVCache:
     def slots(self, page_table: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """The slots (int64, [batch * tokens]) of ``positions`` (integers [batch, tokens]; negative:
         padding, and so is its slot) of the sequences of ``page_table`` [batch, pages].  A position
-        past the table gets a slot past the store, which ``write`` reports."""
+        past the table, or on a page outside the store, gets a slot past the store, which ``write``
+        reports."""
         pages, page = self.k_codes.shape[:2]
         at = positions.long()
         index = page_table.long().gather(1, (at.clamp_min(0) // page).clamp_max(page_table.shape[1] - 1))
-        slot = torch.where(at < page_table.shape[1] * page, index * page + at % page, pages * page)
+        there = (at < page_table.shape[1] * page) & (index >= 0)
+        slot = torch.where(there, index * page + at % page, pages * page)
         return torch.where(at < 0, -1, slot).reshape(-1)

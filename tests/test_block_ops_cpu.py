@@ -154,3 +154,13 @@ def test_cache_slot_numbers():
     got = cache.slots(table, torch.tensor([[0, 15, 16, 31], [5, -1, 32, 17]]))   # 32: past its table
     assert got.dtype == torch.int64
     assert got.tolist() == [64, 79, 32, 47, 117, -1, 144, 1]
+
+
+def test_slots_on_pages_outside_the_store_are_past_it():
+    """A page entry that was never filled in is reported by the write, not taken for padding."""
+    cache = object.__new__(fvq.FP8KVCache)
+    cache.k_codes = torch.empty(6, 16, 1, 8)
+    table = torch.tensor([[3, -1, 6]], dtype=torch.int32)
+    got = cache.slots(table, torch.tensor([[0, 15, 16, 31, 32, -5]]))
+    assert got[:2].tolist() == [48, 63] and got[5] == -1
+    assert (got[2:5] >= 6 * 16).all()
