@@ -179,7 +179,7 @@ bool product_shape(const at::Tensor& x, const at::Tensor& w, const at::Tensor* b
 // linear_act(x, weight, bias, act, gated, residual) -> y
 PyObject* py_linear_act(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
-  if (count != 6 || !PyLong_Check(args[3])) Py_RETURN_NONE;
+  if (count != 6 || !PyLong_Check(args[3]) || !PyBool_Check(args[4])) Py_RETURN_NONE;
   const auto dev = usable_device(reinterpret_cast<const void*>(entries.linear_act), args[0]);
   if (dev < 0) Py_RETURN_NONE;
   bool ok = true;
@@ -187,7 +187,7 @@ PyObject* py_linear_act(PyObject*, PyObject* const* args, Py_ssize_t count) {
   const at::Tensor* w = dense(args[1], at::kBFloat16, dev, 16, &ok);
   const at::Tensor* bias = dense(args[2], at::kBFloat16, dev, 16, &ok, true);
   const at::Tensor* residual = dense(args[5], at::kBFloat16, dev, 16, &ok, true);
-  const bool gated = PyObject_IsTrue(args[4]) == 1;
+  const bool gated = args[4] == Py_True;
   Product p;
   if (x == nullptr || !ok || !product_shape(*x, *w, bias, residual, gated, 8, &p)) Py_RETURN_NONE;
   const int act = static_cast<int>(PyLong_AsLong(args[3]));
@@ -206,7 +206,7 @@ PyObject* py_linear_act(PyObject*, PyObject* const* args, Py_ssize_t count) {
 // fp8_scaled_mm_act(a, scale_a, w, scale_w, bias, act, gated, residual) -> y
 PyObject* py_fp8_scaled_mm_act(PyObject*, PyObject* const* args, Py_ssize_t count) {
   HANDLE_TH_ERRORS
-  if (count != 8 || !PyLong_Check(args[5])) Py_RETURN_NONE;
+  if (count != 8 || !PyLong_Check(args[5]) || !PyBool_Check(args[6])) Py_RETURN_NONE;
   const auto dev = usable_device(reinterpret_cast<const void*>(entries.fp8_scaled_mm_act), args[0]);
   if (dev < 0) Py_RETURN_NONE;
   bool ok = true;
@@ -216,7 +216,7 @@ PyObject* py_fp8_scaled_mm_act(PyObject*, PyObject* const* args, Py_ssize_t coun
   const at::Tensor* sw = dense(args[3], at::kFloat, dev, 16, &ok);
   const at::Tensor* bias = dense(args[4], at::kBFloat16, dev, 16, &ok, true);
   const at::Tensor* residual = dense(args[7], at::kBFloat16, dev, 16, &ok, true);
-  const bool gated = PyObject_IsTrue(args[6]) == 1;
+  const bool gated = args[6] == Py_True;
   Product p;
   if (a == nullptr || !ok || !product_shape(*a, *w, bias, residual, gated, 16, &p) ||
       sa->numel() != p.m || sw->numel() != p.wn)
