@@ -66,7 +66,7 @@ __device__ __forceinline__ uint2 dequantize4(uint32_t codes, float scale) {
 
 // 32-byte accesses: a warp's are whole sectors whichever way they are split up
 __device__ __forceinline__ void load32(const void* p, uint32_t (&w)[8]) {
-  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]),
                  "=r"(w[7])
                : "l"(p));
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheW
   for (int k = 0; k < kRows; ++k) {
     const uint32_t row = min(first + k * kStep, rows - 1);  // whole warps at the shuffles
     const uint32_t token = divide(row, by_heads), head = row - token * by_heads.d;
-    slot[k] = first + k * kStep < rows ? __ldg(a.slots + token) : -1;
+    slot[k] = first + k * kStep < rows ? a.slots[token] : -1;
     const uint16_t* x = src.x + token * src.token_stride + head * src.head_stride;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheW
       if constexpr (kElems == 16) {
         load32(x + j * 16, v[k][i]);
       } else {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(x + j * 8));
+        const uint4 q = *reinterpret_cast<const uint4*>(x + j * 8);
         v[k][i][0] = q.x, v[k][i][1] = q.y, v[k][i][2] = q.z, v[k][i][3] = q.w;
       }
     }
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kCacheThreads)
   const uint8_t* codes = values ? a.v_codes : a.k_codes;
   const float* scales = values ? a.v_scale : a.k_scale;
   const int64_t b = blockIdx.y;
-  const int32_t len_raw = __ldg(a.lengths + b);
+  const int32_t len_raw = a.lengths[b];
   const int64_t most = a.pages_per_seq * a.page < a.max_len ? a.pages_per_seq * a.page : a.max_len;
   const int64_t len = len_raw < most ? len_raw : most;
   if (len_raw > most && blockIdx.x == 0 && threadIdx.x == 0 && !values)
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kCacheThreads)
       const uint32_t pos = static_cast<uint32_t>(pos0) + t;              // below 2^31
       if (pos >= len) continue;
       const uint32_t p = divide(pos, by_page);
-      const int64_t page = __ldg(table + p);
+      const int64_t page = table[p];
       if (page < 0 || page >= a.num_pages) {
         if (vec == 0 && !values) atomicOr(err_word, kErrCachePage);
         continue;
@@ -201,13 +201,13 @@ __global__ void __launch_bounds__(kCacheThreads)
       const int64_t slot = page * a.page + (pos - p * by_page.d);
       const uint8_t* at = codes + (slot * a.heads * a.d + static_cast<int64_t>(vec) * kCodes);
       if constexpr (kCodes == 16) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
+        const uint4 v = *reinterpret_cast<const uint4*>(at);
         c[u][0] = v.x, c[u][1] = v.y, c[u][2] = v.z, c[u][3] = v.w;
       } else {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+        const uint2 v = *reinterpret_cast<const uint2*>(at);
         c[u][0] = v.x, c[u][1] = v.y;
       }
-      s[u] = __ldg(scales + slot * a.heads + divide(vec, by_row));
+      s[u] = scales[slot * a.heads + divide(vec, by_row)];
     }
 #pragma unroll
     for (int u = 0; u < kReadUnroll; ++u) {

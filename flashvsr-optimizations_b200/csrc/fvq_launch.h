@@ -3,7 +3,10 @@
 // They follow one another in a block, each a few microseconds long at a few rows, so every one
 // is launched as a programmatic dependent of the kernel before it: it lets the next one start
 // setting up (grid_launch_dependents) and waits for the previous one to complete
-// (grid_dependency_wait) before any of its threads touches global memory.
+// (grid_dependency_wait) before any of its threads touches global memory.  A kernel may so be
+// running while another writes what it is going to read: it reads with ordinary loads, never
+// through the read-only path (__ldg, ld.global.nc, __restrict__), whose lines nothing promises
+// to refresh inside a running kernel.
 #pragma once
 
 #include <cuda_runtime.h>

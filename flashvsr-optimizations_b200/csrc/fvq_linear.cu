@@ -236,8 +236,8 @@ template <bool kF8>
 __device__ __forceinline__ ColumnParam column_param(const LinearArgs& a, int row, bool inside) {
   ColumnParam c = {1.0f, 0.0f};
   if (inside) {
-    if constexpr (kF8) c.scale = __ldg(a.sw + row);
-    if (a.bias != nullptr) c.bias = __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + row)) << 16);
+    if constexpr (kF8) c.scale = a.sw[row];
+    if (a.bias != nullptr) c.bias = __uint_as_float(static_cast<uint32_t>(a.bias[row]) << 16);
   }
   return c;
 }
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int nb = t % n_blocks, mb = t / n_blocks;
       const int row0 = mb * kPairTokens + static_cast<int>(rank) * 128 + quad * 32;
       const int row = mb * kPairTokens + static_cast<int>(rank) * 128 + trow;
-      const float sx = kF8 && row < a.m ? __ldg(a.sx + row) : 0.0f;
+      const float sx = kF8 && row < a.m ? a.sx[row] : 0.0f;
       const uint64_t sx2 = f2_pack(sx, sx);
       const int buf = i & 1;
       const int tile_col = nb * out_cols;
@@ -705,8 +705,8 @@ template <bool kF8>
 __global__ void __launch_bounds__(kSplitThreads, 1)
     linear_split_kernel(const __grid_constant__ CUtensorMap tmap_x,
                         const __grid_constant__ CUtensorMap tmap_w, const SplitPlan p,
-                        const int gated, const uint16_t* __restrict__ residual,
-                        uint16_t* __restrict__ y, const LinearArgs a) {
+                        const int gated, const uint16_t* residual,
+                        uint16_t* y, const LinearArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   if ((smem_u32(smem) & 1023u) != 0) {
     if (threadIdx.x == 0) atomicOr(a.err_word, kErrSmemAlign);
@@ -896,12 +896,12 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   float4 sg = make_float4(1.0f, 1.0f, 1.0f, 1.0f), su = sg;
   if (in_columns) {
     if (a.bias != nullptr) {
-      bg = __ldg(reinterpret_cast<const uint2*>(a.bias + col));
-      if (gated) bu = __ldg(reinterpret_cast<const uint2*>(a.bias + a.n + col));
+      bg = *reinterpret_cast<const uint2*>(a.bias + col);
+      if (gated) bu = *reinterpret_cast<const uint2*>(a.bias + a.n + col);
     }
     if constexpr (kF8) {
-      sg = __ldg(reinterpret_cast<const float4*>(a.sw + col));
-      if (gated) su = __ldg(reinterpret_cast<const float4*>(a.sw + a.n + col));
+      sg = *reinterpret_cast<const float4*>(a.sw + col);
+      if (gated) su = *reinterpret_cast<const float4*>(a.sw + a.n + col);
     }
   }
   __syncwarp();
@@ -938,8 +938,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       if (token >= a.m) break;
       const int64_t dst = static_cast<int64_t>(token) * a.n + col;
       uint2 res = make_uint2(0, 0);
-      if (residual != nullptr) res = __ldg(reinterpret_cast<const uint2*>(residual + dst));
-      const float sx = kF8 ? __ldg(a.sx + token) : 1.0f;
+      if (residual != nullptr) res = *reinterpret_cast<const uint2*>(residual + dst);
+      const float sx = kF8 ? a.sx[token] : 1.0f;
       uint64_t z[2], u[2];
       affine(total(t, row), sx, sg, bg, z);
       if (gated) affine(total(t, row + out_rows), sx, su, bu, u);
@@ -973,7 +973,7 @@ constexpr int kVecSmemMax = 72 * 1024;
 
 __device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
@@ -1001,10 +1001,10 @@ __device__ __forceinline__ void unpack16(const uint4& v, uint64_t (&f)[kF8 ? 8 :
 
 template <bool kF8, int kM>
 __global__ void __launch_bounds__(kVecThreads, kVecCtas)
-    linear_vector_kernel(const uint8_t* __restrict__ x, const int64_t x_bytes,
-                         const uint8_t* __restrict__ w, const int k_bytes, const int kw,
-                         const int gated, const uint16_t* __restrict__ residual,
-                         uint16_t* __restrict__ y, const LinearArgs a) {
+    linear_vector_kernel(const uint8_t* x, const int64_t x_bytes,
+                         const uint8_t* w, const int k_bytes, const int kw,
+                         const int gated, const uint16_t* residual,
+                         uint16_t* y, const LinearArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
   grid_launch_dependents();
   grid_dependency_wait();
@@ -1039,7 +1039,7 @@ __global__ void __launch_bounds__(kVecThreads, kVecCtas)
   load(slice * 32);
   for (int i = threadIdx.x; i < kM * slices; i += kVecThreads) {
     const int t = i / slices;
-    xs[i] = t < a.m ? __ldg(reinterpret_cast<const uint4*>(x + t * x_bytes) + (i - t * slices))
+    xs[i] = t < a.m ? reinterpret_cast<const uint4*>(x + t * x_bytes)[i - t * slices]
                     : make_uint4(0, 0, 0, 0);
   }
   __syncthreads();
@@ -1117,17 +1117,17 @@ __global__ void __launch_bounds__(kVecThreads, kVecCtas)
     z += p[c * kM + t];
     if (gated) u += p[(c + 2) * kM + t];
   }
-  if constexpr (kF8) z = z * __ldg(a.sx + t) * __ldg(a.sw + col);
-  if (a.bias != nullptr) z += __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + col)) << 16);
+  if constexpr (kF8) z = z * a.sx[t] * a.sw[col];
+  if (a.bias != nullptr) z += __uint_as_float(static_cast<uint32_t>(a.bias[col]) << 16);
   float unused;
   f2_split(activate2_any(a.act, f2_pack(z, 0.0f)), z, unused);
   if (gated) {
-    if constexpr (kF8) u = u * __ldg(a.sx + t) * __ldg(a.sw + a.n + col);
-    if (a.bias != nullptr) u += __uint_as_float(static_cast<uint32_t>(__ldg(a.bias + a.n + col)) << 16);
+    if constexpr (kF8) u = u * a.sx[t] * a.sw[a.n + col];
+    if (a.bias != nullptr) u += __uint_as_float(static_cast<uint32_t>(a.bias[a.n + col]) << 16);
     z *= u;
   }
   const int64_t dst = static_cast<int64_t>(t) * a.n + col;
-  if (residual != nullptr) z += __uint_as_float(static_cast<uint32_t>(__ldg(residual + dst)) << 16);
+  if (residual != nullptr) z += __uint_as_float(static_cast<uint32_t>(residual[dst]) << 16);
   y[dst] = __bfloat16_as_ushort(__float2bfloat16_rn(z));
 }
 

@@ -125,7 +125,6 @@ __device__ __forceinline__ void add_f32(uint64_t (&s)[kPairs], const float* p, i
     }
   } else if constexpr (kVec == 2) {
 #pragma unroll
-#pragma unroll
     for (int i = 0; i < kPairs; ++i)
       if (at.inner(i) || at(i) < d) s[i] = f2_add(s[i], *reinterpret_cast<const uint64_t*>(p + at(i)));
   } else {

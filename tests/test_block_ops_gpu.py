@@ -932,3 +932,42 @@ def test_large_store():
         assert (got[1] == 0).all()
     del codes, scales, cache
     torch.cuda.empty_cache()
+
+
+def test_store_written_and_read_back_to_back():
+    """Each kernel may start while the one before it runs; it reads what that one stored."""
+    cache = fvq.FP8KVCache(24, 16, 4, 64)
+    table = torch.randperm(24, device="cuda").to(torch.int32).reshape(2, 12)
+    at = torch.arange(192, device="cuda").expand(2, 192)
+    slots = cache.slots(table, at)
+    lengths = torch.full((2,), 192, dtype=torch.int32, device="cuda")
+    values = [randn(384, 4, 64, seed=s) for s in range(8)]
+    got = []
+    for i in range(64):
+        cache.write(values[i % 8], values[(i + 3) % 8], slots)
+        got.append(cache.read(table, lengths, 192))
+    for i, (k, v) in enumerate(got):
+        for y, x in ((k, values[i % 8]), (v, values[(i + 3) % 8])):
+            if i < 8:
+                inside(y.reshape(384, 4, 64), x.double(), (2.0 ** -4 + 2.0 ** -7) * x.double().abs()
+                       + 2.0 ** -9 * x.double().abs().amax(-1, keepdim=True) / 448)
+            else:
+                assert torch.equal(y, got[i - 8][0 if y is k else 1])
+    assert ops.read_device_error() == 0
+
+
+@pytest.mark.parametrize("m", [1, 24])
+def test_product_operands_written_just_before(m):
+    """A weight that the kernel before wrote in place, over one that was just multiplied."""
+    x = randn(m, 256, seed=1)
+    ws = [randn(128, 256, seed=2 + i) for i in range(4)]
+    w = torch.empty_like(ws[0])
+    one = torch.ones(256, dtype=BF16, device="cuda")
+    got = []
+    for i in range(32):
+        w.copy_(ws[i % 4])
+        got.append(ops.linear_act(ops.linear_act(x, w), ws[0][:, :128].contiguous(), gated=1))
+    for i in range(4, 32):
+        assert torch.equal(got[i], got[i - 4])
+    x2 = ops.rms_norm(x, one)
+    assert torch.equal(ops.linear_act(x2, ws[1], gated=True), ops.linear_act(x2, ws[1], gated=1))
