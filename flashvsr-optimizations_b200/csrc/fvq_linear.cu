@@ -21,8 +21,8 @@
 //     CTAs until every SM streams its share of W, and each CTA sends its partial sums to the
 //     one that owns their tokens, through distributed shared memory; they are added in rank
 //     order (no atomics, no workspace, the same bits on every run).
-//   linear_vector_kernel  one or two tokens: W streamed through registers by plain 16-byte
-//     loads and fp32 FMAs, x in shared memory.  No tensor-core pipeline to set up, fill and
+//   linear_vector_kernel  one or two tokens: W streamed through rings in shared memory by bulk
+//     copies, fp32 FMAs, x in registers.  No tensor-core pipeline to set up, fill and
 //     drain, which is half of the split kernel's time at this size.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -960,24 +960,30 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 }
 
 // ---------------------------------------------------------------- one or two tokens
-// A warp takes four W rows (gated: two Wg rows and the same columns' Wu rows) and every
-// `kw`-th 512-byte slice of their K; the `kw` warps of a row group are in one CTA and join
-// their sums through shared memory in warp order.
+// W is one stream of bytes.  Its rows are taken in pairs (gated: column c's Wg and Wu rows),
+// every CTA an equal range of them; the CTA's eight warps are groups of `kw`, a group takes
+// every (8 / kw)-th pair, and a warp always the same `kw`-th of K, so that its part of x stays
+// in its registers.  A warp's parts of its pairs come through a ring of its own by bulk copies
+// and are waited for by it alone; only the sums of a block of pairs meet in shared memory (in
+// warp order), where one thread per output applies the epilogue.
 constexpr int kVecWarps = 8;
 constexpr int kVecThreads = 32 * kVecWarps;
-constexpr int kVecRows = 4;
-constexpr int kVecUnroll = 2;          // slices in flight: 8 loads of 16 bytes a lane
 constexpr int kVecTokensMax = 2;
-constexpr int kVecCtas = 2;            // per SM (three: spills, and slower from 8960 x 1536 on)
-constexpr int kVecSmemMax = 72 * 1024;
+constexpr int kVecSlotsMax = 8;
+constexpr int kVecGrid = 2;            // CTAs per SM
+constexpr int kVecPieces = 256;        // 16-byte pieces of a row that a warp takes at most
+constexpr int kVecRing = 11 * 1024;    // of a warp (two CTAs fit an SM), more where two slots need it
+constexpr int kVecHead = 1024;         // barriers
+constexpr int kVecPart = 2 * kVecThreads * kVecWarps * 4;
+constexpr int kVecSmemMax = kVecHead + kVecPart + kVecWarps * 2 * 2 * kVecPieces * 16;
 
-__device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
+struct VecPlan {
+  int k_bytes;
+  int kw_log;             // warps that share a row: 1 << kw_log
+  int per;                // 16-byte pieces of a row per warp
+  int slots, ring_bytes;  // of a warp
+  int each, more;         // pairs of rows per CTA, and one more for the first `more`
+};
 
 // 16 bytes of operand -> pairs of fp32: 4 (bf16) or 8 (E4M3)
 template <bool kF8>
@@ -999,136 +1005,177 @@ __device__ __forceinline__ void unpack16(const uint4& v, uint64_t (&f)[kF8 ? 8 :
   }
 }
 
-template <bool kF8, int kM>
-__global__ void __launch_bounds__(kVecThreads, kVecCtas)
-    linear_vector_kernel(const uint8_t* x, const int64_t x_bytes,
-                         const uint8_t* w, const int k_bytes, const int kw,
-                         const int gated, const uint16_t* residual,
-                         uint16_t* y, const LinearArgs a) {
+template <bool kF8, int kM, int kS>
+__global__ void __launch_bounds__(kVecThreads, 2)
+    linear_vector_kernel(const uint8_t* x, const int64_t x_bytes, const uint8_t* w, const VecPlan p,
+                         const int gated, const uint16_t* residual, uint16_t* y, const LinearArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr int kPairs = kF8 ? 8 : 4;
+  constexpr int kValues = 2 * kM;                  // sums of a pair of rows
+  constexpr int kBlock = kVecThreads / kValues;    // pairs per block
+  auto* lost = reinterpret_cast<volatile int*>(smem + kVecWarps * kVecSlotsMax * 8);
+  auto* part = reinterpret_cast<float*>(smem + kVecHead);  // [2][kBlock][kw][kValues]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kw = 1 << p.kw_log, groups = kVecWarps >> p.kw_log;
+  const int group = warp >> p.kw_log, slice = warp & (kw - 1);
+  auto* bar = reinterpret_cast<uint64_t*>(smem) + warp * kVecSlotsMax;
+  uint8_t* ring = smem + kVecHead + kVecPart + warp * p.ring_bytes;
+  const int unit0 = static_cast<int>(blockIdx.x) * p.each + min(static_cast<int>(blockIdx.x), p.more);
+  const int total = p.each + (static_cast<int>(blockIdx.x) < p.more ? 1 : 0);  // pairs of the CTA
+  const int piece0 = slice * p.per, len = min(p.per, p.k_bytes / 16 - piece0);  // of this warp, len > 0
+  const int mine = total > group ? ((total - 1 - group) >> (3 - p.kw_log)) + 1 : 0;  // pairs of this warp
+  const uint32_t row_bytes = static_cast<uint32_t>(len) * 16u, slot_bytes = static_cast<uint32_t>(p.per) * 32u;
+  static_assert(kVecWarps == 8, "3 is its logarithm");
+
+  if (lane == 0) {
+    for (int i = 0; i < p.slots; ++i) mbar_init(&bar[i], 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (threadIdx.x == 0) *lost = 0;
   grid_launch_dependents();
   grid_dependency_wait();
-  constexpr int kPairs = kF8 ? 8 : 4;
-  constexpr int kValues = kVecRows * kM;
-  uint4* xs = reinterpret_cast<uint4*>(smem);                     // [kM][k_bytes / 16]
-  float* part = reinterpret_cast<float*>(smem + kM * k_bytes);    // [warps][kValues]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int slice = warp % kw;
-  const int slices = k_bytes / 16;                                // 16-byte pieces of a row
-  const int group = static_cast<int>(blockIdx.x) * (kVecWarps / kw) + warp / kw;
-  const int out_cols = gated ? kVecRows / 2 : kVecRows;
-  const int col0 = group * out_cols;
-  const uint4* rows[kVecRows];
-#pragma unroll
-  for (int r = 0; r < kVecRows; ++r) {
-    // a group past the last column reads the last rows and stores nothing
-    const int c = min(col0 + (gated ? r & 1 : r), a.n - 1);
-    rows[r] = reinterpret_cast<const uint4*>(w + (static_cast<int64_t>(c) + (gated && r >= 2 ? a.n : 0)) * k_bytes);
-  }
-  uint4 wv[kVecUnroll][kVecRows];
-  const auto load = [&](int base) {
-#pragma unroll
-    for (int u = 0; u < kVecUnroll; ++u) {
-      const int at = base + u * kw * 32 + lane;
-#pragma unroll
-      for (int r = 0; r < kVecRows; ++r)
-        wv[u][r] = at < slices ? ld_stream_v4(rows[r] + at) : make_uint4(0, 0, 0, 0);
-    }
+  const auto fetch = [&](int i, int slot) {  // lane 0: the warp's i-th pair
+    if (i >= mine) return;
+    const int64_t unit = unit0 + group + i * groups;
+    const uint8_t* from = w + (gated ? unit : 2 * unit) * p.k_bytes + piece0 * 16;
+    uint8_t* to = ring + slot * slot_bytes;
+    mbar_arrive_expect_tx(&bar[slot], 2 * row_bytes);
+    bulk_load(to, from, row_bytes, &bar[slot]);
+    bulk_load(to + p.per * 16, from + (gated ? static_cast<int64_t>(a.n) : int64_t(1)) * p.k_bytes, row_bytes,
+              &bar[slot]);
   };
-  const int step = kVecUnroll * kw * 32;
-  load(slice * 32);
-  for (int i = threadIdx.x; i < kM * slices; i += kVecThreads) {
-    const int t = i / slices;
-    xs[i] = t < a.m ? reinterpret_cast<const uint4*>(x + t * x_bytes)[i - t * slices]
-                    : make_uint4(0, 0, 0, 0);
-  }
-  __syncthreads();
-  uint64_t acc[kVecRows][kM];
+  if (lane == 0)
+    for (int i = 0; i < p.slots; ++i) fetch(i, i);
+  uint4 xr[kM][kS];
 #pragma unroll
-  for (int r = 0; r < kVecRows; ++r)
+  for (int t = 0; t < kM; ++t)
 #pragma unroll
-    for (int t = 0; t < kM; ++t) acc[r][t] = 0;
-  for (int base = slice * 32; base < slices; base += step) {
-    uint4 now[kVecUnroll][kVecRows];
-#pragma unroll
-    for (int u = 0; u < kVecUnroll; ++u)
-#pragma unroll
-      for (int r = 0; r < kVecRows; ++r) now[u][r] = wv[u][r];
-    if (base + step < slices) load(base + step);
-#pragma unroll
-    for (int u = 0; u < kVecUnroll; ++u) {
-      const int at = base + u * kw * 32 + lane;
-      if (at >= slices) continue;
-      uint64_t xf[kM][kPairs];
-#pragma unroll
-      for (int t = 0; t < kM; ++t) unpack16<kF8>(xs[t * slices + at], xf[t]);
-#pragma unroll
-      for (int r = 0; r < kVecRows; ++r) {
-        uint64_t wf[kPairs];
-        unpack16<kF8>(now[u][r], wf);
-#pragma unroll
-        for (int t = 0; t < kM; ++t)
-#pragma unroll
-          for (int i = 0; i < kPairs; ++i) acc[r][t] = f2_fma(wf[i], xf[t][i], acc[r][t]);
-      }
+    for (int i = 0; i < kS; ++i) {
+      const int at = lane + 32 * i;
+      xr[t][i] = make_uint4(0, 0, 0, 0);
+      if (at < len && t < a.m) xr[t][i] = reinterpret_cast<const uint4*>(x + t * x_bytes)[piece0 + at];
     }
-  }
-  // Sums over the warp: while a lane holds several values, each step exchanges half of them
-  // (the upper lanes keep the upper half), so that the last lanes hold one value each.
-  float v[kValues];
-#pragma unroll
-  for (int r = 0; r < kVecRows; ++r)
-#pragma unroll
-    for (int t = 0; t < kM; ++t) {
-      float lo, hi;
-      f2_split(acc[r][t], lo, hi);
-      v[r * kM + t] = lo + hi;
-    }
-  int index = 0;
-#pragma unroll
-  for (int o = 16, have = kValues; o > 0; o >>= 1) {
-    if (have > 1) {
-      have /= 2;
-      const bool upper = (lane & o) != 0;
-#pragma unroll
-      for (int i = 0; i < kValues / 2; ++i) {
-        if (i >= have) break;
-        const float give = upper ? v[i] : v[i + have];
-        const float keep = upper ? v[i + have] : v[i];
-        v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
-      }
-      if (upper) index += have;
-    } else {
-      v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], o);
-    }
-  }
-  if ((lane & (32 / kValues - 1)) == 0) part[warp * kValues + index] = v[0];
-  __syncthreads();
-  // one thread per output of the CTA
-  const int outs = out_cols * kM;
+  __syncthreads();  // the barriers and the flag are initialised
+
+  const int outs = gated ? 1 : 2;  // outputs of a pair, for each token
   const int id = static_cast<int>(threadIdx.x);
-  if (id >= kVecWarps / kw * outs) return;
-  const int g = id / outs, j = id - g * outs, c = j / kM, t = j - c * kM;
-  const int col = (static_cast<int>(blockIdx.x) * (kVecWarps / kw) + g) * out_cols + c;
-  if (col >= a.n || t >= a.m) return;
-  float z = 0.0f, u = 0.0f;
-  for (int q = 0; q < kw; ++q) {
-    const float* p = part + (g * kw + q) * kValues;
-    z += p[c * kM + t];
-    if (gated) u += p[(c + 2) * kM + t];
+  const int out_pair = gated ? id / kM : id / kValues, out_row = gated ? 0 : id / kM % 2, out_t = id % kM;
+  int slot = 0;
+  uint32_t phases = 0;  // bit s: parity of slot s
+  int i = 0;            // pairs of this warp so far
+  for (int base = 0, buf = 0; base < total; base += kBlock, buf ^= 1) {
+    // this thread's output of the block; what its epilogue reads is under way meanwhile
+    const int unit = base + out_pair;
+    const int col = (unit0 + unit) * outs + out_row;
+    const bool output = out_pair < kBlock && unit < total && out_t < a.m;
+    const int64_t dst = static_cast<int64_t>(out_t) * a.n + col;
+    float sx = 1.0f, sg = 1.0f, su = 1.0f, bg = 0.0f, bu = 0.0f, res = 0.0f;
+    if (output) {
+      const auto bf16 = [](const uint16_t* at) { return __uint_as_float(static_cast<uint32_t>(*at) << 16); };
+      if constexpr (kF8) {
+        sx = a.sx[out_t];
+        sg = a.sw[col];
+        if (gated) su = a.sw[a.n + col];
+      }
+      if (a.bias != nullptr) {
+        bg = bf16(a.bias + col);
+        if (gated) bu = bf16(a.bias + a.n + col);
+      }
+      if (residual != nullptr) res = bf16(residual + dst);
+    }
+    float* sums = part + buf * (kBlock * kVecWarps * kValues);
+    for (int u = group; u < kBlock && base + u < total; u += groups, ++i) {
+      // As in the streaming norm: a wait that runs out is reported and waited for once more, so
+      // that no copy is in flight when the CTA exits.
+      const uint32_t parity = (phases >> slot) & 1u;
+      if (*lost == 0 && !mbar_wait_bounded(&bar[slot], parity, a.wait_limit)) {
+        atomicOr(a.err_word, kErrWaitProducer);
+        if (!mbar_wait_bounded(&bar[slot], parity,
+                               a.wait_limit > kDefaultWaitLimit ? a.wait_limit : kDefaultWaitLimit))
+          *lost = 1;  // later pairs are not waited for; the output is undefined
+      }
+      phases ^= 1u << slot;
+      const uint4* rows = reinterpret_cast<const uint4*>(ring + slot * slot_bytes);
+      uint64_t acc[2][kM];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int t = 0; t < kM; ++t) acc[r][t] = 0;
+#pragma unroll
+      for (int j = 0; j < kS; ++j) {
+        const int at = lane + 32 * j;
+        if (at >= len) continue;
+        if constexpr (kM * kS * kPairs > 24) {  // unpacked anew for every pair, or it spills
+#pragma unroll
+          for (int t = 0; t < kM; ++t)
+            asm volatile("" : "+r"(xr[t][j].x), "+r"(xr[t][j].y), "+r"(xr[t][j].z), "+r"(xr[t][j].w));
+        }
+        uint64_t xf[kM][kPairs];
+#pragma unroll
+        for (int t = 0; t < kM; ++t) unpack16<kF8>(xr[t][j], xf[t]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          uint64_t wf[kPairs];
+          unpack16<kF8>(rows[r * p.per + at], wf);
+#pragma unroll
+          for (int t = 0; t < kM; ++t)
+#pragma unroll
+            for (int e = 0; e < kPairs; ++e) acc[r][t] = f2_fma(wf[e], xf[t][e], acc[r][t]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) fetch(i + p.slots, slot);
+      if (++slot == p.slots) slot = 0;
+      // Sums over the warp: while a lane holds several values, each step exchanges half of them
+      // (the upper lanes keep the upper half), so that the last lanes hold one value each.
+      float v[kValues];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int t = 0; t < kM; ++t) {
+          float lo, hi;
+          f2_split(acc[r][t], lo, hi);
+          v[r * kM + t] = lo + hi;
+        }
+      int index = 0;
+#pragma unroll
+      for (int o = 16, have = kValues; o > 0; o >>= 1) {
+        if (have > 1) {
+          have /= 2;
+          const bool upper = (lane & o) != 0;
+#pragma unroll
+          for (int e = 0; e < kValues / 2; ++e) {
+            if (e >= have) break;
+            const float give = upper ? v[e] : v[e + have];
+            const float keep = upper ? v[e + have] : v[e];
+            v[e] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
+          }
+          if (upper) index += have;
+        } else {
+          v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], o);
+        }
+      }
+      if ((lane & (32 / kValues - 1)) == 0) sums[((u << p.kw_log) + slice) * kValues + index] = v[0];
+    }
+    __syncthreads();  // (the other half of `part` was read before the block's last barrier)
+    if (output) {
+      float z = 0.0f, u = 0.0f;
+      const float* at = sums + (out_pair << p.kw_log) * kValues + out_row * kM + out_t;
+      for (int q = 0; q < kw; ++q) z += at[q * kValues];
+      if (gated)
+        for (int q = 0; q < kw; ++q) u += at[q * kValues + kM];
+      if constexpr (kF8) z = z * sx * sg;
+      z += bg;
+      float unused;
+      f2_split(activate2_any(a.act, f2_pack(z, 0.0f)), z, unused);
+      if (gated) {
+        if constexpr (kF8) u = u * sx * su;
+        z *= u + bu;
+      }
+      y[dst] = __bfloat16_as_ushort(__float2bfloat16_rn(z + res));
+    }
   }
-  if constexpr (kF8) z = z * a.sx[t] * a.sw[col];
-  if (a.bias != nullptr) z += __uint_as_float(static_cast<uint32_t>(a.bias[col]) << 16);
-  float unused;
-  f2_split(activate2_any(a.act, f2_pack(z, 0.0f)), z, unused);
-  if (gated) {
-    if constexpr (kF8) u = u * a.sx[t] * a.sw[a.n + col];
-    if (a.bias != nullptr) u += __uint_as_float(static_cast<uint32_t>(a.bias[a.n + col]) << 16);
-    z *= u;
-  }
-  const int64_t dst = static_cast<int64_t>(t) * a.n + col;
-  if (residual != nullptr) z += __uint_as_float(static_cast<uint32_t>(residual[dst]) << 16);
-  y[dst] = __bfloat16_as_ushort(__float2bfloat16_rn(z));
 }
 
 // ---------------------------------------------------------------- host side
@@ -1205,30 +1252,68 @@ cudaError_t launch_split(const LinearProblem& l, const LinearArgs& a, const Spli
                           p.split, mx, mw, p, l.gated ? 1 : 0, l.residual, l.y, a);
 }
 
-template <bool kF8, int kM>
-cudaError_t launch_vector(const LinearProblem& l, const LinearArgs& a, cudaStream_t st) {
-  const int elem = kF8 ? 1 : 2;
-  const int k_bytes = static_cast<int>(l.k * elem);
-  const int64_t out_cols = l.gated ? kVecRows / 2 : kVecRows;
-  const int64_t groups = (l.n + out_cols - 1) / out_cols;
-  // warps per row group: enough for sixteen warps an SM, while a warp keeps a slice of K
-  int kw = 1;
-  while (kw < kVecWarps && groups * kw < 16 * sm_count() && kw * 512 < k_bytes) kw *= 2;
-  const int bytes = kM * k_bytes + kVecWarps * kVecRows * kM * 4;
+// The vector kernel's plan; false where a row does not fit the warps that may share it.
+bool plan_vector(const LinearProblem& l, VecPlan* p, int* grid) {
+  const int64_t k_bytes = l.k * (l.fp8 ? 1 : 2), pieces = k_bytes / 16;
+  if (pieces > kVecWarps * kVecPieces) return false;
+  const int64_t units = l.gated ? l.n : l.n / 2;
+  *grid = static_cast<int>(units < kVecGrid * sm_count() ? units : kVecGrid * sm_count());
+  p->each = static_cast<int>(units / *grid);
+  p->more = static_cast<int>(units % *grid);
+  // Warps that share a row: a warp spends about 450 cycles on a pair beside its share of the
+  // bytes (the wait, the refill, the sum over the lanes), so many pairs want whole rows and few
+  // pairs all eight warps; two slots should fit the ring.
+  const int per_slice = (l.fp8 ? 100 : 50) * (l.m == 1 ? 2 : 3) / 2;
+  int64_t best = INT64_MAX;
+  for (int log = 3; log >= 0; --log) {
+    const int64_t per = (pieces + (1 << log) - 1) >> log;
+    if (log < 3 && per > kVecRing / 64) break;
+    if (log > 0 && (pieces >> log) < 32) continue;  // every warp has a share
+    const int64_t turns = (p->each + (p->more > 0 ? 1 : 0) + (kVecWarps >> log) - 1) / (kVecWarps >> log);
+    const int64_t cost = turns * (450 + per_slice * ((per + 31) / 32));
+    if (cost < best) {
+      best = cost;
+      p->kw_log = log;
+    }
+  }
+  p->k_bytes = static_cast<int>(k_bytes);
+  p->per = static_cast<int>((pieces + (1 << p->kw_log) - 1) >> p->kw_log);
+  const int slot_bytes = p->per * 32;
+  p->slots = kVecRing / slot_bytes;
+  if (p->slots < 2) p->slots = 2;
+  if (p->slots > kVecSlotsMax) p->slots = kVecSlotsMax;
+  p->ring_bytes = p->slots * slot_bytes;
+  return true;
+}
+
+template <bool kF8, int kM, int kS>
+cudaError_t launch_vector(const LinearProblem& l, const LinearArgs& a, const VecPlan& p, int grid, cudaStream_t st) {
   static ContextCache attr_done;
-  auto* kernel = linear_vector_kernel<kF8, kM>;
-  if (cudaError_t e = ensure_max_dynamic_smem(attr_done, reinterpret_cast<const void*>(kernel),
-                                              kVecSmemMax + kVecWarps * kVecRows * kM * 4))
+  auto* kernel = linear_vector_kernel<kF8, kM, kS>;
+  if (cudaError_t e = ensure_max_dynamic_smem(attr_done, reinterpret_cast<const void*>(kernel), kVecSmemMax))
     return e;
-  const int64_t ctas = (groups + kVecWarps / kw - 1) / (kVecWarps / kw);
-  return launch_dependent(kernel, static_cast<unsigned>(ctas), kVecThreads, bytes, st, 0,
-                          static_cast<const uint8_t*>(l.x), l.x_stride * elem,
-                          static_cast<const uint8_t*>(l.w), k_bytes, kw, l.gated ? 1 : 0, l.residual, l.y, a);
+  return launch_dependent(kernel, static_cast<unsigned>(grid), kVecThreads,
+                          kVecHead + kVecPart + kVecWarps * p.ring_bytes, st, 0, static_cast<const uint8_t*>(l.x),
+                          l.x_stride * (kF8 ? 1 : 2), static_cast<const uint8_t*>(l.w), p, l.gated ? 1 : 0,
+                          l.residual, l.y, a);
+}
+
+template <bool kF8, int kM>
+cudaError_t launch_vector_by_width(const LinearProblem& l, const LinearArgs& a, const VecPlan& p, int grid,
+                                   cudaStream_t st) {
+  if (p.per <= 64) return launch_vector<kF8, kM, 2>(l, a, p, grid, st);
+  if (p.per <= 96) return launch_vector<kF8, kM, 3>(l, a, p, grid, st);
+  if (p.per <= 128) return launch_vector<kF8, kM, 4>(l, a, p, grid, st);
+  if (p.per <= 160) return launch_vector<kF8, kM, 5>(l, a, p, grid, st);
+  if (p.per <= 192) return launch_vector<kF8, kM, 6>(l, a, p, grid, st);
+  return launch_vector<kF8, kM, kVecPieces / 32>(l, a, p, grid, st);
 }
 
 template <bool kF8>
-cudaError_t launch_vector_by_tokens(const LinearProblem& l, const LinearArgs& a, cudaStream_t st) {
-  return l.m == 1 ? launch_vector<kF8, 1>(l, a, st) : launch_vector<kF8, 2>(l, a, st);
+cudaError_t launch_vector_by_tokens(const LinearProblem& l, const LinearArgs& a, const VecPlan& p, int grid,
+                                    cudaStream_t st) {
+  return l.m == 1 ? launch_vector_by_width<kF8, 1>(l, a, p, grid, st)
+                  : launch_vector_by_width<kF8, 2>(l, a, p, grid, st);
 }
 
 // How many clusters of `split` of the split kernel's CTAs run at a time: a cluster stays inside
@@ -1384,9 +1469,10 @@ cudaError_t launch_linear(const LinearProblem& l, uint64_t wait_limit, cudaStrea
   a.err_word = error_word_ptr();
   if (a.err_word == nullptr) return cudaErrorInvalidSymbol;
   const int mode = linear_kernel_mode();
-  const int64_t x_smem = l.m * l.k * (l.fp8 ? 1 : 2);
-  if (mode == 0 && l.m <= kVecTokensMax && x_smem <= kVecSmemMax)
-    return l.fp8 ? launch_vector_by_tokens<true>(l, a, st) : launch_vector_by_tokens<false>(l, a, st);
+  VecPlan v;
+  int grid;
+  if (mode == 0 && l.m <= kVecTokensMax && plan_vector(l, &v, &grid))
+    return l.fp8 ? launch_vector_by_tokens<true>(l, a, v, grid, st) : launch_vector_by_tokens<false>(l, a, v, grid, st);
   double split_cost, pair_cost;
   const SplitPlan p = l.fp8 ? plan_split<true>(l, a.k_tiles, &split_cost)
                             : plan_split<false>(l, a.k_tiles, &split_cost);

@@ -313,7 +313,7 @@ def test_product_by_size(fp8, m, n, k, gated):
 @pytest.mark.parametrize("m", [1, 2, 3, 4, 5])
 @pytest.mark.parametrize("n,k", [(8, 16), (16, 528), (72, 1536), (1000, 8960), (8960, 1536), (264, 12288), (40, 20480)])
 def test_product_few_rows(fp8, m, n, k):
-    """One or two rows (the form that reads W through registers), and the next counts."""
+    """One or two rows (the form that streams W past x), and the next counts."""
     check_product(m, n, k, fp8)
     check_product(m, n, k, fp8, act="gelu_tanh", gated=True, residual=False)
     check_product(m, n, k, fp8, bias=False, act="silu", gated=True)
@@ -971,3 +971,37 @@ def test_product_operands_written_just_before(m):
         assert torch.equal(got[i], got[i - 4])
     x2 = ops.rms_norm(x, one)
     assert torch.equal(ops.linear_act(x2, ws[1], gated=True), ops.linear_act(x2, ws[1], gated=1))
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("n,k", [(8, 16384), (16, 16400), (80008, 16), (77000, 144), (1184, 1536), (2376, 8960),
+                                 (9000, 512), (600, 4096), (5000, 400), (304, 2816), (40, 33024)])
+def test_product_few_rows_shares_of_a_row(m, n, k, fp8):
+    """One to eight warps a row, rings of few and many slots, several blocks a CTA, rows too long."""
+    check_product(m, n, k, fp8, act="silu")
+    check_product(m, n, k, fp8, act="silu", gated=True, residual=False)
+
+
+def test_product_few_rows_nan_and_infinity_stay_in_their_row():
+    x, w = randn(2, 528, seed=1), randn(1400, 528, seed=2)
+    clean = ops.linear_act(x, w)
+    w[33], w[34, 7], w[700] = float("nan"), float("inf"), float("nan")
+    y = ops.linear_act(x, w)
+    hit = torch.zeros(2, 1400, dtype=torch.bool, device="cuda")
+    hit[:, 33], hit[:, 34], hit[:, 700] = True, True, True
+    assert torch.equal(~torch.isfinite(y), hit) and torch.equal(y[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("m,n,k,gated", [(1, 264, 1536, False), (2, 3000, 8960, True), (1, 80000, 64, False)])
+def test_product_few_rows_wait_limit(m, n, k, gated):
+    """A wait that runs out is reported; a copy that landed before its only test gives the result."""
+    x, w = randn(m, k, seed=1), randn(2 * n if gated else n, k, seed=2, std=k ** -0.5)
+    want = ops.linear_act(x, w, act="silu", gated=gated)
+    ops.set_wait_limit(1)
+    try:
+        y = ops.linear_act(x, w, act="silu", gated=gated)
+        assert ops.read_device_error() != 0 or torch.equal(y, want)
+    finally:
+        ops.set_wait_limit(0)
+    assert torch.equal(ops.linear_act(x, w, act="silu", gated=gated), want)
