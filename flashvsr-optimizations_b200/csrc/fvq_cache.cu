@@ -7,11 +7,16 @@
 // Both are HBM-bound copies with a conversion, keys and values in one launch.  Writing gives
 // a row of d <= 512 values to a power-of-two group of lanes (16 values a lane, 8 where
 // alignment allows no more), so that its maximum needs only shuffles; reading gives 16 (or 8)
-// codes to a thread, four vectors in flight each.  Row and position arithmetic is 32-bit with multiplications in
-// place of divisions: with 64-bit divisions both were bound by issue slots (reading 4 x 7680
-// tokens of 12 heads of 128 took 78 us).  Slot and page numbers come from the device and are
-// checked there: a negative slot is padding and stores nothing, a slot or page past the store
-// touches nothing (the rows read are zero) and sets a bit of the device error word.
+// codes to a thread, four vectors in flight each.  Row and position arithmetic is 32-bit with
+// multiplications in place of divisions: with 64-bit divisions both were bound by issue slots
+// (reading 4 x 7680 tokens of 12 heads of 128 took 78 us).  Slot and page numbers come from the
+// device and are checked there: a negative slot is padding and stores nothing, a slot or page
+// past the store touches nothing (the rows read are zero) and sets a bit of the device error
+// word.
+//
+// Measured on a B200, back to back in a CUDA graph (a copy moves 6.5 TB/s), heads of 128, 12 a
+// token: writing 64 tokens 1.4 us, 7680 tokens 12.5 us (71 MB, 5.7 TB/s, 1.5 us of it start and
+// end); reading 4 x 7680 tokens 40.6 us (247 MB, 6.1 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

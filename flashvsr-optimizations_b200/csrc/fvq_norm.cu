@@ -24,6 +24,13 @@
 //     the row's buffer, by bulk copies (kVec = 2).
 // In the first two forms, and with other strides, such rows take element-wise accesses
 // (kVec = 1): neighbouring lanes read neighbouring elements, so the sectors fetched are the same.
+//
+// Measured on a B200, launches back to back in a CUDA graph over operands larger than L2 (a copy
+// moves 6.5 TB/s): one row of 1536 in E4M3 1.9 us; 15360 x 1536 with a bf16 residual to E4M3
+// 27 us (6.1 TB/s); 92160 rows of 128 8.9 us (5.3 TB/s, 1.7 us of it start and end); 4099 x 2048
+// with an fp32 residual 17.7 us (5.7 TB/s), 4099 x 2047 21.3 us (bounds, shifts and copies of
+// the ragged ends are instructions that the aligned form does not have).  More warps a row than
+// the rings need cost time (15360 x 1536 to bf16: one warp 14.9 us, two 18.8, four 25.0).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -367,10 +374,11 @@ __global__ void __launch_bounds__(kLanes == 0 ? kNormMaxThreads : kNormThreads)
 }
 
 // ---------------------------------------------------------------- many long rows
-// (No grid_launch_dependents here: with the next kernel let in early, 15360 rows of 1536 took
-// 29.5 us instead of 28.2.)  One CTA of 16 warps per SM.  A group of `kGroup` warps walks rows group by group over the
+// One CTA of 16 warps per SM.  A group of `kGroup` warps walks rows group by group over the
 // grid; each group owns a ring of `slots` row buffers (x's row, then the residual's), one
-// mbarrier each.  A slot is refilled as soon as the group holds its row in registers.
+// mbarrier each.  A slot is refilled as soon as the group holds its row in registers.  (No
+// grid_launch_dependents here: with the next kernel let in early, 15360 rows of 1536 took
+// 29.5 us instead of 28.2.)
 constexpr int kStreamWarps = 16;
 constexpr int kStreamThreads = 32 * kStreamWarps;
 constexpr int kStreamSmem = 216 * 1024;

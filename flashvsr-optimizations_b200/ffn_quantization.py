@@ -346,8 +346,8 @@ class FP8GatedFFN(torch.nn.Module):
     Built from three ``nn.Linear``; gate and up are quantized row by row and kept stacked
     (buffers ``qweight`` [2 f, d], ``scale``, ``bias``), so that one product computes both and
     joins them in its epilogue; ``down`` is quantized alike (``down_qweight``, ...).  act: one of
-    ``ops.ACTIVATIONS``.  d and f multiples of 16.  Inputs are bf16 [..., d]; four launches
-    (quantize x, or ``prenorm``'s norm which quantizes its own output; gated product; quantize h;
+    ``ops.ACTIVATIONS``.  d and f multiples of 16, up to 16384 (the row quantizer's).  Inputs are
+    bf16 [..., d]; four launches (quantize x, or ``prenorm``'s norm which quantizes its own output; gated product; quantize h;
     down product).
     """
 

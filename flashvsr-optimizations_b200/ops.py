@@ -870,7 +870,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 
     fp32 accumulation and epilogue, one rounding.  x: bf16 [..., k] (rows may be strided), weight
     in nn.Linear's layout, k and n multiples of 8; act: one of ``ACTIVATIONS`` ("gelu" is the erf
-    form).  From one row to many: few rows run on a kernel bound by reading the weight once."""
+    form).  From one row to many: one or two rows, and few, run on kernels bound by reading the
+    weight once."""
     fast = _fast()
     y = fast.linear_act(x, weight, bias, ACTIVATIONS.get(act), gated, residual) if fast else None
     return _linear_act(x, weight, bias, act, gated, residual) if y is None else y
@@ -928,8 +929,8 @@ def _fp8_cache_write_impl(k, v, slots, k_codes, k_scale, v_codes, v_scale):
         v, v_token, v_head = _cache_rows(v)
         slots = slots.contiguous()
         _launch("fvq_fp8_cache_write", k.device, k.data_ptr(), v.data_ptr(), k.shape[0], heads, d,
-                k_token, k_head, v_token, v_head, slots.data_ptr(), k_codes.data_ptr(), k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(),
-                pages * page)
+                k_token, k_head, v_token, v_head, slots.data_ptr(), k_codes.data_ptr(),
+                k_scale.data_ptr(), v_codes.data_ptr(), v_scale.data_ptr(), pages * page)
 
 
 def _fp8_cache_read_impl(k_codes, k_scale, v_codes, v_scale, page_table, lengths, max_len):
@@ -1028,7 +1029,7 @@ def read_device_error(device: torch.device | None = None) -> int:
 
 def set_linear_kernel(mode: int) -> None:
     """Which kernel ``linear_act`` and ``fp8_scaled_mm_act`` run: 0 by size (default), 1 the split
-    kernel (few rows), 2 the SM-pair kernel."""
+    kernel (few rows), 2 the SM-pair kernel, whatever the number of rows."""
     _lib.call("fvq_set_linear_kernel", mode)
 
 

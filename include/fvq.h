@@ -405,8 +405,9 @@ int fvq_rms_norm(const uint16_t* x, int64_t rows, int64_t inner, int64_t outer_s
  * elements apart (a multiple of 8, at least k); w: bf16 [n, k], gated [2n, k]; bias: bf16 of
  * as many values as w has rows, or NULL; residual: bf16 [m, n] or NULL; y: bf16 [m, n].
  * n % 8 == 0, k % 8 == 0; every pointer 16-byte aligned.  From one row up; no workspace.
- * Few rows run on a kernel that splits k over clusters (fvq_set_linear_kernel); either
- * kernel gives the same bits on every run, the two differ in the order of the sum over k.
+ * The kernel goes by size (fvq_set_linear_kernel): one or two rows stream W past x, few rows
+ * split k over clusters, many run on SM pairs.  Each gives the same bits on every run; they
+ * differ in the order of the sum over k.
  */
 int fvq_linear_act(const uint16_t* x, int64_t m, int64_t k, int64_t x_stride, const uint16_t* w,
                    int64_t n, const uint16_t* bias, int act, int gated, const uint16_t* residual,
@@ -425,7 +426,7 @@ int fvq_fp8_scaled_mm_act(const uint8_t* a, const float* scale_a, int64_t m, int
 
 /*
  * Library setting: which kernel fvq_linear_act and fvq_fp8_scaled_mm_act run: 0 (the default)
- * by size, 1 the split kernel (few rows), 2 the SM-pair kernel.  Applies to later launches
+ * by size, 1 the split kernel (few rows), 2 the SM-pair kernel, whatever the number of rows.  Applies to later launches
  * from any thread.
  */
 int fvq_set_linear_kernel(int mode);
