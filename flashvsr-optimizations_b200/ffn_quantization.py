@@ -347,8 +347,8 @@ class FP8GatedFFN(torch.nn.Module):
     (buffers ``qweight`` [2 f, d], ``scale``, ``bias``), so that one product computes both and
     joins them in its epilogue; ``down`` is quantized alike (``down_qweight``, ...).  act: one of
     ``ops.ACTIVATIONS``.  d and f multiples of 16, up to 16384 (the row quantizer's).  Inputs are
-    bf16 [..., d]; four launches (quantize x, or ``prenorm``'s norm which quantizes its own output; gated product; quantize h;
-    down product).
+    bf16 [..., d]; four launches (quantize x, or ``prenorm``'s norm which quantizes its own output;
+    gated product; quantize h; down product).
     """
 
     def __init__(self, gate: torch.nn.Linear, up: torch.nn.Linear, down: torch.nn.Linear, act: str = "silu"):
