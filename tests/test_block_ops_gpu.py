@@ -712,6 +712,41 @@ def test_block_run_in_a_graph_and_on_streams():
     assert torch.equal(outs[0], want[3])                   # the slots differ, the attention does not see them
 
 
+@pytest.mark.parametrize("m", [1, 24, 300])
+def test_captured_between_copies_fills_and_a_second_stream(m):
+    """Copies, fills, torch's kernels and events around the operators, captured and eager alike."""
+    ws = [randn(256, 256, seed=s, std=1 / 16) for s in range(2)]
+    x, w, one = randn(m, 256, seed=5), torch.empty_like(ws[0]), randn(256, seed=6)
+    acc, side = torch.empty(m, 256, dtype=BF16, device="cuda"), torch.cuda.Stream()
+
+    def chain():
+        out = []
+        for i in range(4):
+            w.copy_(ws[i % 2])                      # a copy node
+            acc.zero_()                             # a fill node
+            y = ops.linear_act(x, w, act="silu", residual=acc)
+            y.add_(1)                               # a kernel of torch's
+            u = ops.rms_norm(y, one)
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                v = ops.linear_act(u, w, act="relu")
+            z = ops.linear_act(u, w, act="gelu")
+            torch.cuda.current_stream().wait_stream(side)
+            out.append(ops.add_rms_norm(z, v, one)[1])
+        return out
+
+    want = [t.clone() for t in chain()]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = chain()
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 # ---------------------------------------------------------------- modules
 def linear(out_f, in_f, seed, bias=True):
     lin = torch.nn.Linear(in_f, out_f, bias=bias, device="cuda", dtype=BF16)
