@@ -33,8 +33,8 @@
 //           power with it (7680 x 1536 -> 2 * 4480: 75 us without an activation, 84 with one).
 //   split   E4M3 24 x 8960 -> 1536: 8.4 us (13.8 MB of W: 2.1 us at a copy's rate; the rest is the
 //           start, the exchange of partial sums and the epilogue).  bf16 24 x 1536 -> 8960 alike.
-//   vector  bf16 1 x 1536 -> 8960: 7.5 us, 1 x 8960 -> 1536: 7.3 us (27.5 MB, 3.7 TB/s, about
-//           2.5 us of it start and end), 1 x 4096 -> 12288: 17.6 us (5.7 TB/s).
+//   vector  bf16 1 x 1536 -> 8960: 7.2 us, 1 x 8960 -> 1536: 6.8 us (27.5 MB, 4.0 TB/s, about
+//           2.5 us of it start and end), 1 x 4096 -> 12288: 17.1 us (5.9 TB/s).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -996,6 +996,11 @@ struct VecPlan {
   int each, more;         // pairs of rows per CTA, and one more for the first `more`
 };
 
+// 16-byte aligned, bytes a multiple of 16
+__device__ __forceinline__ void l2_prefetch(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
 // 16 bytes of operand -> pairs of fp32: 4 (bf16) or 8 (E4M3)
 template <bool kF8>
 __device__ __forceinline__ void unpack16(const uint4& v, uint64_t (&f)[kF8 ? 8 : 4]) {
@@ -1045,16 +1050,23 @@ __global__ void __launch_bounds__(kVecThreads, 2)
   }
   if (threadIdx.x == 0) *lost = 0;
   grid_launch_dependents();
+  const auto row_of = [&](int i, int r) {  // the warp's part of its i-th pair's row r
+    const int64_t unit = unit0 + group + i * groups;
+    const int64_t row = gated ? unit + (r == 0 ? 0 : a.n) : 2 * unit + r;
+    return w + row * p.k_bytes + piece0 * 16;
+  };
+  // While the kernel before still runs: the first slots' bytes towards L2.  Nothing is read, so
+  // W may be what that kernel writes.  (One row of 1536 x 8960 E4M3 behind its like: 6.5 -> 6.0
+  // us.  The split kernel, whose CTAs take a whole SM, lost by it: 24 rows 10.3 -> 11.3.)
+  if (lane < 2 * p.slots && (lane >> 1) < mine) l2_prefetch(row_of(lane >> 1, lane & 1), row_bytes);
+  __syncwarp();
   grid_dependency_wait();
   const auto fetch = [&](int i, int slot) {  // lane 0: the warp's i-th pair
     if (i >= mine) return;
-    const int64_t unit = unit0 + group + i * groups;
-    const uint8_t* from = w + (gated ? unit : 2 * unit) * p.k_bytes + piece0 * 16;
     uint8_t* to = ring + slot * slot_bytes;
     mbar_arrive_expect_tx(&bar[slot], 2 * row_bytes);
-    bulk_load(to, from, row_bytes, &bar[slot]);
-    bulk_load(to + p.per * 16, from + (gated ? static_cast<int64_t>(a.n) : int64_t(1)) * p.k_bytes, row_bytes,
-              &bar[slot]);
+    bulk_load(to, row_of(i, 0), row_bytes, &bar[slot]);
+    bulk_load(to + p.per * 16, row_of(i, 1), row_bytes, &bar[slot]);
   };
   if (lane == 0)
     for (int i = 0; i < p.slots; ++i) fetch(i, i);
