@@ -95,8 +95,8 @@ def build_binding(force: bool = False) -> Path:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f"-isystem{p}" for p in (root / "include", root / "include/torch/csrc/api/include",
                                       sysconfig.get_paths()["include"], cuda)),
-           str(src), "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10",
-           "-lc10_cuda"]
+           str(src), "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda",
+           "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)

@@ -14,7 +14,7 @@
 
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -82,8 +82,9 @@ c10::DeviceIndex usable_device(const void* entry, PyObject* first) {
   return t.get_device();
 }
 
+// What at::empty ends in for a CUDA tensor, without the dispatch on the way there.
 at::Tensor output(const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
-  return at::empty(sizes, at::TensorOptions().dtype(type).device(like.device()));
+  return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
 }
 
 // rms_norm(x, weight, residual, eps, fp8) -> (y | q, scale | None, new residual | None)
