@@ -6,7 +6,7 @@
 //
 // Operands bf16 (kind::f16) or E4M3 with one fp32 scale per row (kind::f8f6f4); both take
 // 128 bytes of K per row and tile, so one code serves both and only the instruction
-// descriptor differs.  Two kernels:
+// descriptor differs.  Three kernels:
 //
 //   linear_pair_kernel   many tokens: tensor-bound.  Persistent clusters of two CTAs
 //     (cta_group::2, M = 256 tokens, N = bn columns), W and x tiles by TMA through a ring of
@@ -28,11 +28,12 @@
 // Measured on a B200, launches back to back in a CUDA graph, operands larger than L2 in all
 // (a copy moves 6.5 TB/s, cuBLAS reaches 1672 TFLOP/s in bf16 for a moment, 1398 for seconds):
 //   pair    (m x k -> n) bf16 15360 x 8960 -> 1536 with residual: 270 us (1.56 PFLOP/s; the tensor
-//           pipe 80% active).  E4M3 gated 7680 x 1536 -> 2 * 8960: 165 to 215 us with the clock (2.0 to
-//           2.6 PFLOP/s; tensor pipe 72%); the epilogue's arithmetic shares issue slots and
-//           power with it (7680 x 1536 -> 2 * 4480: 75 us without an activation, 84 with one).
-//   split   E4M3 24 x 8960 -> 1536: 8.4 us (13.8 MB of W: 2.1 us at a copy's rate; the rest is the
-//           start, the exchange of partial sums and the epilogue).  bf16 24 x 1536 -> 8960 alike.
+//           pipe 80% active).  E4M3 gated 7680 x 1536 -> 2 * 8960: 165 to 215 us with the clock
+//           (2.0 to 2.6 PFLOP/s; tensor pipe 72%); the epilogue's arithmetic shares issue slots
+//           and power with it (7680 x 1536 -> 2 * 4480: 75 us without an activation, 84 with one).
+//   split   24 x 8960 -> 1536: E4M3 7.0 us (13.8 MB of W: 2.1 us at a copy's rate; the rest is the
+//           start, the exchange of partial sums and the epilogue), bf16 9.2; 24 x 1536 -> 8960:
+//           6.1 and 8.0.
 //   vector  bf16 1 x 1536 -> 8960: 7.2 us, 1 x 8960 -> 1536: 6.8 us (27.5 MB, 4.0 TB/s, about
 //           2.5 us of it start and end), 1 x 4096 -> 12288: 17.1 us (5.9 TB/s).
 #include <cuda.h>
@@ -666,13 +667,15 @@ constexpr int kSplitThreads = 320;                // producer, MMA issuer, eight
 constexpr int kJoinThreads = 256;                 // a power of two, so that a thread keeps its columns
 constexpr int kSplitBarrierBytes = 512;
 // Shared memory: the ring of stages, then the partial sums of this CTA's tokens, as the
-// cluster's CTAs send them (they may arrive while this CTA still multiplies).  An MMA reads
-// 128 W rows; a tile of fewer rows is followed by whatever comes next in shared memory (it
-// ends in accumulator rows that nobody reads), so what follows the ring is at least 16 KB.
-constexpr int kSplitPad = 128 * kKB;
+// cluster's CTAs send them (they may arrive while this CTA still multiplies).
 constexpr int kSplitDataBytes = (232448 - kSplitBarrierBytes) / 1024 * 1024;
-constexpr int kSplitBarrierOff = kSplitDataBytes;
-constexpr int kSplitSmemBytes = kSplitBarrierOff + kSplitBarrierBytes;
+constexpr int kSplitSmemBytes = kSplitDataBytes + kSplitBarrierBytes;
+// Half of an SM, where that leaves a ring of 88 KB: the next call's CTAs then start beside this
+// one's, and the shorter ring costs nothing (E4M3, back to back, whole SM and half: 24 x 8960 ->
+// 1536 7.3 and 7.0 us, 16 x 128 -> 64 2.7 and 2.4; with 80 KB, bf16 24 x 1536 -> 2 x 8960 lost,
+// 13.0 and 13.3).
+constexpr int kSplitHalfBytes = (113 * 1024 - kSplitBarrierBytes) / 1024 * 1024;
+constexpr int kSplitHalfRing = 88 * 1024;
 static_assert(kSplitSmemBytes <= 232448, "split plan exceeds shared memory");
 
 struct SplitBars {
@@ -696,6 +699,7 @@ struct SplitPlan {
   int own;        // tokens per rank: rank r joins tokens [r * own, (r + 1) * own) of the tile
   int own_mul;    // t / own = t * own_mul >> 16, exact for t * own < 2^16
   int part_off;   // of the partial sums in shared memory
+  int bar_off;    // of the barriers, behind them
 };
 
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
@@ -723,7 +727,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     if (threadIdx.x == 0) atomicOr(a.err_word, kErrSmemAlign);
     return;  // every CTA of the cluster sees the same layout
   }
-  auto* bars = reinterpret_cast<SplitBars*>(smem + kSplitBarrierOff);
+  auto* bars = reinterpret_cast<SplitBars*>(smem + p.bar_off);
   int* abort_flag = &bars->abort_flag;
   const int warp = warp_index_uniform();
   const int lane = threadIdx.x & 31;
@@ -824,7 +828,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    const uint32_t idesc = instr_desc<kF8>(128, p.tn);
+    const uint32_t idesc = instr_desc<kF8>(p.wr, p.tn);
     int stage = 0;
     uint32_t phase = 0;
     bool issued_any = false;
@@ -874,13 +878,15 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   tc_fence_after();
   if (warp >= 2) {
     const int quad = warp & 3, half = (warp - 2) >> 2;
-    const int row = quad * 32 + lane;
-    if (quad * 32 < p.wr) {
+    // 128 rows lie in the accumulator's lanes in order, 64 in the first 16 lanes of each quarter
+    const int row = p.wr == 128 ? quad * 32 + lane : quad * 16 + lane;
+    {
       const uint32_t mine = smem_u32(part) + static_cast<uint32_t>((rank * p.own * p.wr + row) * 4);
       for (int c = half * 16; c < p.tn; c += 32) {
         uint32_t r[16];
         tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + c, r);
         tmem_ld_wait();
+        if (p.wr == 64 && lane >= 16) continue;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int t = c + j, owner = (t * p.own_mul) >> 16;
@@ -1271,7 +1277,7 @@ cudaError_t launch_split(const LinearProblem& l, const LinearArgs& a, const Spli
     return e;
   const int64_t out_rows = l.gated ? p.wr / 2 : p.wr;
   const int64_t tiles = ((l.m + p.tn - 1) / p.tn) * ((l.n + out_rows - 1) / out_rows);
-  return launch_dependent(kernel, static_cast<unsigned>(tiles * p.split), kSplitThreads, kSplitSmemBytes, st,
+  return launch_dependent(kernel, static_cast<unsigned>(tiles * p.split), kSplitThreads, p.bar_off + kSplitBarrierBytes, st,
                           p.split, mx, mw, p, l.gated ? 1 : 0, l.residual, l.y, a);
 }
 
@@ -1376,11 +1382,12 @@ int resident_clusters(int split) {
 
 // Both planners estimate cycles per SM from measured rates and take the cheapest tile.
 //
-// Split: a K tile costs its four MMAs, about 137 cycles each whatever their N up to 128 (an
-// M = 128 MMA takes its A rows from shared memory at 32 bytes a cycle), or its bytes: W at an
-// SM's share of HBM (24 bytes a cycle), x from L2.  Half-empty MMAs (64 W rows) pay only when
-// W has few rows.  Setup, drain and output take about 6000 cycles, the exchange of partial
-// sums 2000 more.
+// Split: a K tile costs its four MMAs, or its bytes: W at an SM's share of HBM (24 bytes a
+// cycle), x from L2.  An MMA takes its W rows from shared memory at 32 bytes a cycle: 128 of them
+// about 137 cycles whatever the tokens up to 128, 64 of them half of that up to 32 tokens and as
+// long beyond (24 x 1536 -> 8960: 8.1 us by 64 rows and 9.9 by 128 in bf16, 6.2 and 7.6 in E4M3;
+// with 48 tokens 12.6 and 9.8, 9.3 and 8.1).  Setup, drain and output take about 6000 cycles,
+// the exchange of partial sums 2000 more.
 template <bool kF8>
 SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
   SplitPlan best = {};
@@ -1394,7 +1401,7 @@ SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
       const int tn = static_cast<int>(((l.m + m_tiles - 1) / m_tiles + 15) / 16 * 16);
       if (tn == last_tn) continue;
       last_tn = tn;
-      const double mma = 550.0;
+      const double mma = wr == 64 && tn <= 32 ? 290.0 : 550.0;
       const double bytes = wr * kKB / 24.0 + tn * kKB / 64.0;
       for (int split = 1; split <= kSplitMax && split <= k_tiles; ++split) {
         const int64_t clusters = resident_clusters<kF8>(split);
@@ -1418,9 +1425,13 @@ SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
   best.own = (best.tn + best.split - 1) / best.split;
   best.own_mul = (65536 + best.own - 1) / best.own;
   const int part_bytes = best.split * best.own * best.wr * 4;
-  best.stages = (kSplitDataBytes - (part_bytes > kSplitPad ? part_bytes : kSplitPad)) / (tile_bytes * group);
+  const int stage_bytes = tile_bytes * group;
+  const bool half = (kSplitHalfBytes - part_bytes) / stage_bytes * stage_bytes >= kSplitHalfRing;
+  const int budget = half ? kSplitHalfBytes : kSplitDataBytes;
+  best.stages = (budget - part_bytes) / stage_bytes;
   if (best.stages > kSplitStagesMax) best.stages = kSplitStagesMax;
-  best.part_off = best.stages * tile_bytes * group;
+  best.part_off = best.stages * stage_bytes;
+  best.bar_off = (best.part_off + part_bytes + 1023) / 1024 * 1024;
   best.m_tiles = static_cast<int>((l.m + best.tn - 1) / best.tn);
   best.k_each = k_tiles / best.split;
   best.k_more = k_tiles % best.split;
