@@ -1383,11 +1383,13 @@ int resident_clusters(int split) {
 // Both planners estimate cycles per SM from measured rates and take the cheapest tile.
 //
 // Split: a K tile costs its four MMAs, or its bytes: W at an SM's share of HBM (24 bytes a
-// cycle), x from L2.  An MMA takes its W rows from shared memory at 32 bytes a cycle: 128 of them
-// about 137 cycles whatever the tokens up to 128, 64 of them half of that up to 32 tokens and as
-// long beyond (24 x 1536 -> 8960: 8.1 us by 64 rows and 9.9 by 128 in bf16, 6.2 and 7.6 in E4M3;
-// with 48 tokens 12.6 and 9.8, 9.3 and 8.1).  Setup, drain and output take about 6000 cycles,
-// the exchange of partial sums 2000 more.
+// cycle when all of them read, up to 40 when fewer do), x from L2.  An MMA takes its W rows from
+// shared memory at 32 bytes a cycle: 128 of them about 137 cycles whatever the tokens up to 128,
+// 64 of them half of that up to 32 tokens and more beyond (24 x 1536 -> 8960: 8.1 us by 64 rows
+// and 9.9 by 128 in bf16, 6.2 and 7.6 in E4M3; with 48 tokens 12.6 and 9.8, 9.3 and 8.1).  Setup,
+// drain and output take about 5200 cycles, sending and joining the partial sums 0.35 a sum and,
+// between CTAs, 1200 more (128 x 400 -> 1000 in bf16: 6.3 us on seven CTAs a tile of 128 rows,
+// 4.5 on four of 64).
 template <bool kF8>
 SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
   SplitPlan best = {};
@@ -1401,14 +1403,15 @@ SplitPlan plan_split(const LinearProblem& l, int k_tiles, double* cost) {
       const int tn = static_cast<int>(((l.m + m_tiles - 1) / m_tiles + 15) / 16 * 16);
       if (tn == last_tn) continue;
       last_tn = tn;
-      const double mma = wr == 64 && tn <= 32 ? 290.0 : 550.0;
-      const double bytes = wr * kKB / 24.0 + tn * kKB / 64.0;
+      const double mma = wr == 128 ? 550.0 : tn <= 32 ? 290.0 : 470.0 + 2.0 * tn;
       for (int split = 1; split <= kSplitMax && split <= k_tiles; ++split) {
         const int64_t clusters = resident_clusters<kF8>(split);
         const int64_t waves = (n_tiles * m_tiles + clusters - 1) / clusters;
+        const double share = 24.0 * sm_count() / static_cast<double>(n_tiles * m_tiles * split);  // of HBM
+        const double bytes = wr * kKB / (share < 24.0 ? 24.0 : share > 40.0 ? 40.0 : share) + tn * kKB / 64.0;
         const double c = static_cast<double>(waves) *
-                         ((k_tiles + split - 1) / split * (mma > bytes ? mma : bytes) + 6000.0 +
-                          (split > 1 ? 2000.0 : 0.0) + 0.1 * wr * tn / split);
+                         ((k_tiles + split - 1) / split * (mma > bytes ? mma : bytes) + 5200.0 +
+                          (split > 1 ? 1200.0 : 0.0) + 0.35 * wr * tn);
         if (c < *cost) {
           *cost = c;
           best.wr = wr;
