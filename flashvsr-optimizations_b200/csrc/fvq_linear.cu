@@ -26,7 +26,7 @@
 //     drain, which is half of the split kernel's time at this size.
 //
 // Measured on a B200, launches back to back in a CUDA graph, operands larger than L2 in all
-// (a copy moves 6.5 TB/s, cuBLAS reaches 1672 TFLOP/s in bf16 for a moment, 1398 for seconds):
+// (a copy moves 6.5 TB/s, torch's bf16 product reaches 1672 TFLOP/s for a moment, 1398 for seconds):
 //   pair    (m x k -> n) bf16 15360 x 8960 -> 1536 with residual: 270 us (1.56 PFLOP/s; the tensor
 //           pipe 80% active).  E4M3 gated 7680 x 1536 -> 2 * 8960: 165 to 215 us with the clock
 //           (2.0 to 2.6 PFLOP/s; tensor pipe 72%); the epilogue's arithmetic shares issue slots
