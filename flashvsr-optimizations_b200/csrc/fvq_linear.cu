@@ -670,10 +670,11 @@ constexpr int kSplitBarrierBytes = 512;
 // cluster's CTAs send them (they may arrive while this CTA still multiplies).
 constexpr int kSplitDataBytes = (232448 - kSplitBarrierBytes) / 1024 * 1024;
 constexpr int kSplitSmemBytes = kSplitDataBytes + kSplitBarrierBytes;
-// Half of an SM, where that leaves a ring of 88 KB: the next call's CTAs then start beside this
-// one's, and the shorter ring costs nothing (E4M3, back to back, whole SM and half: 24 x 8960 ->
-// 1536 7.3 and 7.0 us, 16 x 128 -> 64 2.7 and 2.4; with 80 KB, bf16 24 x 1536 -> 2 x 8960 lost,
-// 13.0 and 13.3).
+// Half of the shared memory, where that leaves a ring of 88 KB: a longer one gains nothing, and
+// less of it starts sooner (E4M3, back to back, all of it and half: 24 x 8960 -> 1536 7.3 and 7.0
+// us, 16 x 128 -> 64 2.7 and 2.4; with 80 KB, bf16 24 x 1536 -> 2 x 8960 lost, 13.0 and 13.3).
+// Still one CTA per SM, by its registers: with 96 of them, and so two, the same 24 rows took
+// 8.0 us.
 constexpr int kSplitHalfBytes = (113 * 1024 - kSplitBarrierBytes) / 1024 * 1024;
 constexpr int kSplitHalfRing = 88 * 1024;
 static_assert(kSplitSmemBytes <= 232448, "split plan exceeds shared memory");
