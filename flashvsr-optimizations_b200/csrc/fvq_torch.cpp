@@ -3,10 +3,10 @@
 // A decode step calls these operators on a few rows at a time, where the Python side of a call
 // (argument checks, output allocation, ctypes) takes longer than the kernel.  Each function here
 // takes the common call -- plain CUDA tensors on the current device, contiguous, aligned, of the
-// right types and shapes, with no gradient to record and no mode active -- checks all of that,
-// allocates the outputs and calls libfvq.so, whose entry points ops.py hands over with bind().
-// Anything else returns None, and the Python implementation (which copies, converts or raises)
-// takes the call.  Nothing is computed here.
+// right types and shapes, with no gradient to record and no mode, trace or transform active --
+// checks all of that, allocates the outputs and calls libfvq.so, whose entry points ops.py hands
+// over with bind().  Anything else returns None, and the Python implementation (which copies,
+// converts or raises) takes the call.  Nothing is computed here.
 #include <Python.h>
 
 #include <cstdint>
@@ -16,6 +16,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -34,8 +35,12 @@ struct Entries {
   decltype(&fvq_fp8_cache_read) cache_read = nullptr;
 } entries;
 
-bool modes_active() {
-  return c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled();
+// Whether something has to see the call that only the dispatcher shows it to: a dispatch or function
+// mode, torch.jit.trace (which would record the outputs as constants), a functorch transform.  All
+// but the first two are keys that the thread includes beside the ones it starts with.
+bool interposed() {
+  return c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled() ||
+         !(c10::impl::tls_local_dispatch_key_set().included_ - c10::default_included_set).empty();
 }
 
 bool aligned(const at::Tensor& t, uintptr_t to) {
@@ -76,7 +81,7 @@ void* stream_of(c10::DeviceIndex dev) { return c10::cuda::getCurrentCUDAStream(d
 
 // The device the fast path works on, or -1 when nothing is to be done here.
 c10::DeviceIndex usable_device(const void* entry, PyObject* first) {
-  if (entry == nullptr || !THPVariable_CheckExact(first) || modes_active()) return -1;
+  if (entry == nullptr || !THPVariable_CheckExact(first) || interposed()) return -1;
   const at::Tensor& t = THPVariable_Unpack(first);
   if (!t.defined() || !t.is_cuda() || t.get_device() != c10::cuda::current_device()) return -1;
   return t.get_device();

@@ -599,7 +599,7 @@ def _(x, q1, s1, b1, q2, s2, b2):
 # These operators are called once or more per block and token, where a decode step is bound by
 # its host side.  The common eager call goes straight to the C ABI through _fvq_torch (which
 # returns None for every other: views to copy, odd alignment, wrong arguments, gradients, modes,
-# subclasses); the rest goes through the registered operator, defined directly on a
+# traces, transforms, subclasses); the rest goes through the registered operator, defined directly on a
 # torch.library.Library (about 6 us of dispatch a call against 20 us for the decorator's
 # wrapper).  Inference only: a call that would need a gradient raises when it is asked for.
 _BLOCK_LIB = torch.library.Library("fvq", "FRAGMENT")

@@ -1040,3 +1040,54 @@ def test_product_few_rows_wait_limit(m, n, k, gated):
     finally:
         ops.set_wait_limit(0)
     assert torch.equal(ops.linear_act(x, w, act="silu", gated=gated), want)
+
+
+# ---------------------------------------------------------------- under torch.jit.trace
+@pytest.mark.parametrize("name", ["rms_norm", "add_rms_norm", "rms_norm_fp8", "add_rms_norm_fp8", "linear_act",
+                                  "fp8_scaled_mm_act", "fp8_cache_write", "fp8_cache_read"])
+def test_traced_with_one_input_and_run_with_another(name):
+    """A trace records the operator, not the outputs it had while it was traced."""
+    w, m = randn(64, seed=3), randn(32, 64, seed=4)
+    mq, ms = ops.fp8_row_quant(m)
+    slots = torch.arange(6, device="cuda")
+    table, lens = torch.zeros(1, 2, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+
+    def bits(t):
+        return t.view(torch.uint8) if t.dtype == F8 else t
+
+    def fresh(seed):
+        x, r = randn(6, 64, seed=seed), randn(6, 64, seed=seed + 1)
+        if name == "fp8_scaled_mm_act":
+            return ops.fp8_row_quant(x)
+        if name == "fp8_cache_write":
+            return (x.view(6, 2, 32), r.view(6, 2, 32), *store(3, 4, 2, 32))
+        return store(3, 4, 2, 32, seed=seed) if name == "fp8_cache_read" else (x, r)
+
+    def write(k, v, *cache):
+        ops.fp8_cache_write(k, v, slots, *cache)
+        return cache
+
+    fn = {"rms_norm": lambda x, r: ops.rms_norm(x, w) + r,
+          "add_rms_norm": lambda x, r: ops.add_rms_norm(x, r, w),
+          "rms_norm_fp8": lambda x, r: ops.rms_norm_fp8(x + r, w),
+          "add_rms_norm_fp8": lambda x, r: ops.add_rms_norm_fp8(x, r, w),
+          "linear_act": lambda x, r: ops.linear_act(x + r, m, act="silu"),
+          "fp8_scaled_mm_act": lambda q, s: ops.fp8_scaled_mm_act(q, s, mq, ms),
+          "fp8_cache_write": write,
+          "fp8_cache_read": lambda *cache: ops.fp8_cache_read(*cache, table, lens, 5)}[name]
+    traced = torch.jit.trace(fn, fresh(1), check_trace=False)
+    want, got = fn(*fresh(11)), traced(*fresh(11))
+    if isinstance(want, torch.Tensor):
+        want, got = (want,), (got,)
+    assert len(want) == len(got)
+    for a, b in zip(want, got):
+        assert torch.equal(bits(a), bits(b))
+
+
+def test_traced_prenorm():
+    ffn = fvq.FP8FFN(fvq.QuantLinear(linear(1024, 512, 1), "fp8"), torch.nn.GELU(approximate="tanh"),
+                     fvq.QuantLinear(linear(512, 1024, 3), "fp8"))
+    w = randn(512, seed=6)
+    traced = torch.jit.trace(lambda x: ffn.prenorm(x, w), (randn(3, 512, seed=7),), check_trace=False)
+    x = randn(3, 512, seed=8)
+    assert torch.equal(traced(x), ffn.prenorm(x, w))
