@@ -16,6 +16,7 @@ import ctypes
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -601,8 +602,12 @@ def _(x, q1, s1, b1, q2, s2, b2):
 # returns None for every other: views to copy, odd alignment, wrong arguments, gradients, modes,
 # traces, transforms, subclasses); the rest goes through the registered operator, defined directly on a
 # torch.library.Library (about 6 us of dispatch a call against 20 us for the decorator's
-# wrapper).  Inference only: a call that would need a gradient raises when it is asked for.
+# wrapper).  Inference only: a call that would need a gradient raises when it is asked for, one on
+# a forward-mode tangent at once.
 _BLOCK_LIB = torch.library.Library("fvq", "FRAGMENT")
+
+
+_NO_GRADIENT = "no gradient formula (this library's operators are for inference)"
 
 
 class _NoGradient(torch.autograd.Function):
@@ -615,7 +620,12 @@ class _NoGradient(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        raise RuntimeError(f"{ctx.name}: no gradient formula (this library's operators are for inference)")
+        raise RuntimeError(f"{ctx.name}: {_NO_GRADIENT}")
+
+
+def _has_tangent(args) -> bool:
+    return torch._C._is_fwd_grad_enabled() and any(
+        isinstance(a, torch.Tensor) and forward_ad.unpack_dual(a).tangent is not None for a in args)
 
 
 def _define(schema: str, impl, fake):
@@ -627,6 +637,8 @@ def _define(schema: str, impl, fake):
     fn = getattr(torch.ops.fvq, name).default
 
     def call(*args):
+        if forward_ad._current_level >= 0 and _has_tangent(args):
+            raise RuntimeError(f"{name}: {_NO_GRADIENT}")
         if torch.is_grad_enabled() and any(isinstance(a, torch.Tensor) and a.requires_grad for a in args):
             return _NoGradient.apply(name, fn, *args)
         return fn(*args)

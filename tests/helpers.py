@@ -51,3 +51,26 @@ def gpu_rcp_table(x_bits: np.ndarray, g: float) -> dict:
     args = np.array(O.rcp_arguments(x_bits, g), dtype=np.uint32)
     res = fvq.ops.rcp_approx_probe(torch.from_numpy(args.view(np.float32)).cuda())
     return table_from(args, res.cpu().numpy().view(np.uint32))
+
+
+def calls_with_a_tangent(device: str) -> list:
+    """Calls of the block operators, each with one argument that carries a forward-mode tangent
+    (make and call them inside a dual level)."""
+    import torch
+    from torch.autograd.forward_ad import make_dual
+    from flashvsr_optimizations_b200 import ops
+
+    def dual(t):
+        return make_dual(t, torch.ones_like(t))
+    p = torch.ones(8, 64, dtype=torch.bfloat16, device=device)
+    s, i = torch.ones(8, 1, device=device), torch.zeros(1, dtype=torch.int32, device=device)
+    kv, slots = p.view(8, 1, 64), torch.arange(8, device=device)
+    q = p.to(torch.float8_e4m3fn)
+    codes, scale = q.view(2, 4, 1, 64), s.view(2, 4, 1)
+    x = dual(p)
+    return [lambda: ops.rms_norm(x), lambda: ops.rms_norm(p, dual(p[0])), lambda: ops.add_rms_norm(p, x),
+            lambda: ops.rms_norm_fp8(x), lambda: ops.add_rms_norm_fp8(x, p), lambda: ops.linear_act(x, p),
+            lambda: ops.linear_act(p, x), lambda: ops.linear_act(p, p, residual=dual(torch.ones_like(p[:, :8]))),
+            lambda: ops.fp8_scaled_mm_act(q, dual(s), q, s),
+            lambda: ops.fp8_cache_write(kv, dual(kv), slots, codes, scale, codes, scale),
+            lambda: ops.fp8_cache_read(codes, dual(scale), codes, scale, i.view(1, 1), i, 4)]

@@ -7,6 +7,7 @@ import torch
 
 import flashvsr_optimizations_b200 as fvq
 from flashvsr_optimizations_b200 import _lib, ops
+from helpers import calls_with_a_tangent
 
 BF16, F32, F8 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
 
@@ -164,3 +165,14 @@ def test_slots_on_pages_outside_the_store_are_past_it():
     got = cache.slots(table, torch.tensor([[0, 15, 16, 31, 32, -5]]))
     assert got[:2].tolist() == [48, 63] and got[5] == -1
     assert (got[2:5] >= 6 * 16).all()
+
+
+def test_forward_mode_tangents_are_refused():
+    """The outputs carry no tangent, so it would be dropped without a word."""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        for call in calls_with_a_tangent("cpu"):
+            with pytest.raises(RuntimeError, match="no gradient formula"):
+                call()
+    with pytest.raises(RuntimeError, match="no gradient formula"):
+        torch.func.jvp(ops.rms_norm, (torch.ones(4, 64),), (torch.ones(4, 64),))

@@ -16,6 +16,7 @@ import torch
 
 import flashvsr_optimizations_b200 as fvq
 from flashvsr_optimizations_b200 import ops
+from helpers import calls_with_a_tangent
 
 pytestmark = pytest.mark.gpu
 
@@ -1091,3 +1092,13 @@ def test_traced_prenorm():
     traced = torch.jit.trace(lambda x: ffn.prenorm(x, w), (randn(3, 512, seed=7),), check_trace=False)
     x = randn(3, 512, seed=8)
     assert torch.equal(traced(x), ffn.prenorm(x, w))
+
+
+def test_forward_mode_tangents_are_refused():
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        for call in calls_with_a_tangent("cuda"):
+            with pytest.raises(RuntimeError, match="no gradient formula"):
+                call()
+        x = randn(4, 64)
+        assert torch.equal(ops.rms_norm(forward_ad.unpack_dual(forward_ad.make_dual(x, x)).primal), ops.rms_norm(x))
