@@ -52,7 +52,7 @@ const at::Tensor* plain(PyObject* obj, at::ScalarType type, c10::DeviceIndex dev
   if (!THPVariable_CheckExact(obj)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(obj);
   if (!t.defined() || !t.is_cuda() || !t.has_storage() || t.layout() != at::kStrided || t.is_neg() ||
-      t.scalar_type() != type || t.get_device() != dev)
+      t._is_zerotensor() || t.scalar_type() != type || t.get_device() != dev)
     return nullptr;
   if ((t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined()) return nullptr;
   return &t;

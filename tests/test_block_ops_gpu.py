@@ -1102,3 +1102,14 @@ def test_forward_mode_tangents_are_refused():
                 call()
         x = randn(4, 64)
         assert torch.equal(ops.rms_norm(forward_ad.unpack_dual(forward_ad.make_dual(x, x)).primal), ops.rms_norm(x))
+
+
+def test_tensors_without_memory_are_materialised():
+    """A weight, bias or residual of zeros that torch holds without storage is not an absent one."""
+    x, w = randn(8, 64, seed=1), randn(16, 64, seed=2)
+
+    def zeros(*shape):
+        return torch._efficientzerotensor(*shape, dtype=BF16, device="cuda")
+    assert torch.equal(ops.rms_norm(x, zeros(64)), torch.zeros_like(x))
+    assert torch.equal(ops.linear_act(x, w, zeros(16), residual=zeros(8, 16)), ops.linear_act(x, w))
+    assert torch.equal(ops.linear_act(zeros(8, 64), w), torch.zeros(8, 16, dtype=BF16, device="cuda"))
