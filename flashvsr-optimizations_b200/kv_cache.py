@@ -55,6 +55,8 @@ class FP8KVCache:
         reports."""
         pages, page = self.k_codes.shape[:2]
         at = positions.long()
+        if page_table.shape[1] == 0:  # no entry to gather
+            return torch.where(at < 0, -1, pages * page).reshape(-1)
         index = page_table.long().gather(1, (at.clamp_min(0) // page).clamp_max(page_table.shape[1] - 1))
         there = (at < page_table.shape[1] * page) & (index >= 0)
         slot = torch.where(there, index * page + at % page, pages * page)

@@ -176,3 +176,14 @@ def test_forward_mode_tangents_are_refused():
                 call()
     with pytest.raises(RuntimeError, match="no gradient formula"):
         torch.func.jvp(ops.rms_norm, (torch.ones(4, 64),), (torch.ones(4, 64),))
+
+
+def test_slots_of_a_table_without_pages():
+    """Every position is past such a table; nothing is looked up in it (on a GPU that would be a
+    device-side assertion)."""
+    cache = object.__new__(fvq.FP8KVCache)
+    cache.k_codes = torch.empty(6, 16, 1, 8)
+    got = cache.slots(torch.empty(2, 0, dtype=torch.int32), torch.tensor([[0, -1, 40], [-3, 15, 1 << 40]]))
+    assert got.dtype == torch.int64 and got[1] == -1 and got[3] == -1
+    assert (got[[0, 2, 4, 5]] >= 6 * 16).all()
+    assert cache.slots(torch.empty(2, 0, dtype=torch.int32), torch.empty(2, 0, dtype=torch.int64)).shape == (0,)
