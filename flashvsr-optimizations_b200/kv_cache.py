@@ -54,6 +54,10 @@ class FP8KVCache:
         past the table, or on a page outside the store, gets a slot past the store, which ``write``
         reports."""
         pages, page = self.k_codes.shape[:2]
+        if page_table.dim() != 2 or positions.dim() != 2 or positions.shape[0] != page_table.shape[0] or \
+                any(t.dtype.is_floating_point or t.dtype == torch.bool for t in (page_table, positions)):
+            raise ValueError("FP8KVCache.slots: expected integers, page_table [batch, pages] and positions "
+                             f"[batch, tokens], got {tuple(page_table.shape)} and {tuple(positions.shape)}")
         at = positions.long()
         if page_table.shape[1] == 0:  # no entry to gather
             return torch.where(at < 0, -1, pages * page).reshape(-1)

@@ -187,3 +187,14 @@ def test_slots_of_a_table_without_pages():
     assert got.dtype == torch.int64 and got[1] == -1 and got[3] == -1
     assert (got[[0, 2, 4, 5]] >= 6 * 16).all()
     assert cache.slots(torch.empty(2, 0, dtype=torch.int32), torch.empty(2, 0, dtype=torch.int64)).shape == (0,)
+
+
+def test_slots_refuse_what_is_no_table_and_positions():
+    cache = object.__new__(fvq.FP8KVCache)
+    cache.k_codes = torch.empty(6, 16, 1, 8)
+    table, at = torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 3, dtype=torch.int64)
+    assert cache.slots(table.long(), at.int()).tolist() == [0] * 12
+    for bad in ((table, at[:1]), (table[:1], at), (table[0], at), (table, at[:, 0]), (table.float(), at),
+                (table, at.double()), (table, at.bool())):
+        with pytest.raises(ValueError, match="FP8KVCache.slots"):
+            cache.slots(*bad)
