@@ -458,7 +458,9 @@ __global__ void __launch_bounds__(kNumThreads, 1)
         if (elect_one()) tc_commit(&bars->acc_full);
         __syncwarp();
       }
-      if (warp_aborted(bars) && issued_any) {
+      // Nothing issued may run on when TMEM and the ring go, whichever warp gives up, and when: so
+      // this waits whether or not the flag is up by now.
+      if (issued_any) {
         if (elect_one()) tc_commit(&bars->teardown);
         __syncwarp();
         if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))
@@ -954,7 +956,9 @@ __global__ void __launch_bounds__(kNumThreads, 1)
         }
         __syncwarp();
       }
-      if (warp_aborted(bars) && issued_any) {
+      // Nothing issued may run on when TMEM and the ring go, whichever warp gives up, and when: so
+      // this waits whether or not the flag is up by now.
+      if (issued_any) {
         if (elect_one()) tc_commit_pair(smem_u32(&bars->teardown));
         __syncwarp();
         if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))
@@ -1234,7 +1238,9 @@ __global__ void __launch_bounds__(kNumThreads, 1)
         if (elect_one()) tc_commit(&bars->acc_full);
         __syncwarp();
       }
-      if (warp_aborted(bars) && issued_any) {
+      // Nothing issued may run on when TMEM and the ring go, whichever warp gives up, and when: so
+      // this waits whether or not the flag is up by now.
+      if (issued_any) {
         if (elect_one()) tc_commit(&bars->teardown);
         __syncwarp();
         if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))
@@ -1532,7 +1538,9 @@ __global__ void __launch_bounds__(kNumThreads, 1)
         }
         __syncwarp();
       }
-      if (warp_aborted(bars) && issued_any) {
+      // Nothing issued may run on when TMEM and the ring go, whichever warp gives up, and when: so
+      // this waits whether or not the flag is up by now.
+      if (issued_any) {
         if (elect_one()) tc_commit_pair(smem_u32(&bars->teardown));
         __syncwarp();
         if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))

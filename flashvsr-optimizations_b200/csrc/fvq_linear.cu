@@ -476,7 +476,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         __syncwarp();
       }
-      if (warp_aborted(abort_flag) && issued_any) {
+      // Nothing issued may run on when TMEM and the ring go, whichever warp gives up, and when: so
+      // this waits whether or not the flag is up by now.
+      if (issued_any) {
         if (elect_one()) tc_commit_pair(smem_u32(&bars->teardown));
         __syncwarp();
         if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))
@@ -861,7 +863,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         phase ^= 1u;
       }
     }
-    if (warp_aborted(abort_flag) && issued_any) {
+    // as in the pair kernel: whether or not a warp has given up by now
+    if (issued_any) {
       if (elect_one()) tc_commit(&bars->teardown);
       __syncwarp();
       if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))

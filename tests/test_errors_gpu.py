@@ -73,3 +73,41 @@ def test_fused_quantizer_grid_wait_timeout_sets_error_word():
     torch.cuda.synchronize()
     assert ops.read_device_error() == 0
     assert g.item() == g_ref.item() and torch.equal(q, q_ref) and torch.equal(s, s_ref)
+
+
+# Waits that run out in the middle of a kernel: from shorter than a first load to longer than the
+# whole launch.  Bits 0 to 2 of the error word are waits of the producer, the MMA issuer and the
+# epilogue; bit 3, a teardown that did not complete, must not appear, and a result without a bit is
+# the result.
+LIMITS = [1000, 1500, 2000, 3000, 4000, 6000, 8000, 12000, 16000, 32000, 64000]
+
+
+def give_up(call, want):
+    try:
+        for limit in LIMITS:
+            ops.set_wait_limit(limit)
+            got = call()
+            flags = ops.read_device_error()
+            assert flags & ~7 == 0, (limit, flags)
+            if flags == 0:
+                assert torch.equal(got, want), limit
+    finally:
+        ops.set_wait_limit(0)
+    assert torch.equal(call(), want)
+    assert ops.read_device_error() == 0
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("m,n,k", [(24, 1536, 8960), (128, 8960, 1536), (16, 64, 64), (100, 264, 16384)])
+def test_split_product_gives_up_anywhere(m, n, k, fp8):
+    x = torch.randn(m, k, generator=torch.Generator("cuda").manual_seed(1), device="cuda").to(torch.bfloat16)
+    w = torch.randn(n, k, generator=torch.Generator("cuda").manual_seed(2), device="cuda").to(torch.bfloat16)
+    if fp8:
+        args, fn = (*ops.fp8_row_quant(x), *ops.fp8_row_quant(w)), ops.fp8_scaled_mm_act
+    else:
+        args, fn = (x, w), ops.linear_act
+    ops.set_linear_kernel(1)
+    try:
+        give_up(lambda: fn(*args), fn(*args))
+    finally:
+        ops.set_linear_kernel(0)
