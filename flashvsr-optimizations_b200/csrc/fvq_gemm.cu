@@ -502,7 +502,9 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     asm("mov.b64 %0, {%1, %1};" : "=l"(alpha2) : "f"(alpha));
     uint32_t amax2 = 0;  // max |h| of the low and high columns, bf16 magnitude bits
     for (int i = 0; i < seq.count; ++i) {
-      if (!mbar_wait_bounded(&bars->acc_full, static_cast<uint32_t>(i) & 1u, wait_limit)) {
+      // one outcome for the warp: tcgen05.ld and the shuffles below need all of its lanes
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(&bars->acc_full, static_cast<uint32_t>(i) & 1u,
+                                                     wait_limit))) {
         flag_error(bars, kErrWaitEpilogue);
         break;
       }
@@ -978,7 +980,9 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     const uint32_t acc_empty_addr = even_addr(&bars->acc_empty);
     uint32_t amax2 = 0;  // max |out| of the low and high columns (amax_out)
     for (int i = 0; i < count; ++i) {
-      if (!mbar_wait_cluster_bounded(&bars->acc_full, static_cast<uint32_t>(i) & 1u, wait_limit)) {
+      // one outcome for the warp: tcgen05.ld and the shuffles below need all of its lanes
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait_cluster_bounded(
+                                       &bars->acc_full, static_cast<uint32_t>(i) & 1u, wait_limit))) {
         flag_error(bars, kErrWaitEpilogue);
         break;
       }
@@ -1267,7 +1271,9 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       seq.at(i, mb, nb, half);
       const int row = mb * BM + trow;
       const float sa = row < m ? __ldg(sa_rows + row) : 0.0f;
-      if (!mbar_wait_bounded(&bars->acc_full, static_cast<uint32_t>(i) & 1u, wait_limit)) {
+      // one outcome for the warp: tcgen05.ld and the shuffles below need all of its lanes
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(&bars->acc_full, static_cast<uint32_t>(i) & 1u,
+                                                     wait_limit))) {
         flag_error(bars, kErrWaitEpilogue);
         break;
       }
@@ -1566,7 +1572,9 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       const int row0 = mbp * 2 * BM + static_cast<int>(rank) * BM;  // this CTA's first row
       const int row = row0 + trow;
       const float sa = row < m ? __ldg(sa_rows + row) : 0.0f;
-      if (!mbar_wait_cluster_bounded(&bars->acc_full, static_cast<uint32_t>(i) & 1u, wait_limit)) {
+      // one outcome for the warp: tcgen05.ld and the shuffles below need all of its lanes
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait_cluster_bounded(
+                                       &bars->acc_full, static_cast<uint32_t>(i) & 1u, wait_limit))) {
         flag_error(bars, kErrWaitEpilogue);
         break;
       }

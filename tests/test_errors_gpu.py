@@ -111,3 +111,32 @@ def test_split_product_gives_up_anywhere(m, n, k, fp8):
         give_up(lambda: fn(*args), fn(*args))
     finally:
         ops.set_linear_kernel(0)
+
+
+def fp8_rows(m, k, seed):
+    x = torch.randn(m, k, generator=torch.Generator("cuda").manual_seed(seed), device="cuda")
+    return ops.fp8_row_quant(x.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("m,n,k", [(512, 1024, 1536), (1000, 1536, 8960)])
+@pytest.mark.parametrize("kind", ["nvfp4", "nvfp4_gelu", "fp8"])
+def test_one_sm_gemm_gives_up_anywhere(kind, m, n, k):
+    if kind == "fp8":
+        (a, sa), (w, sw) = fp8_rows(m, k, 1), fp8_rows(n, k, 2)
+
+        def call():
+            return ops.fp8_scaled_mm(a, sa, w, sw)
+    else:
+        (a, asf), (w, wsf) = _operands(m, n, k, seed=3)
+        g = torch.ones(1, device="cuda")
+
+        def call():
+            return ops.nvfp4_gemm(a, asf, g, w, wsf, g, gelu=kind == "nvfp4_gelu")[0]
+    from flashvsr_optimizations_b200 import _lib
+    _lib.call("fvq_set_gemm_pairing", 0)
+    _lib.call("fvq_set_fp8_gemm_pairing", 0)
+    try:
+        give_up(call, call())
+    finally:
+        _lib.call("fvq_set_gemm_pairing", 1)
+        _lib.call("fvq_set_fp8_gemm_pairing", 1)
