@@ -750,6 +750,8 @@ struct PairBarriers {
   uint64_t acc_full;                // the pair's accumulator is complete
   uint64_t acc_empty;               // even CTA: both epilogues drained their TMEM
   uint64_t teardown;
+  uint64_t odd_done;                // even CTA: the odd one's producer has ended,
+  uint32_t odd_fills;               // after this many fills of its stages
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -801,6 +803,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     mbar_init(&bars->acc_full, 1);
     mbar_init(&bars->acc_empty, 2 * kEpiWarps);
     mbar_init(&bars->teardown, 1);
+    mbar_init(&bars->odd_done, 1);
     bars->abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -827,9 +830,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     // (the whole warp runs the loop; one elected lane issues the copies)
     grid_dependency_wait();
     if (count > 0) {
-      uint32_t armed[kPairStages];
-#pragma unroll
-      for (int s = 0; s < kPairStages; ++s) armed[s] = 0;
+      uint32_t fills = 0;
       int stage = 0;
       uint32_t phase = 0;
       for (int i = 0; i < count && !warp_aborted(bars); ++i) {
@@ -868,21 +869,25 @@ __global__ void __launch_bounds__(kNumThreads, 1)
               tma_load_3d_pair(ssfb, &tmap_sfb, bar, 0, 0, nb * (k / 64) + kt * 4);
           }
           __syncwarp();
-          armed[stage] += 1;
+          ++fills;
           if (++stage == kPairStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-      // the even CTA's stage barriers count both CTAs' loads; the odd CTA's land
-      // before the even CTA's MMAs consume the stage, which the final cluster
-      // barrier waits for
-      for (int s = 0; even && s < kPairStages; ++s) {
-        if (armed[s] > 0 &&
-            !warp_wait_cluster_bounded(&bars->full[s], (armed[s] - 1) & 1u, teardown_limit))
-          warp_flag_error(bars, kErrWaitTeardown);
-      }
+      const auto bytes = [&](uint32_t f) {
+        int mbp_unused, nb_unused, half;
+        seq.at(static_cast<int>(f) / num_k_tiles, mbp_unused, nb_unused, half);
+        return static_cast<uint32_t>(half < 0 ? kPairStageBytes : kPairStageBytes - kPairQuarterBBytes);
+      };
+      if (!pair_drain_loads<kPairStages>(rank, bars->full, &bars->odd_done, &bars->odd_fills, fills,
+                                         bytes, teardown_limit))
+        warp_flag_error(bars, kErrWaitTeardown);
+      // the odd CTA: the even one's MMAs, and their arrivals here, are over (its MMA warp may have
+      // one wait and its own teardown ahead)
+      if (!even && !warp_wait_cluster_bounded(&bars->teardown, 0, limit_times(teardown_limit, 3)))
+        warp_flag_error(bars, kErrWaitTeardown);
     }
   } else if (warp == 1) {
     if (count > 0 && even) {
@@ -960,12 +965,9 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       }
       // Nothing issued may run on when TMEM and the ring go, whichever warp gives up, and when: so
       // this waits whether or not the flag is up by now.
-      if (issued_any) {
-        if (elect_one()) tc_commit_pair(smem_u32(&bars->teardown));
-        __syncwarp();
-        if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))
-          warp_flag_error(bars, kErrWaitTeardown);
-      }
+      pair_commit_teardown(&bars->teardown, rank, issued_any);
+      if (!warp_wait_cluster_bounded(&bars->teardown, 0, teardown_limit))
+        warp_flag_error(bars, kErrWaitTeardown);
     }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
@@ -1375,6 +1377,8 @@ struct F8PairBarriers {
   uint64_t acc_full;         // the pair's accumulator is complete
   uint64_t acc_empty;        // even CTA: both epilogues drained their TMEM
   uint64_t teardown;
+  uint64_t odd_done;         // even CTA: the odd one's producer has ended,
+  uint32_t odd_fills;        // after this many fills of its stages
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -1429,6 +1433,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     mbar_init(&bars->acc_full, 1);
     mbar_init(&bars->acc_empty, 2 * kEpiWarps);
     mbar_init(&bars->teardown, 1);
+    mbar_init(&bars->odd_done, 1);
     bars->abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -1450,9 +1455,7 @@ __global__ void __launch_bounds__(kNumThreads, 1)
     // ------------------------------------------------------------ producer (both CTAs)
     // (the whole warp runs the loop; one elected lane issues the copies)
     if (count > 0) {
-      uint32_t armed[kStages];
-#pragma unroll
-      for (int s = 0; s < kStages; ++s) armed[s] = 0;
+      uint32_t fills = 0;
       int stage = 0;
       uint32_t phase = 0;
       for (int i = 0; i < count && !warp_aborted(bars); ++i) {
@@ -1476,21 +1479,21 @@ __global__ void __launch_bounds__(kNumThreads, 1)
                              nb * BN + static_cast<int>(rank) * (BN / 2));
           }
           __syncwarp();
-          armed[stage] += 1;
+          ++fills;
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-      // the even CTA's stage barriers count both CTAs' loads; the odd CTA's land
-      // before the even CTA's MMAs consume the stage, which the final cluster
-      // barrier waits for
-      for (int s = 0; even && s < kStages; ++s) {
-        if (armed[s] > 0 &&
-            !warp_wait_cluster_bounded(&bars->full[s], (armed[s] - 1) & 1u, teardown_limit))
-          warp_flag_error(bars, kErrWaitTeardown);
-      }
+      const auto bytes = [](uint32_t) { return static_cast<uint32_t>(kF8PairStageBytes); };
+      if (!pair_drain_loads<kStages>(rank, bars->full, &bars->odd_done, &bars->odd_fills, fills,
+                                     bytes, teardown_limit))
+        warp_flag_error(bars, kErrWaitTeardown);
+      // the odd CTA: the even one's MMAs, and their arrivals here, are over (its MMA warp may have
+      // one wait and its own teardown ahead)
+      if (!even && !warp_wait_cluster_bounded(&bars->teardown, 0, limit_times(teardown_limit, 3)))
+        warp_flag_error(bars, kErrWaitTeardown);
     }
   } else if (warp == 1) {
     if (count > 0 && even) {
@@ -1546,12 +1549,9 @@ __global__ void __launch_bounds__(kNumThreads, 1)
       }
       // Nothing issued may run on when TMEM and the ring go, whichever warp gives up, and when: so
       // this waits whether or not the flag is up by now.
-      if (issued_any) {
-        if (elect_one()) tc_commit_pair(smem_u32(&bars->teardown));
-        __syncwarp();
-        if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))
-          warp_flag_error(bars, kErrWaitTeardown);
-      }
+      pair_commit_teardown(&bars->teardown, rank, issued_any);
+      if (!warp_wait_cluster_bounded(&bars->teardown, 0, teardown_limit))
+        warp_flag_error(bars, kErrWaitTeardown);
     }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)

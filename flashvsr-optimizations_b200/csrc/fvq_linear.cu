@@ -189,12 +189,6 @@ __device__ __forceinline__ bool warp_aborted(const int* abort_flag) {
   return __shfl_sync(0xFFFFFFFFu, *reinterpret_cast<const volatile int*>(abort_flag), 0) != 0;
 }
 
-__device__ __forceinline__ void pause_ns(uint64_t ns) {
-  const uint64_t start = global_timer_ns();
-  for (int i = 0; i < (1 << 20) && global_timer_ns() - start < ns; ++i) {
-  }
-}
-
 // ---------------------------------------------------------------- many tokens
 constexpr int kPairTokens = 256;                  // per pair; 128 per CTA
 constexpr int kPairABytes = 128 * kKB;            // 16 KB
@@ -220,6 +214,8 @@ struct PairBars {
   uint64_t acc_empty[2];          // even CTA: both epilogues drained the accumulator
   uint64_t res_full[kPairEpiWarps][2];  // residual chunk landed in the warp's staging buffer
   uint64_t teardown;
+  uint64_t odd_done;              // even CTA: the odd one's producer has ended,
+  uint32_t odd_fills;             // after this many fills of its stages
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -359,6 +355,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       for (int w = 0; w < kPairEpiWarps; ++w) mbar_init(&bars->res_full[w][b], 1);
     }
     mbar_init(&bars->teardown, 1);
+    mbar_init(&bars->odd_done, 1);
     bars->abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -379,9 +376,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (both CTAs)
-    uint32_t armed[kPairStages];
-#pragma unroll
-    for (int s = 0; s < kPairStages; ++s) armed[s] = 0;
+    uint32_t fills = 0;
     const uint32_t w_bytes = static_cast<uint32_t>(bn / 2) * kKB;
     const int k_step = kF8 ? kKB : kKB / 2;  // elements
     int stage = 0;
@@ -406,7 +401,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           tma_load_2d_pair(sa + kPairABytes, &tmap_w, bar, kt * k_step, w_row);
         }
         __syncwarp();
-        armed[stage] += 1;
+        ++fills;
         if (++stage == kPairStages) {
           stage = 0;
           phase ^= 1u;
@@ -414,16 +409,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
     }
     grid_launch_dependents();  // this CTA's last tile is on its way
-    // the even CTA's stage barriers count both CTAs' loads; the odd CTA's land before the
-    // even CTA passes the final cluster barrier
-    for (int s = 0; even && s < kPairStages; ++s) {
-      if (armed[s] > 0 &&
-          !warp_wait_cluster_bounded(&bars->full[s], (armed[s] - 1) & 1u, teardown_limit))
-        warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
-    }
-    // after an abort the even CTA may not have armed a stage that this one has loads for: no
-    // barrier counts them, so give them time to land before the CTA may exit
-    if (!even && warp_aborted(abort_flag)) pause_ns(100000);
+    if (!pair_drain_loads<kPairStages>(cta, bars->full, &bars->odd_done, &bars->odd_fills, fills,
+                                       [&](uint32_t) { return kPairABytes + w_bytes; }, teardown_limit))
+      warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
+    // the odd CTA: the even one's MMAs, and their arrivals here, are over (its MMA warp may have one
+    // wait and its own teardown ahead)
+    if (!even && !warp_wait_cluster_bounded(&bars->teardown, 0, limit_times(teardown_limit, 3)))
+      warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
     if constexpr (kSplitK) cluster_sync();  // the partial sums are in place
   } else if (warp == 1) {
     if (even) {
@@ -478,12 +470,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       // Nothing issued may run on when TMEM and the ring go, whichever warp gives up, and when: so
       // this waits whether or not the flag is up by now.
-      if (issued_any) {
-        if (elect_one()) tc_commit_pair(smem_u32(&bars->teardown));
-        __syncwarp();
-        if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))
-          warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
-      }
+      pair_commit_teardown(&bars->teardown, cta, issued_any);
+      if (!warp_wait_cluster_bounded(&bars->teardown, 0, teardown_limit))
+        warp_flag(abort_flag, a.err_word, kErrWaitTeardown);
     }
     if constexpr (kSplitK) cluster_sync();
   } else {
@@ -863,7 +852,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         phase ^= 1u;
       }
     }
-    // as in the pair kernel: whether or not a warp has given up by now
+    // as in the pair kernel, whether or not a warp has given up by now
     if (issued_any) {
       if (elect_one()) tc_commit(&bars->teardown);
       __syncwarp();

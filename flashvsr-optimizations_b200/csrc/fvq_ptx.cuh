@@ -245,6 +245,57 @@ __device__ __forceinline__ bool warp_wait_cluster_bounded(uint64_t* bar, uint32_
   return __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, 0) != 0;
 }
 
+// Counts `bytes` on a local mbarrier as a landed copy would.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
+               : "memory");
+}
+
+// n waits' worth of a limit, which may be as good as none.
+__device__ __forceinline__ uint64_t limit_times(uint64_t limit_ns, uint32_t n) {
+  return limit_ns < (uint64_t(1) << 56) ? n * limit_ns : limit_ns;
+}
+
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// How the producer warps of a CTA pair end.  Both CTAs' loads of a fill are counted on the even
+// CTA's stage barrier, which the even CTA arms for both; fill f goes to stage f % kStages.  A CTA
+// that gives up may have issued fewer fills than the other, by at most kStages (a stage is filled
+// again only after the MMAs on its last fill): then a barrier waits for bytes that never come,
+// or loads land that no barrier counts.  So the odd CTA says how many fills it issued, the even CTA
+// takes the odd one's bytes off the fills that only it issued itself, arms those that only the odd
+// one issued, and waits until everything has landed (the odd one is held by the pair's last
+// barrier meanwhile).  `fills`: this CTA's; bytes(f): of one CTA's share of fill f.  Called by a
+// converged warp; false when a wait ran out.
+template <int kStages, class Bytes>
+__device__ __forceinline__ bool pair_drain_loads(uint32_t cta, uint64_t* full, uint64_t* odd_done,
+                                                 uint32_t* odd_fills, uint32_t fills, Bytes bytes,
+                                                 uint64_t limit_ns) {
+  if ((cta & 1u) != 0) {
+    if (elect_one()) {
+      st_cluster_u32(mapa_shared(smem_u32(odd_fills), cta & ~1u), fills);
+      mbar_arrive_cluster(mapa_shared(smem_u32(odd_done), cta & ~1u));
+    }
+    __syncwarp();
+    return true;
+  }
+  // the odd CTA's producer ends within one wait of its own
+  bool ok = warp_wait_cluster_bounded(odd_done, 0, limit_times(limit_ns, 2));
+  const uint32_t said = ok ? *reinterpret_cast<volatile uint32_t*>(odd_fills) : fills;
+  const uint32_t theirs = __shfl_sync(0xFFFFFFFFu, said, 0);  // lane 0's wait saw it
+  if (elect_one()) {
+    for (uint32_t f = theirs; f < fills; ++f) mbar_complete_tx(&full[f % kStages], bytes(f));
+    for (uint32_t f = fills; f < theirs; ++f) mbar_arrive_expect_tx(&full[f % kStages], bytes(f));
+  }
+  __syncwarp();
+  const uint32_t most = fills > theirs ? fills : theirs;
+  for (uint32_t s = 0; s < kStages && s < most; ++s)
+    ok &= warp_wait_cluster_bounded(&full[s], ((most - 1 - s) / kStages) & 1u, limit_ns);
+  return ok;
+}
+
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_dst, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                    smem_u32(smem_dst)),
@@ -293,6 +344,23 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t cluster_addr) {
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
           cluster_addr)
       : "memory");
+}
+
+// How the MMA warp of a pair's even CTA ends: both CTAs' `teardown` barriers complete with its last
+// MMA, after every arrival that its commits owe either CTA; without any MMA (a commit would have
+// nothing to track), at once.  Called by a converged warp, by the lane that issued the MMAs.
+__device__ __forceinline__ void pair_commit_teardown(uint64_t* teardown, uint32_t cta, bool issued_any) {
+  const uint32_t own = smem_u32(teardown), odd = mapa_shared(smem_u32(teardown), cta | 1u);
+  if (elect_one()) {
+    if (issued_any) {
+      tc_commit_pair(own);
+      tc_commit_pair(odd);
+    } else {
+      mbar_arrive_cluster(own);
+      mbar_arrive_cluster(odd);
+    }
+  }
+  __syncwarp();
 }
 
 // Tiled tensor loads into this CTA's shared memory whose completion is counted

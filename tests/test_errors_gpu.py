@@ -140,3 +140,48 @@ def test_one_sm_gemm_gives_up_anywhere(kind, m, n, k):
     finally:
         _lib.call("fvq_set_gemm_pairing", 1)
         _lib.call("fvq_set_fp8_gemm_pairing", 1)
+
+
+@pytest.mark.parametrize("m,n,k", [(256, 256, 512), (512, 1024, 1536), (1536, 1536, 8960), (7680, 1536, 1536)])
+@pytest.mark.parametrize("kind", ["nvfp4", "nvfp4_replicated", "fp8", "bf16_product", "fp8_product", "gated_product"])
+def test_pair_gemm_gives_up_anywhere(kind, m, n, k):
+    """Either CTA of a pair may give up first, with loads of the other's on the way."""
+    from flashvsr_optimizations_b200 import _lib
+    if kind == "fp8" or kind == "fp8_product":
+        (a, sa), (w, sw) = fp8_rows(m, k, 1), fp8_rows(n, k, 2)
+        fn = ops.fp8_scaled_mm if kind == "fp8" else ops.fp8_scaled_mm_act
+
+        def call():
+            return fn(a, sa, w, sw)
+    elif kind.endswith("product"):
+        gated = kind == "gated_product"
+        x = torch.randn(m, k, generator=torch.Generator("cuda").manual_seed(1), device="cuda").to(torch.bfloat16)
+        w = torch.randn(n, k, generator=torch.Generator("cuda").manual_seed(2), device="cuda").to(torch.bfloat16)
+        r = torch.randn(m, n // (1 + gated), generator=torch.Generator("cuda").manual_seed(3), device="cuda")
+
+        def call():
+            return ops.linear_act(x, w, act="silu", gated=gated, residual=r.to(torch.bfloat16))
+    else:
+        (a, asf), (w, wsf) = _operands(m, n, k, seed=3)
+        g = torch.ones(1, device="cuda")
+        lib = _lib.load()
+        rep = torch.empty(lib.fvq_w_scales_replicated_bytes(n, k), dtype=torch.uint8, device="cuda")
+        st = torch.cuda.current_stream().cuda_stream
+        _lib.call("fvq_replicate_w_scales", wsf.data_ptr(), n, k, rep.data_ptr(), st)
+
+        def call():
+            if kind == "nvfp4":
+                return ops.nvfp4_gemm(a, asf, g, w, wsf, g)[0]
+            out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+            _lib.call("fvq_nvfp4_gemm_wrep", a.data_ptr(), asf.data_ptr(), g.data_ptr(), w.data_ptr(), rep.data_ptr(),
+                      g.data_ptr(), None, out.data_ptr(), m, n, k, st)
+            return out
+    _lib.call("fvq_set_gemm_pairing", 2 if kind == "nvfp4_replicated" else 1)
+    _lib.call("fvq_set_fp8_gemm_pairing", 2)
+    ops.set_linear_kernel(2)
+    try:
+        give_up(call, call())
+    finally:
+        _lib.call("fvq_set_gemm_pairing", 1)
+        _lib.call("fvq_set_fp8_gemm_pairing", 1)
+        ops.set_linear_kernel(0)
