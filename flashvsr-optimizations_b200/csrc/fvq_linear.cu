@@ -793,6 +793,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
+  uint64_t acc_limit = wait_limit;  // on the wait for the accumulator
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -823,7 +824,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     const uint32_t idesc = instr_desc<kF8>(p.wr, p.tn);
     int stage = 0;
     uint32_t phase = 0;
-    bool issued_any = false;
+    int done = 0;  // steps issued
     for (int i = 0; i < steps; ++i) {
       if (!warp_wait_bounded(&bars->full[stage], phase, wait_limit)) {
         warp_flag(abort_flag, a.err_word, kErrWaitMma);
@@ -846,14 +847,17 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         if (i == steps - 1) tc_commit(&bars->acc_full);
       }
       __syncwarp();
-      issued_any = true;
+      ++done;
       if (++stage == p.stages) {
         stage = 0;
         phase ^= 1u;
       }
     }
-    // as in the pair kernel, whether or not a warp has given up by now
-    if (issued_any) {
+    // Nothing issued may run on when TMEM and the ring go, whichever warp gives up, and when: the wait
+    // for acc_full below, or where that was not committed, one here.
+    if (done == steps) {
+      acc_limit = teardown_limit;
+    } else if (done > 0) {
       if (elect_one()) tc_commit(&bars->teardown);
       __syncwarp();
       if (!warp_wait_bounded(&bars->teardown, 0, teardown_limit))
@@ -863,7 +867,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   // ------------------------------------------------------------ partial sums to their owners
   // part[(source rank * own + t - owner's first token) * wr + row] of the owner of token t
   float* part = reinterpret_cast<float*>(smem + p.part_off);
-  if (!mbar_wait_bounded(&bars->acc_full, 0, wait_limit) &&
+  if (!mbar_wait_bounded(&bars->acc_full, 0, acc_limit) &&
       *reinterpret_cast<volatile int*>(abort_flag) == 0)
     flag(abort_flag, a.err_word, kErrWaitEpilogue);
   __syncwarp();
