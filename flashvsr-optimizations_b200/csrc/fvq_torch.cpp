@@ -17,10 +17,10 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/fvq.h"
@@ -35,12 +35,23 @@ struct Entries {
   decltype(&fvq_fp8_cache_read) cache_read = nullptr;
 } entries;
 
-// Whether something has to see the call that only the dispatcher shows it to: a dispatch or function
-// mode, torch.jit.trace (which would record the outputs as constants), a functorch transform.  All
-// but the first two are keys that the thread includes beside the ones it starts with.
+// Whether something has to see the call that only the dispatcher shows it to: a dispatch mode,
+// torch.jit.trace (which would record the outputs as constants) or a functorch transform, all of
+// them keys that the thread includes beside the ones it starts with; a function mode; a forward-mode
+// level, whose tangents the Python path refuses.
 bool interposed() {
-  return c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled() ||
-         !(c10::impl::tls_local_dispatch_key_set().included_ - c10::default_included_set).empty();
+  return !(c10::impl::tls_local_dispatch_key_set().included_ - c10::default_included_set).empty() ||
+         at::impl::torch_function_mode_enabled() ||
+         torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
+}
+
+// The keys of a strided CUDA tensor in memory; any other (a conjugate or negated view, zeros without
+// storage, a wrapper) makes it one for the dispatcher.
+bool plain_keys(const at::Tensor& t) {
+  constexpr c10::DispatchKeySet kPlain({c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA,
+                                        c10::DispatchKey::ADInplaceOrView, c10::DispatchKey::AutocastCUDA});
+  const c10::DispatchKeySet keys = t.key_set();
+  return (keys.raw_repr() & ~kPlain.raw_repr()) == 0 && keys.has(c10::DispatchKey::CUDA);
 }
 
 bool aligned(const at::Tensor& t, uintptr_t to) {
@@ -51,10 +62,9 @@ bool aligned(const at::Tensor& t, uintptr_t to) {
 const at::Tensor* plain(PyObject* obj, at::ScalarType type, c10::DeviceIndex dev) {
   if (!THPVariable_CheckExact(obj)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(obj);
-  if (!t.defined() || !t.is_cuda() || !t.has_storage() || t.layout() != at::kStrided || t.is_neg() ||
-      t._is_zerotensor() || t.scalar_type() != type || t.get_device() != dev)
+  if (!t.defined() || !plain_keys(t) || !t.has_storage() || t.scalar_type() != type || t.get_device() != dev)
     return nullptr;
-  if ((t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined()) return nullptr;
+  if (t.requires_grad() && c10::GradMode::is_enabled()) return nullptr;
   return &t;
 }
 
