@@ -9,7 +9,9 @@ from __future__ import annotations
 import ctypes
 import importlib.machinery
 import importlib.util
+import sys
 import threading
+import warnings
 from pathlib import Path
 
 _HERE = Path(__file__).resolve().parent
@@ -168,22 +170,40 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
 
 
 _binding = None
+_binding_missing = False
+
+
+def _load_binding():
+    import torch
+    loader = importlib.machinery.ExtensionFileLoader("_fvq_torch", str(BINDING_PATH))
+    mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_fvq_torch", loader))
+    loader.exec_module(mod)
+    here = f"{torch.__version__.split('+')[0]} {sys.version_info.major}.{sys.version_info.minor}"
+    built_for = getattr(mod, "built_for", "of unknown versions")
+    if built_for != here:
+        raise ImportError(f"built for torch and Python {built_for}, these are {here}")
+    lib = load()
+    mod.bind(*(ctypes.cast(getattr(lib, f"fvq_{n}"), _vp).value
+               for n in ("rms_norm", "linear_act", "fp8_scaled_mm_act", "fp8_cache_write",
+                         "fp8_cache_read")))
+    return mod
 
 
 def binding():
-    """The module _fvq_torch (csrc/fvq_torch.cpp), bound to libfvq.so's entry points."""
-    global _binding
-    if _binding is None:
-        if not BINDING_PATH.exists():
-            raise FileNotFoundError(
-                f"{BINDING_PATH} is missing: build it with `python flashvsr-optimizations_b200/build.py`")
-        lib = load()
-        loader = importlib.machinery.ExtensionFileLoader("_fvq_torch", str(BINDING_PATH))
-        mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_fvq_torch", loader))
-        loader.exec_module(mod)
-        mod.bind(*(ctypes.cast(getattr(lib, f"fvq_{n}"), _vp).value
-                   for n in ("rms_norm", "linear_act", "fp8_scaled_mm_act", "fp8_cache_write",
-                             "fp8_cache_read")))
+    """The module _fvq_torch (csrc/fvq_torch.cpp), bound to libfvq.so's entry points; None, after one
+    warning, where it is missing or was not built for this torch: the same kernels are then reached
+    through the registered operators, with more of the host's time a call."""
+    global _binding, _binding_missing
+    if _binding is None and not _binding_missing:
+        try:
+            mod = _load_binding()
+        except ImportError as e:
+            with _lock:
+                told, _binding_missing = _binding_missing, True
+            if not told:
+                warnings.warn(f"{BINDING_PATH.name} cannot be used ({e}): calls of the block operators take longer; "
+                              "build it with `python flashvsr-optimizations_b200/build.py`", RuntimeWarning, stacklevel=4)
+            return None
         with _lock:
             _binding = _binding or mod
     return _binding

@@ -22,6 +22,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include "../../include/fvq.h"
 
@@ -372,4 +373,17 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fvq_torch", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fvq_torch() { return PyModule_Create(&module); }
+#define FVQ_TEXT_(x) #x
+#define FVQ_TEXT(x) FVQ_TEXT_(x)
+
+PyMODINIT_FUNC PyInit__fvq_torch() {
+  PyObject* m = PyModule_Create(&module);
+  // compared by the loader: what is used of torch changes between its versions
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for",
+                                                 TORCH_VERSION " " FVQ_TEXT(PY_MAJOR_VERSION) "." FVQ_TEXT(
+                                                     PY_MINOR_VERSION)) != 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -650,7 +650,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(d
 
 
 def _fast():
-    """The short path's module; None while a graph is traced."""
+    """The short path's module; None while a graph is traced, and where there is none."""
     return None if torch.compiler.is_compiling() else (_lib._binding or _lib.binding())
 
 

@@ -198,3 +198,26 @@ def test_slots_refuse_what_is_no_table_and_positions():
                 (table, at.double()), (table, at.bool())):
         with pytest.raises(ValueError, match="FP8KVCache.slots"):
             cache.slots(*bad)
+
+
+@pytest.mark.parametrize("why", ["missing", "no library", "another torch"])
+def test_without_the_binding_the_registered_operators_serve(why, monkeypatch, tmp_path):
+    """One warning, and the calls go on as the registered operators take them."""
+    import warnings
+    path = tmp_path / "_fvq_torch.so"
+    if why == "no library":
+        path.write_bytes(b"not a library")
+    monkeypatch.setattr(_lib, "BINDING_PATH", _lib.BINDING_PATH if why == "another torch" else path)
+    if why == "another torch":
+        monkeypatch.setattr(torch, "__version__", "1.0.0")
+    monkeypatch.setattr(_lib, "_binding", None)
+    monkeypatch.setattr(_lib, "_binding_missing", False)
+    x = torch.zeros(4, 64, dtype=BF16)
+    with pytest.warns(RuntimeWarning, match="_fvq_torch.so cannot be used"):
+        with pytest.raises(RuntimeError, match="expected CUDA tensors"):
+            ops.rms_norm(x)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        with pytest.raises(RuntimeError, match="expected CUDA tensors"):
+            ops.linear_act(x, x)
+    assert _lib.binding() is None

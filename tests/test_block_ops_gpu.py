@@ -1113,3 +1113,23 @@ def test_tensors_without_memory_are_materialised():
     assert torch.equal(ops.rms_norm(x, zeros(64)), torch.zeros_like(x))
     assert torch.equal(ops.linear_act(x, w, zeros(16), residual=zeros(8, 16)), ops.linear_act(x, w))
     assert torch.equal(ops.linear_act(zeros(8, 64), w), torch.zeros(8, 16, dtype=BF16, device="cuda"))
+
+
+def test_without_the_binding(monkeypatch):
+    """The registered operators give the short path's results."""
+    from flashvsr_optimizations_b200 import _lib
+    x, r, w, m = randn(24, 64, seed=1), randn(24, 64, seed=2), randn(64, seed=3), randn(72, 64, seed=4)
+    cache, slots = store(3, 16, 1, 64), torch.arange(24, device="cuda")
+    table, lens = torch.arange(2, dtype=torch.int32, device="cuda").view(1, 2), torch.ones(1, dtype=torch.int32, device="cuda") * 24
+
+    def run():
+        y, s = ops.add_rms_norm(x, r, w)
+        q, scale = ops.rms_norm_fp8(s, w)
+        ops.fp8_cache_write(y.view(24, 1, 64), s.view(24, 1, 64), slots, *cache)
+        return (y, s, q.view(torch.uint8), scale, ops.linear_act(y, m, act="silu"),
+                ops.fp8_scaled_mm_act(q, scale, q, scale), *ops.fp8_cache_read(*cache, table, lens, 30))
+    want = run()
+    monkeypatch.setattr(_lib, "_binding", None)
+    monkeypatch.setattr(_lib, "_binding_missing", True)
+    for a, b in zip(want, run()):
+        assert torch.equal(a, b)
