@@ -170,3 +170,17 @@ def test_fp8_entry_points_check_arguments():
     l2 = _lib.FvqLinearFp8(b, b, None, 8960, 1536)
     assert _rc("fvq_fp8_ffn", b, 4, ctypes.byref(l1), ctypes.byref(l2), b, b, 16,
                None) == _lib.FVQ_EWORKSPACE
+
+
+def test_build_script_without_torch(monkeypatch, capsys):
+    """The C ABI builds where torch is not installed; only the torch binding is left out."""
+    import importlib.util
+    import sys
+    spec = importlib.util.spec_from_file_location("fvq_build", _lib.LIB_PATH.parent / "build.py")
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    monkeypatch.setattr(mod, "build", lambda *args: mod.LIB)
+    monkeypatch.setitem(sys.modules, "torch", None)
+    mod.main([])
+    out = capsys.readouterr().out
+    assert "libfvq.so" in out and "_fvq_torch.so not built" in out
