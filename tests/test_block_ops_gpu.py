@@ -1133,3 +1133,29 @@ def test_without_the_binding(monkeypatch):
     monkeypatch.setattr(_lib, "_binding_missing", True)
     for a, b in zip(want, run()):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- bf16 and E4M3 from one call of the C entry
+# rows of 8, 16 and 32 lanes, with one and two rows a group; a CTA a row of 8 and of 16 values a thread; streamed by
+# one to sixteen warps a row; each on and off 16 bytes
+@pytest.mark.parametrize("rows,d", [(7, 33), (5, 64), (20000, 64), (9, 128), (40000, 121), (3, 256), (20000, 250), (6, 512),
+                                    (20000, 511), (2, 1536), (3, 2047), (1, 16384), (5, 9001), (5001, 1536), (4800, 2047),
+                                    (2400, 4096), (1200, 8200), (700, 16384), (700, 16383)])
+@pytest.mark.parametrize("residual", [None, BF16, F32], ids=["none", "bf16", "fp32"])
+def test_norm_with_both_outputs(rows, d, residual):
+    from flashvsr_optimizations_b200 import _lib
+    x, w = randn(rows, d, seed=1, std=2.0), randn(d, seed=2)
+    r = None if residual is None else randn(rows, d, seed=3, dtype=residual)
+    y, new = torch.empty_like(x), None if r is None else torch.empty_like(r)
+    q, scale = torch.empty_like(x, dtype=F8), torch.empty(rows, 1, device="cuda")
+    _lib.call("fvq_rms_norm", x.data_ptr(), rows, 1, d, 0, d, w.data_ptr(), 1e-6, None if r is None else r.data_ptr(),
+              int(residual == F32), None if r is None else new.data_ptr(), y.data_ptr(), q.data_ptr(), scale.data_ptr(),
+              torch.cuda.current_stream().cuda_stream)
+    s, v = norm64(x, r, w, 1e-6)
+    tol = 2.0 ** -17
+    if r is not None:
+        assert torch.equal(new, (x.float() + r.float()).to(residual))
+    inside(y, v, v.abs() * (HALF_BF16 + tol))
+    want = (v.abs().amax(-1, keepdim=True) / 448).clamp_min(1e-12)
+    inside(scale, want, want * tol)
+    codes_inside(q, scale, v, tol)
