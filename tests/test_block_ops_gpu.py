@@ -1159,3 +1159,23 @@ def test_norm_with_both_outputs(rows, d, residual):
     want = (v.abs().amax(-1, keepdim=True) / 448).clamp_min(1e-12)
     inside(scale, want, want * tol)
     codes_inside(q, scale, v, tol)
+
+
+@pytest.mark.parametrize("limit", [1, 1000, 1500, 2000, 3000, 5000, 10000])
+@pytest.mark.parametrize("m,n,k,gated", [(1, 264, 1536, False), (2, 3000, 8960, True), (1, 80000, 64, False),
+                                         (1, 12288, 4096, False)])
+def test_product_few_rows_right_whatever_the_wait_limit(m, n, k, gated, limit):
+    """A wait that runs out is reported and waited for again before its slot is read: the result is right either way."""
+    x, w = randn(m, k, seed=1), randn(2 * n if gated else n, k, seed=2, std=k ** -0.5)
+    xq, wq = ops.fp8_row_quant(x), ops.fp8_row_quant(w)
+    calls = (lambda: ops.linear_act(x, w, act="silu", gated=gated),
+             lambda: ops.fp8_scaled_mm_act(*xq, *wq, act="silu", gated=gated))
+    want = [call() for call in calls]
+    ops.set_wait_limit(limit)
+    try:
+        for call, y in zip(calls, want):
+            got = call()
+            assert ops.read_device_error() in (0, 1)         # bit 0: a load's wait
+            assert torch.equal(got, y)
+    finally:
+        ops.set_wait_limit(0)
