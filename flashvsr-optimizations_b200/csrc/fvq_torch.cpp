@@ -90,6 +90,13 @@ const T* in(const at::Tensor* t) {
 
 void* stream_of(c10::DeviceIndex dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
 
+// Releases the interpreter's lock; taken again before an exception (a tensor whose memory may not be
+// written throws at data_ptr) becomes a Python error.
+struct Unlocked {
+  PyThreadState* const state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 // The device the fast path works on, or -1 when nothing is to be done here.
 c10::DeviceIndex usable_device(const void* entry, PyObject* first) {
   if (entry == nullptr || !THPVariable_CheckExact(first) || interposed()) return -1;
@@ -144,14 +151,15 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
   }
   if (r != nullptr) fresh = output(*x, sizes, r->scalar_type());
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = entries.rms_norm(in<uint16_t>(x), rows, inner, outer, step, d, in<uint16_t>(w),
-                        static_cast<float>(eps), ptr(r), f32 ? 1 : 0,
-                        r != nullptr ? fresh.data_ptr() : nullptr,
-                        fp8 ? nullptr : static_cast<uint16_t*>(y.data_ptr()),
-                        fp8 ? static_cast<uint8_t*>(y.data_ptr()) : nullptr,
-                        fp8 ? static_cast<float*>(scale.data_ptr()) : nullptr, stream_of(dev));
-  Py_END_ALLOW_THREADS
+  {
+    const Unlocked unlocked;
+    rc = entries.rms_norm(in<uint16_t>(x), rows, inner, outer, step, d, in<uint16_t>(w),
+                          static_cast<float>(eps), ptr(r), f32 ? 1 : 0,
+                          r != nullptr ? fresh.data_ptr() : nullptr,
+                          fp8 ? nullptr : static_cast<uint16_t*>(y.data_ptr()),
+                          fp8 ? static_cast<uint8_t*>(y.data_ptr()) : nullptr,
+                          fp8 ? static_cast<float*>(scale.data_ptr()) : nullptr, stream_of(dev));
+  }
   if (rc != FVQ_OK) Py_RETURN_NONE;  // the Python path repeats the call and raises
   PyObject* out = PyTuple_New(3);
   if (out == nullptr) return nullptr;
@@ -210,11 +218,12 @@ PyObject* py_linear_act(PyObject*, PyObject* const* args, Py_ssize_t count) {
   const int act = static_cast<int>(PyLong_AsLong(args[3]));
   at::Tensor y = output(*x, p.out, at::kBFloat16);
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = entries.linear_act(in<uint16_t>(x), p.m, p.k, p.stride, in<uint16_t>(w), p.n, in<uint16_t>(bias),
-                          act, gated ? 1 : 0, in<uint16_t>(residual), static_cast<uint16_t*>(y.data_ptr()),
-                          stream_of(dev));
-  Py_END_ALLOW_THREADS
+  {
+    const Unlocked unlocked;
+    rc = entries.linear_act(in<uint16_t>(x), p.m, p.k, p.stride, in<uint16_t>(w), p.n, in<uint16_t>(bias),
+                            act, gated ? 1 : 0, in<uint16_t>(residual), static_cast<uint16_t*>(y.data_ptr()),
+                            stream_of(dev));
+  }
   if (rc != FVQ_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
@@ -241,12 +250,13 @@ PyObject* py_fp8_scaled_mm_act(PyObject*, PyObject* const* args, Py_ssize_t coun
   const int act = static_cast<int>(PyLong_AsLong(args[5]));
   at::Tensor y = output(*a, p.out, at::kBFloat16);
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = entries.fp8_scaled_mm_act(in<uint8_t>(a), in<float>(sa), p.m, p.k, p.stride, in<uint8_t>(w),
-                                 in<float>(sw), p.n, in<uint16_t>(bias), act, gated ? 1 : 0,
-                                 in<uint16_t>(residual), static_cast<uint16_t*>(y.data_ptr()),
-                                 stream_of(dev));
-  Py_END_ALLOW_THREADS
+  {
+    const Unlocked unlocked;
+    rc = entries.fp8_scaled_mm_act(in<uint8_t>(a), in<float>(sa), p.m, p.k, p.stride, in<uint8_t>(w),
+                                   in<float>(sw), p.n, in<uint16_t>(bias), act, gated ? 1 : 0,
+                                   in<uint16_t>(residual), static_cast<uint16_t*>(y.data_ptr()),
+                                   stream_of(dev));
+  }
   if (rc != FVQ_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
@@ -284,13 +294,14 @@ PyObject* py_cache_write(PyObject*, PyObject* const* args, Py_ssize_t count) {
       slots->size(0) != k->size(0))
     Py_RETURN_NONE;
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = entries.cache_write(in<uint16_t>(k), in<uint16_t>(v), k->size(0), k->size(1), k->size(2),
-                           k->stride(0), k->stride(1), v->stride(0), v->stride(1), in<int64_t>(slots),
-                           static_cast<uint8_t*>(t[0]->data_ptr()), static_cast<float*>(t[1]->data_ptr()),
-                           static_cast<uint8_t*>(t[2]->data_ptr()), static_cast<float*>(t[3]->data_ptr()),
-                           t[0]->size(0) * t[0]->size(1), stream_of(dev));
-  Py_END_ALLOW_THREADS
+  {
+    const Unlocked unlocked;
+    rc = entries.cache_write(in<uint16_t>(k), in<uint16_t>(v), k->size(0), k->size(1), k->size(2),
+                             k->stride(0), k->stride(1), v->stride(0), v->stride(1), in<int64_t>(slots),
+                             static_cast<uint8_t*>(t[0]->data_ptr()), static_cast<float*>(t[1]->data_ptr()),
+                             static_cast<uint8_t*>(t[2]->data_ptr()), static_cast<float*>(t[3]->data_ptr()),
+                             t[0]->size(0) * t[0]->size(1), stream_of(dev));
+  }
   if (rc != FVQ_OK) Py_RETURN_NONE;
   for (const auto* s : t)  // written in place
     if (!s->is_inference()) s->unsafeGetTensorImpl()->bump_version();
@@ -316,13 +327,14 @@ PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t count) {
   const int64_t sizes[4] = {table->size(0), max_len, t[0]->size(2), t[0]->size(3)};
   at::Tensor k = output(*t[0], sizes, at::kBFloat16), v = output(*t[0], sizes, at::kBFloat16);
   int rc;
-  Py_BEGIN_ALLOW_THREADS
-  rc = entries.cache_read(in<uint8_t>(t[0]), in<float>(t[1]), in<uint8_t>(t[2]), in<float>(t[3]),
-                          t[0]->size(0), t[0]->size(1), sizes[2], sizes[3], in<int32_t>(table), sizes[0],
-                          table->size(1), in<int32_t>(lengths), max_len,
-                          static_cast<uint16_t*>(k.data_ptr()), static_cast<uint16_t*>(v.data_ptr()),
-                          stream_of(dev));
-  Py_END_ALLOW_THREADS
+  {
+    const Unlocked unlocked;
+    rc = entries.cache_read(in<uint8_t>(t[0]), in<float>(t[1]), in<uint8_t>(t[2]), in<float>(t[3]),
+                            t[0]->size(0), t[0]->size(1), sizes[2], sizes[3], in<int32_t>(table), sizes[0],
+                            table->size(1), in<int32_t>(lengths), max_len,
+                            static_cast<uint16_t*>(k.data_ptr()), static_cast<uint16_t*>(v.data_ptr()),
+                            stream_of(dev));
+  }
   if (rc != FVQ_OK) Py_RETURN_NONE;
   PyObject* out = PyTuple_New(2);
   if (out == nullptr) return nullptr;

@@ -1179,3 +1179,14 @@ def test_product_few_rows_right_whatever_the_wait_limit(m, n, k, gated, limit):
             assert torch.equal(got, y)
     finally:
         ops.set_wait_limit(0)
+
+
+def test_a_store_that_may_not_be_written_raises():
+    """torch can mark a tensor's memory so that asking for a pointer to write throws."""
+    cache = store(2, 4, 1, 64)
+    x, slots = randn(3, 1, 64), torch.arange(3, device="cuda")
+    torch._C._set_throw_on_mutable_data_ptr(cache[0])
+    with pytest.raises(RuntimeError):
+        ops.fp8_cache_write(x, x, slots, *cache)
+    cache = store(2, 4, 1, 64)
+    ops.fp8_cache_write(x, x, slots, *cache)                 # the interpreter goes on
