@@ -36,7 +36,8 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Division by a fixed divisor, exact below 2^31.
+// Division by a fixed divisor, exact below 2^31 (Granlund and Montgomery, "Division by invariant
+// integers using multiplication", 1994).
 struct Divider {
   uint32_t d, mul;
   int shift;

@@ -1,12 +1,13 @@
 // fvq_launch.h -- launches of the block operators' kernels.
 //
 // They follow one another in a block, each a few microseconds long at a few rows, so every one
-// is launched as a programmatic dependent of the kernel before it: it lets the next one start
-// setting up (grid_launch_dependents) and waits for the previous one to complete
-// (grid_dependency_wait) before any of its threads touches global memory.  A kernel may so be
-// running while another writes what it is going to read: it reads with ordinary loads, never
-// through the read-only path (__ldg, ld.global.nc, __restrict__), whose lines nothing promises
-// to refresh inside a running kernel.
+// is launched as a programmatic dependent of the kernel before it.  All but the streaming norm,
+// which lost by it, let the next one start setting up (grid_launch_dependents).  Each waits for the
+// previous one to complete (grid_dependency_wait) before any of its threads reads or writes global
+// memory; the product of one or two rows sends L2 prefetches of W ahead of that wait, which read
+// nothing.  A kernel may so be running while another writes what it is going to read: it reads
+// with ordinary loads, never through the read-only path (__ldg, ld.global.nc, __restrict__),
+// whose lines nothing promises to refresh inside a running kernel.
 #pragma once
 
 #include <cuda_runtime.h>

@@ -27,13 +27,14 @@
 //
 // Measured on a B200, launches back to back in a CUDA graph, operands larger than L2 in all
 // (a copy moves 6.5 TB/s, torch's bf16 product reaches 1672 TFLOP/s for a moment, 1398 for seconds):
-//   pair    (m x k -> n) bf16 15360 x 8960 -> 1536 with residual: 270 us (1.56 PFLOP/s; the tensor
-//           pipe 80% active).  E4M3 gated 7680 x 1536 -> 2 * 8960: 165 to 215 us with the clock
-//           (2.0 to 2.6 PFLOP/s; tensor pipe 72%); the epilogue's arithmetic shares issue slots
-//           and power with it (7680 x 1536 -> 2 * 4480: 75 us without an activation, 84 with one).
-//   split   24 x 8960 -> 1536: E4M3 7.0 us (13.8 MB of W: 2.1 us at a copy's rate; the rest is the
-//           start, the exchange of partial sums and the epilogue), bf16 9.2; 24 x 1536 -> 8960:
-//           6.1 and 8.0.
+//   pair    (m x k -> n) bf16 15360 x 8960 -> 1536 with residual: 270 to 280 us (1.51 to
+//           1.56 PFLOP/s).  E4M3 gated 7680 x 1536 -> 2 * 8960: 165 to 215 us with the clock (2.0
+//           to 2.6 PFLOP/s).  At 4096 rows of the same products the tensor pipe is 80% and 72%
+//           active; the epilogue's arithmetic shares issue slots and power with it (7680 x 1536
+//           -> 2 * 4480: 75 us without an activation, 84 with one).
+//   split   24 x 8960 -> 1536: E4M3 7.0 us, with bias and residual 7.5 (13.8 MB of W: 2.1 us at a
+//           copy's rate; the rest is the start, the exchange of partial sums and the epilogue),
+//           bf16 9.2 and 9.7; 24 x 1536 -> 8960: 6.1 and, bf16, 8.0.
 //   vector  bf16 1 x 1536 -> 8960: 7.2 us, 1 x 8960 -> 1536: 6.8 us (27.5 MB, 4.0 TB/s, about
 //           2.5 us of it start and end), 1 x 4096 -> 12288: 17.1 us (5.9 TB/s).
 #include <cuda.h>

@@ -312,7 +312,8 @@ __device__ __forceinline__ float row_reduce(float v, float* smem, Op op) {
 
 __device__ __forceinline__ const uint16_t* x_row(const NormArgs& a, int64_t row) {
   if (a.inner == 1) return a.x + row * a.outer_stride;
-  // row / inner, exact below 2^31: (n + umulhi(n, m)) >> l with m, l of the launcher
+  // row / inner, exact below 2^31 (Granlund and Montgomery, "Division by invariant integers using
+  // multiplication", 1994): (n + umulhi(n, m)) >> l with m, l of the launcher
   const uint32_t n = static_cast<uint32_t>(row);
   const uint32_t outer = (n + __umulhi(n, a.inner_mul)) >> a.inner_shift;
   const uint32_t in = n - outer * static_cast<uint32_t>(a.inner);
@@ -715,7 +716,7 @@ cudaError_t launch_rms_norm(const NormArgs& args, uint64_t wait_limit, cudaStrea
   if (d <= 256) return norm_short<32>(a, vec, st);
   if (d <= 512) return norm_short<32, 16>(a, vec, st);
   {
-    // warps per row: rings of two rows per group within the shared memory, 64 values a lane
+    // warps per row: rings of two rows per group within the shared memory, 72 values a lane
     StreamPlan p;
     const int res = a.residual == nullptr ? 0 : a.residual_f32 ? 4 : 2, slack = vec ? 0 : 16;
     p.x_bytes = (2 * d + slack + 15) / 16 * 16;

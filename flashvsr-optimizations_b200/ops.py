@@ -768,7 +768,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor |
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor | None = None,
                  eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
     """(q float8_e4m3fn like x, scale fp32 [..., 1]): rms_norm's fp32 value v quantized with one scale
-    per row, scale = max(max|v| / 448, 1e-12), q = v / scale -- the input of ``fp8_scaled_mm`` and
+    per row, scale = max(max|v| / 448, 1e-12), q = v * (1 / scale) -- the input of ``fp8_scaled_mm`` and
     ``fp8_scaled_mm_act`` without a bf16 copy in between."""
     fast = _fast()
     got = fast.rms_norm(x, weight, None, eps, True) if fast else None
@@ -990,7 +990,7 @@ def fp8_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cod
     k, v: bf16 [tokens, heads, d] (strided views of a fused projection are read in place); codes
     float8_e4m3fn [pages, page, heads, d] and scales fp32 [pages, page, heads], written in place.
     Token t goes to slot slots[t] = page index * page + offset (int64): one scale per token and
-    head, scale = max(max|x| / 448, 1e-12), q = x / scale.  A negative slot is padding (nothing is
+    head, scale = max(max|x| / 448, 1e-12), q = x * (1 / scale).  A negative slot is padding (nothing is
     stored); one past the store is skipped and sets bit 6 of ``read_device_error()``.  The slots
     of one call must differ: what a repeated slot then holds is undefined."""
     fast = _fast()
@@ -1041,7 +1041,9 @@ def read_device_error(device: torch.device | None = None) -> int:
 
 def set_linear_kernel(mode: int) -> None:
     """Which kernel ``linear_act`` and ``fp8_scaled_mm_act`` run: 0 by size (default), 1 the split
-    kernel (few rows), 2 the SM-pair kernel, whatever the number of rows."""
+    kernel (few rows), 2 the SM-pair kernel, whatever the number of rows.  For tests and
+    measurements: like the other settings of the library it is the process's, and changes the
+    kernel, and with it the order of the sums, for every caller."""
     _lib.call("fvq_set_linear_kernel", mode)
 
 

@@ -425,18 +425,20 @@ int fvq_fp8_scaled_mm_act(const uint8_t* a, const float* scale_a, int64_t m, int
                           uint16_t* y, void* stream);
 
 /*
- * Library setting: which kernel fvq_linear_act and fvq_fp8_scaled_mm_act run: 0 (the default)
- * by size, 1 the split kernel (few rows), 2 the SM-pair kernel, whatever the number of rows.  Applies to later launches
- * from any thread.
+ * Library setting, for tests and measurements: which kernel fvq_linear_act and
+ * fvq_fp8_scaled_mm_act run: 0 (the default) by size, 1 the split kernel (few rows), 2 the SM-pair
+ * kernel, whatever the number of rows.  Process-wide: it applies to later launches from any
+ * thread, and changes the order of their sums over k.
  */
 int fvq_set_linear_kernel(int mode);
 
 /*
  * Paged FP8 store of attention keys and values: codes E4M3 [num_slots, heads, d], scales fp32
  * [num_slots, heads], `page` consecutive slots being one page.  A row of k and v (one token,
- * one head) is stored as fvq_fp8_row_quantize's formula has it,
+ * one head) is stored with a scale of its own,
  *   scale = max(max|x| / 448, 1e-12),  q = e4m3_rn(x * (1 / scale)),
- * and read back as bf16(q * scale).
+ * and read back as bf16(q * scale).  (fvq_fp8_row_quantize divides by the scale: the codes differ
+ * where the quotient lies within 2^-24 of the middle between two of them.)
  *
  * write: token t goes to slot slots[t] (device int64); a negative slot is padding and stores
  * nothing; a slot >= num_slots stores nothing and sets bit 6 of the device error word
